@@ -1,0 +1,571 @@
+"""Performance cases of the language-model serving operators (parakeet_amd.lm): what a decoder-only model
+that follows the speech decoder needs beside its matrix products.
+
+  plan     page tables and slot maps from request lengths (lm.kv_plan)
+  store    rows into the 4-bit paged cache and back out of it (lm.kv4_store, lm.kv4_load)
+  attend   attention over that cache, single tokens and whole prompts (lm.kv4_attend)
+  sample   temperature, top-k, top-p and min-p from given uniform numbers (lm.sample)
+
+`own` chooses between the plain forms below (elementary torch operations, 32 bits) and the framework's kernels.
+
+The cache.  Channels are held in blocks of 32: four-bit floating point codes (sign, values 0 .5 1 1.5 2 3 4 6) and
+one power-of-two scale byte 2^(b - 127) a block; b = 255 marks a block that held a NaN or an infinity.  A page holds
+`page` tokens; a (page, kv head) record is K codes [page][D/2] | V codes [page/8][16][8][D/32] | K scales
+[page][D/32] | V scales [D/32][page].  In the V codes, entry [a][r][i] has the D/16 channels from r D/16 of token
+8a + i; low nibbles come first.
+"""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+SIZEOF = {"f32": 4, "f16": 2, "bf16": 2}
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+# ---- the cases ----
+
+def listed():
+    return [
+        # one live session takes its next token: the page plan of every decode step, where only latency counts
+        dict(name="plan_one", kind="plan", requests=1, length=700, fresh=0.0, page=64),
+        # a full server's step: most of 512 sessions take a token, some bring prompts, some shrink or end
+        dict(name="plan_sessions", kind="plan", requests=512, length=8191, fresh=0.06, page=16),
+        # the new tokens' rows of 64 sessions, one layer of one decode step
+        dict(name="store_step", kind="store", tokens=64, heads=8, dim=128, dtype="bf16", page=64),
+        # one layer of a batch of prompts, rows cut out of a joint QKV product
+        dict(name="store_prompts", kind="store", tokens=24577, heads=8, dim=128, dtype="bf16", page=64),
+        # one live session's next token, a short turn, the smaller model width of the speech encoders (512 = 8 x 64)
+        dict(name="attend_one", kind="attend", requests=1, new=1, length=733, heads=8, kv_heads=8, dim=64, dtype="bf16",
+             page=64, window=0),
+        # a server's decode step: 64 sessions of uneven length, one of them still empty
+        dict(name="attend_sessions", kind="attend", requests=64, new=1, length=4097, heads=32, kv_heads=8, dim=128,
+             dtype="bf16", page=64, window=0),
+        # two day-long transcripts held as context, few rows and a long axis
+        dict(name="attend_long", kind="attend", requests=2, new=1, length=200003, heads=16, kv_heads=2, dim=128,
+             dtype="f16", page=128, window=0),
+        # prompts of uneven length, some behind what their session already holds (1024 = 8 x 128 wide, 32 heads on 8)
+        dict(name="attend_prompts", kind="attend", requests=4, new=2047, length=4095, heads=32, kv_heads=8, dim=128,
+             dtype="bf16", page=64, window=0),
+        # one live session's token: the speech decoder's own 8193 token logits, cut out of its joint rows
+        dict(name="sample_one", kind="sample", rows=1, vocab=8193, pad=5, dtype="f32", filters="both"),
+        # 512 sessions over the turn-taking model's vocabulary, each with its own settings
+        dict(name="sample_sessions", kind="sample", rows=512, vocab=1027, pad=0, dtype="f32", filters="mixed"),
+        # one session, a large vocabulary, top-p alone
+        dict(name="sample_large_one", kind="sample", rows=1, vocab=128001, pad=0, dtype="bf16", filters="top_p"),
+        # a server's step over a large vocabulary, each row with its own settings
+        dict(name="sample_large_64", kind="sample", rows=64, vocab=128001, pad=0, dtype="bf16", filters="mixed"),
+    ]
+
+
+def draw(rng):
+    def log(lo, hi):
+        return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+    kind = rng.choice(("plan", "store", "attend", "attend", "attend", "sample", "sample"))
+    if kind == "plan":
+        return dict(kind=kind, requests=log(1, 512), length=log(16, 8191), fresh=rng.choice((0.0, 0.02, 0.06)),
+                    page=rng.choice((16, 32, 64, 128, 256)))
+    dim = rng.choice((64, 128, 128, 256))
+    page = rng.choice((16, 32, 64, 128, 256))
+    dtype = rng.choice(("bf16", "f16"))
+    if kind == "store":
+        heads = rng.choice((1, 2, 3, 4, 8))
+        return dict(kind=kind, tokens=log(1, 24577 * 1024 // (heads * dim) // 2), heads=heads, dim=dim,
+                    dtype=rng.choice(("bf16", "f16", "f32")), page=page)
+    if kind == "attend":
+        kv_heads = rng.choice((1, 2, 4, 8))
+        heads = kv_heads * rng.choice((1, 2, 3, 4, 8))
+        window = rng.choice((0, 0, 0, log(1, 2000)))
+        width = kv_heads * dim
+        if rng.random() < 0.6:      # decode steps, one token or a few drafted ones
+            requests = log(1, 512)
+            return dict(kind=kind, requests=requests, new=rng.choice((1, 1, 1, 2, 5)),
+                        length=log(5, max(6, min(200003, 64 * 4097 * 1024 // (2 * width * requests)))), heads=heads,
+                        kv_heads=kv_heads, dim=dim, dtype=dtype, page=page, window=window)
+        requests = log(1, 16)
+        new = log(16, 2047)
+        most = int(4 * 2047 * 4095 * 32 * 128 / (4.0 * requests * new * heads * dim))
+        return dict(kind=kind, requests=requests, new=new, length=log(new, max(new + 1, min(16384, most))), heads=heads,
+                    kv_heads=kv_heads, dim=dim, dtype=dtype, page=page, window=window)
+    vocab = log(64, 200001)
+    return dict(kind=kind, rows=log(1, min(512, max(1, 64 * 128001 // vocab))), vocab=vocab, pad=rng.choice((0, 0, 5, 64)),
+                dtype=rng.choice(("f32", "f16", "bf16")), filters=rng.choice(("none", "top_k", "top_p", "both", "mixed")))
+
+
+# ---- their inputs ----
+
+def _pages(length, page):
+    return (length + page - 1) // page
+
+
+def _lengths(case, g):
+    """(new tokens, tokens held with them) of each request, on the host: spread evenly up to what the case allows, in an
+    order and with offsets of the seed's; the first as long as allowed, and one empty where there are many."""
+    B, q, n = case["requests"], case["new"], case["length"]
+
+    def spread(most):
+        rank = torch.cat([torch.tensor([B]), torch.randperm(B - 1, generator=g) + 1])
+        return (most * rank // B).clamp(min=1)
+
+    news = spread(q) if q > 8 else torch.full((B,), q)
+    lens = spread(n)
+    lens[1:] -= torch.randint(0, n // (4 * B) + 1, (B - 1,), generator=g)
+    lens = torch.maximum(lens, news)
+    if B > 8:
+        lens[B // 2] = 0      # a session that holds nothing yet: its queries see no key
+    return news, lens
+
+
+def prepare(case, seed):
+    return globals()["_prepare_" + case["kind"]](case, torch.Generator().manual_seed(seed),
+                                                 torch.Generator("cuda").manual_seed(seed))
+
+
+def _fresh(case):
+    return int(round(case["fresh"] * case["requests"]))
+
+
+def _tokens(case):
+    return case["requests"] + _fresh(case) * case["length"]
+
+
+def _prepare_plan(case, g, gd):
+    B, n, page = case["requests"], case["length"], case["page"]
+    width = _pages(n, page) + 1
+    old = torch.randint(1, n, (B,), generator=g)
+    new = old + 1                                                      # a token each
+    order, ends = torch.randperm(B, generator=g), B // 32
+    fresh = order < _fresh(case)
+    new = torch.where(fresh, old, new)                                 # whole prompts, from nothing
+    old = torch.where(fresh, 0, old)
+    new = torch.where(order >= B - ends, torch.where(order % 2 == 0, 0, old // 2), new)    # ended, or cut back
+    held = _pages(old, page)
+    total = int(held.sum())
+    n_pages = B * width + 8
+    ids = torch.randperm(n_pages, generator=g)
+    table = torch.zeros(B, width, dtype=torch.int64)
+    mask = torch.arange(width) < held[:, None]
+    table[mask] = ids[:total]
+    free = n_pages - total
+    head = int(torch.randint(0, n_pages, (1,), generator=g))
+    ring = torch.zeros(n_pages, dtype=torch.int64)
+    ring[(head + torch.arange(free)) % n_pages] = ids[total:]
+    cap = _tokens(case)                                                # the slot map is padded, as a captured graph has it
+    dev = lambda t: t.to(torch.int32).cuda()  # noqa: E731
+    empty = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    return dict(kind="plan", page=page, old=dev(old), new=dev(new), table=dev(table), ring=dev(ring),
+                state=dev(torch.tensor([head, free])), state_out=empty(2), lens=empty(B), ok=empty(B), first=empty(B + 1),
+                slots=empty(cap), pos=empty(cap))
+
+
+def _prepare_store(case, g, gd):
+    N, H, D, page = case["tokens"], case["heads"], case["dim"], case["page"]
+    n_pages = _pages(N, page) + 3
+    rows = torch.randn(N, 3, H, D, generator=gd, device="cuda")        # K and V are cut out of a joint QKV product
+    rows *= torch.exp(0.7 * torch.randn(1, 3, H, D, generator=gd, device="cuda"))     # channels of uneven size
+    rows = rows.to(DTYPES[case["dtype"]])
+    slots = torch.randperm(n_pages * page, generator=g)[:N] if N < 512 else torch.randperm(n_pages, generator=g)[
+        torch.arange(N) // page] * page + torch.arange(N) % page
+    slots = slots.to(torch.int32).cuda()
+    cache = torch.zeros(n_pages, H, page * (D + D // 16), dtype=torch.uint8, device="cuda")
+    back = torch.zeros(2, N, H, D, dtype=rows.dtype, device="cuda")
+    return dict(kind="store", page=page, k=rows[:, 1], v=rows[:, 2], slots=slots, cache=cache, k_back=back[0], v_back=back[1])
+
+
+def _prepare_attend(case, g, gd):
+    B, Hq, H, D, page = case["requests"], case["heads"], case["kv_heads"], case["dim"], case["page"]
+    news, lens = _lengths(case, g)
+    held = _pages(lens, page)
+    total = int(held.sum())
+    n_pages = total + 2
+    ids = torch.randperm(n_pages, generator=g)
+    table = torch.zeros(B, _pages(case["length"], page) + 1, dtype=torch.int64)
+    table[torch.arange(table.shape[1]) < held[:, None]] = ids[:total]
+    cache = torch.zeros(n_pages, H, page * (D + D // 16), dtype=torch.uint8, device="cuda")
+    size = torch.exp(0.7 * torch.randn(2, 1, H, D, generator=gd, device="cuda"))      # channels of uneven size
+    step = max(1, (1 << 26) // (page * H * D))
+    for p in range(0, n_pages, step):
+        n = min(step, n_pages - p)
+        kv = torch.randn(2, n * page, H, D, generator=gd, device="cuda") * size
+        cache[p:p + n] = _records(kv[0], kv[1], page)
+    first = torch.zeros(B + 1, dtype=torch.int64)
+    first[1:] = torch.cumsum(news, 0)
+    N = int(first[-1])
+    q = torch.randn(N, Hq + 2 * H, D, generator=gd, device="cuda").to(DTYPES[case["dtype"]])[:, :Hq]
+    out = torch.zeros(N, Hq, D, dtype=q.dtype, device="cuda")
+    return dict(kind="attend", page=page, window=case["window"], scale=1.0 / math.sqrt(D), q=q, cache=cache, max_new=case["new"],
+                max_len=case["length"], table=table.to(torch.int32).cuda(), lens=lens.to(torch.int32).cuda(),
+                first=first.to(torch.int32).cuda(), out=out, lse=torch.zeros(N, Hq, device="cuda"))
+
+
+def _prepare_sample(case, g, gd):
+    B, V = case["rows"], case["vocab"]
+    x = torch.randn(B, V + case["pad"], generator=gd, device="cuda") * 2.0
+    top = torch.randint(0, V, (B, 12), generator=gd, device="cuda")    # what the model has in mind, over a broad tail
+    x.scatter_add_(1, top, 6.0 * torch.rand(B, 12, generator=gd, device="cuda") + 3.0)
+    x[torch.rand(x.shape, generator=gd, device="cuda") < 0.03] = -math.inf      # tokens that the caller bars
+    x = x.to(DTYPES[case["dtype"]])[:, :V]
+    u = torch.rand(B, generator=gd, device="cuda")
+    f, r = case["filters"], torch.rand(4, B, generator=g)
+    temperature = 0.5 + 0.8 * r[0]
+    top_k = torch.where(r[1] < 0.5, 50, 1 + (r[1] * 200).long())
+    top_p = 0.8 + 0.19 * r[2]
+    min_p = torch.where(r[3] < 0.5, 0.05, 0.1 * r[3])
+    row = torch.arange(B)
+    if f in ("none", "top_p"):
+        top_k = torch.zeros_like(top_k)
+    if f in ("none", "top_k"):
+        top_p = torch.ones_like(top_p)
+    if f != "mixed":
+        min_p = torch.zeros_like(min_p)
+    else:                                                              # each row its own kind of filter, some greedy
+        top_k = torch.where(row % 4 < 2, top_k, 0)
+        top_p = torch.where(row % 4 % 3 == 0, 1.0, top_p)
+        min_p = torch.where(row % 8 == 5, min_p, 0.0)
+        temperature = torch.where(row % 16 == 7, 0.0, temperature)
+    return dict(kind="sample", logits=x, u=u, temperature=temperature.float().cuda(), top_k=top_k.to(torch.int32).cuda(),
+                top_p=top_p.float().cuda(), min_p=min_p.float().cuda(),
+                token=torch.zeros(B, dtype=torch.int32, device="cuda"), prob=torch.zeros(B, device="cuda"),
+                kept=torch.zeros(B, dtype=torch.int32, device="cuda"))
+
+
+# ---- one pass ----
+
+_loaded = []
+
+
+def _lm():
+    if not _loaded:
+        import __graft_entry__
+        __graft_entry__.load_package()
+        from parakeet_amd import lm
+        _loaded.append(lm)
+    return _loaded[0]
+
+
+def run(state):
+    s = state
+    if not own:
+        return globals()["_plain_" + s["kind"]](s)
+    lm = _lm()
+    if s["kind"] == "plan":
+        lm.kv_plan(s["old"], s["new"], s["table"], s["ring"], s["state"], s["page"], state_out=s["state_out"], lens=s["lens"],
+                   ok=s["ok"], first=s["first"], slots=s["slots"], pos=s["pos"])
+        return {k: s[k] for k in ("table", "ring", "state_out", "lens", "ok", "first", "slots", "pos")}
+    if s["kind"] == "store":
+        lm.kv4_store(s["k"], s["v"], s["slots"], s["cache"], s["page"])
+        lm.kv4_load(s["cache"], s["slots"], s["k_back"], s["v_back"], s["page"])
+        return {"k": s["k_back"], "v": s["v_back"]}
+    if s["kind"] == "attend":
+        lm.kv4_attend(s["q"], s["cache"], s["table"], s["lens"], s["out"], s["page"], first=s["first"], max_new=s["max_new"],
+                      max_len=s["max_len"], scale=s["scale"], window=s["window"], lse=s["lse"])
+        return {"out": s["out"], "lse": s["lse"]}
+    lm.sample(s["logits"], s["u"], s["token"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
+              min_p=s["min_p"], prob=s["prob"], kept=s["kept"])
+    return {"token": s["token"], "prob": s["prob"], "kept": s["kept"]}
+
+
+def _plain_plan(s):
+    """Request b holds old[b] tokens and is to hold new[b].  Pages it lacks come from the front of the ring of free
+    pages, in the order of the requests, as long as the running sum of the pages lacked fits the ring's count; pages
+    that it gives up go behind the ring's end."""
+    page, n, width = s["page"], s["ring"].numel(), s["table"].shape[1]
+    old, new, head, count = s["old"].long(), s["new"].long(), s["state"][0].long(), s["state"][1].long()
+    ranged = (old >= 0) & (new >= 0) & (old <= width * page) & (new <= width * page)
+    had, want = (old + page - 1) // page, (new + page - 1) // page
+    lack = torch.where(ranged, (want - had).clamp(min=0), 0)
+    upto = torch.cumsum(lack, 0)
+    ok = ranged & ((lack == 0) | (upto <= count))
+    lens = torch.where(ok, new, old)
+    j = torch.arange(width, device=old.device)
+    taken = ok[:, None] & (j >= had[:, None]) & (j < want[:, None])
+    place = (head + (upto - lack)[:, None] + j - had[:, None]) % n
+    table = torch.where(taken, s["ring"][place], s["table"])
+    freed = torch.where(ok, (had - want).clamp(min=0), 0)
+    behind = torch.cumsum(freed, 0)
+    gone = (j >= want[:, None]) & (j < (want + freed)[:, None])
+    place = (head + count + (behind - freed)[:, None] + j - want[:, None]) % n
+    ring = torch.cat([s["ring"], s["ring"][:1]]).scatter(0, torch.where(gone, place, n).reshape(-1),
+                                                         s["table"].reshape(-1))[:n]
+    used = torch.where(ok, lack, 0).sum()
+    state = torch.stack([(head + used) % n, count - used + freed.sum()])
+    more = torch.where(ranged, (new - old).clamp(min=0), 0)
+    first = torch.cat([more.new_zeros(1), torch.cumsum(more, 0)])
+    t = torch.arange(s["slots"].numel(), device=old.device)
+    b = torch.searchsorted(first[1:], t, right=True).clamp(max=old.numel() - 1)
+    p = old[b] + t - first[b]
+    live = (t < first[-1]) & ok[b]
+    slot = table.long()[b, (p // page).clamp(0, width - 1)] * page + p % page
+    i32 = lambda x: x.to(torch.int32)  # noqa: E731
+    return {"table": table, "ring": ring, "state_out": i32(state), "lens": i32(lens), "ok": i32(ok), "first": i32(first),
+            "slots": i32(torch.where(live, slot, -1)), "pos": i32(torch.where(live, p, -1))}
+
+
+def _pow2(e):
+    """2^e of whole numbers -126 .. 127."""
+    return (e.int() + 127 << 23).view(torch.float32)
+
+
+def _codes(x):
+    """Blocks of 32 as (code 0 .. 15, scale byte): the scale that puts the largest value between 3.5 and 7, every value
+    to the nearest level, ties to the even code."""
+    b = x.float().unflatten(-1, (-1, 32))
+    top = b.abs().amax(-1, keepdim=True)
+    m, e = torch.frexp(top)
+    e = torch.where(top == 0, -120, (e - 3 + (m > 0.875).to(e.dtype)).clamp(-120, 127))
+    y = b.abs() * _pow2(-e)
+    code = ((y > 0.25).to(torch.uint8) + (y >= 0.75) + (y > 1.25) + (y >= 1.75) + (y > 2.5) + (y >= 3.5) + (y > 5.0)
+            + 8 * (b < 0)).to(torch.uint8)
+    bad = ~torch.isfinite(top)
+    return (torch.where(bad, 0, code).to(torch.uint8).flatten(-2),
+            torch.where(bad, 255, e + 127).squeeze(-1).to(torch.uint8))
+
+
+def _values(code, scale):
+    """What codes [..., D] and scale bytes [..., D/32] stand for, in 32 bits."""
+    level = torch.tensor(LEVELS + tuple(-v for v in LEVELS), device=code.device)
+    s = torch.where(scale == 255, math.nan, _pow2(scale.int() - 127))
+    return (level[code.long()].unflatten(-1, (-1, 32)) * s[..., None]).flatten(-2)
+
+
+def _records(k, v, page):
+    """Whole pages of rows k, v [n page, H, D] as the cache holds them: [n, H, page (D + D/16)] bytes."""
+    H, D = k.shape[1:]
+    n = k.shape[0] // page
+    (kc, ks), (vc, vs) = _codes(k), _codes(v)
+    pair = lambda c: c[..., 0::2] | c[..., 1::2] << 4  # noqa: E731
+    kc = pair(kc).view(n, page, H, D // 2).permute(0, 2, 1, 3).reshape(n, H, -1)
+    vc = pair(vc).view(n, page // 8, 8, H, 16, D // 32).permute(0, 3, 1, 4, 2, 5).reshape(n, H, -1)
+    ks = ks.view(n, page, H, D // 32).permute(0, 2, 1, 3).reshape(n, H, -1)
+    vs = vs.view(n, page, H, D // 32).permute(0, 2, 3, 1).reshape(n, H, -1)
+    return torch.cat([kc, vc, ks, vs], -1)
+
+
+def _rows(records, page, D):
+    """The values k, v [..., H, page, D] that records [..., H, bytes] stand for."""
+    kc, vc, ks, vs = torch.split(records, [page * D // 2, page * D // 2, page * D // 32, page * D // 32], -1)
+    both = lambda c: torch.stack([c & 15, c >> 4], -1).flatten(-2)  # noqa: E731
+    vc = vc.unflatten(-1, (page // 8, 16, 8, D // 32)).transpose(-3, -2).flatten(-4)
+    vs = vs.unflatten(-1, (D // 32, page)).transpose(-1, -2)
+    return (_values(both(kc).unflatten(-1, (page, D)), ks.unflatten(-1, (page, D // 32))),
+            _values(both(vc).unflatten(-1, (page, D)), vs))
+
+
+def _plain_store(s):
+    page, cache, slots = s["page"], s["cache"], s["slots"].long()
+    N, H, D = s["k"].shape
+    at, off = slots // page, slots % page
+    (kc, ks), (vc, vs) = _codes(s["k"]), _codes(s["v"])
+    pair = lambda c: c[..., 0::2] | c[..., 1::2] << 4  # noqa: E731
+    # byte places of one row in its record
+    i = torch.arange(D // 2, device=cache.device)
+    g = torch.arange(D // 32, device=cache.device)
+    k_at = off[:, None] * (D // 2) + i
+    v_at = page * D // 2 + ((off[:, None] // 8 * 16 + i // (D // 32)) * 8 + off[:, None] % 8) * (D // 32) + i % (D // 32)
+    ks_at = page * D + off[:, None] * (D // 32) + g
+    vs_at = page * D + page * D // 32 + g * page + off[:, None]
+    places = torch.cat([k_at, v_at, ks_at, vs_at], -1)[:, None].expand(N, H, -1)
+    data = torch.cat([pair(kc), pair(vc), ks, vs], -1)
+    h = torch.arange(H, device=cache.device)[:, None].expand(N, H, places.shape[-1])
+    cache[at[:, None, None].expand_as(h), h, places] = data
+    got = cache[at[:, None, None].expand_as(h), h, places]             # and back
+    both = lambda c: torch.stack([c & 15, c >> 4], -1).flatten(-2)  # noqa: E731
+    kc, vc, ks, vs = torch.split(got, [D // 2, D // 2, D // 32, D // 32], -1)
+    return {"k": _values(both(kc), ks).to(s["k"].dtype), "v": _values(both(vc), vs).to(s["v"].dtype)}
+
+
+def _plain_attend(s):
+    """softmax(scale q K^T) V over the keys that query i of request b sees: its own place p = lens - new + i and those
+    before it, the last `window` of them where a window is set.  A query that sees none gives zeros, lse -inf."""
+    q, table, lens, page, D = s["q"], s["table"].long(), s["lens"].long(), s["page"], s["q"].shape[-1]
+    B, Hq, H = table.shape[0], q.shape[1], s["cache"].shape[1]
+    used = -(-s["max_len"] // page)
+    k, v = _rows(s["cache"][table[:, :used]].transpose(1, 2), page, D)            # [B, H, pages, page, D]
+    k, v = k.flatten(2, 3), v.flatten(2, 3)
+    L = k.shape[2]
+    first = s["first"].long()
+    new = first[1:] - first[:-1]
+    i = torch.arange(s["max_new"], device=q.device)
+    row = (first[:-1, None] + i).clamp(max=q.shape[0] - 1)                        # [B, max_new]
+    p = lens[:, None] - new[:, None] + i
+    j = torch.arange(L, device=q.device)
+    see = (j <= p[..., None]) & (i < new[:, None])[..., None]
+    if s["window"]:
+        see &= j > p[..., None] - s["window"]
+    see = see[:, None, None]                                                      # [B, 1, 1, max_new, L]
+    qq = q[row].float().unflatten(2, (H, Hq // H)).permute(0, 2, 3, 1, 4)         # [B, H, G, max_new, D]
+    z = torch.matmul(qq.flatten(2, 3), k.transpose(2, 3)).unflatten(2, (Hq // H, -1)) * s["scale"]
+    z = z.masked_fill(~see, -math.inf)
+    top = z.amax(-1, keepdim=True)
+    e = torch.exp(z - torch.where(top == -math.inf, 0.0, top))
+    total = e.sum(-1, keepdim=True)
+    o = torch.matmul(e.flatten(2, 3), v).unflatten(2, (Hq // H, -1)) / torch.where(total == 0, 1.0, total)
+    lse = (top + torch.log(total)).squeeze(-1)
+    live = i < new[:, None]
+    out = torch.zeros(q.shape[0] + 1, Hq, D, device=q.device)
+    place = torch.where(live, row, q.shape[0]).flatten()
+    out[place] = o.permute(0, 3, 1, 2, 4).flatten(2, 3).flatten(0, 1)
+    back = torch.zeros(q.shape[0] + 1, Hq, device=q.device)
+    back[place] = lse.permute(0, 3, 1, 2).flatten(2, 3).flatten(0, 1)
+    return {"out": out[:-1].to(q.dtype), "lse": back[:-1]}
+
+
+def _share(total, part):
+    """floor(total part / 2^31) of whole numbers."""
+    return (total >> 31) * part + (((total & (2 ** 31 - 1)) * part) >> 31)
+
+
+def _plain_sample(s):
+    """Weights are whole numbers, round(2^30 exp((x - max) / T)), so that no sum depends on its order.  By falling
+    value (ties: rising index) the first top_k are kept, of these the ones with less than top_p of their mass before
+    them, of these the ones with at least min_p of the largest weight; the first always.  The token is the first, by
+    rising index, whose running kept weight exceeds u of the kept total."""
+    x = s["logits"].float()
+    B, V = x.shape
+    x = torch.where(torch.isnan(x), -math.inf, x)
+    t = s["temperature"]
+    greedy = ~(t > 0)
+    inv = torch.where(greedy, 1.0, 1.0 / t).clamp(max=3e38)
+    top = x.amax(-1, keepdim=True)
+    z = torch.where(x == top, 0.0, (x - top) * inv[:, None])
+    w = torch.where(x == -math.inf, 0, torch.round(torch.exp(z) * 2.0 ** 30).long())
+    order = torch.sort(x, dim=-1, descending=True, stable=True).indices
+    ws = w.gather(-1, order)
+    rank = torch.arange(V, device=x.device)
+    k = torch.where(greedy, 1, torch.where(s["top_k"] > 0, s["top_k"], V))
+    in_k = rank < k[:, None]
+    total = torch.where(in_k, ws, 0).sum(-1)
+    p = (s["top_p"].clamp(0, 1) * 2.0 ** 31).long()
+    before = torch.cumsum(ws, -1) - ws
+    keep = in_k & (before < _share(total, p)[:, None]) & (ws >= torch.ceil(s["min_p"].clamp(0, 1) * 2.0 ** 30).long()[:, None])
+    keep[:, 0] = True
+    keep &= (top > -math.inf)
+    kept = keep.sum(-1)
+    wk = torch.zeros_like(w).scatter(-1, order, torch.where(keep, ws, 0))
+    mass = wk.sum(-1)
+    u = (s["u"].clamp(0, 1) * 2.0 ** 31).long().clamp(max=2 ** 31 - 1)
+    over = torch.cumsum(wk, -1) > _share(mass, u)[:, None]
+    token = torch.where(over, rank, V).amin(-1)
+    prob = wk.gather(-1, token.clamp(max=V - 1)[:, None])[:, 0].float() / mass.clamp(min=1).float()
+    token = torch.where(kept > 0, token, -1)
+    return {"token": token.to(torch.int32), "prob": prob, "kept": kept.to(torch.int32)}
+
+
+# ---- what a pass cannot do without ----
+
+def work(case):
+    c = case
+    if c["kind"] == "plan":
+        return {"bytes": 20.0 * c["requests"] + 8.0 * _tokens(c) * (1 + 1 / c["page"]), "flops": 0}
+    if c["kind"] == "store":
+        values = 2.0 * c["tokens"] * c["heads"] * c["dim"]
+        return {"bytes": values * (2 * SIZEOF[c["dtype"]] + 2 * 17 / 32) + 8.0 * c["tokens"], "flops": 0}
+    if c["kind"] == "attend":
+        news, lens = _lengths(c, torch.Generator().manual_seed(1))
+        rows, place = int(news.sum()), lens - news     # of a query's place p, its keys: min(p + 1, window)
+        low = place.clamp(min=0)
+        W = c["window"] or c["length"]
+        upto = lambda n: torch.where(n <= W, n * (n + 1) // 2, W * (W + 1) // 2 + (n - W) * W)  # noqa: E731
+        pairs = int((upto(lens) - upto(low)).clamp(min=0).sum())
+        seen = int(torch.minimum(lens, W - 1 + lens - low).sum())
+        return {"bytes": seen * c["kv_heads"] * c["dim"] * 2 * 17 / 32 + rows * c["heads"] * (c["dim"] * 4.0 + 4),
+                "flops": 4.0 * c["dim"] * c["heads"] * pairs}
+    return {"bytes": float(c["rows"]) * c["vocab"] * SIZEOF[c["dtype"]] + 36.0 * c["rows"], "flops": 0}
+
+
+# ---- the same from the definitions, in 64 bits ----
+
+def exact(case, seed):
+    return {"store": _exact_store, "attend": _exact_attend, "sample": _exact_sample}.get(case["kind"], lambda *a: None)(
+        case, prepare(case, seed))
+
+
+def _exact_pow2(e):
+    return (e.long() + 1023 << 52).view(torch.float64)
+
+
+def _exact_store(case, s):
+    found = {}
+    level = torch.tensor(LEVELS, dtype=torch.float64, device="cuda")
+    for name in ("k", "v"):
+        x = s[name].double().unflatten(-1, (-1, 32))
+        top = x.abs().amax(-1, keepdim=True)
+        e = torch.floor(torch.log2(torch.where(top > 0, top, 1.0)))    # top is 2^e .. 2^(e+1)
+        e = torch.where(top >= _exact_pow2(e + 1), e + 1, torch.where(top < _exact_pow2(e), e - 1, e)) - 2
+        e = torch.where(top > 7 * _exact_pow2(e), e + 1, e).clamp(-120, 127)
+        y = x.abs() / _exact_pow2(e)
+        best, code = torch.full_like(y, math.inf), torch.zeros_like(y, dtype=torch.long)
+        for c in (0, 2, 4, 6, 1, 3, 5, 7):                             # even codes first: they win ties
+            d = (y - level[c]).abs()
+            code, best = torch.where(d < best, c, code), torch.minimum(d, best)
+        found[name] = (level[code] * _exact_pow2(e) * torch.sign(x)).flatten(-2)
+    return found
+
+
+def _exact_attend(case, s):
+    D, page = case["dim"], case["page"]
+    B, Hq, H = case["requests"], case["heads"], case["kv_heads"]
+    first, lens, table = s["first"].tolist(), s["lens"].tolist(), s["table"].long()
+    level = torch.tensor(LEVELS + tuple(-v for v in LEVELS), dtype=torch.float64, device="cuda")
+    q = s["q"].double()
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device="cuda")
+    d = torch.arange(D, device="cuda")
+    per = D // 16
+    for b in range(B):
+        n, new = lens[b], first[b + 1] - first[b]
+        if n == 0:
+            continue
+        t = torch.arange(n, device="cuda")
+        pages, off = table[b, t // page], t % page
+        k_at = off[:, None] * (D // 2) + d // 2
+        v_at = page * D // 2 + ((off[:, None] // 8 * 16 + d // per) * 8 + off[:, None] % 8) * (D // 32) + d % per // 2
+        ks_at = page * D + off[:, None] * (D // 32) + d // 32
+        vs_at = page * (D + D // 32) + d // 32 * page + off[:, None]
+        for h in range(H):
+            rec = s["cache"][:, h]
+            value = lambda at, sat, odd: level[((rec[pages[:, None], at] >> (4 * odd)) & 15).long()] * _exact_pow2(  # noqa: E731
+                rec[pages[:, None], sat].long() - 127)
+            k, v = value(k_at, ks_at, (d % 2).to(torch.uint8)), value(v_at, vs_at, (d % 2).to(torch.uint8))
+            for i0 in range(0, new, 512):
+                i1 = min(new, i0 + 512)
+                p = n - new + torch.arange(i0, i1, device="cuda")
+                see = t <= p[:, None]
+                if case["window"]:
+                    see &= t > p[:, None] - case["window"]
+                for hq in range(h * (Hq // H), (h + 1) * (Hq // H)):
+                    r = slice(first[b] + i0, first[b] + i1)
+                    z = (q[r, hq] @ k.T * s["scale"]).masked_fill(~see, -math.inf)
+                    lse[r, hq] = torch.logsumexp(z, -1)
+                    out[r, hq] = torch.softmax(z, -1) @ v
+    return {"out": out, "lse": lse}
+
+
+def _exact_sample(case, s):
+    """The token's probability among the kept ones; which token it is and how many are kept are whole numbers."""
+    x = s["logits"].double().cpu()
+    B, V = x.shape
+    prob = torch.zeros(B, dtype=torch.float64)
+    for b in range(B):
+        t, k, p, m = (float(s[n][b]) for n in ("temperature", "top_k", "top_p", "min_p"))
+        order = torch.argsort(x[b], descending=True, stable=True)
+        if t <= 0:
+            prob[b] = 1.0
+            continue
+        w = torch.exp((x[b] - x[b].max()) / t)
+        n = int(k) if k > 0 else V
+        order = order[:n]
+        sw = w[order]
+        before = torch.cumsum(sw, 0) - sw
+        keep = (before < min(p, 1.0) * sw.sum()) & (sw >= m)
+        keep[0] = True
+        order = order[keep]
+        kept = torch.zeros(V, dtype=torch.float64)
+        kept[order] = w[order]
+        run_ = torch.cumsum(kept, 0)
+        at = min(int(torch.searchsorted(run_, float(s["u"][b]) * run_[-1], right=True)), int(order.max()))
+        prob[b] = kept[at] / run_[-1]
+    return {"token": None, "prob": prob, "kept": None}
