@@ -315,7 +315,7 @@ def _codes(x):
     b = x.float().unflatten(-1, (-1, 32))
     top = b.abs().amax(-1, keepdim=True)
     m, e = torch.frexp(top)
-    e = torch.where(top == 0, -120, (e - 3 + (m > 0.875).to(e.dtype)).clamp(-120, 127))
+    e = torch.where(top == 0, -120, (e - 3 + (m > 0.875).to(e.dtype)).clamp(-120, 125))
     y = b.abs() * _pow2(-e)
     code = ((y > 0.25).to(torch.uint8) + (y >= 0.75) + (y > 1.25) + (y >= 1.75) + (y > 2.5) + (y >= 3.5) + (y > 5.0)
             + 8 * (b < 0)).to(torch.uint8)
@@ -495,7 +495,7 @@ def _exact_store(case, s):
         top = x.abs().amax(-1, keepdim=True)
         e = torch.floor(torch.log2(torch.where(top > 0, top, 1.0)))    # top is 2^e .. 2^(e+1)
         e = torch.where(top >= _exact_pow2(e + 1), e + 1, torch.where(top < _exact_pow2(e), e - 1, e)) - 2
-        e = torch.where(top > 7 * _exact_pow2(e), e + 1, e).clamp(-120, 127)
+        e = torch.where(top > 7 * _exact_pow2(e), e + 1, e).clamp(-120, 125)
         y = x.abs() / _exact_pow2(e)
         best, code = torch.full_like(y, math.inf), torch.zeros_like(y, dtype=torch.long)
         for c in (0, 2, 4, 6, 1, 3, 5, 7):                             # even codes first: they win ties
