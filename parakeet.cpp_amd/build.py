@@ -1,6 +1,7 @@
 """Build recipe for the native libraries (gfx950 only, built in-tree).
 
-  libparakeet_hip.so      HIP kernels + C ABI      (csrc/pk_decode.hip)
+  libparakeet_hip.so      HIP kernels + C ABI      (csrc/pk_decode.hip: the decode loop,
+                          csrc/pk_lm.hip: the language-model serving operators)
   libparakeet_decoder.so  C++ decoder API           (csrc/parakeet_decoder.cpp, csrc/gguf_reader.cpp)
   libpk_calib.so          copy kernel of known size (csrc/pk_calib.hip), used by bench.py to scale
                           hardware byte counters
@@ -48,7 +49,8 @@ def build_hip():
     out = os.path.join(HERE, "libparakeet_hip.so")
     # PK_TIMELINE=1 compiles the decode loop's per-wave checkpoint timeline (profiling builds only)
     extra = ["-DPK_TIMELINE"] if os.environ.get("PK_TIMELINE") else []
-    _run([HIPCC, *HIP_FLAGS, *extra, "-shared", os.path.join(CSRC, "pk_decode.hip"), "-o", out + ".tmp"])
+    srcs = [os.path.join(CSRC, f) for f in ("pk_decode.hip", "pk_lm.hip")]
+    _run([HIPCC, *HIP_FLAGS, *extra, "-shared", *srcs, "-o", out + ".tmp"])
     os.replace(out + ".tmp", out)
     return out
 

@@ -1,0 +1,139 @@
+// lm_plan.h -- page tables and slot maps from request lengths (pk_kv_plan).
+#pragma once
+
+#include "lm_common.h"
+#include "parakeet_lm.h"
+
+namespace pklm {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanTokens = 4;   // consecutive tokens of one thread: one 16-byte store for each map
+
+// Three running sums over the requests: new tokens (where a token's request is found), pages lacked (where its page
+// is in the ring), pages given up (where they go behind the ring's end).  Every workgroup makes all three in its LDS
+// from the two length arrays, at most 32 KB of reads, so that nothing is exchanged between workgroups and one launch
+// does it all; each then takes its share of the tokens and of the pages given up.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, int wide) {
+    __shared__ int s_first[PK_LM_MAX_REQUESTS + 1], s_lack[PK_LM_MAX_REQUESTS + 1], s_free[PK_LM_MAX_REQUESTS + 1];
+    __shared__ int s_wave[3][kPlanThreads / 64], s_used;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int B = a.requests, most = a.width * a.page;
+    const int count = min(max(a.state[1], 0), a.n_pages);
+    int head = a.state[0] % a.n_pages;
+    if (head < 0) head += a.n_pages;
+
+    // this thread's run of requests, their sums, and what lies before them
+    const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    int tokens = 0, lack = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int o = a.old_len[b], n = a.new_len[b];
+        if (o < 0 || n < 0 || o > most || n > most) continue;
+        tokens += max(n - o, 0);
+        lack += max((n + a.page - 1) / a.page - (o + a.page - 1) / a.page, 0);
+    }
+    if (tid == 0) s_used = 0;
+    if (tid == 0 && B == 0) s_first[0] = s_free[0] = 0;   // no thread below has a last request
+    const int st = wave_scan(tokens), sl = wave_scan(lack);
+    if (lane == 63) s_wave[0][wave] = st, s_wave[1][wave] = sl;
+    __syncthreads();
+    int at = st - tokens, al = sl - lack, freed = 0, used = 0;
+    for (int w = 0; w < wave; ++w) at += s_wave[0][w], al += s_wave[1][w];
+    for (int b = b0; b < b1; ++b) {
+        const int o = a.old_len[b], n = a.new_len[b];
+        const bool ranged = !(o < 0 || n < 0 || o > most || n > most);
+        const int had = (o + a.page - 1) / a.page, want = (n + a.page - 1) / a.page;
+        const int need = ranged ? max(want - had, 0) : 0;
+        const bool ok = ranged && (need == 0 || al + need <= count);
+        s_first[b] = at;
+        s_lack[b] = ok ? al : -1;                       // -1: not served
+        if (ranged) at += max(n - o, 0);
+        al += need;
+        if (ok && need) used = al;
+        s_free[b] = ok ? max(had - want, 0) : 0;
+        freed += s_free[b];
+        if (blockIdx.x == 0) {
+            a.ok[b] = ok;
+            a.lens[b] = ok ? n : o;
+            a.first[b] = s_first[b];
+        }
+    }
+    const int sf = wave_scan(freed);
+    if (lane == 63) s_wave[2][wave] = sf;
+    if (used) atomicMax(&s_used, used);
+    if (b0 < b1 && b1 == B) s_first[B] = at;
+    __syncthreads();
+    int af = sf - freed;
+    for (int w = 0; w < wave; ++w) af += s_wave[2][w];
+    for (int b = b0; b < b1; ++b) {
+        const int f = s_free[b];
+        s_free[b] = af;
+        af += f;
+    }
+    if (b0 < b1 && b1 == B) s_free[B] = af;
+    __syncthreads();
+    const int total = s_first[B], gone = s_free[B];
+    if (blockIdx.x == 0 && tid == 0) {
+        a.first[B] = total;
+        a.state_out[0] = (head + s_used) % a.n_pages;
+        a.state_out[1] = min(count - s_used + gone, a.n_pages);
+    }
+
+    const int64_t stride = (int64_t)gridDim.x * kPlanThreads, me = (int64_t)blockIdx.x * kPlanThreads + tid;
+    for (int64_t t0 = me * kPlanTokens; t0 < max(total, a.n_tokens); t0 += stride * kPlanTokens) {
+        int b = 0;
+        if (t0 < total) {                               // the last request that begins at or before t0
+            int hi = B;
+            while (hi - b > 1) {
+                const int mid = (b + hi) >> 1;
+                if (s_first[mid] <= t0) b = mid; else hi = mid;
+            }
+        }
+        v4i slot, pos;
+#pragma unroll
+        for (int i = 0; i < kPlanTokens; ++i) {
+            const int64_t t = t0 + i;
+            slot[i] = pos[i] = -1;
+            if (t >= total) continue;
+            while (t >= s_first[b + 1]) ++b;
+            const int al_b = s_lack[b];
+            if (al_b < 0) continue;
+            const int o = a.old_len[b], p = o + (int)(t - s_first[b]), j = p / a.page, had = (o + a.page - 1) / a.page;
+            int id;
+            if (j < had) {
+                id = a.table[b * a.table_stride + j];
+            } else {
+                int r = head + al_b + (j - had);
+                if (r >= a.n_pages) r -= a.n_pages;
+                id = a.ring[r];
+                // the page's first token is new: it enters the page into the table
+                if (p == j * a.page) a.table[b * a.table_stride + j] = id;
+            }
+            slot[i] = id * a.page + (p - j * a.page);
+            pos[i] = p;
+        }
+        if (t0 + kPlanTokens <= a.n_tokens && wide) {
+            *(v4i *)(a.slots + t0) = slot;
+            if (a.pos) *(v4i *)(a.pos + t0) = pos;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPlanTokens; ++i)
+                if (t0 + i < a.n_tokens) {
+                    a.slots[t0 + i] = slot[i];
+                    if (a.pos) a.pos[t0 + i] = pos[i];
+                }
+        }
+    }
+    for (int64_t f = me; f < gone; f += stride) {       // pages given up, in the order of the requests
+        int b = 0, hi = B;
+        while (hi - b > 1) {
+            const int mid = (b + hi) >> 1;
+            if (s_free[mid] <= f) b = mid; else hi = mid;
+        }
+        if (count + f >= a.n_pages) continue;           // a ring that says it holds more than there are
+        const int want = (a.new_len[b] + a.page - 1) / a.page;
+        const int r = (int)(((int64_t)head + count + f) % a.n_pages);
+        a.ring[r] = a.table[b * a.table_stride + want + (f - s_free[b])];
+    }
+}
+
+}  // namespace pklm

@@ -60,6 +60,7 @@ extern char **environ;
 #include "parakeet_hip.h"
 #include "enc_proj_rule.h"
 #include "host_outputs.h"
+#include "last_error.h"
 #include "pk_device.h"
 
 namespace {
@@ -572,6 +573,17 @@ constexpr int kChainFrames = 8192;
 int open_loop_lock(int device);
 
 }  // namespace
+
+int pk_fail(int rc, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return rc;
+}
+void pk_fail_clear() { g_err.clear(); }
 
 extern "C" {
 

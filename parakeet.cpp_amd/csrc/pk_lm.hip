@@ -1,0 +1,237 @@
+// pk_lm.hip -- language-model serving operators: host side + C ABI of parakeet_lm.h.
+//
+// Each entry point checks its descriptor, chooses a launch and enqueues it on the caller's stream.  The kernels are in
+// lm_plan.h, lm_cache.h, lm_attend.h and lm_sample.h.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "last_error.h"
+#include "lm_attend.h"
+#include "lm_cache.h"
+#include "lm_plan.h"
+#include "lm_sample.h"
+#include "parakeet_lm.h"
+
+namespace {
+
+using namespace pklm;
+
+bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
+int log2i(int v) { return 31 - __builtin_clz((unsigned)v); }
+
+int launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? PK_OK : pk_fail(PK_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
+}
+
+// What pk_kv4_store, _load and _attend ask of the cache; 0 = fine.
+int check_cache(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
+    if (!page_ok(page)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: pages of %d tokens (16, 32, 64, 128 or 256)", what, page);
+    if (dim != 64 && dim != 128 && dim != 256)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, dim);
+    if (heads <= 0 || n_pages <= 0) return pk_fail(PK_ERR_ARG, "%s: %d heads, %d pages", what, heads, n_pages);
+    if ((int64_t)n_pages * page > INT32_MAX)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d pages of %d tokens: slots are 32 bits", what, n_pages, page);
+    if (!cache || !aligned(cache, 16)) return pk_fail(PK_ERR_ARG, "%s: the cache is NULL or not aligned to 16 bytes", what);
+    const Record rec{page, dim};
+    if (page_stride % 16 || page_stride < heads * rec.bytes())
+        return pk_fail(PK_ERR_ARG, "%s: page_stride %lld bytes (a multiple of 16, at least %lld)", what, (long long)page_stride,
+                       (long long)(heads * rec.bytes()));
+    return PK_OK;
+}
+
+template <class T, bool Store>
+void launch_rows(const pk_kv4_rows_desc &d, int wide, hipStream_t s) {
+    const int64_t units = (int64_t)d.n_rows * d.heads * 2 * (d.head_dim / 8);
+    const unsigned grid = (unsigned)((units + kRowThreads - 1) / kRowThreads);
+    if (d.head_dim == 64) rows_kernel<T, 64, Store><<<grid, kRowThreads, 0, s>>>(d, wide);
+    else if (d.head_dim == 128) rows_kernel<T, 128, Store><<<grid, kRowThreads, 0, s>>>(d, wide);
+    else rows_kernel<T, 256, Store><<<grid, kRowThreads, 0, s>>>(d, wide);
+}
+
+template <bool Store>
+int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
+    pk_fail_clear();
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (int rc = check_cache(what, d->cache, d->page_stride, d->page, d->n_pages, d->heads, d->head_dim)) return rc;
+    if (d->n_rows < 0) return pk_fail(PK_ERR_ARG, "%s: %d rows", what, d->n_rows);
+    if (d->n_rows == 0) return PK_OK;
+    const int size = d->dtype == PK_DTYPE_F32 ? 4 : 2;
+    if (d->dtype != PK_DTYPE_F32 && d->dtype != PK_DTYPE_F16 && d->dtype != PK_DTYPE_BF16)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
+    if (!d->k || !d->v || !d->slots) return pk_fail(PK_ERR_ARG, "%s: NULL rows or slots", what);
+    if (!aligned(d->k, size) || !aligned(d->v, size) || !aligned(d->slots, 4))
+        return pk_fail(PK_ERR_ARG, "%s: rows or slots not aligned to their type", what);
+    if ((int64_t)d->n_rows * d->heads * d->head_dim / 4 > (int64_t)INT32_MAX * kRowThreads)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d heads in one call", what, d->n_rows, d->heads);
+    const int per = 16 / size;
+    const int wide = aligned(d->k, 16) && aligned(d->v, 16) && d->k_row % per == 0 && d->k_head % per == 0 &&
+                     d->v_row % per == 0 && d->v_head % per == 0;
+    const hipStream_t s = (hipStream_t)stream;
+    if (d->dtype == PK_DTYPE_F32) launch_rows<F32, Store>(*d, wide, s);
+    else if (d->dtype == PK_DTYPE_F16) launch_rows<F16, Store>(*d, wide, s);
+    else launch_rows<BF16, Store>(*d, wide, s);
+    return launched(what);
+}
+
+// Arrival counters of the tiles whose keys are split, at the workspace's beginning whatever the call's shape, so that
+// no call's partial sums lie where another's counters are.  A split call has fewer tiles than this (attend_shape).
+constexpr int kCounters = 1024;
+
+// How a call's work is dealt out, from its host-known sizes alone.
+struct AttendShape {
+    int tiles, chunk, splits;
+    int64_t part_bytes;
+    int64_t bytes() const { return splits > 1 ? kCounters * 4 + part_bytes : 0; }
+};
+
+int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
+    const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads);
+    const int64_t tiles = (rows + 15) / 16, pairs = (int64_t)d.requests * d.kv_heads;
+    // keys of one 16-row tile: its rows span at most 16 tokens
+    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 32) : d.max_len;
+    const int64_t want = 2 * kCounters, each = std::max<int64_t>(pairs * tiles, 1);   // split: at most kCounters tiles
+    int64_t splits = std::max<int64_t>(std::min<int64_t>(want / each, (keys + 255) / 256), 1);
+    int64_t chunk = ((keys + splits - 1) / splits + 127) / 128 * 128;
+    chunk = std::max<int64_t>(chunk, 128);
+    splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
+    if (pairs * tiles * splits > INT32_MAX)
+        return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
+                       (long long)rows);
+    s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
+    s.part_bytes = pairs * tiles * splits * 16 * (d.head_dim + 2) * 4;
+    return PK_OK;
+}
+
+int attend_check(const pk_kv4_attend_desc *d) {
+    const char *what = "pk_kv4_attend";
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (d->dtype != PK_DTYPE_F16 && d->dtype != PK_DTYPE_BF16) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d (f16 or bf16)", what, d->dtype);
+    if (d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads)
+        return pk_fail(PK_ERR_ARG, "%s: %d query heads on %d kv heads", what, d->heads, d->kv_heads);
+    if (d->requests < 0 || d->n_rows < 0 || d->max_new < 0 || d->max_len < 0 || d->window < 0 || d->width <= 0)
+        return pk_fail(PK_ERR_ARG, "%s: %d requests, %d rows, max_new %d, max_len %d, window %d, table width %d", what, d->requests, d->n_rows,
+                       d->max_new, d->max_len, d->window, d->width);
+    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, d->head_dim);
+    return PK_OK;
+}
+
+template <class T>
+void launch_attend(const AttendParams &p, int dim, unsigned grid, hipStream_t s) {
+    if (dim == 64) attend_kernel<T, 64><<<grid, kAttendThreads, 0, s>>>(p);
+    else if (dim == 128) attend_kernel<T, 128><<<grid, kAttendThreads, 0, s>>>(p);
+    else attend_kernel<T, 256><<<grid, kAttendThreads, 0, s>>>(p);
+}
+
+}  // namespace
+
+extern "C" {
+
+PK_API int pk_kv_plan(const pk_kv_plan_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_kv_plan";
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (d->requests < 0 || d->requests > PK_LM_MAX_REQUESTS)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests (at most %d)", what, d->requests, PK_LM_MAX_REQUESTS);
+    if (!page_ok(d->page)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: pages of %d tokens (16, 32, 64, 128 or 256)", what, d->page);
+    if (d->width <= 0 || d->n_pages <= 0 || d->n_tokens < 0)
+        return pk_fail(PK_ERR_ARG, "%s: table width %d, %d pages, %d tokens", what, d->width, d->n_pages, d->n_tokens);
+    if ((int64_t)d->n_pages * d->page > INT32_MAX || (int64_t)std::max(d->requests, 1) * d->width * d->page > INT32_MAX)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests x %d pages, %d pages of %d tokens: positions and slots are 32 bits", what, d->requests,
+                       d->width, d->n_pages, d->page);
+    if (!d->ring || !d->state || !d->state_out || !d->first || (d->n_tokens && !d->slots) ||
+        (d->requests && (!d->old_len || !d->new_len || !d->table || !d->lens || !d->ok)))
+        return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
+    if (d->requests > 1 && d->table_stride < d->width)
+        return pk_fail(PK_ERR_ARG, "%s: table rows %lld apart, %d wide", what, (long long)d->table_stride, d->width);
+    if (d->state == d->state_out || d->lens == d->old_len || d->lens == d->new_len)
+        return pk_fail(PK_ERR_ARG, "%s: state_out and lens are written while state and the lengths are read", what);
+    const int wide = aligned(d->slots, 16) && aligned(d->pos, 16);
+    const int64_t per = kPlanThreads * kPlanTokens;
+    const unsigned grid = (unsigned)std::min<int64_t>(std::max<int64_t>((d->n_tokens + per - 1) / per, 1), 512);
+    plan_kernel<<<grid, kPlanThreads, 0, (hipStream_t)stream>>>(*d, wide);
+    return launched(what);
+}
+
+PK_API int pk_kv4_store(const pk_kv4_rows_desc *d, void *stream) { return rows_call<true>("pk_kv4_store", d, stream); }
+PK_API int pk_kv4_load(const pk_kv4_rows_desc *d, void *stream) { return rows_call<false>("pk_kv4_load", d, stream); }
+
+PK_API int pk_kv4_attend_workspace(const pk_kv4_attend_desc *d, int64_t *bytes) {
+    pk_fail_clear();
+    if (int rc = attend_check(d)) return rc;
+    if (!bytes) return pk_fail(PK_ERR_ARG, "pk_kv4_attend_workspace: NULL result");
+    AttendShape s;
+    if (int rc = attend_shape(*d, s)) return rc;
+    *bytes = s.bytes();
+    return PK_OK;
+}
+
+PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_kv4_attend";
+    if (int rc = attend_check(d)) return rc;
+    if (int rc = check_cache(what, d->cache, d->page_stride, d->page, d->n_pages, d->kv_heads, d->head_dim)) return rc;
+    if (d->n_rows == 0 || d->requests == 0 || d->max_new == 0) return PK_OK;
+    if (!d->q || !d->out || !d->table || !d->lens) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
+    if (!aligned(d->q, 2) || !aligned(d->out, 2) || !aligned(d->lse, 4))
+        return pk_fail(PK_ERR_ARG, "%s: q, out or lse not aligned to its type", what);
+    if (!d->first && (d->n_rows != d->requests || d->max_new != 1))
+        return pk_fail(PK_ERR_ARG, "%s: without first, one query per request: %d rows, %d requests, max_new %d", what, d->n_rows, d->requests, d->max_new);
+    if (d->requests > 1 && d->table_stride < d->width)
+        return pk_fail(PK_ERR_ARG, "%s: table rows %lld apart, %d wide", what, (long long)d->table_stride, d->width);
+    AttendShape sh;
+    if (int rc = attend_shape(*d, sh)) return rc;
+    if (sh.bytes() > 0 && (!d->workspace || !aligned(d->workspace, 16) || d->workspace_bytes < sh.bytes()))
+        return pk_fail(PK_ERR_ARG, "%s: a workspace of %lld bytes is wanted, aligned to 16 (%lld given)", what, (long long)sh.bytes(),
+                       (long long)(d->workspace ? d->workspace_bytes : 0));
+    AttendParams p;
+    p.q = d->q, p.out = d->out, p.lse = d->lse, p.cache = (const uint8_t *)d->cache;
+    p.table = d->table, p.lens = d->lens, p.first = d->first;
+    p.arrived = (int *)d->workspace;
+    p.part = (float *)((char *)d->workspace + kCounters * 4);
+    p.q_row = d->q_row, p.q_head = d->q_head, p.out_row = d->out_row, p.out_head = d->out_head;
+    p.page_stride = d->page_stride, p.table_stride = d->table_stride;
+    p.n_rows = d->n_rows, p.requests = d->requests, p.heads = d->heads, p.kv_heads = d->kv_heads;
+    p.page = d->page, p.page_shift = log2i(d->page), p.n_pages = d->n_pages, p.width = d->width;
+    p.max_len = d->max_len, p.window = d->window, p.group = d->heads / d->kv_heads;
+    p.tiles = sh.tiles, p.splits = sh.splits, p.chunk = sh.chunk, p.scale = d->scale;
+    p.vec = aligned(d->q, 16) && d->q_row % 8 == 0 && d->q_head % 8 == 0;
+    const unsigned grid = (unsigned)((int64_t)d->requests * d->kv_heads * sh.tiles * sh.splits);
+    if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, d->head_dim, grid, (hipStream_t)stream);
+    else launch_attend<BF16>(p, d->head_dim, grid, (hipStream_t)stream);
+    return launched(what);
+}
+
+PK_API int pk_sample_workspace(const pk_sample_desc *d, int64_t *bytes) {
+    pk_fail_clear();
+    if (!d || !bytes) return pk_fail(PK_ERR_ARG, "pk_sample_workspace: no descriptor or result");
+    *bytes = 0;
+    return PK_OK;
+}
+
+PK_API int pk_sample(const pk_sample_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_sample";
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (d->rows < 0 || d->vocab <= 0 || d->vocab > PK_LM_MAX_VOCAB)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d logits (1 .. %d)", what, d->rows, d->vocab, PK_LM_MAX_VOCAB);
+    if (d->rows == 0) return PK_OK;
+    if (!d->logits || !d->u || !d->token) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
+    if (d->dtype != PK_DTYPE_F32 && d->dtype != PK_DTYPE_F16 && d->dtype != PK_DTYPE_BF16)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
+    if (!aligned(d->logits, d->dtype == PK_DTYPE_F32 ? 4 : 2)) return pk_fail(PK_ERR_ARG, "%s: logits not aligned to their type", what);
+    const hipStream_t s = (hipStream_t)stream;
+    const unsigned grid = (unsigned)d->rows;
+    if (d->dtype == PK_DTYPE_F32) sample_kernel<F32><<<grid, kSampleThreads, 0, s>>>(*d);
+    else if (d->dtype == PK_DTYPE_F16) sample_kernel<F16><<<grid, kSampleThreads, 0, s>>>(*d);
+    else sample_kernel<BF16><<<grid, kSampleThreads, 0, s>>>(*d);
+    return launched(what);
+}
+
+}  // extern "C"

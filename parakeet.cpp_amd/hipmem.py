@@ -73,5 +73,62 @@ class DeviceArray:
             pass
 
 
+NUMPY_TYPES = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16, "i32": np.int32, "u8": np.uint8}
+
+
+class Tensor:
+    """A device array with a shape, element type ("f32", "f16", "bf16", "i32", "u8") and strides, as
+    much of a tensor as the operators of ``lm`` ask for.  bf16 comes and goes as its 16-bit patterns."""
+
+    def __init__(self, shape, dtype: str, buffer: DeviceArray | None = None, offset: int = 0, strides=None):
+        self.shape, self.dtype = tuple(int(n) for n in shape), dtype
+        self.itemsize = np.dtype(NUMPY_TYPES[dtype]).itemsize
+        self.buffer = DeviceArray(self.numel() * self.itemsize) if buffer is None else buffer
+        self.offset = offset                      # elements
+        if strides is None:
+            strides, n = [], 1
+            for k in reversed(self.shape):
+                strides.insert(0, n)
+                n *= k
+        self._strides = tuple(strides)
+
+    @classmethod
+    def from_numpy(cls, a: np.ndarray, dtype: str | None = None):
+        """dtype: only to say that uint16 patterns are bf16 ones."""
+        kinds = {np.dtype(v): k for k, v in NUMPY_TYPES.items()}
+        a = np.ascontiguousarray(a)
+        return cls(a.shape, dtype or kinds[a.dtype], DeviceArray.from_numpy(a))
+
+    def numel(self):
+        return int(np.prod(self.shape, dtype=np.int64))
+
+    def data_ptr(self):
+        return self.buffer.ptr + self.offset * self.itemsize
+
+    def stride(self):
+        return self._strides
+
+    def is_contiguous(self):
+        n = 1
+        for k, s in zip(reversed(self.shape), reversed(self._strides)):
+            if k > 1 and s != n:
+                return False
+            n *= k
+        return True
+
+    def view(self, shape, strides=None, offset: int = 0):
+        """The same memory under another shape: strides and offset in elements."""
+        return Tensor(shape, self.dtype, self.buffer, self.offset + offset, strides)
+
+    def numpy(self) -> np.ndarray:
+        """A host copy, strides followed."""
+        kind = NUMPY_TYPES[self.dtype]
+        flat = self.buffer.to_numpy(kind, self.buffer.nbytes // self.itemsize)
+        return np.lib.stride_tricks.as_strided(flat[self.offset:], self.shape, [s * self.itemsize for s in self._strides]).copy()
+
+    def zero(self):
+        self.buffer.zero()
+
+
 def synchronize():
     _check(hip().hipDeviceSynchronize(), "hipDeviceSynchronize")
