@@ -20,7 +20,7 @@
 
 namespace pklm {
 
-constexpr int kAttendThreads = 256, kAttendWaves = 4;
+constexpr int kAttendThreads = 512, kAttendWaves = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttendParams {
@@ -30,10 +30,10 @@ struct AttendParams {
     const uint8_t *cache;
     const int *table, *lens, *first;
     int *arrived;       // [tiles] how many splits of a tile are done
-    float *part;        // [splits][rows][D + 2]
+    float *part;        // [tiles][splits][16 columns][D sums, maximum, total, 2 unused]
     int64_t q_row, q_head, out_row, out_head, page_stride, table_stride;
     int n_rows, requests, heads, kv_heads, page, page_shift, n_pages, width, max_len, window, group;
-    int tiles, splits, chunk, vec;
+    int tiles, splits, chunk, vec, vec_out;
     float scale;
 };
 
@@ -48,7 +48,7 @@ struct Queries {
     u4 b[Planes][D / 32];
 
     template <class T>
-    __device__ void load(const typename T::Raw *row, bool vec) {
+    __device__ void load(const typename T::Raw *row, bool vec, bool negate) {
         const int g = (threadIdx.x & 63) >> 4;
         const typename T::Raw *p = row + g * (D / 4);
 #pragma unroll
@@ -60,6 +60,9 @@ struct Queries {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) raw[i] = p[8 * ks + i];
             }
+            if (negate)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[i] ^= 0x8000;
             if (Planes == 1) {
                 b[0][ks] = *(u4 *)raw;
             } else {
@@ -89,18 +92,196 @@ __device__ inline v4f mfma(u4 a, u4 b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
-// One 16-column tile, its keys dealt to the four waves 32 at a time; `splits` workgroups share a tile's keys.
+// max and sum over the four lanes g of a column
+__device__ inline float column_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float column_sum(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Values that workgroups on other XCDs read within the launch: written through to, and read from, where all XCDs meet.
+// base is the same in the whole wave, at counts floats.
+__device__ inline void store_shared(float *base, unsigned at, v4f v) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, 4 * at, 0, 16);
+}
+__device__ inline v4f load_shared(const float *base, unsigned at) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc((float *)base, 0, 0x7FFFFFFF, 0x00020000);
+    return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(r, 4 * at, 0, 16));
+}
+
+// One step's operands of a lane: 32 keys, of K two rows' D/4 channels, of V 8 keys' D/16 channels.
+template <int D>
+struct KeyTile {
+    static constexpr int kKWords = D / 32, kVWords = D == 64 ? 4 : D / 16;
+    unsigned k[2][kKWords], v[kVWords];
+    unsigned ks[2];
+    u2 vs;
+
+    // id0, id1: pages of the tile's two 16-key halves (the same page where pages are larger), -1: none
+    __device__ void load(const AttendParams &a, const Record &rec, int64_t head_at, int kb, int id0, int id1) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+        const uint8_t *rec0 = a.cache + max(id0, 0) * a.page_stride + head_at;
+        const uint8_t *rec1 = a.cache + max(id1, 0) * a.page_stride + head_at;
+        const int koff = (kb + 8 * (c >> 2) + (c & 3)) & (a.page - 1), voff = (kb + 8 * g) & (a.page - 1);
+        const uint8_t *krec = c < 8 ? rec0 : rec1, *vrec = g < 2 ? rec0 : rec1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint8_t *code = krec + (koff + 4 * t) * (D / 2) + g * (D / 8);
+            if (D == 64) *(u2 *)k[t] = *(const u2 *)code;
+            else
+#pragma unroll
+                for (int i = 0; i < D / 128; ++i) *(u4 *)&k[t][4 * i] = *(const u4 *)(code + 16 * i);
+            const uint8_t *sc = krec + rec.k_scales() + (koff + 4 * t) * (D / 32) + g * (D / 4) / 32;
+            ks[t] = D == 256 ? *(const uint16_t *)sc : *sc;
+        }
+        const uint8_t *code = vrec + rec.v_codes() + (voff >> 3) * (4 * D) + c * (D / 4);
+#pragma unroll
+        for (int i = 0; i < kVWords / 4; ++i) *(u4 *)&v[4 * i] = *(const u4 *)(code + 16 * i);
+        vs = *(const u2 *)(vrec + rec.v_scales() + (c * (D / 16) / 32) * a.page + voff);
+    }
+    // key j's word w of V codes (D = 64: its 16 bits, in the low half)
+    __device__ unsigned v_word(int j, int w) const {
+        return D == 64 ? (j & 1 ? v[j >> 1] >> 16 : v[j >> 1]) : v[j * (D / 128 > 0 ? D / 128 : 1) + w];
+    }
+};
+
+// Online softmax of 16 columns over 32 keys a step, on one wave.
+template <int D, int Planes>
+struct Softmax {
+    static constexpr int kTiles = D / 16;
+    v4f acc[kTiles];      // O^T: channel (D/16)(4g + i) + n of column c in acc[n][i]
+    float m, l;           // largest score so far (before the scale), this lane's share of the sum
+
+    __device__ void clear() {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) acc[n] = v4f{0, 0, 0, 0};
+        m = -INFINITY, l = 0;
+    }
+
+    __device__ void scores(const KeyTile<D> &x, const Queries<D, Planes> &q, v4f (&s)[2]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks) {
+                const unsigned sb = D == 256 ? x.ks[t] >> (8 * (ks / 4)) & 255u : x.ks[t];
+                const u4 k8 = unpack8(x.k[t][ks], __uint_as_float(sb << 23));
+#pragma unroll
+                for (int n = 0; n < Planes; ++n) s[t] = mfma(k8, q.b[n][ks], s[t]);
+            }
+        }
+    }
+
+    // Keys vk .. vk + 7 of this lane: [lo, hi) is what its column sees, [lo_all, hi_all) what any column sees.  Scores
+    // of keys not seen become -inf.  What lies at keys that no column sees may be anything: their V scale becomes 1.  A
+    // NaN block of V that only some columns see is taken out, and those columns are made NaN.
+    __device__ void mask(v4f (&s)[2], u2 &vs, int vk, bool fine, int lo, int hi, int lo_all, int hi_all) {
+        unsigned nan_keys = 0, seen = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = vk + j, at = 8 * (j & 3);
+            if (fine && key < hi && key >= lo) seen |= 1u << j;
+            else s[j >> 2][j & 3] = -INFINITY;
+            const bool dead = !fine || key >= hi_all || key < lo_all;
+            const bool nan = (vs[j >> 2] >> at & 255u) == 255u;
+            if (!dead && nan) nan_keys |= 1u << j;
+            if (dead || nan) vs[j >> 2] = (vs[j >> 2] & ~(255u << at)) | 127u << at;
+        }
+        if (__any(nan_keys != 0)) {
+            u4 va, pa;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                va[j] = (nan_keys >> (2 * j) & 1 ? 0x3F80u : 0) | (nan_keys >> (2 * j + 1) & 1 ? 0x3F800000u : 0);
+                pa[j] = (seen >> (2 * j) & 1 ? 0x3F80u : 0) | (seen >> (2 * j + 1) & 1 ? 0x3F800000u : 0);
+            }
+            const v4f n = mfma(va, pa, v4f{0, 0, 0, 0});      // how many such keys each column sees, by channel entry
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n[i] > 0)
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) acc[t][i] = __builtin_nanf("");
+        }
+    }
+
+    __device__ void add(const v4f (&s)[2], const KeyTile<D> &x, u2 vs, float to_log2) {
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = column_max(top);
+        if (__any(top > m)) {
+            const float m2 = fmaxf(m, top);
+            const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - m2) * to_log2);
+            m = m2;
+            l *= keep;
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][i] *= keep;
+        }
+        const float shift = m == -INFINITY ? 0.0f : m;
+        u4 ph, pl;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // subtracted first: s to_log2 - m to_log2 in one rounding is not 0 at s = m, and large scores overflow by it
+            const float a = __builtin_amdgcn_exp2f((s[j >> 1][2 * (j & 1)] - shift) * to_log2);
+            const float b = __builtin_amdgcn_exp2f((s[j >> 1][2 * (j & 1) + 1] - shift) * to_log2);
+            l += a + b;
+            ph[j] = pack_bf16(a, b);
+            if (Planes == 2)      // an f16 result wants more than bf16's 8 bits of P: the rest of it as a second product
+                pl[j] = pack_bf16(a - __uint_as_float(ph[j] << 16), b - __uint_as_float(ph[j] & 0xFFFF0000u));
+        }
+        float vscale[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vscale[j] = __uint_as_float((vs[j >> 2] >> (8 * (j & 3)) & 255u) << 23);
+        // two channels at a time: a byte of each key's codes
+        auto two = [&](auto sel, int word, v4f &even, v4f &odd) {
+            constexpr int kSel = decltype(sel)::value;
+            u4 ve, vo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v_word(2 * j, word), vscale[2 * j], kSel);
+                const bf2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v_word(2 * j + 1, word), vscale[2 * j + 1], kSel);
+                const unsigned au = __builtin_bit_cast(unsigned, a), bu = __builtin_bit_cast(unsigned, b);
+                ve[j] = __builtin_amdgcn_perm(bu, au, 0x05040100u);
+                vo[j] = __builtin_amdgcn_perm(bu, au, 0x07060302u);
+            }
+            even = mfma(ve, ph, even);
+            odd = mfma(vo, ph, odd);
+            if (Planes == 2) {
+                even = mfma(ve, pl, even);
+                odd = mfma(vo, pl, odd);
+            }
+        };
+#pragma unroll
+        for (int w = 0; w < (D == 64 ? 1 : D / 128); ++w) {
+            two(std::integral_constant<int, 0>{}, w, acc[8 * w + 0], acc[8 * w + 1]);
+            two(std::integral_constant<int, 1>{}, w, acc[8 * w + 2], acc[8 * w + 3]);
+            if constexpr (D > 64) {
+                two(std::integral_constant<int, 2>{}, w, acc[8 * w + 4], acc[8 * w + 5]);
+                two(std::integral_constant<int, 3>{}, w, acc[8 * w + 6], acc[8 * w + 7]);
+            }
+        }
+    }
+};
+
+// One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.
 template <class T, int D>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendParams a) {
+__global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
-    constexpr int kTiles = D / 16;                          // channel tiles of O^T, and channels of a V entry
-    constexpr int kWords = D / 32 >= 4 ? D / 128 : 1;       // 32-bit words of a V entry (D = 64: half of one)
+    constexpr int kTiles = D / 16, kRow = D + 4;
     using Raw = typename T::Raw;
     __shared__ float s_m[kAttendWaves][16], s_l[kAttendWaves][16];
-    __shared__ float s_o[kAttendWaves][16][D + 4];
+    __shared__ float s_o[4][16][kRow];
     __shared__ int s_last;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     int id = blockIdx.x;
     const int hk = id % a.kv_heads;
     id /= a.kv_heads;
@@ -119,228 +300,148 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendParams a) 
     auto begin_of = [&](int p) { return a.window ? max(p + 1 - a.window, 0) : 0; };
     const int hi = max(place0 + tok + 1, 0), lo = begin_of(place0 + tok);
     const int hi_min = max(place0 + tok_a + 1, 0), hi_max = max(place0 + tok_b + 1, 0);
-    const int lo_min = begin_of(place0 + tok_a) & ~31, lo_max = begin_of(place0 + tok_b);
-    const int mine = max((hi_max - lo_min + a.chunk - 1) / a.chunk, 1);     // splits with keys in them
+    const int lo_min = begin_of(place0 + tok_a), lo_max = begin_of(place0 + tok_b), start = lo_min & ~31;
+    const int mine = max((hi_max - start + a.chunk - 1) / a.chunk, 1);     // splits with keys in them
     if (split >= mine) return;
-    const int k0 = lo_min + split * a.chunk, k1 = min(k0 + a.chunk, hi_max);
+    const int k0 = start + split * a.chunk, k1 = min(k0 + a.chunk, hi_max);
 
     Queries<D, Planes> q;
-    q.template load<T>((const Raw *)a.q + (q0 + tok) * a.q_row + head * a.q_head, a.vec);
+    q.template load<T>((const Raw *)a.q + (q0 + tok) * a.q_row + head * a.q_head, a.vec, a.scale < 0);
+    // the scale's sign is in the queries; a scale of zero would make 0 * -inf of a key not seen
+    const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
 
     const Record rec{a.page, D};
     const int64_t head_at = hk * rec.bytes();
     const int *table = a.table + b * a.table_stride;
     const int last_page = max(held - 1, 0) >> a.page_shift;
+    auto page_of = [&](int key) {
+        const int p = table[min(key >> a.page_shift, last_page)];
+        return (unsigned)p < (unsigned)a.n_pages ? p : -1;
+    };
 
-    v4f acc[kTiles];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) acc[n] = v4f{0, 0, 0, 0};
-    float m = -INFINITY, l = 0;
-    const float to_log2 = a.scale * kLog2e;
-
-    for (int kb = k0 + 32 * wave; kb < k1; kb += 32 * kAttendWaves) {
-        // two 16-row code tiles; row 4x + i of tile t is key kb + 8x + 4t + i
-        const int kk = kb + 8 * (c >> 2) + (c & 3);
-        const int kp = table[min(kk >> a.page_shift, last_page)];
-        const int vk = kb + 8 * g;
-        const int vp = table[min(vk >> a.page_shift, last_page)];
-        const bool kfine = (unsigned)kp < (unsigned)a.n_pages, vfine = (unsigned)vp < (unsigned)a.n_pages;
-        const uint8_t *krec = a.cache + (kfine ? kp : 0) * a.page_stride + head_at;
-        const uint8_t *vrec = a.cache + (vfine ? vp : 0) * a.page_stride + head_at;
-        const int koff = kk & (a.page - 1), voff = vk & (a.page - 1);
-
-        v4f s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            s[t] = v4f{0, 0, 0, 0};
-            const uint8_t *code = krec + (koff + 4 * t) * (D / 2) + g * (D / 8);
-            const uint8_t *sc = krec + rec.k_scales() + (koff + 4 * t) * (D / 32) + g * (D / 4) / 32;
-            unsigned w[D / 32];
-            if (D == 64) *(u2 *)w = *(const u2 *)code;
-            else
-#pragma unroll
-                for (int i = 0; i < D / 128; ++i) *(u4 *)&w[4 * i] = *(const u4 *)(code + 16 * i);
-#pragma unroll
-            for (int ks = 0; ks < D / 32; ++ks) {
-                const u4 k8 = unpack8(w[ks], __uint_as_float((unsigned)sc[ks / 4] << 23));
-#pragma unroll
-                for (int n = 0; n < Planes; ++n) s[t] = mfma(k8, q.b[n][ks], s[t]);
-            }
+    Softmax<D, Planes> sm;
+    sm.clear();
+    constexpr int kStride = 32 * kAttendWaves;
+    int kb = k0 + 32 * wave;
+    if (kb < k1) {
+        // the next step's operands are on their way while this one's are worked on, the pages after that looked up
+        KeyTile<D> cur, next;
+        int id0 = page_of(kb), id1 = page_of(kb + 16);
+        int n0 = page_of(kb + kStride), n1 = page_of(kb + kStride + 16);
+        cur.load(a, rec, head_at, kb, id0, id1);
+        for (;;) {
+            const int nb = kb + kStride < k1 ? kb + kStride : kb;
+            const int l0 = nb == kb ? id0 : n0, l1 = nb == kb ? id1 : n1;
+            next.load(a, rec, head_at, nb, l0, l1);
+            n0 = page_of(nb + kStride), n1 = page_of(nb + kStride + 16);
+            v4f s[2];
+            sm.scores(cur, q, s);
+            u2 vs = cur.vs;
+            if (kb + 32 > hi_min || kb < lo_max || id0 < 0 || id1 < 0)
+                sm.mask(s, vs, kb + 8 * g, (g < 2 ? id0 : id1) >= 0, lo, hi, lo_min, hi_max);
+            sm.add(s, cur, vs, to_log2);
+            if (nb == kb) break;
+            cur = next;
+            kb = nb, id0 = l0, id1 = l1;
         }
-        // V: 8 keys x D/16 channels, 8 scale bytes
-        unsigned vw[8 * kWords];
-        const uint8_t *vcode = vrec + rec.v_codes() + (voff >> 3) * (4 * D) + c * (D / 4);
-        if (D == 64) {
-            const u4 h = *(const u4 *)vcode;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vw[2 * i] = h[i] & 0xFFFFu, vw[2 * i + 1] = h[i] >> 16;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2 * kWords; ++i) *(u4 *)&vw[4 * i] = *(const u4 *)(vcode + 16 * i);
-        }
-        u2 vs = *(const u2 *)(vrec + rec.v_scales() + (c * (D / 16) / 32) * a.page + voff);
+    }
 
-        float p[8];
+    // the eight waves' sums into one, each brought to the common maximum first
+    float l = column_sum(sm.l);
+    if (g == 0) s_m[wave][c] = sm.m, s_l[wave][c] = l;
+    __syncthreads();
+    float M = s_m[0][c];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+    for (int w = 1; w < kAttendWaves; ++w) M = fmaxf(M, s_m[w][c]);
+    const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm.m - M) * to_log2);
+    const int live = min(rows - tile * 16, 16);
+    float *mine_o = &s_o[wave & 3][c][kTiles * 4 * g];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[4 * t + i] = s[t][i] * to_log2;
-        unsigned nan_keys = 0;
-        if (kb + 32 > hi_min || kb < lo_max || !__all(vfine)) {
-            // some key of the 32 is not seen by some column: its score goes, and so does what its V holds.  A NaN block
-            // seen by some columns alone is taken out and marked for those.
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = vk + j, at = 8 * (j & 3);
-                if (!vfine || key >= hi || key < lo) p[j] = -INFINITY;
-                const bool dead = !vfine || key >= hi_max || key < lo_min;     // what lies there may be anything
-                const bool nan = (vs[j >> 2] >> at & 255u) == 255u;
-                if (!dead && nan) nan_keys |= 1u << j;
-                if (dead || nan) vs[j >> 2] = (vs[j >> 2] & ~(255u << at)) | 127u << at;
-            }
-        }
-        if (__any(nan_keys != 0)) {
-            u4 va, pa;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                va[j] = (nan_keys >> (2 * j) & 1 ? 0x3F80u : 0) | (nan_keys >> (2 * j + 1) & 1 ? 0x3F800000u : 0);
-                const bool see0 = vfine && vk + 2 * j < hi && vk + 2 * j >= lo;
-                const bool see1 = vfine && vk + 2 * j + 1 < hi && vk + 2 * j + 1 >= lo;
-                pa[j] = (see0 ? 0x3F80u : 0) | (see1 ? 0x3F800000u : 0);
-            }
-            v4f n = {0, 0, 0, 0};
-            n = mfma(va, pa, n);
+    for (int round = 0; round < 2; ++round) {
+        if (wave >> 2 == round && c < live)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (n[i] > 0)
 #pragma unroll
-                    for (int t = 0; t < kTiles; ++t) acc[t][i] = __builtin_nanf("");
-        }
-
-        float top = p[0];
+                for (int n = 0; n < kTiles; n += 4) {
+                    v4f x = {sm.acc[n][i] * f, sm.acc[n + 1][i] * f, sm.acc[n + 2][i] * f, sm.acc[n + 3][i] * f};
+                    v4f *at = (v4f *)(mine_o + kTiles * i + n);
+                    if (round) x += *at;
+                    *at = x;
+                }
+        __syncthreads();
+    }
+    constexpr int kQuads = D / 4;       // 4 channels a thread from here on
+    const int64_t at = ((int64_t)b * a.kv_heads + hk) * a.tiles + tile;
+    float *all = a.part + at * a.splits * 16 * kRow;      // under 2^31 bytes: at most 1,024 splits of 16 rows
+    auto finish = [&](int col, int quad, v4f o, float top, float total) {
+        const int r = tile * 16 + col, t = r / a.group, h = hk * a.group + r % a.group;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        Raw *out = (Raw *)a.out + (int64_t)(q0 + t) * a.out_row + h * a.out_head + 4 * quad;
+        Raw v[4];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, p[j]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > m)) {
-            const float m2 = fmaxf(m, top), keep = exp2f(m == -INFINITY ? -INFINITY : m - m2);
-            m = m2;
-            l *= keep;
+        for (int i = 0; i < 4; ++i) v[i] = T::put(o[i] * inv);
+        if (a.vec_out) *(u2 *)out = *(u2 *)v;
+        else
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n)
+            for (int i = 0; i < 4; ++i) out[i] = v[i];
+        if (a.lse && quad == 0)
+            a.lse[(int64_t)(q0 + t) * a.heads + h] = total == 0.0f ? -INFINITY : top * to_log2 * kLn2 + logf(total);
+    };
+    for (int u = threadIdx.x; u < live * kQuads; u += kAttendThreads) {
+        const int col = u / kQuads, quad = u % kQuads;
+        v4f o = *(v4f *)&s_o[0][col][4 * quad];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][i] *= keep;
-        }
-        const float shift = m == -INFINITY ? 0.0f : m;
-        u4 ph, pl;
+        for (int w = 1; w < 4; ++w) o += *(v4f *)&s_o[w][col][4 * quad];
+        float top = s_m[0][col], total = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = __builtin_amdgcn_exp2f(p[2 * j] - shift), y = __builtin_amdgcn_exp2f(p[2 * j + 1] - shift);
-            l += x + y;
-            ph[j] = pack_bf16(x, y);
-            if (Planes == 2)      // an f16 result wants more than bf16's 8 bits of P: the rest of it as a second product
-                pl[j] = pack_bf16(x - __uint_as_float(ph[j] << 16), y - __uint_as_float(ph[j] & 0xFFFF0000u));
-        }
-        float vscale[8];
+        for (int w = 1; w < kAttendWaves; ++w) top = fmaxf(top, s_m[w][col]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vscale[j] = __uint_as_float((vs[j >> 2] >> (8 * (j & 3)) & 255u) << 23);
-        // two channels at a time: a byte of each key's codes
-        auto two = [&](auto sel, int word, v4f &even, v4f &odd) {
-            constexpr int kSel = decltype(sel)::value;
-            u4 ve, vo;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bf2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[2 * j * kWords + word], vscale[2 * j], kSel);
-                const bf2 y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[(2 * j + 1) * kWords + word], vscale[2 * j + 1], kSel);
-                const unsigned xu = __builtin_bit_cast(unsigned, x), yu = __builtin_bit_cast(unsigned, y);
-                ve[j] = __builtin_amdgcn_perm(yu, xu, 0x05040100u);
-                vo[j] = __builtin_amdgcn_perm(yu, xu, 0x07060302u);
-            }
-            even = mfma(ve, ph, even);
-            odd = mfma(vo, ph, odd);
-            if (Planes == 2) {
-                even = mfma(ve, pl, even);
-                odd = mfma(vo, pl, odd);
-            }
-        };
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-            two(std::integral_constant<int, 0>{}, w, acc[8 * w + 0], acc[8 * w + 1]);
-            two(std::integral_constant<int, 1>{}, w, acc[8 * w + 2], acc[8 * w + 3]);
-            if constexpr (D > 64) {
-                two(std::integral_constant<int, 2>{}, w, acc[8 * w + 4], acc[8 * w + 5]);
-                two(std::integral_constant<int, 3>{}, w, acc[8 * w + 6], acc[8 * w + 7]);
-            }
+        for (int w = 0; w < kAttendWaves; ++w)      // with no maximum the sums are 0, or NaN
+            total += s_l[w][col] * (top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((s_m[w][col] - top) * to_log2));
+        if (mine == 1) {
+            finish(col, quad, o, top, total);
+        } else {
+            const unsigned p = (split * 16 + col) * kRow;
+            store_shared(all, p + 4 * quad, o);
+            if (quad == 0) store_shared(all, p + D, v4f{top, total, 0, 0});
         }
     }
+    if (mine == 1) return;
 
-    // the four waves' sums into one
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (g == 0) s_m[wave][c] = m, s_l[wave][c] = l;
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[wave][c][kTiles * (4 * g + i) + n] = acc[n][i];
+    // splits meet in memory; the last to arrive joins them
+    __builtin_amdgcn_s_waitcnt(0);        // this thread's sums have landed
     __syncthreads();
-    const int live = min(rows - tile * 16, 16);
-    const int col = threadIdx.x >> 4, part = threadIdx.x & 15;         // 16 threads a column, D/16 channels each
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kAttendWaves; ++w) M = fmaxf(M, s_m[w][col]);
-    const float shift = M == -INFINITY ? 0.0f : M;
-    float L = 0, o[kTiles];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) o[n] = 0;
-#pragma unroll
-    for (int w = 0; w < kAttendWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(s_m[w][col] - shift);
-        L += f * s_l[w][col];
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) o[n] += f * s_o[w][col][part * kTiles + n];
+    if (threadIdx.x == 0) {
+        s_last = __hip_atomic_fetch_add(&a.arrived[at], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mine - 1;
+        if (s_last) __hip_atomic_store(&a.arrived[at], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    const int row2 = tile * 16 + col;
-    if (mine > 1) {
-        // splits meet in memory; the last to arrive adds them up
-        const int64_t at = ((int64_t)b * a.kv_heads + hk) * a.tiles + tile;
-        float *p = a.part + ((at * a.splits + split) * 16 + col) * (D + 2);
-        if (col < live) {
-            if (part == 0) p[D] = M, p[D + 1] = L;
+    __syncthreads();
+    if (!s_last) return;
+    for (int u = threadIdx.x; u < live * kQuads; u += kAttendThreads) {
+        const int col = u / kQuads, quad = u % kQuads;
+        v4f o = {0, 0, 0, 0};
+        float top = -INFINITY, total = 0;
+        // batches of 8 splits, their loads together
+        for (int i0 = 0; i0 < mine; i0 += 8) {
+            v4f x[8], ml[8];
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) p[part * kTiles + n] = o[n];
-        }
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            s_last = atomicAdd(&a.arrived[at], 1) == mine - 1;
-            if (s_last) atomicExch(&a.arrived[at], 0);
-        }
-        __syncthreads();
-        if (!s_last) return;
-        __threadfence();
-        if (col >= live) return;
-        const float *all = a.part + (at * a.splits * 16 + col) * (D + 2);
-        M = -INFINITY;
-        for (int i = 0; i < mine; ++i) M = fmaxf(M, all[(int64_t)i * 16 * (D + 2) + D]);
-        const float sh = M == -INFINITY ? 0.0f : M;
-        L = 0;
+            for (int i = 0; i < 8; ++i) {
+                const unsigned p = (min(i0 + i, mine - 1) * 16 + col) * kRow;
+                x[i] = load_shared(all, p + 4 * quad), ml[i] = load_shared(all, p + D);
+            }
+            float t2 = top;
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n) o[n] = 0;
-        for (int i = 0; i < mine; ++i) {
-            const float *pi = all + (int64_t)i * 16 * (D + 2);
-            const float f = __builtin_amdgcn_exp2f(pi[D] - sh);
-            L += f * pi[D + 1];
+            for (int i = 0; i < 8; ++i) t2 = fmaxf(t2, ml[i][0]);
+            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - t2) * to_log2);
+            o *= keep, total *= keep, top = t2;
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) o[n] += f * pi[part * kTiles + n];
+            for (int i = 0; i < 8; ++i) {
+                const float w = t2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((ml[i][0] - t2) * to_log2);
+                if (i0 + i < mine) o += x[i] * w, total += ml[i][1] * w;
+            }
         }
+        finish(col, quad, o, top, total);
     }
-    if (col >= live) return;
-    const int tok2 = row2 / a.group, head2 = hk * a.group + row2 % a.group;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    Raw *out = (Raw *)a.out + (int64_t)(q0 + tok2) * a.out_row + head2 * a.out_head + part * kTiles;
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) out[n] = T::put(o[n] * inv);
-    if (a.lse && part == 0) a.lse[(int64_t)(q0 + tok2) * a.heads + head2] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 }  // namespace pklm

@@ -95,16 +95,15 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t tiles = (rows + 15) / 16, pairs = (int64_t)d.requests * d.kv_heads;
     // keys of one 16-row tile: its rows span at most 16 tokens
     const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 32) : d.max_len;
-    const int64_t want = 2 * kCounters, each = std::max<int64_t>(pairs * tiles, 1);   // split: at most kCounters tiles
+    const int64_t want = kCounters, each = std::max<int64_t>(pairs * tiles, 1);   // split: fewer than kCounters tiles
     int64_t splits = std::max<int64_t>(std::min<int64_t>(want / each, (keys + 255) / 256), 1);
-    int64_t chunk = ((keys + splits - 1) / splits + 127) / 128 * 128;
-    chunk = std::max<int64_t>(chunk, 128);
+    int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + 255) / 256 * 256, 256);
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
     if (pairs * tiles * splits > INT32_MAX)
         return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
                        (long long)rows);
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
-    s.part_bytes = pairs * tiles * splits * 16 * (d.head_dim + 2) * 4;
+    s.part_bytes = pairs * tiles * splits * 16 * (d.head_dim + 4) * 4;
     return PK_OK;
 }
 
@@ -202,6 +201,7 @@ PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
     p.max_len = d->max_len, p.window = d->window, p.group = d->heads / d->kv_heads;
     p.tiles = sh.tiles, p.splits = sh.splits, p.chunk = sh.chunk, p.scale = d->scale;
     p.vec = aligned(d->q, 16) && d->q_row % 8 == 0 && d->q_head % 8 == 0;
+    p.vec_out = aligned(d->out, 8) && d->out_row % 4 == 0 && d->out_head % 4 == 0;
     const unsigned grid = (unsigned)((int64_t)d->requests * d->kv_heads * sh.tiles * sh.splits);
     if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, d->head_dim, grid, (hipStream_t)stream);
     else launch_attend<BF16>(p, d->head_dim, grid, (hipStream_t)stream);
