@@ -106,15 +106,11 @@ __device__ inline float column_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Values that workgroups on other XCDs read within the launch: written through to, and read from, where all XCDs meet.
-// base is the same in the whole wave, at counts floats.
 __device__ inline void store_shared(float *base, unsigned at, v4f v) {
-    const auto r = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000);
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, 4 * at, 0, 16);
+    store_shared4((unsigned *)base, at, __builtin_bit_cast(u4, v));
 }
 __device__ inline v4f load_shared(const float *base, unsigned at) {
-    const auto r = __builtin_amdgcn_make_buffer_rsrc((float *)base, 0, 0x7FFFFFFF, 0x00020000);
-    return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(r, 4 * at, 0, 16));
+    return __builtin_bit_cast(v4f, load_shared4((const unsigned *)base, at));
 }
 
 // One step's operands of a lane: 32 keys, of K two rows' D/4 channels, of V 8 keys' D/16 channels.

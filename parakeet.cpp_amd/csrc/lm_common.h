@@ -50,15 +50,58 @@ struct Record {
     __host__ __device__ int v_scales() const { return page * dim + page * (dim / 32); }
 };
 
-template <class T>
-__device__ inline T wave_scan(T v) {   // inclusive sum over the wave
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+// Whole-wave scans and sums in the vector unit: lanes 1, 2, 4 and 8 before within rows of 16, then the last lanes of
+// the rows before (a shuffle through LDS takes several times as long, and there are six in a row).
+template <int Ctrl, int RowMask>
+__device__ inline unsigned from_lane(unsigned v, unsigned none) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)none, (int)v, Ctrl, RowMask, 0xF, false);
+}
+template <int Ctrl, int RowMask>
+__device__ inline unsigned long long from_lane(unsigned long long v, unsigned long long none) {
+    return (unsigned long long)from_lane<Ctrl, RowMask>((unsigned)(v >> 32), (unsigned)(none >> 32)) << 32 |
+           from_lane<Ctrl, RowMask>((unsigned)v, (unsigned)none);
+}
+template <int Ctrl, int RowMask>
+__device__ inline int from_lane(int v, int none) { return (int)from_lane<Ctrl, RowMask>((unsigned)v, (unsigned)none); }
+template <int Ctrl, int RowMask>
+__device__ inline float from_lane(float v, float none) {
+    return __uint_as_float(from_lane<Ctrl, RowMask>(__float_as_uint(v), __float_as_uint(none)));
+}
+template <class V, class F>
+__device__ inline V wave_scan(V v, V none, F f) {      // inclusive; lane 63 has all
+    v = f(v, from_lane<0x111, 0xF>(v, none));
+    v = f(v, from_lane<0x112, 0xF>(v, none));
+    v = f(v, from_lane<0x114, 0xF>(v, none));
+    v = f(v, from_lane<0x118, 0xF>(v, none));
+    v = f(v, from_lane<0x142, 0xA>(v, none));
+    v = f(v, from_lane<0x143, 0xC>(v, none));
     return v;
+}
+template <class V>
+__device__ inline V wave_scan(V v) {
+    return wave_scan(v, V(0), [](V a, V b) { return a + b; });
+}
+__device__ inline unsigned lane_value(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ inline int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ inline float lane_value(float v, int lane) { return __uint_as_float(lane_value(__float_as_uint(v), lane)); }
+__device__ inline unsigned long long lane_value(unsigned long long v, int lane) {
+    return (unsigned long long)lane_value((unsigned)(v >> 32), lane) << 32 | lane_value((unsigned)v, lane);
+}
+template <class V>
+__device__ inline V wave_sum(V v) { return lane_value(wave_scan(v), 63); }
+__device__ inline float wave_max(float v) {
+    return lane_value(wave_scan(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); }), 63);
+}
+
+// Values that workgroups on other XCDs read within the launch: written through to, and read from, where all XCDs meet.
+// base is the same in the whole wave, at counts 32-bit words from it, below 2^29.
+__device__ inline void store_shared4(unsigned *base, unsigned at, u4 v) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(v, r, 4 * at, 0, 16);
+}
+__device__ inline u4 load_shared4(const unsigned *base, unsigned at) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc((unsigned *)base, 0, 0x7FFFFFFF, 0x00020000);
+    return __builtin_amdgcn_raw_buffer_load_b128(r, 4 * at, 0, 16);
 }
 
 }  // namespace pklm

@@ -1,4 +1,14 @@
 // lm_sample.h -- one token per row of logits (pk_sample).
+//
+// Weights are whole numbers, so sums are exact and the same in any order, and atomics may build them.  In the order
+// (falling logit, rising index) the kept tokens are a prefix, so the filters come down to one cut: the last kept token.
+// Every token has a rank word of 64 bits, its logit's ordered bits over its inverted index; kept is rank >= cut.
+//
+// To find the cut, tokens are binned by their distance from the largest logit, (max - x) / T in bins of 22/1,024
+// (weights round to none at 21.5), and the bins' (count, weight) sums are scanned.  That names the bin in which
+// the count reaches top_k or the weight reaches top_p's share.  The tokens up to that bin, or where they are too many
+// those of that bin alone, are listed and sorted, one a thread: the cut is a place in the list, and of a whole list the
+// token too.  A bin with more tokens than that (many equal logits) is split by the rank words' digits instead.
 #pragma once
 
 #include "lm_common.h"
@@ -6,25 +16,49 @@
 
 namespace pklm {
 
-constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
+typedef unsigned long long u64;
+
+constexpr float kReach = 22.0f;            // distance that the bins cover
+constexpr int kWholeMost = 64;            // a list with all kept tokens has at most so many: they are compared each with each
+constexpr int kCountShift = 46;            // (count, weight) of up to 2^15 tokens in one word: 2^15 2^30 < 2^46
+constexpr u64 kMassMask = (1ull << kCountShift) - 1;
 
 // f32 order as unsigned order; both zeros alike
 __device__ inline unsigned order_key(float x) {
     const unsigned b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ inline u64 rank_of(float x, int i) { return (u64)order_key(x) << 32 | (0xFFFFFFFFu - (unsigned)i); }
 // floor(total * part / 2^31), part <= 2^31
-__device__ inline unsigned long long share(unsigned long long total, unsigned long long part) {
-    return (total >> 31) * part + (((total & 0x7FFFFFFFull) * part) >> 31);
-}
+__device__ inline u64 share(u64 total, u64 part) { return (total >> 31) * part + (((total & 0x7FFFFFFFull) * part) >> 31); }
+__device__ inline u64 part31(float p) { return (u64)(fminf(fmaxf(p, 0.0f), 1.0f) * 2147483648.0f); }
 
-struct RowFilter {
-    float top, inv;      // largest logit, 1 / temperature
-    __device__ unsigned weight(float x) const {
-        if (x == -INFINITY) return 0;
-        const float z = x == top ? 0.0f : (x - top) * inv;
-        return (unsigned)rintf(expf(z) * 1073741824.0f);
+// One row's settings and what follows from its largest logit.
+struct RowRule {
+    float top, inv;
+    unsigned least;      // min_p's weight
+    int k;               // how many at most
+    u64 p;               // top_p in 2^-31
+    bool k_on, p_on;
+
+    __device__ void settings(const pk_sample_desc &a, int b) {
+        const float t = a.temperature ? a.temperature[b] : 1.0f;
+        const bool greedy = !(t > 0);
+        inv = greedy ? 1.0f : fminf(1.0f / t, 3e38f);
+        const int top_k = a.top_k ? a.top_k[b] : 0;
+        k = greedy ? 1 : top_k;
+        k_on = greedy || (top_k > 0 && top_k < a.vocab);
+        p = part31(a.top_p ? a.top_p[b] : 1.0f);
+        p_on = p < 0x80000000ull;
+        least = (unsigned)ceilf(fminf(fmaxf(a.min_p ? a.min_p[b] : 0.0f, 0.0f), 1.0f) * 1073741824.0f);
     }
+    __device__ float distance(float x) const { return x == top ? 0.0f : (x - top) * inv; }
+    __device__ unsigned weight(float x) const {
+        return x == -INFINITY ? 0u : (unsigned)rintf(expf(distance(x)) * 1073741824.0f);
+    }
+    // the steps from x to the bin are monotone, so bins keep the order; tokens without a weight are in none, or the last
+    template <int Bins>
+    __device__ int bin(float x) const { return (int)fminf(distance(x) * (-Bins / kReach), (float)(Bins - 1)); }
 };
 
 template <class T>
@@ -33,183 +67,701 @@ __device__ inline float logit(const typename T::Raw *row, int i) {
     return x != x ? -INFINITY : x;
 }
 
-// One workgroup a row.  The kept set is a prefix of the order (falling logit, rising index), so it is one cut: a key and
-// how many of that key's tokens.  The cut is found digit by digit from histograms of (count, weight).
-template <class T>
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(pk_sample_desc a) {
-    using Raw = typename T::Raw;
-    typedef unsigned long long u64;
-    __shared__ u64 s_top, s_mass[256], s_wm[kSampleWaves], s_r[4];
-    __shared__ unsigned s_cnt[256], s_wc[kSampleWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab, b = blockIdx.x;
-    const Raw *row = (const Raw *)a.logits + (int64_t)b * a.logits_row;
+// Where a cut was found: the token's rank word and the weight up to it, itself included.
+struct Cut {
+    u64 rank, mass;
+};
 
-    // the largest logit, lowest index
-    u64 best = 0;
-    for (int i = tid; i < V; i += kSampleThreads) {
-        const u64 k = (u64)order_key(logit<T>(row, i)) << 32 | (0xFFFFFFFFu - (unsigned)i);
-        best = best > k ? best : k;
+__device__ inline float logit_of(u64 rank) {
+    const unsigned k = (unsigned)(rank >> 32);
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+__device__ inline int index_of(u64 rank) { return (int)(0xFFFFFFFFu - (unsigned)rank); }
+
+// What a workgroup of BS threads keeps in LDS to find a cut.
+template <int BS, int Bins>
+struct CutScratch {
+    static constexpr int kThreads = BS, kBins = Bins, kCounted = BS / 4;
+    u64 mass[Bins];                  // (count, weight) of a bin in one word; then running weight
+    unsigned count[Bins];            // running count of tokens
+    u64 list[BS], list_mass[BS];     // rank words, falling once sorted; running weight
+    unsigned list_w[BS];             // weight
+    u64 wave_mass[BS / 64];
+    unsigned wave_count[BS / 64];
+    u64 digit_mass[256];
+    unsigned digit_count[256];
+    u64 digit_at[3];
+    int n[2], bin[2], found[2];      // by count, by weight: tokens listed, bin reached, place in the list
+    int digit;
+
+    // before the barrier that precedes everything below
+    __device__ void clear() {
+        for (int i = threadIdx.x; i < Bins; i += BS) mass[i] = 0;
+        if (threadIdx.x < 2) n[threadIdx.x] = 0, bin[threadIdx.x] = -1;
     }
-    if (tid == 0) s_top = 0;
-    __syncthreads();
-    for (int d = 32; d; d >>= 1) {
-        const u64 o = __shfl_xor(best, d);
-        best = best > o ? best : o;
+    __device__ u64 mass_to(int b) const { return b < 0 ? 0 : mass[b]; }
+    __device__ unsigned count_to(int b) const { return b < 0 ? 0 : count[b]; }
+
+    // a running sum over the threads: what lies before this one's, from its wave's inclusive sum
+    __device__ u64 before(u64 inclusive, u64 own) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 63) wave_mass[wave] = inclusive;
+        __syncthreads();
+        u64 v = inclusive - own;
+#pragma unroll
+        for (int w = 0; w < BS / 64; ++w)
+            if (w < wave) v += wave_mass[w];
+        return v;
     }
-    if (lane == 0) atomicMax(&s_top, best);
-    __syncthreads();
-    best = s_top;
-    const unsigned top_key = (unsigned)(best >> 32);
-    const int top_at = (int)(0xFFFFFFFFu - (unsigned)best);
-    const float temperature = a.temperature ? a.temperature[b] : 1.0f;
-    const bool none = top_key == order_key(-INFINITY);
-    if (none || !(temperature > 0)) {
-        if (tid == 0) {
-            a.token[b] = none ? -1 : top_at;
-            if (a.prob) a.prob[b] = none ? 0.0f : 1.0f;
-            if (a.kept) a.kept[b] = none ? 0 : 1;
+
+    // Running sums of m, c, Bins / BS a thread (bin tid Bins / BS + i), into mass and count.
+    __device__ void scan(u64 (&m)[Bins / BS], unsigned (&c)[Bins / BS]) {
+        constexpr int kPer = Bins / BS;
+        const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) m[i] += m[i - 1], c[i] += c[i - 1];
+        const unsigned ic = wave_scan(c[kPer - 1]);
+        if (lane == 63) wave_count[wave] = ic;
+        const u64 bm = before(wave_scan(m[kPer - 1]), m[kPer - 1]);
+        unsigned bc = ic - c[kPer - 1];
+#pragma unroll
+        for (int w = 0; w < BS / 64; ++w)
+            if (w < wave) bc += wave_count[w];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mass[tid * kPer + i] = bm + m[i], count[tid * kPer + i] = bc + c[i];
+        __syncthreads();
+    }
+
+    // The bin in which the running count (kind 0) or weight (kind 1) reaches `want`; -1: never.  Once a kind.
+    __device__ int reach(int kind, u64 want) {
+        for (int i = threadIdx.x; i < Bins; i += BS) {
+            const u64 here = kind ? mass[i] : count[i];
+            const u64 prior = i == 0 ? 0 : kind ? mass[i - 1] : count[i - 1];
+            if (prior < want && want <= here) bin[kind] = i;
         }
+        __syncthreads();
+        return bin[kind];
+    }
+
+    // list[0 .. n), n <= BS, into falling order, and its running weights.  Short lists: each word's place is the number
+    // of larger ones, some lanes a word.  Longer ones: a bitonic network, one word a thread, steps within a wave by lane
+    // exchanges.
+    __device__ void sort(int n_list, const RowRule &rule) {
+        const int tid = threadIdx.x;
+        if (n_list <= kCounted) {
+            constexpr int kLanes = BS / kCounted;
+            const int j = tid / kLanes;
+            const u64 v = j < n_list ? list[j] : 0;
+            int larger = 0;
+#pragma unroll 4
+            for (int i = tid % kLanes; i < n_list; i += kLanes) larger += list[i] > v;
+#pragma unroll
+            for (int d = kLanes / 2; d; d >>= 1) larger += __shfl_xor(larger, d);
+            __syncthreads();
+            if (j < n_list && tid % kLanes == 0) list[larger] = v;
+            __syncthreads();
+            const u64 u = tid < n_list ? list[tid] : 0;
+            const u64 w = tid < n_list ? rule.weight(logit_of(u)) : 0;
+            const u64 run = before(wave_scan(w), w) + w;
+            if (tid < n_list) list_mass[tid] = run, list_w[tid] = (unsigned)w;
+        } else {
+            int size = 64;
+            while (size < n_list) size <<= 1;
+            u64 v = tid < n_list ? list[tid] : 0;
+            for (int k = 2; k <= size; k <<= 1)
+                for (int j = k >> 1; j; j >>= 1) {
+                    u64 o = 0;
+                    if (j >= 64) {
+                        __syncthreads();
+                        list[tid] = v;
+                        __syncthreads();
+                        o = list[tid ^ j];
+                    } else if ((tid & ~63) < size) {
+                        o = __shfl_xor(v, j);
+                    }
+                    const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
+                    v = (o > v) == larger ? o : v;
+                }
+            const u64 w = tid < n_list ? rule.weight(logit_of(v)) : 0;
+            const u64 run = before(wave_scan(w), w) + w;      // the barrier in it: list has been read
+            list[tid] = v, list_mass[tid] = run, list_w[tid] = (unsigned)w;
+        }
+        __syncthreads();
+    }
+
+    // The place in the sorted list at which mass0 and its running weight reach `want`.
+    __device__ int place(int n_list, u64 mass0, u64 want) {
+        const int tid = threadIdx.x;
+        if (tid < n_list && mass0 + list_mass[tid] >= want && (tid == 0 || mass0 + list_mass[tid - 1] < want)) found[1] = tid;
+        __syncthreads();
+        return found[1];
+    }
+};
+
+// The token at which the count (kind 0) or the weight (kind 1) reaches `want`, among all that `each` gives (each(f) calls
+// f(rank, weight) for this thread's ones), without a list: eight bits of the rank words at a time.
+template <class Scratch, class Each>
+__device__ inline Cut cut_by_digits(Scratch &s, int kind, u64 want, Each each) {
+    u64 prefix = 0, c0 = 0, m0 = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 256; i += Scratch::kThreads) s.digit_mass[i] = 0, s.digit_count[i] = 0;
+        __syncthreads();
+        each([&](u64 r, unsigned w) {
+            if (shift == 56 || (r >> (shift + 8)) == prefix) {
+                atomicAdd(&s.digit_count[r >> shift & 255u], 1u);
+                atomicAdd(&s.digit_mass[r >> shift & 255u], (u64)w);
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int d = 255;
+            for (; d > 0; --d) {
+                if ((kind ? m0 + s.digit_mass[d] : c0 + s.digit_count[d]) >= want) break;
+                c0 += s.digit_count[d], m0 += s.digit_mass[d];
+            }
+            s.digit_at[0] = c0, s.digit_at[1] = m0, s.digit_at[2] = s.digit_mass[d], s.digit = d;
+        }
+        __syncthreads();
+        c0 = s.digit_at[0], m0 = s.digit_at[1], prefix = prefix << 8 | (unsigned)s.digit;
+    }
+    const Cut cut{prefix, m0 + s.digit_at[2]};
+    __syncthreads();
+    return cut;
+}
+
+// The cut of a row whose bins are scanned.  list(kind, first, last) lists the tokens of some bins; each(f) is as above.
+// Returns how many tokens the cut leaves where the list holds all of them, else -1.
+template <class Scratch, class List, class Each>
+__device__ inline int find_cut(Scratch &s, const RowRule &rule, u64 &cut, List list, Each each) {
+    u64 total = s.mass[Scratch::kBins - 1];
+    int kept = -1, n = 0;
+    bool whole = false;
+    // lists the bins up to b, or b alone
+    auto listed = [&](int kind, int b) {
+        whole = s.count_to(b) <= kWholeMost;
+        n = s.count_to(b) - (whole ? 0 : s.count_to(b - 1));
+        if (n > Scratch::kThreads) return false;
+        list(kind, whole ? 0 : b, b);
+        s.sort(n, rule);
+        return true;
+    };
+    bool have = false;       // a list with every token that may be kept
+    if (rule.k_on) {
+        const int b = s.reach(0, (u64)rule.k);
+        if (b >= 0) {
+            if (listed(0, b)) {
+                const int at = rule.k - 1 - (whole ? 0 : (int)s.count_to(b - 1));
+                cut = s.list[at], total = s.list_mass[at] + (whole ? 0 : s.mass_to(b - 1));
+                have = whole;
+                if (whole) kept = at + 1;
+            } else {
+                const Cut c = cut_by_digits(s, 0, (u64)rule.k, each);
+                cut = c.rank, total = c.mass;
+            }
+        }
+    }
+    if (rule.p_on) {
+        u64 need = share(total, rule.p);
+        need = need ? need : 1;              // the first token is kept whatever the share
+        u64 c;
+        if (have) {
+            const int at = s.place(n, 0, need);
+            c = s.list[at], kept = at + 1;
+        } else {
+            const int b = s.reach(1, need);
+            if (listed(1, b)) {
+                const int at = s.place(n, whole ? 0 : s.mass_to(b - 1), need);
+                c = s.list[at];
+                if (whole) kept = at + 1;    // a whole list by weight ends before any cut by count that had none
+            } else {
+                c = cut_by_digits(s, 1, need, each).rank;
+            }
+        }
+        cut = cut > c ? cut : c;
+    }
+    return kept;
+}
+
+// Sets a row's results.
+__device__ inline void answer(const pk_sample_desc &a, int b, int token, unsigned w, u64 total, unsigned kept) {
+    a.token[b] = token;
+    if (a.prob) a.prob[b] = total ? (float)w / (float)total : 0.0f;
+    if (a.kept) a.kept[b] = (int)kept;
+}
+__device__ inline u64 drawn(const pk_sample_desc &a, int b, u64 total) {
+    const u64 u = part31(a.u[b]);
+    return share(total, u > 0x7FFFFFFFull ? 0x7FFFFFFFull : u);
+}
+
+// The drawn token of the first `kept` of a sorted list.
+template <class Scratch>
+__device__ inline void answer_from_list(Scratch &s, const pk_sample_desc &a, int b, const RowRule &rule, int kept) {
+    const int tid = threadIdx.x;
+    if (tid < kept && s.list_w[tid] >= rule.least && (tid == kept - 1 || s.list_w[tid + 1] < rule.least)) s.found[0] = tid + 1;
+    __syncthreads();
+    kept = s.found[0];
+    const u64 total = s.list_mass[kept - 1], t = drawn(a, b, total);
+    int lanes = 64;
+    while (lanes > 1 && kept * lanes > Scratch::kThreads) lanes >>= 1;
+    const int j = tid / lanes;
+    const unsigned own = j < kept ? (unsigned)s.list[j] : 0;       // inverted indices
+    u64 before = 0;
+#pragma unroll 4
+    for (int i = tid & (lanes - 1); i < kept; i += lanes) {
+        const unsigned other = (unsigned)s.list[i], w = s.list_w[i];
+        before += other > own ? w : 0;
+    }
+    for (int d = lanes >> 1; d; d >>= 1) before += __shfl_xor(before, d);
+    if (j < kept && (tid & (lanes - 1)) == 0) {
+        const unsigned w = s.list_w[j];
+        if (before <= t && t < before + w) answer(a, b, index_of(s.list[j]), w, total, kept);
+    }
+}
+
+// A row on one workgroup, its tokens in registers: wave w has tokens (w n + e) 64 + lane, e < n <= E.
+template <class T, int BS, int E>
+__global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
+    constexpr int kWaves = BS / 64, kBins = 1024;
+    __shared__ CutScratch<BS, kBins> s;
+    __shared__ float s_max[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab, b = blockIdx.x;
+    const auto *row = (const typename T::Raw *)a.logits + (int64_t)b * a.logits_row;
+    const int n = (V + BS - 1) / BS, base = wave * n * 64 + lane;
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = base + e * 64;
+        x[e] = e < n && i < V ? logit<T>(row, i) : -INFINITY;
+    }
+    RowRule rule;
+    rule.settings(a, b);
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
+    top = wave_max(top);
+    if (lane == 0) s_max[wave] = top;
+    s.clear();
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_max[w]);
+    rule.top = top;
+    if (top == -INFINITY) {
+        if (tid == 0) answer(a, b, -1, 0, 0, 0);
         return;
     }
-    const RowFilter f{logit<T>(row, top_at), fminf(1.0f / temperature, 3e38f)};
-    const int top_k = a.top_k ? a.top_k[b] : 0;
-    const float top_p = a.top_p ? a.top_p[b] : 1.0f, min_p = a.min_p ? a.min_p[b] : 0.0f;
-    const u64 P = (u64)(fminf(fmaxf(top_p, 0.0f), 1.0f) * 2147483648.0f);
-    const unsigned least = (unsigned)ceilf(fminf(fmaxf(min_p, 0.0f), 1.0f) * 1073741824.0f);
-
-    // sums over all, then the cut by count, then the cut by weight
-    u64 cut_mass = 0;            // weight of the kept prefix so far
-    unsigned cut_key = 0, cut_ties = 0xFFFFFFFFu;   // kept: key > cut_key, or the first cut_ties of cut_key
-    auto block_sum = [&](u64 m, unsigned n) {
-        for (int d = 32; d; d >>= 1) m += __shfl_xor(m, d), n += __shfl_xor(n, d);
-        __syncthreads();
-        if (lane == 0) s_wm[wave] = m, s_wc[wave] = n;
-        __syncthreads();
-        if (tid == 0) {
-            u64 M = 0;
-            unsigned N = 0;
-            for (int w = 0; w < kSampleWaves; ++w) M += s_wm[w], N += s_wc[w];
-            s_r[0] = M, s_r[1] = N;
+    unsigned w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = e < n ? rule.weight(x[e]) : 0;
+    u64 cut = 0;
+    if (rule.k_on || rule.p_on) {
+        int bin[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            bin[e] = e < n && w[e] ? rule.bin<kBins>(x[e]) : kBins;
+            if (e < n && w[e]) atomicAdd(&s.mass[bin[e]], (1ull << kCountShift) | w[e]);
         }
         __syncthreads();
-    };
-    {
-        u64 m = 0;
-        for (int i = tid; i < V; i += kSampleThreads) m += f.weight(logit<T>(row, i));
-        block_sum(m, 0);
-        cut_mass = s_r[0];
-    }
-    // the key in which a running count (by_count) or weight first reaches `want` (>= 1, and reached)
-    auto find = [&](bool by_count, u64 want, unsigned &key, unsigned &ties, u64 &before) {
-        unsigned prefix = 0;
-        u64 above_c = 0, above_m = 0;
-        unsigned here = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) s_cnt[tid] = 0, s_mass[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < V; i += kSampleThreads) {
-                const float x = logit<T>(row, i);
-                const unsigned k = order_key(x);
-                if (shift == 24 || (k >> (shift + 8)) == prefix) {
-                    atomicAdd(&s_cnt[k >> shift & 255u], 1u);
-                    atomicAdd(&s_mass[k >> shift & 255u], (u64)f.weight(x));
-                }
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int d = 255;
-                u64 c = above_c, m = above_m;
-                for (; d > 0; --d) {
-                    if ((by_count ? c + s_cnt[d] : m + s_mass[d]) >= want) break;
-                    c += s_cnt[d], m += s_mass[d];
-                }
-                s_r[0] = (u64)d, s_r[1] = c, s_r[2] = m, s_r[3] = s_cnt[d];
-            }
-            __syncthreads();
-            prefix = prefix << 8 | (unsigned)s_r[0];
-            above_c = s_r[1], above_m = s_r[2], here = (unsigned)s_r[3];
+        constexpr int kPer = kBins / BS;
+        u64 bm[kPer];
+        unsigned bc[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const u64 both = s.mass[tid * kPer + i];
+            bm[i] = both & kMassMask, bc[i] = (unsigned)(both >> kCountShift);
         }
-        key = prefix, ties = here;
-        before = by_count ? above_c : above_m;
-        if (by_count) s_wm[0] = above_m;     // read back below, before the next use
-    };
-    auto weight_of_key = [&](unsigned k) {
-        return f.weight(__uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k));
-    };
-    if (top_k > 0 && top_k < V) {
-        u64 before;
-        find(true, (u64)top_k, cut_key, cut_ties, before);
-        __syncthreads();
-        cut_ties = (unsigned)(top_k - before);
-        cut_mass = s_wm[0] + (u64)cut_ties * weight_of_key(cut_key);
+        s.scan(bm, bc);
+        auto each = [&](auto f) {            // seldom wanted: from memory again
+            for (int i = tid; i < V; i += BS) {
+                const float y = logit<T>(row, i);
+                const unsigned wt = rule.weight(y);
+                if (wt) f(rank_of(y, i), wt);
+            }
+        };
+        auto list = [&](int kind, int first, int last) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < n && bin[e] >= first && bin[e] <= last) s.list[atomicAdd(&s.n[kind], 1)] = rank_of(x[e], base + e * 64);
+            __syncthreads();
+        };
+        const int left = find_cut(s, rule, cut, list, each);
+        if (left > 0 && left <= kWholeMost) {
+            answer_from_list(s, a, b, rule, left);
+            return;
+        }
     }
-    const u64 need = share(cut_mass, P);
-    if (need == 0) {
-        cut_key = top_key, cut_ties = 1;
-    } else {
-        unsigned key, ties;
-        u64 before;
-        find(false, need, key, ties, before);
-        const u64 w = weight_of_key(key);
-        const unsigned t = (unsigned)((need - before + w - 1) / w);
-        if (key > cut_key || (key == cut_key && t < cut_ties)) cut_key = key, cut_ties = t;
-    }
-    // waves own runs of the row: which tie is the last, sums, then the token
-    const int seg = (V + kSampleWaves * 64 - 1) / (kSampleWaves * 64) * 64, w0 = min(wave * seg, V), w1 = min(w0 + seg, V);
-    unsigned n = 0;
-    for (int i = w0 + lane; i < w1; i += 64) n += order_key(logit<T>(row, i)) == cut_key;
-    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-    __syncthreads();
-    if (lane == 0) s_wc[wave] = n;
-    __syncthreads();
-    unsigned ties_before = 0;
-    for (int w = 0; w < wave; ++w) ties_before += s_wc[w];
+    // kept weights; each wave's sum, then the token in the wave that the drawn weight falls to
+    const float cut_x = cut ? logit_of(cut) : -INFINITY;
+    const int cut_i = cut ? index_of(cut) : 0;
     u64 mass = 0;
-    unsigned kept = 0, seen = ties_before;
-    auto weigh = [&](int i, unsigned &run) -> unsigned {    // the kept weight of lane's token, ~0u where not kept
-        const float x = i < w1 ? logit<T>(row, i) : -INFINITY;
-        const unsigned k = i < w1 ? order_key(x) : 0;
-        const u64 tie = __ballot(i < w1 && k == cut_key);
-        const unsigned rank = run + __popcll(tie & ((1ull << lane) - 1));
-        run += __popcll(tie);
-        const bool in = i < w1 && (k > cut_key || (k == cut_key && rank < cut_ties));
-        const unsigned w = in ? f.weight(x) : 0;
-        return in && (w >= least || i == top_at) ? w : ~0u;
-    };
-    for (int i0 = w0; i0 < w1; i0 += 64) {
-        const unsigned w = weigh(i0 + lane, seen);
-        if (w != ~0u) mass += w, ++kept;
-    }
-    for (int d = 32; d; d >>= 1) mass += __shfl_xor(mass, d), kept += __shfl_xor(kept, d);
-    __syncthreads();
-    if (lane == 0) s_wm[wave] = mass, s_wc[wave] = kept;
+    unsigned kept = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (e < n) {
+            const bool in = w[e] && w[e] >= rule.least && (x[e] > cut_x || (x[e] == cut_x && base + e * 64 <= cut_i));
+            w[e] = in ? w[e] : 0;
+            mass += w[e], kept += in;
+        }
+    mass = wave_sum(mass), kept = wave_sum(kept);
+    __syncthreads();                         // wave_mass may still be read
+    if (lane == 0) s.wave_mass[wave] = mass, s.wave_count[wave] = kept;
     __syncthreads();
     u64 total = 0, lead = 0;
     unsigned all = 0;
-    for (int w = 0; w < kSampleWaves; ++w) {
-        if (w < wave) lead += s_wm[w];
-        total += s_wm[w], all += s_wc[w];
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+        if (v < wave) lead += s.wave_mass[v];
+        total += s.wave_mass[v], all += s.wave_count[v];
     }
-    u64 U = (u64)(fminf(fmaxf(a.u[b], 0.0f), 1.0f) * 2147483648.0f);
-    if (U > 0x7FFFFFFFull) U = 0x7FFFFFFFull;
-    const u64 t = share(total, U);
-    if (lead > t || lead + s_wm[wave] <= t) return;         // another wave's run has the token
-    seen = ties_before;
-    for (int i0 = w0; i0 < w1; i0 += 64) {
-        const unsigned w = weigh(i0 + lane, seen);
-        const u64 run = wave_scan((u64)(w == ~0u ? 0 : w));
-        const u64 hit = __ballot(lead + run > t);
-        if (hit) {
-            const int at = __ffsll(hit) - 1;
-            if (lane == at) {
-                a.token[b] = i0 + lane;
-                if (a.prob) a.prob[b] = (float)w / (float)total;
-                if (a.kept) a.kept[b] = (int)all;
-            }
-            return;
+    const u64 t = drawn(a, b, total);
+    if (lead > t || lead + mass <= t) return;
+    u64 sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = e < n ? wave_sum((u64)w[e]) : 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (lead <= t && t < lead + sum[e]) {
+            const u64 hit = __ballot(lead + wave_scan((u64)w[e]) > t);
+            if (lane == __ffsll(hit) - 1) answer(a, b, base + e * 64, w[e], total, all);
         }
-        lead += __shfl(run, 63);
+        lead += sum[e];
+    }
+}
+
+// ---- rows too long for one workgroup's registers ----
+//
+// Three launches over chunks of rows: the largest logit of each chunk; the bins' sums of each chunk, which the row's last
+// chunk to arrive adds up and names the bins to list from; the kept weight of each chunk's 16 runs with the listed
+// tokens beside, from which the row's last chunk finds the cut, the run and the token.
+
+constexpr int kSplitThreads = 1024, kSplitBins = 1024, kSplitCap = kSplitThreads, kRuns = kSplitThreads / 64, kMaxChunks = 32;
+
+// What is listed of a row: the tokens of the bins first .. last, and of bin_k.
+struct RowPick {
+    int first, last, bin_k, n;
+    u64 total, mass_first, mass_k;  // weight of the row; before first; before bin_k less what first .. last hold
+    unsigned count_k, unused;       // tokens before bin_k, likewise
+};
+
+struct SplitRows {
+    float *chunk_max;               // [rows][chunks]
+    u64 *hist;                      // [rows][chunks][kSplitBins] (count, weight)
+    RowPick *pick;                  // [rows]
+    u64 *run_mass;                  // [rows][chunks * kRuns]
+    u64 *list_rank;                 // [rows][kSplitCap]
+    unsigned *run_kept;
+    int *arrived_hist, *arrived_pick, *listed;       // [rows], zero between calls
+    int row0, chunks, per;          // first row of this launch; tokens of a run: 64 per
+};
+
+template <class V>
+__device__ inline void put_shared(V *p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <class V>
+__device__ inline V get_shared(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether this workgroup is the last of `of` to get here; what each had put_shared before is then seen by it.
+__device__ inline bool last_to_arrive(int *counter, int of, int *s_flag) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *s_flag = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1;
+        if (*s_flag) put_shared(counter, 0);
+    }
+    __syncthreads();
+    return *s_flag;
+}
+
+// kBatch logits, step apart, from memory together: -inf at and behind `end`.
+constexpr int kBatch = 8;
+template <class T>
+__device__ inline void load_batch(const typename T::Raw *row, int i, int step, int end, float (&x)[kBatch]) {
+    typename T::Raw raw[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) raw[e] = row[min(i + e * step, end - 1)];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+        x[e] = T::get(raw[e]);
+        if (x[e] != x[e] || i + e * step >= end) x[e] = -INFINITY;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kSplitThreads) void sample_max_kernel(pk_sample_desc a, SplitRows w) {
+    __shared__ float s_max[kRuns];
+    const int tid = threadIdx.x, chunk = blockIdx.x % w.chunks, r = blockIdx.x / w.chunks;
+    const auto *row = (const typename T::Raw *)a.logits + (int64_t)(w.row0 + r) * a.logits_row;
+    const int size = w.per * kSplitThreads, i0 = chunk * size, i1 = min(i0 + size, a.vocab);
+    float top = -INFINITY;
+    for (int i = i0 + tid; i < i1; i += kBatch * kSplitThreads) {
+        float x[kBatch];
+        load_batch<T>(row, i, kSplitThreads, i1, x);
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) top = fmaxf(top, x[e]);
+    }
+    top = wave_max(top);
+    if ((tid & 63) == 0) s_max[tid >> 6] = top;
+    __syncthreads();
+    if (tid < 64) {
+        top = wave_max(s_max[tid % kRuns]);
+        if (tid == 0) w.chunk_max[r * w.chunks + chunk] = top;
+    }
+}
+
+__device__ inline float row_max(const SplitRows &w, int r) {
+    float top = w.chunk_max[r * w.chunks];
+    for (int c = 1; c < w.chunks; ++c) top = fmaxf(top, w.chunk_max[r * w.chunks + c]);
+    return top;
+}
+
+template <class T>
+__global__ __launch_bounds__(kSplitThreads, 8) void sample_hist_kernel(pk_sample_desc a, SplitRows w) {
+    static_assert(kSplitBins == kSplitThreads, "a bin a thread");
+    __shared__ CutScratch<kSplitThreads, kSplitBins> s;
+    __shared__ int s_flag;
+    const int tid = threadIdx.x, chunk = blockIdx.x % w.chunks, r = blockIdx.x / w.chunks;
+    const auto *row = (const typename T::Raw *)a.logits + (int64_t)(w.row0 + r) * a.logits_row;
+    const int size = w.per * kSplitThreads, i0 = chunk * size, i1 = min(i0 + size, a.vocab);
+    float x[kBatch];
+    load_batch<T>(row, i0 + tid, kSplitThreads, i1, x);       // on its way while the settings are read
+    RowRule rule;
+    rule.settings(a, w.row0 + r);
+    rule.top = row_max(w, r);
+    s.clear();
+    if ((!rule.k_on && !rule.p_on) || rule.top == -INFINITY) return;
+    __syncthreads();
+    for (int i = i0 + tid;;) {
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            const unsigned wt = rule.weight(x[e]);
+            if (wt) atomicAdd(&s.mass[rule.bin<kSplitBins>(x[e])], (1ull << kCountShift) | wt);
+        }
+        i += kBatch * kSplitThreads;
+        if (i - tid >= i1) break;
+        load_batch<T>(row, i, kSplitThreads, i1, x);
+    }
+    __syncthreads();
+    u64 *hist = w.hist + (int64_t)r * w.chunks * kSplitBins;
+    put_shared(&hist[(int64_t)chunk * kSplitBins + tid], s.mass[tid]);
+    if (!last_to_arrive(&w.arrived_hist[r], w.chunks, &s_flag)) return;
+
+    // two bins of every other chunk a thread, so that all loads are on their way together
+    const int pair = tid & 511, half = tid >> 9;
+    u64 m2[2] = {0, 0};
+    unsigned c2[2] = {0, 0};
+#pragma unroll 8
+    for (int c = half; c < w.chunks; c += 2) {
+        const u4 v = load_shared4((const unsigned *)hist, 2 * (c * kSplitBins + 2 * pair));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const u64 both = (u64)v[2 * i + 1] << 32 | v[2 * i];
+            m2[i] += both & kMassMask, c2[i] += (unsigned)(both >> kCountShift);
+        }
+    }
+    __syncthreads();
+    if (half)
+        for (int i = 0; i < 2; ++i) s.mass[2 * pair + i] = m2[i], s.count[2 * pair + i] = c2[i];
+    __syncthreads();
+    if (!half)
+        for (int i = 0; i < 2; ++i) s.mass[2 * pair + i] += m2[i], s.count[2 * pair + i] += c2[i];
+    __syncthreads();
+    u64 mass[1] = {s.mass[tid]};
+    unsigned count[1] = {s.count[tid]};
+    s.scan(mass, count);
+    auto mass_to = [&](int bin) { return s.mass_to(bin); };
+    auto count_to = [&](int bin) { return s.count_to(bin); };
+    RowPick p{kSplitBins, kSplitBins - 1, -1, 0, 0, 0, 0, 0, 0};
+    u64 low = s.mass[kSplitBins - 1], high = low;          // between which the kept total after top_k lies
+    if (rule.k_on) {
+        p.bin_k = s.reach(0, (u64)rule.k);
+        if (p.bin_k >= 0) p.first = p.last = p.bin_k, low = mass_to(p.bin_k - 1), high = mass_to(p.bin_k);
+    }
+    if (rule.p_on) {
+        const u64 need_low = share(low, rule.p), need_high = share(high, rule.p);
+        const int b0 = s.reach(1, need_low ? need_low : 1);
+        __syncthreads();                                    // b0 is read by all before it is written again
+        const int b1 = s.reach(1, need_high ? need_high : 1);
+        p.first = p.bin_k >= 0 ? min(b0, p.bin_k) : b0, p.last = p.bin_k >= 0 ? min(b1, p.bin_k) : b1;
+    }
+    if (p.first < kSplitBins && count_to(max(p.last, p.bin_k)) <= kWholeMost) p.first = 0, p.last = max(p.last, p.bin_k);     // all that may be kept
+    if (tid == 0) {
+        const unsigned ranged = count_to(p.last) - count_to(p.first - 1);
+        const bool apart = p.bin_k > p.last;
+        p.total = s.mass[kSplitBins - 1], p.mass_first = mass_to(p.first - 1);
+        if (p.bin_k >= 0) {
+            p.mass_k = mass_to(p.bin_k - 1) - (apart ? mass_to(p.last) - p.mass_first : 0);
+            p.count_k = count_to(p.bin_k - 1) - (apart ? ranged : 0);
+            if (!apart) p.mass_k = p.mass_first, p.count_k = count_to(p.first - 1);
+        }
+        p.n = (int)(ranged + (apart ? count_to(p.bin_k) - count_to(p.bin_k - 1) : 0));
+        w.pick[r] = p;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample_desc a, SplitRows w) {
+    __shared__ CutScratch<kSplitThreads, kSplitBins> s;
+    __shared__ u64 s_run[kMaxChunks * kRuns], s_row[kMaxChunks];
+    __shared__ int s_flag, s_at;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunk = blockIdx.x % w.chunks, r = blockIdx.x / w.chunks, b = w.row0 + r, V = a.vocab, runs = w.chunks * kRuns;
+    const auto *row = (const typename T::Raw *)a.logits + (int64_t)b * a.logits_row;
+    const int run = chunk * kRuns + wave, run_size = 64 * w.per;
+    const int from = run * run_size + lane, end = min((run + 1) * run_size, V);
+    float x[kBatch];
+    if (from - lane < end) load_batch<T>(row, from, 64, end, x);      // on its way while the settings are read
+    RowPick p = w.pick[r];
+    RowRule rule;
+    rule.settings(a, b);
+    rule.top = row_max(w, r);
+    if (rule.top == -INFINITY) {
+        if (chunk == 0 && tid == 0) answer(a, b, -1, 0, 0, 0);
+        return;
+    }
+    if (!rule.k_on && !rule.p_on) p = RowPick{kSplitBins, kSplitBins - 1, -1, 0, 0, 0, 0, 0, 0};
+    const bool crowded = p.n > kSplitCap;
+    if (!crowded) {
+        if (tid == 0) s.n[0] = 0;
+        __syncthreads();
+        // this wave's run: what lies in the bins before the listed ones is kept whatever the cut
+        u64 mass = 0;
+        unsigned kept = 0;
+        for (int i0 = from; i0 - lane < end; i0 += 64 * kBatch) {
+            if (i0 != from) load_batch<T>(row, i0, 64, end, x);
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int bin = rule.bin<kSplitBins>(x[e]);
+                if (bin > p.last && bin != p.bin_k) continue;      // most tokens: no weight is worked out
+                const unsigned wt = rule.weight(x[e]);
+                if (wt && bin < p.first) {
+                    if (wt >= rule.least) mass += wt, ++kept;
+                } else if (wt) {
+                    const int at = atomicAdd(&s.n[0], 1);
+                    if (at < kSplitCap) s.list[at] = rank_of(x[e], i0 + e * 64);
+                }
+            }
+        }
+        mass = wave_sum(mass), kept = wave_sum(kept);
+        if (lane == 0) put_shared(&w.run_mass[(int64_t)r * runs + run], mass), put_shared(&w.run_kept[(int64_t)r * runs + run], kept);
+        // the chunk's listed tokens, behind those of the chunks that came before it
+        __syncthreads();
+        const int n = min(s.n[0], kSplitCap);
+        if (tid == 0 && n) s_at = __hip_atomic_fetch_add(&w.listed[r], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        for (int j = tid; j < n; j += kSplitThreads) {
+            const int at = s_at + j;
+            if (at < kSplitCap) put_shared(&w.list_rank[(int64_t)r * kSplitCap + at], s.list[j]);
+        }
+    }
+    if (!last_to_arrive(&w.arrived_pick[r], w.chunks, &s_flag)) return;
+
+    u64 cut = 0;
+    unsigned kept = 0;
+    if (!crowded) {
+        const int n = p.n;
+        if (tid < n) s.list[tid] = get_shared(&w.list_rank[(int64_t)r * kSplitCap + tid]);
+        if (tid < runs) {
+            s_run[tid] = get_shared(&w.run_mass[(int64_t)r * runs + tid]);
+            kept = get_shared(&w.run_kept[(int64_t)r * runs + tid]);
+        }
+        if (tid == 0) put_shared(&w.listed[r], 0);
+        __syncthreads();
+        if (n) {
+            s.sort(n, rule);
+            u64 total = p.total;
+            int left = n;                    // of the list
+            if (p.bin_k >= 0) left = rule.k - (int)p.count_k, total = p.mass_k + s.list_mass[left - 1];
+            if (rule.p_on) {
+                const u64 need = share(total, rule.p);
+                left = min(left, s.place(n, p.mass_first, need ? need : 1) + 1);
+            }
+            if (p.first == 0 && left <= kWholeMost) {
+                answer_from_list(s, a, b, rule, left);
+                return;
+            }
+            cut = s.list[left - 1];
+            if (tid < left) {
+                const unsigned wt = s.list_w[tid];
+                if (wt >= rule.least) atomicAdd(&s_run[index_of(s.list[tid]) / run_size], (u64)wt), ++kept;
+            }
+        }
+    } else {
+        // more tokens at the cut than the list holds: this workgroup goes over the row by itself
+        auto each = [&](auto f) {
+            for (int i = tid; i < V; i += kSplitThreads) {
+                const float x = logit<T>(row, i);
+                const unsigned wt = rule.weight(x);
+                if (wt) f(rank_of(x, i), wt);
+            }
+        };
+        u64 total = p.total;
+        if (p.bin_k >= 0) {
+            const Cut c = cut_by_digits(s, 0, (u64)rule.k, each);
+            cut = c.rank, total = c.mass;
+        }
+        if (rule.p_on) {
+            const u64 need = share(total, rule.p);
+            const Cut c = cut_by_digits(s, 1, need ? need : 1, each);
+            cut = cut > c.rank ? cut : c.rank;
+        }
+        for (int q = wave; q < runs; q += kRuns) {
+            u64 mass = 0;
+            for (int e = 0; e < w.per; ++e) {
+                const int i = q * run_size + e * 64 + lane;
+                if (i >= V) break;
+                const float x = logit<T>(row, i);
+                const unsigned wt = rule.weight(x);
+                if (wt && wt >= rule.least && rank_of(x, i) >= cut) mass += wt, ++kept;
+            }
+            mass = wave_sum(mass);
+            if (lane == 0) s_run[q] = mass;
+        }
+    }
+    kept = wave_sum(kept);
+    if (lane == 0) s.wave_count[wave] = kept;
+    __syncthreads();
+    // running sums over the runs (at most 512: the first waves), then the one in which the drawn weight falls
+    {
+        u64 m = tid < runs ? s_run[tid] : 0;
+        const u64 im = wave_scan(m);
+        if (lane == 63) s.wave_mass[wave] = im;
+        __syncthreads();
+        u64 before = im - m, total = 0;
+        for (int v = 0; v < kRuns; ++v) {
+            if (v < wave) before += s.wave_mass[v];
+            total += s.wave_mass[v];
+        }
+        const u64 t = drawn(a, b, total);
+        if (tid < runs && before <= t && t < before + m) s.bin[0] = tid, s.digit_at[0] = before;
+        __syncthreads();
+        const int q = s.bin[0];
+        const u64 lead = s.digit_at[0];
+        unsigned all = 0;
+        for (int v = 0; v < kRuns; ++v) all += s.wave_count[v];
+        // its rows of 64 tokens, two a wave at most
+        unsigned wt[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = wave + h * kRuns, i = q * run_size + e * 64 + lane;
+            wt[h] = 0;
+            if (e < w.per && i < V) {
+                const float x = logit<T>(row, i);
+                const unsigned v = rule.weight(x);
+                if (v && v >= rule.least && rank_of(x, i) >= cut) wt[h] = v;
+            }
+            const u64 sum = wave_sum((u64)wt[h]);
+            if (lane == 0 && e < w.per) s_row[e] = sum;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = wave + h * kRuns;
+            if (e >= w.per) break;
+            u64 at = lead;
+            for (int v = 0; v < e; ++v) at += s_row[v];
+            if (at > t || at + s_row[e] <= t) continue;
+            const u64 hit = __ballot(at + wave_scan((u64)wt[h]) > t);
+            if (lane == __ffsll(hit) - 1) answer(a, b, q * run_size + e * 64 + lane, wt[h], total, all);
+        }
     }
 }
 

@@ -121,6 +121,64 @@ int attend_check(const pk_kv4_attend_desc *d) {
     return PK_OK;
 }
 
+// Sampling.  A row of up to kRowVocab logits is one workgroup's, its tokens in registers; longer rows are cut in chunks.
+constexpr int kRowVocab = 16384, kSplitRowsMost = 512, kSplitGroups = 2048;
+
+struct SampleShape {
+    int per, chunks, rows;       // tokens a thread takes of a chunk, chunks of a row, rows of a launch
+    // counters first, the same place for every shape: they are zero between calls
+    static constexpr int64_t kCounterBytes = 3 * kSplitRowsMost * 4;
+    int64_t max_at, hist_at, pick_at, run_mass_at, list_rank_at, run_kept_at, bytes;
+};
+
+SampleShape sample_shape(int rows, int vocab) {
+    SampleShape s{};
+    if (vocab <= kRowVocab) return s;
+    // about 16 chunks a row: fewer leave one session's row on few workgroups, more are slow to add up
+    s.per = std::min(std::max((vocab + 16 * kSplitThreads - 1) / (16 * kSplitThreads), 4), kMaxChunks);
+    s.chunks = (vocab + s.per * kSplitThreads - 1) / (s.per * kSplitThreads);
+    s.rows = std::min({rows, kSplitRowsMost, std::max(kSplitGroups / s.chunks, 1)});
+    int64_t at = SampleShape::kCounterBytes;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const int64_t n = s.rows, runs = (int64_t)s.chunks * kRuns;
+    s.max_at = take(n * s.chunks * 4);
+    s.hist_at = take(n * s.chunks * kSplitBins * 8);
+    s.pick_at = take(n * sizeof(RowPick));
+    s.run_mass_at = take(n * runs * 8);
+    s.list_rank_at = take(n * kSplitCap * 8);
+    s.run_kept_at = take(n * runs * 4);
+    s.bytes = at;
+    return s;
+}
+
+template <class T>
+void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s) {
+    const unsigned rows = (unsigned)d.rows;
+    if (d.vocab <= 1024) sample_row_kernel<T, 256, 4><<<rows, 256, 0, s>>>(d);
+    else if (d.vocab <= 2048) sample_row_kernel<T, 256, 8><<<rows, 256, 0, s>>>(d);
+    else if (d.vocab <= 4096) sample_row_kernel<T, 1024, 4><<<rows, 1024, 0, s>>>(d);
+    else if (d.vocab <= kRowVocab) sample_row_kernel<T, 1024, 16><<<rows, 1024, 0, s>>>(d);
+    else {
+        char *w = (char *)d.workspace;
+        SplitRows p;
+        p.arrived_hist = (int *)w, p.arrived_pick = p.arrived_hist + kSplitRowsMost, p.listed = p.arrived_pick + kSplitRowsMost;
+        p.chunk_max = (float *)(w + sh.max_at), p.hist = (u64 *)(w + sh.hist_at), p.pick = (RowPick *)(w + sh.pick_at);
+        p.run_mass = (u64 *)(w + sh.run_mass_at), p.list_rank = (u64 *)(w + sh.list_rank_at);
+        p.run_kept = (unsigned *)(w + sh.run_kept_at);
+        p.chunks = sh.chunks, p.per = sh.per;
+        for (p.row0 = 0; p.row0 < d.rows; p.row0 += sh.rows) {
+            const unsigned grid = (unsigned)(std::min(sh.rows, d.rows - p.row0) * sh.chunks);
+            sample_max_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
+            if (d.temperature || d.top_k || d.top_p) sample_hist_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
+            sample_pick_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
+        }
+    }
+}
+
 template <class T>
 void launch_attend(const AttendParams &p, int dim, unsigned grid, hipStream_t s) {
     if (dim == 64) attend_kernel<T, 64><<<grid, kAttendThreads, 0, s>>>(p);
@@ -208,29 +266,38 @@ PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
     return launched(what);
 }
 
+static int sample_check(const char *what, const pk_sample_desc *d) {
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (d->rows < 0 || d->vocab <= 0 || d->vocab > PK_LM_MAX_VOCAB)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d logits (1 .. %d)", what, d->rows, d->vocab, PK_LM_MAX_VOCAB);
+    return PK_OK;
+}
+
 PK_API int pk_sample_workspace(const pk_sample_desc *d, int64_t *bytes) {
     pk_fail_clear();
-    if (!d || !bytes) return pk_fail(PK_ERR_ARG, "pk_sample_workspace: no descriptor or result");
-    *bytes = 0;
+    if (int rc = sample_check("pk_sample_workspace", d)) return rc;
+    if (!bytes) return pk_fail(PK_ERR_ARG, "pk_sample_workspace: NULL result");
+    *bytes = sample_shape(d->rows, d->vocab).bytes;
     return PK_OK;
 }
 
 PK_API int pk_sample(const pk_sample_desc *d, void *stream) {
     pk_fail_clear();
     const char *what = "pk_sample";
-    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
-    if (d->rows < 0 || d->vocab <= 0 || d->vocab > PK_LM_MAX_VOCAB)
-        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d logits (1 .. %d)", what, d->rows, d->vocab, PK_LM_MAX_VOCAB);
+    if (int rc = sample_check(what, d)) return rc;
     if (d->rows == 0) return PK_OK;
     if (!d->logits || !d->u || !d->token) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
     if (d->dtype != PK_DTYPE_F32 && d->dtype != PK_DTYPE_F16 && d->dtype != PK_DTYPE_BF16)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
     if (!aligned(d->logits, d->dtype == PK_DTYPE_F32 ? 4 : 2)) return pk_fail(PK_ERR_ARG, "%s: logits not aligned to their type", what);
+    const SampleShape sh = sample_shape(d->rows, d->vocab);
+    if (sh.bytes > 0 && (!d->workspace || !aligned(d->workspace, 16) || d->workspace_bytes < sh.bytes))
+        return pk_fail(PK_ERR_ARG, "%s: a workspace of %lld bytes is wanted, aligned to 16 (%lld given)", what, (long long)sh.bytes,
+                       (long long)(d->workspace ? d->workspace_bytes : 0));
     const hipStream_t s = (hipStream_t)stream;
-    const unsigned grid = (unsigned)d->rows;
-    if (d->dtype == PK_DTYPE_F32) sample_kernel<F32><<<grid, kSampleThreads, 0, s>>>(*d);
-    else if (d->dtype == PK_DTYPE_F16) sample_kernel<F16><<<grid, kSampleThreads, 0, s>>>(*d);
-    else sample_kernel<BF16><<<grid, kSampleThreads, 0, s>>>(*d);
+    if (d->dtype == PK_DTYPE_F32) launch_sample<F32>(*d, sh, s);
+    else if (d->dtype == PK_DTYPE_F16) launch_sample<F16>(*d, sh, s);
+    else launch_sample<BF16>(*d, sh, s);
     return launched(what);
 }
 
