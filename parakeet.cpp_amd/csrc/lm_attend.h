@@ -267,6 +267,49 @@ struct Softmax {
     }
 };
 
+// Splits meet in memory: whether this workgroup is the last of its tile to arrive, and joins them.
+__device__ inline bool last_split(const AttendParams &a, int64_t at, int mine, int *s_last) {
+    __builtin_amdgcn_s_waitcnt(0);        // this thread's sums have landed
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *s_last = __hip_atomic_fetch_add(&a.arrived[at], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mine - 1;
+        if (*s_last) __hip_atomic_store(&a.arrived[at], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return *s_last;
+}
+
+// all: [splits][Cols][D sums, maximum, total, 2 unused]; finish(column, quad, sums of its 4 channels, maximum, total)
+template <int D, int Cols, int Threads, class Finish>
+__device__ inline void join_splits(const float *all, int live, int mine, float to_log2, Finish finish) {
+    constexpr int kQuads = D / 4, kRow = D + 4;
+    for (int u = threadIdx.x; u < live * kQuads; u += Threads) {
+        const int col = u / kQuads, quad = u % kQuads;
+        v4f o = {0, 0, 0, 0};
+        float top = -INFINITY, total = 0;
+        // batches of 8 splits, their loads together
+        for (int i0 = 0; i0 < mine; i0 += 8) {
+            v4f x[8], ml[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned p = (min(i0 + i, mine - 1) * Cols + col) * kRow;
+                x[i] = load_shared(all, p + 4 * quad), ml[i] = load_shared(all, p + D);
+            }
+            float t2 = top;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t2 = fmaxf(t2, ml[i][0]);
+            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - t2) * to_log2);
+            o *= keep, total *= keep, top = t2;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = t2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((ml[i][0] - t2) * to_log2);
+                if (i0 + i < mine) o += x[i] * w, total += ml[i][1] * w;
+            }
+        }
+        finish(col, quad, o, top, total);
+    }
+}
+
 // One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.
 template <class T, int D>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kernel(AttendParams a) {
@@ -402,42 +445,366 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
             if (quad == 0) store_shared(all, p + D, v4f{top, total, 0, 0});
         }
     }
-    if (mine == 1) return;
+    if (mine == 1 || !last_split(a, at, mine, &s_last)) return;
+    join_splits<D, 16, kAttendThreads>(all, live, mine, to_log2, finish);
+}
 
-    // splits meet in memory; the last to arrive joins them
-    __builtin_amdgcn_s_waitcnt(0);        // this thread's sums have landed
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s_last = __hip_atomic_fetch_add(&a.arrived[at], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mine - 1;
-        if (s_last) __hip_atomic_store(&a.arrived[at], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// ---- many query rows: prompts ----
+//
+// A workgroup takes 128 columns, a wave 32 of them, and goes over the keys 64 at a time.  K's and V's values are
+// unpacked to bf16 once for the four waves, into LDS, two buffers deep: the next 64 keys' bytes are on their way from
+// memory while these are worked on.  v_mfma_f32_32x32x16_bf16: a lane holds 16 scores of 32 keys of its own column, so
+// the maximum crosses lanes once per 64 keys; row 8b + 4h + i of a score tile stands for key 16 (b / 2) + 8h + 4 (b % 2) + i,
+// which makes a lane's scores its own operand of O^T as above.  V lies transposed, row 16j + r holding channel
+// (D/16) r + j: rows that 16 lanes write together are adjacent.
+
+constexpr int kPromptThreads = 256, kPromptCols = 128, kPromptKeys = 64;
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ inline v16f mfma32(u4 a, u4 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+// One thread's share of 64 keys' bytes: of K a quarter of a key's channels, of V half the channels of an entry of 8 keys.
+template <int D>
+struct PromptBytes {
+    unsigned k[D / 32], v[8], ks;
+    u2 vs;
+
+    __device__ void load(const AttendParams &a, const Record &rec, int64_t head_at, int kb, int kid, int vid) {
+        const int t = threadIdx.x, kkey = kb + (t >> 2), quarter = t & 3;
+        const int vkey = kb + (t >> 5) * 8, r = (t >> 1) & 15, half = t & 1;
+        const uint8_t *krec = a.cache + max(kid, 0) * a.page_stride + head_at, *vrec = a.cache + max(vid, 0) * a.page_stride + head_at;
+        const int koff = kkey & (a.page - 1), voff = vkey & (a.page - 1);
+        const uint8_t *code = krec + koff * (D / 2) + quarter * (D / 8);
+        if (D == 64) *(u2 *)k = *(const u2 *)code;
+        else
+#pragma unroll
+            for (int i = 0; i < D / 128; ++i) *(u4 *)&k[4 * i] = *(const u4 *)(code + 16 * i);
+        const uint8_t *sc = krec + rec.k_scales() + koff * (D / 32) + quarter * (D / 4) / 32;
+        ks = D == 256 ? *(const uint16_t *)sc : *sc;
+        const uint8_t *vcode = vrec + rec.v_codes() + (voff >> 3) * (4 * D) + r * (D / 4);
+        if (D == 64) {
+            const u4 w = *(const u4 *)vcode;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[2 * i] = w[i] >> (8 * half), v[2 * i + 1] = w[i] >> (16 + 8 * half);
+        } else if (D == 128) {
+            *(u4 *)&v[0] = *(const u4 *)vcode, *(u4 *)&v[4] = *(const u4 *)(vcode + 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = *(const unsigned *)(vcode + 8 * i + 4 * half);
+        }
+        vs = *(const u2 *)(vrec + rec.v_scales() + (r * (D / 16) / 32) * a.page + voff);
     }
-    __syncthreads();
-    if (!s_last) return;
-    for (int u = threadIdx.x; u < live * kQuads; u += kAttendThreads) {
-        const int col = u / kQuads, quad = u % kQuads;
-        v4f o = {0, 0, 0, 0};
-        float top = -INFINITY, total = 0;
-        // batches of 8 splits, their loads together
-        for (int i0 = 0; i0 < mine; i0 += 8) {
-            v4f x[8], ml[8];
+};
+
+template <int D>
+struct alignas(16) PromptTile {
+    static constexpr int kKRow = D * 2 + 16, kVRow = kPromptKeys * 2 + 16;     // bytes; the pads spread rows over banks
+    uint8_t k[kPromptKeys * kKRow], v[D * kVRow];
+
+    uint8_t nan[kPromptKeys][D / 32];       // of an edge tile: blocks of V that are NaN
+
+    // What lies at keys without a page may be anything; so at an edge, where some column does not see some key, at keys
+    // outside [lo, hi), which no column sees.  NaN blocks of the others are taken out there and marked.
+    __device__ void stage(const PromptBytes<D> &x, int kb, bool edge, bool vfine, int lo, int hi) {
+        const int t = threadIdx.x, key = t >> 2, quarter = t & 3;
+        uint8_t *krow = k + key * kKRow + quarter * (D / 2);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned p = (min(i0 + i, mine - 1) * 16 + col) * kRow;
-                x[i] = load_shared(all, p + 4 * quad), ml[i] = load_shared(all, p + D);
-            }
-            float t2 = top;
+        for (int w = 0; w < D / 32; ++w) {
+            const unsigned sb = D == 256 ? x.ks >> (8 * (w / 4)) & 255u : x.ks;
+            *(u4 *)(krow + 16 * w) = unpack8(x.k[w], __uint_as_float(sb << 23));
+        }
+        const int a8 = t >> 5, r = (t >> 1) & 15, half = t & 1;
+        u2 vs = x.vs;
+        if (edge || !vfine) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t2 = fmaxf(t2, ml[i][0]);
-            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - t2) * to_log2);
-            o *= keep, total *= keep, top = t2;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = t2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((ml[i][0] - t2) * to_log2);
-                if (i0 + i < mine) o += x[i] * w, total += ml[i][1] * w;
+            for (int j = 0; j < 8; ++j) {
+                const int at = 8 * (j & 3), kj = kb + 8 * a8 + j;
+                const bool dead = !vfine || kj >= hi || kj < lo, bad = (vs[j >> 2] >> at & 255u) == 255u;
+                if (edge) nan[8 * a8 + j][r * (D / 16) / 32] = bad && !dead;     // by all threads of the block alike
+                if (bad || dead) vs[j >> 2] = (vs[j >> 2] & ~(255u << at)) | 127u << at;
             }
         }
-        finish(col, quad, o, top, total);
+        float scale[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) scale[j] = __uint_as_float((vs[j >> 2] >> (8 * (j & 3)) & 255u) << 23);
+        constexpr int kEach = D / 32;                  // channels of this thread, two a byte
+        auto two = [&](auto sel, int shift) {
+            constexpr int kSel = decltype(sel)::value;
+            u4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bf2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v[2 * j] >> shift, scale[2 * j], kSel);
+                const bf2 q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v[2 * j + 1] >> shift, scale[2 * j + 1], kSel);
+                const unsigned pu = __builtin_bit_cast(unsigned, p), qu = __builtin_bit_cast(unsigned, q);
+                even[j] = __builtin_amdgcn_perm(qu, pu, 0x05040100u);
+                odd[j] = __builtin_amdgcn_perm(qu, pu, 0x07060302u);
+            }
+            const int n = half * kEach + 2 * kSel;
+            *(u4 *)(v + (n * 16 + r) * kVRow + a8 * 16) = even;
+            *(u4 *)(v + ((n + 1) * 16 + r) * kVRow + a8 * 16) = odd;
+        };
+        const int shift = D == 128 ? 16 * half : 0;
+        two(std::integral_constant<int, 0>{}, shift);
+        if constexpr (D >= 128) two(std::integral_constant<int, 1>{}, shift);
+        if constexpr (D == 256) {
+            two(std::integral_constant<int, 2>{}, shift);
+            two(std::integral_constant<int, 3>{}, shift);
+        }
     }
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_prompt_kernel(AttendParams a) {
+    constexpr int Planes = __is_same(T, F16) ? 2 : 1;
+    constexpr int kSteps = D / 16, kTiles = D / 32, kRow = D + 4;
+    using Raw = typename T::Raw;
+    __shared__ PromptTile<D> s_tile[2];
+    __shared__ int s_missing[2], s_last;
+
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, c = lane & 31;
+    // the last tiles of a prompt see the most keys: they go first
+    int id = blockIdx.x;
+    const int hk = id % a.kv_heads;
+    id /= a.kv_heads;
+    const int b = id % a.requests;
+    id /= a.requests;
+    const int split = id % a.splits, tile = a.tiles - 1 - id / a.splits;
+
+    const int f0 = a.first ? a.first[b] : b, f1 = a.first ? a.first[b + 1] : b + 1;
+    const int q0 = max(f0, 0), q1 = min(f1, a.n_rows), rows = (q1 - q0) * a.group, row0 = tile * kPromptCols;
+    if (q1 <= q0 || row0 >= rows) return;
+    const int held = max(min(min(a.lens[b], a.max_len), a.width * a.page), 0);
+    const int place0 = held - (f1 - q0);
+    auto end_of = [&](int r) { return max(place0 + r / a.group + 1, 0); };
+    auto begin_of = [&](int r) { return a.window ? max(place0 + r / a.group + 1 - a.window, 0) : 0; };
+    const int row_last = min(row0 + kPromptCols, rows) - 1;
+    const int hi_min = end_of(row0), hi_max = end_of(row_last), lo_min = begin_of(row0), lo_max = begin_of(row_last);
+    const int start = lo_min & ~(kPromptKeys - 1);
+    const int mine = max((hi_max - start + a.chunk - 1) / a.chunk, 1);
+    if (split >= mine) return;
+    const int k0 = start + split * a.chunk, k1 = min(k0 + a.chunk, hi_max);
+
+    // this wave's columns
+    const int wrow0 = row0 + wave * 32, row = min(wrow0 + c, rows - 1), tok = row / a.group, head = hk * a.group + row % a.group;
+    const int hi = end_of(row), lo = begin_of(row);
+    const int whi_min = end_of(min(wrow0, rows - 1)), whi_max = end_of(min(wrow0 + 31, rows - 1));
+    const int wlo_min = begin_of(min(wrow0, rows - 1)), wlo_max = begin_of(min(wrow0 + 31, rows - 1));
+    u4 q[Planes][kSteps];
+    {
+        const Raw *p = (const Raw *)a.q + (int64_t)(q0 + tok) * a.q_row + head * a.q_head + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+            unsigned short raw[8];
+            if (a.vec) {
+                *(u4 *)raw = *(const u4 *)(p + 16 * ks);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[i] = p[16 * ks + i];
+            }
+            if (a.scale < 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[i] ^= 0x8000;
+            if (Planes == 1) {
+                q[0][ks] = *(u4 *)raw;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = T::get(raw[2 * j]), y = T::get(raw[2 * j + 1]);
+                    const unsigned top = pack_bf16(x, y);
+                    q[0][ks][j] = top;
+                    q[Planes - 1][ks][j] = pack_bf16(x - __uint_as_float(top << 16), y - __uint_as_float(top & 0xFFFF0000u));
+                }
+            }
+        }
+    }
+    const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+
+    const Record rec{a.page, D};
+    const int64_t head_at = hk * rec.bytes();
+    const int *table = a.table + b * a.table_stride;
+    const int last_page = max(held - 1, 0) >> a.page_shift;
+    auto page_of = [&](int key) {
+        const int p = table[min(key >> a.page_shift, last_page)];
+        return (unsigned)p < (unsigned)a.n_pages ? p : -1;
+    };
+
+    v16f acc[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] = 0;
+    float m = -INFINITY, l = 0;
+
+    const int kkey = t >> 2, vkey = (t >> 5) * 8;        // of 64, in this thread's staging
+    auto edge_at = [&](int kb) { return kb + kPromptKeys > hi_min || kb < lo_max; };
+    if (k0 < k1) {
+        PromptBytes<D> bytes;
+        int kid = page_of(k0 + kkey), vid = page_of(k0 + vkey);
+        bytes.load(a, rec, head_at, k0, kid, vid);
+        if (t < 2) s_missing[t] = -1;
+        __syncthreads();
+        if (kid < 0 || vid < 0) s_missing[0] = k0;       // which tile of this buffer lacks a page
+        s_tile[0].stage(bytes, k0, edge_at(k0), vid >= 0, lo_min, hi_max);
+        kid = page_of(k0 + kPromptKeys + kkey), vid = page_of(k0 + kPromptKeys + vkey);
+        __syncthreads();
+        int buf = 0;
+        for (int kb = k0; kb < k1; kb += kPromptKeys, buf ^= 1) {
+            const bool more = kb + kPromptKeys < k1;
+            const bool fine = kid >= 0 && vid >= 0, vfine = vid >= 0;
+            if (more) {
+                bytes.load(a, rec, head_at, kb + kPromptKeys, kid, vid);
+                kid = page_of(kb + 2 * kPromptKeys + kkey), vid = page_of(kb + 2 * kPromptKeys + vkey);
+            }
+
+            if (kb < whi_max && kb + kPromptKeys > wlo_min) {
+                const PromptTile<D> &x = s_tile[buf];
+                v16f s[2];
+                const int krow = 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[u][i] = 0;
+#pragma unroll
+                    for (int ks = 0; ks < kSteps; ++ks) {
+                        const u4 kk = *(const u4 *)(x.k + (32 * u + krow) * PromptTile<D>::kKRow + 32 * ks + 16 * h);
+#pragma unroll
+                        for (int n = 0; n < Planes; ++n) s[u] = mfma32(kk, q[n][ks], s[u]);
+                    }
+                }
+                const bool missing = s_missing[buf] == kb;
+                if (kb + kPromptKeys > whi_min || kb < wlo_max || missing) {
+                    const bool edge = edge_at(kb);
+                    unsigned bad = 0;             // channel blocks whose NaN this column sees
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int at = 32 * (i >> 4) + 16 * (i >> 3 & 1) + 8 * h + (i & 7), key = kb + at;
+                        const bool see = key < hi && key >= lo && !(missing && page_of(key) < 0);
+                        if (!see) s[i >> 4][i & 15] = -INFINITY;
+                        else if (edge)
+#pragma unroll
+                            for (int j = 0; j < D / 32; ++j) bad |= (unsigned)x.nan[at][j] << j;
+                    }
+                    bad |= (unsigned)__shfl_xor((int)bad, 32);
+                    if (__any(bad != 0))
+#pragma unroll
+                        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int r = (8 * (i >> 2) + 4 * h + (i & 3)) & 15;
+                                if (bad >> (r * (D / 16) / 32) & 1) acc[n][i] = __builtin_nanf("");
+                            }
+                }
+                float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+                {
+                    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                    top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+                }
+                // sums are brought to a new maximum only where it has outgrown the old one by 2^6
+                if (__any((top - m) * to_log2 > 6.0f)) {
+                    const float m2 = fmaxf(m, top);
+                    const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - m2) * to_log2);
+                    m = m2;
+                    l *= keep;
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[n][i] *= keep;
+                }
+                const float shift = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        u4 ph, pl;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float e0 = __builtin_amdgcn_exp2f((s[u][8 * g + 2 * j] - shift) * to_log2);
+                            const float e1 = __builtin_amdgcn_exp2f((s[u][8 * g + 2 * j + 1] - shift) * to_log2);
+                            l += e0 + e1;
+                            ph[j] = pack_bf16(e0, e1);
+                            if (Planes == 2) pl[j] = pack_bf16(e0 - __uint_as_float(ph[j] << 16), e1 - __uint_as_float(ph[j] & 0xFFFF0000u));
+                        }
+#pragma unroll
+                        for (int n = 0; n < kTiles; ++n) {
+                            const u4 vv = *(const u4 *)(x.v + (32 * n + c) * PromptTile<D>::kVRow + 64 * u + 32 * g + 16 * h);
+                            acc[n] = mfma32(vv, ph, acc[n]);
+                            if (Planes == 2) acc[n] = mfma32(vv, pl, acc[n]);
+                        }
+                    }
+            }
+            if (more) {
+                const int nb = kb + kPromptKeys;
+                if (!fine) s_missing[buf ^ 1] = nb;
+                s_tile[buf ^ 1].stage(bytes, nb, edge_at(nb), vfine, lo_min, hi_max);
+            }
+            __syncthreads();
+        }
+    }
+    {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const bool live = wrow0 + c < rows;
+    // entry r of D/16 channels from acc[n][8 b + ..]: this lane has the entries 4h + i and 8 + 4h + i
+    auto entry = [&](int half, int i, float (&v)[D / 16]) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) v[2 * n] = acc[n][4 * half + i], v[2 * n + 1] = acc[n][8 + 4 * half + i];
+        return 8 * half + 4 * h + i;
+    };
+    auto lse_of = [&](float top, float total) { return total == 0.0f ? -INFINITY : top * to_log2 * kLn2 + logf(total); };
+    if (mine == 1) {
+        if (!live) return;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        Raw *out = (Raw *)a.out + (int64_t)(q0 + tok) * a.out_row + head * a.out_head;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[D / 16];
+                const int r = entry(half, i, v);
+                alignas(8) Raw w[D / 16];
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) w[j] = T::put(v[j] * inv);
+                Raw *o = out + r * (D / 16);
+                if (a.vec_out)
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) ((u2 *)o)[j] = ((u2 *)w)[j];
+                else
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) o[j] = w[j];
+            }
+        if (a.lse && h == 0) a.lse[(int64_t)(q0 + tok) * a.heads + head] = lse_of(m, l);
+        return;
+    }
+    const int64_t at = ((int64_t)b * a.kv_heads + hk) * a.tiles + tile;
+    float *all = a.part + at * a.splits * kPromptCols * kRow;
+    if (live) {
+        const unsigned p = (split * kPromptCols + wave * 32 + c) * kRow;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[D / 16];
+                const int r = entry(half, i, v);
+#pragma unroll
+                for (int j = 0; j < D / 16; j += 4) store_shared(all, p + r * (D / 16) + j, v4f{v[j], v[j + 1], v[j + 2], v[j + 3]});
+            }
+        if (h == 0) store_shared(all, p + D, v4f{m, l, 0, 0});
+    }
+    if (!last_split(a, at, mine, &s_last)) return;
+    join_splits<D, kPromptCols, kPromptThreads>(all, min(rows - row0, kPromptCols), mine, to_log2, [&](int col, int quad, v4f o, float top, float total) {
+        const int r = row0 + col, tk = r / a.group, hd = hk * a.group + r % a.group;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        Raw *out = (Raw *)a.out + (int64_t)(q0 + tk) * a.out_row + hd * a.out_head + 4 * quad;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = T::put(o[i] * inv);
+        if (a.lse && quad == 0) a.lse[(int64_t)(q0 + tk) * a.heads + hd] = lse_of(top, total);
+    });
 }
 
 }  // namespace pklm

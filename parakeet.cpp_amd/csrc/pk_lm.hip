@@ -82,28 +82,36 @@ int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
 // Arrival counters of the tiles whose keys are split, at the workspace's beginning whatever the call's shape, so that
 // no call's partial sums lie where another's counters are.  A split call has fewer tiles than this (attend_shape).
 constexpr int kCounters = 1024;
+// more query rows of a request and kv head than this go to the prompt kernel
+constexpr int kPromptFrom = 64;
 
 // How a call's work is dealt out, from its host-known sizes alone.
 struct AttendShape {
-    int tiles, chunk, splits;
+    bool prompt;             // attend_prompt_kernel, 128 query rows a workgroup; else attend_kernel, 16
+    int cols, tiles, chunk, splits;
     int64_t part_bytes;
     int64_t bytes() const { return splits > 1 ? kCounters * 4 + part_bytes : 0; }
 };
 
 int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
-    const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads);
-    const int64_t tiles = (rows + 15) / 16, pairs = (int64_t)d.requests * d.kv_heads;
-    // keys of one 16-row tile: its rows span at most 16 tokens
-    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 32) : d.max_len;
-    const int64_t want = kCounters, each = std::max<int64_t>(pairs * tiles, 1);   // split: fewer than kCounters tiles
-    int64_t splits = std::max<int64_t>(std::min<int64_t>(want / each, (keys + 255) / 256), 1);
-    int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + 255) / 256 * 256, 256);
+    const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
+    s.prompt = rows > kPromptFrom;
+    s.cols = s.prompt ? kPromptCols : 16;
+    const int step = s.prompt ? kPromptKeys : 32 * kAttendWaves;
+    const int64_t tiles = (rows + s.cols - 1) / s.cols;
+    // keys of one tile: its rows span at most as many tokens
+    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + s.cols + 64) : d.max_len;
+    // split where the tiles leave the card's 256 CUs short of work (so fewer than kCounters tiles), into no less than
+    // 256 (512) keys
+    const int64_t want = s.prompt ? 512 : kCounters, least = s.prompt ? 512 : 256, each = std::max<int64_t>(pairs * tiles, 1);
+    int64_t splits = std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
+    const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
     if (pairs * tiles * splits > INT32_MAX)
         return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
                        (long long)rows);
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
-    s.part_bytes = pairs * tiles * splits * 16 * (d.head_dim + 4) * 4;
+    s.part_bytes = pairs * tiles * splits * s.cols * (d.head_dim + 4) * 4;
     return PK_OK;
 }
 
@@ -179,11 +187,17 @@ void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s
     }
 }
 
+template <class T, int D>
+void launch_attend(const AttendParams &p, bool prompt, unsigned grid, hipStream_t s) {
+    if (prompt) attend_prompt_kernel<T, D><<<grid, kPromptThreads, 0, s>>>(p);
+    else attend_kernel<T, D><<<grid, kAttendThreads, 0, s>>>(p);
+}
+
 template <class T>
-void launch_attend(const AttendParams &p, int dim, unsigned grid, hipStream_t s) {
-    if (dim == 64) attend_kernel<T, 64><<<grid, kAttendThreads, 0, s>>>(p);
-    else if (dim == 128) attend_kernel<T, 128><<<grid, kAttendThreads, 0, s>>>(p);
-    else attend_kernel<T, 256><<<grid, kAttendThreads, 0, s>>>(p);
+void launch_attend(const AttendParams &p, bool prompt, int dim, unsigned grid, hipStream_t s) {
+    if (dim == 64) launch_attend<T, 64>(p, prompt, grid, s);
+    else if (dim == 128) launch_attend<T, 128>(p, prompt, grid, s);
+    else launch_attend<T, 256>(p, prompt, grid, s);
 }
 
 }  // namespace
@@ -261,8 +275,8 @@ PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
     p.vec = aligned(d->q, 16) && d->q_row % 8 == 0 && d->q_head % 8 == 0;
     p.vec_out = aligned(d->out, 8) && d->out_row % 4 == 0 && d->out_head % 4 == 0;
     const unsigned grid = (unsigned)((int64_t)d->requests * d->kv_heads * sh.tiles * sh.splits);
-    if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, d->head_dim, grid, (hipStream_t)stream);
-    else launch_attend<BF16>(p, d->head_dim, grid, (hipStream_t)stream);
+    if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, sh.prompt, d->head_dim, grid, (hipStream_t)stream);
+    else launch_attend<BF16>(p, sh.prompt, d->head_dim, grid, (hipStream_t)stream);
     return launched(what);
 }
 

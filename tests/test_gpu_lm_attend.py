@@ -135,9 +135,10 @@ def test_scales_and_large_values():
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("D", [64, 128, 256])
-def test_nan_reaches_only_those_that_see_it(dtype, D):
+@pytest.mark.parametrize("news", [(50, 60, 1), (25, 30, 1)])      # many query rows of a request, and few
+def test_nan_reaches_only_those_that_see_it(dtype, D, news):
     """A NaN block of K makes the queries that see its key NaN, one of V its 32 channels; no other query or channel."""
-    p = problem(11, D, 32, 4, 2, [100, 60, 33], [50, 60, 1], dtype)
+    p = problem(11, D, 32, 4, 2, [100, 60, 33], news, dtype)
     page = 32
 
     def poison(b, t, h, part, block):
@@ -151,6 +152,7 @@ def test_nan_reaches_only_those_that_see_it(dtype, D):
     poison(0, 90, 1, "k", 0)
     poison(1, 0, 1, "v", 0)
     poison(1, 59, 0, "v", 1)
+    poison(1, 40, 1, "v", D // 32 - 1)
     out, _ = check(p)
     assert np.isnan(out).any() and not np.isnan(out).all()
     p["cache"][p["table"][2, 1], 0, page * D + page * D // 32 + 1] = 255      # key 33 of request 2: not held
@@ -158,11 +160,12 @@ def test_nan_reaches_only_those_that_see_it(dtype, D):
     check(p, window=9)
     p["q"] = p["q"].copy()
     bad = R.to_dtype(np.array([np.nan, np.inf, -np.inf]), dtype)
-    p["q"][3, 0, 5], p["q"][60, 1, 0], p["q"][70, 2, D - 1] = bad
+    second = news[0] + 10
+    p["q"][1, 0, 5], p["q"][second, 1, 0], p["q"][second + 10, 2, D - 1] = bad
     out, lse = run(p)
-    for i, h in ((3, 0), (60, 1), (70, 2)):
+    for i, h in ((1, 0), (second, 1), (second + 10, 2)):
         assert np.isnan(out[i, h]).all() and np.isnan(lse[i, h])
-    assert not np.isnan(out[4:20]).any()
+    assert not np.isnan(lse[2:news[0] // 4]).any()
 
 
 def test_page_ids_out_of_range_are_skipped():
@@ -172,6 +175,26 @@ def test_page_ids_out_of_range_are_skipped():
     p["table"][0, :7] = -5                     # nothing left to see
     out, lse = check(p)
     assert (out[0] == 0).all() and np.isneginf(lse[0]).all()
+    for D, page in ((64, 16), (128, 32), (128, 64), (256, 16)):
+        p = problem(14, D, page, 4, 2, [300, 90], [80, 90], "bf16")
+        p["table"][0, 1], p["table"][0, 200 // page], p["table"][1, 0] = -1, 1 << 30, len(p["cache"])
+        check(p)
+        check(p, window=70)
+
+
+def test_few_rows_and_many_rows_agree():
+    """The last queries of a prompt in one call and in calls of their own: two kernels, one definition."""
+    for dtype, D in (("bf16", 128), ("f16", 64)):
+        p = problem(17, D, 64, 8, 2, [700], [90], dtype)
+        a, la = check(p)
+        few = dict(p, q=np.ascontiguousarray(p["q"][-5:]), first=np.array([0, 5], np.int32), news=np.array([5], np.int32))
+        b, lb = check(few)
+        assert np.allclose(a[-5:], b, atol=3 * R.UNIT[dtype] * np.abs(a[-5:]).max()) and np.allclose(la[-5:], lb, atol=1e-5)
+
+
+def test_prompts_over_a_long_axis():
+    check(problem(18, 128, 64, 16, 2, [4500, 130], [17, 130], "bf16"))
+    check(problem(19, 64, 32, 8, 8, [3000], [129], "f16"), window=1500)
 
 
 def test_lengths_are_cut_at_max_len_and_table():
