@@ -324,9 +324,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
     int id = blockIdx.x;
     const int hk = id % a.kv_heads;
     id /= a.kv_heads;
-    const int b = id % a.requests;
-    id /= a.requests;
-    const int tile = id % a.tiles, split = id / a.tiles;
+    // Workgroups go round the 8 XCDs and within one round its 4 shader engines, in order: with 8 heads and 4 requests
+    // each engine would get one request alone, and a long one would leave the others idle (measured: a quarter of the
+    // slots in use).  So the requests are turned on by one from tile to tile.
+    const int turn = id / a.requests, b = (id + turn) % a.requests;
+    const int tile = turn % a.tiles, split = turn / a.tiles;
 
     const int f0 = a.first ? a.first[b] : b, f1 = a.first ? a.first[b + 1] : b + 1;
     const int q0 = max(f0, 0), q1 = min(f1, a.n_rows), rows = (q1 - q0) * a.group;
@@ -472,6 +474,17 @@ struct PromptBytes {
     unsigned k[D / 32], v[8], ks;
     u2 vs;
 
+    // What is made of the bytes is made after this point, not before (the compiler would).
+    __device__ void pin() {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(k[i]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(v[i]));
+        unsigned a = vs[0], b = vs[1];
+        asm volatile("" : "+v"(ks), "+v"(a), "+v"(b));
+        vs = u2{a, b};
+    }
+
     __device__ void load(const AttendParams &a, const Record &rec, int64_t head_at, int kb, int kid, int vid) {
         const int t = threadIdx.x, kkey = kb + (t >> 2), quarter = t & 3;
         const int vkey = kb + (t >> 5) * 8, r = (t >> 1) & 15, half = t & 1;
@@ -508,7 +521,19 @@ struct alignas(16) PromptTile {
 
     // What lies at keys without a page may be anything; so at an edge, where some column does not see some key, at keys
     // outside [lo, hi), which no column sees.  NaN blocks of the others are taken out there and marked.
-    __device__ void stage(const PromptBytes<D> &x, int kb, bool edge, bool vfine, int lo, int hi) {
+    __device__ void clean(PromptBytes<D> &x, int kb, bool edge, bool vfine, int lo, int hi) {
+        const int t = threadIdx.x, a8 = t >> 5, r = (t >> 1) & 15;
+        if (edge || !vfine) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = 8 * (j & 3), kj = kb + 8 * a8 + j;
+                const bool dead = !vfine || kj >= hi || kj < lo, bad = (x.vs[j >> 2] >> at & 255u) == 255u;
+                if (edge) nan[8 * a8 + j][r * (D / 16) / 32] = bad && !dead;     // by all threads of the block alike
+                if (bad || dead) x.vs[j >> 2] = (x.vs[j >> 2] & ~(255u << at)) | 127u << at;
+            }
+        }
+    }
+    __device__ void stage(const PromptBytes<D> &x) {
         const int t = threadIdx.x, key = t >> 2, quarter = t & 3;
         uint8_t *krow = k + key * kKRow + quarter * (D / 2);
 #pragma unroll
@@ -517,16 +542,7 @@ struct alignas(16) PromptTile {
             *(u4 *)(krow + 16 * w) = unpack8(x.k[w], __uint_as_float(sb << 23));
         }
         const int a8 = t >> 5, r = (t >> 1) & 15, half = t & 1;
-        u2 vs = x.vs;
-        if (edge || !vfine) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int at = 8 * (j & 3), kj = kb + 8 * a8 + j;
-                const bool dead = !vfine || kj >= hi || kj < lo, bad = (vs[j >> 2] >> at & 255u) == 255u;
-                if (edge) nan[8 * a8 + j][r * (D / 16) / 32] = bad && !dead;     // by all threads of the block alike
-                if (bad || dead) vs[j >> 2] = (vs[j >> 2] & ~(255u << at)) | 127u << at;
-            }
-        }
+        const u2 vs = x.vs;
         float scale[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) scale[j] = __uint_as_float((vs[j >> 2] >> (8 * (j & 3)) & 255u) << 23);
@@ -569,9 +585,8 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
     int id = blockIdx.x;
     const int hk = id % a.kv_heads;
     id /= a.kv_heads;
-    const int b = id % a.requests;
-    id /= a.requests;
-    const int split = id % a.splits, tile = a.tiles - 1 - id / a.splits;
+    const int turn = id / a.requests, b = (id + turn) % a.requests;       // turned on: see attend_kernel
+    const int split = turn % a.splits, tile = a.tiles - 1 - turn / a.splits;
 
     const int f0 = a.first ? a.first[b] : b, f1 = a.first ? a.first[b + 1] : b + 1;
     const int q0 = max(f0, 0), q1 = min(f1, a.n_rows), rows = (q1 - q0) * a.group, row0 = tile * kPromptCols;
@@ -647,33 +662,63 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
         if (t < 2) s_missing[t] = -1;
         __syncthreads();
         if (kid < 0 || vid < 0) s_missing[0] = k0;       // which tile of this buffer lacks a page
-        s_tile[0].stage(bytes, k0, edge_at(k0), vid >= 0, lo_min, hi_max);
+        s_tile[0].clean(bytes, k0, edge_at(k0), vid >= 0, lo_min, hi_max);
+        s_tile[0].stage(bytes);
         kid = page_of(k0 + kPromptKeys + kkey), vid = page_of(k0 + kPromptKeys + vkey);
+        bytes.load(a, rec, head_at, k0 + kPromptKeys, kid, vid);
+        int kid2 = page_of(k0 + 2 * kPromptKeys + kkey), vid2 = page_of(k0 + 2 * kPromptKeys + vkey);
         __syncthreads();
         int buf = 0;
+        // While a tile is worked on, the next one is unpacked (between the products of Q and K, which leave the vector
+        // unit free) and the one after that is on its way from memory; behind the last one the last page is read again.
         for (int kb = k0; kb < k1; kb += kPromptKeys, buf ^= 1) {
-            const bool more = kb + kPromptKeys < k1;
-            const bool fine = kid >= 0 && vid >= 0, vfine = vid >= 0;
-            if (more) {
-                bytes.load(a, rec, head_at, kb + kPromptKeys, kid, vid);
-                kid = page_of(kb + 2 * kPromptKeys + kkey), vid = page_of(kb + 2 * kPromptKeys + vkey);
-            }
-
-            if (kb < whi_max && kb + kPromptKeys > wlo_min) {
-                const PromptTile<D> &x = s_tile[buf];
-                v16f s[2];
+            const int nb = kb + kPromptKeys;
+            PromptTile<D> &next = s_tile[buf ^ 1];
+            if (kid < 0 || vid < 0) s_missing[buf ^ 1] = nb;
+            next.clean(bytes, nb, edge_at(nb), vid >= 0, lo_min, hi_max);
+            const bool active = kb < whi_max && nb > wlo_min;
+            v16f s[2];
+            const PromptTile<D> &x = s_tile[buf];
+            {
+                // all operands first, so that no product waits for its own; the two halves' products in turn, the next
+                // tile's unpacking between them
                 const int krow = 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3);
+                constexpr int kAhead = kSteps < 8 ? kSteps : 8;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[u][i] = 0;
 #pragma unroll
-                    for (int ks = 0; ks < kSteps; ++ks) {
-                        const u4 kk = *(const u4 *)(x.k + (32 * u + krow) * PromptTile<D>::kKRow + 32 * ks + 16 * h);
+                for (int k8 = 0; k8 < kSteps; k8 += kAhead) {
+                    u4 kk[2][kAhead];
 #pragma unroll
-                        for (int n = 0; n < Planes; ++n) s[u] = mfma32(kk, q[n][ks], s[u]);
+                    for (int ks = 0; ks < kAhead; ++ks)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            kk[u][ks] = *(const u4 *)(x.k + (32 * u + krow) * PromptTile<D>::kKRow + 32 * (k8 + ks) + 16 * h);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (k8 + kAhead >= kSteps) bytes.pin();
+#pragma unroll
+                    for (int ks = 0; ks < kAhead; ++ks)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int n = 0; n < Planes; ++n) s[u] = mfma32(kk[u][ks], q[n][k8 + ks], s[u]);
+                    if (k8 + kAhead >= kSteps) {
+                        next.stage(bytes);
+#pragma unroll
+                        for (int i = 0; i < 2 * kAhead * Planes; ++i) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x202, 8 / Planes, 0);
+                        }
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+            }
+            kid = kid2, vid = vid2;
+            bytes.load(a, rec, head_at, kb + 2 * kPromptKeys, kid, vid);
+            kid2 = page_of(kb + 3 * kPromptKeys + kkey), vid2 = page_of(kb + 3 * kPromptKeys + vkey);
+            if (active) {
                 const bool missing = s_missing[buf] == kb;
                 if (kb + kPromptKeys > whi_min || kb < wlo_max || missing) {
                     const bool edge = edge_at(kb);
@@ -715,32 +760,59 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
 #pragma unroll
                         for (int i = 0; i < 16; ++i) acc[n][i] *= keep;
                 }
-                const float shift = m == -INFINITY ? 0.0f : m;
+                const float shift = m == -INFINITY ? 0.0f : m * to_log2;
+                if (__any(fabsf(shift) > 0x1p24f)) {
+                    // s to_log2 - shift in one rounding is not 0 at s = m: nothing beside what it is beyond such scores
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        u4 ph, pl;
+                        for (int i = 0; i < 16; ++i) s[u][i] = m == -INFINITY ? s[u][i] * to_log2 : (s[u][i] - m) * to_log2;
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float e0 = __builtin_amdgcn_exp2f((s[u][8 * g + 2 * j] - shift) * to_log2);
-                            const float e1 = __builtin_amdgcn_exp2f((s[u][8 * g + 2 * j + 1] - shift) * to_log2);
-                            l += e0 + e1;
-                            ph[j] = pack_bf16(e0, e1);
-                            if (Planes == 2) pl[j] = pack_bf16(e0 - __uint_as_float(ph[j] << 16), e1 - __uint_as_float(ph[j] & 0xFFFF0000u));
-                        }
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int n = 0; n < kTiles; ++n) {
-                            const u4 vv = *(const u4 *)(x.v + (32 * n + c) * PromptTile<D>::kVRow + 64 * u + 32 * g + 16 * h);
-                            acc[n] = mfma32(vv, ph, acc[n]);
-                            if (Planes == 2) acc[n] = mfma32(vv, pl, acc[n]);
-                        }
+                        for (int i = 0; i < 16; ++i) s[u][i] = __builtin_fmaf(s[u][i], to_log2, -shift);
+                }
+                // 16 keys at a time: their products with V run beside the next ones' exponentials
+                u4 ph[4], pl[4];
+                auto exponentials = [&](int g) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float e0 = __builtin_amdgcn_exp2f(s[g >> 1][8 * (g & 1) + 2 * j]);
+                        const float e1 = __builtin_amdgcn_exp2f(s[g >> 1][8 * (g & 1) + 2 * j + 1]);
+                        l += e0 + e1;
+                        ph[g][j] = pack_bf16(e0, e1);
+                        if (Planes == 2)
+                            pl[g][j] = pack_bf16(e0 - __uint_as_float(ph[g][j] << 16), e1 - __uint_as_float(ph[g][j] & 0xFFFF0000u));
                     }
-            }
-            if (more) {
-                const int nb = kb + kPromptKeys;
-                if (!fine) s_missing[buf ^ 1] = nb;
-                s_tile[buf ^ 1].stage(bytes, nb, edge_at(nb), vfine, lo_min, hi_max);
+                };
+                u4 vv[2][kTiles];
+                auto operands = [&](int g) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+                        vv[g & 1][n] = *(const u4 *)(x.v + (32 * n + c) * PromptTile<D>::kVRow + 32 * g + 16 * h);
+                };
+                operands(0);
+                __builtin_amdgcn_sched_barrier(0);
+                exponentials(0);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (g < 3) operands(g + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (g < 3) exponentials(g + 1);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) {
+                        acc[n] = mfma32(vv[g & 1][n], ph[g], acc[n]);
+                        if (Planes == 2) acc[n] = mfma32(vv[g & 1][n], pl[g], acc[n]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, Planes, 1);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 8 / kTiles > 0 ? 8 / kTiles : 1, 1);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 4, 1);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             __syncthreads();
         }

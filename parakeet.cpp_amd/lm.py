@@ -302,7 +302,7 @@ def kv4_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: in
         raise TypeError(f"table: {table.dtype} (int32)")
     tp, ts = _rows(table, width, "table")
     if max_len is None:
-        max_len = min(width * page, 2 ** 31 - 1)
+        max_len = min(width * page, 2 ** 31 - 4097)
     head = (qp, op, 0 if lse is None else _f32(lse, (n, heads), "lse"), cp, tp, _i32(lens, (B,), "lens"),
             0 if first is None else _i32(first, (B + 1,), "first"))
     tail = (qr, qh, our, oh, ps, ts, n, B, heads, kv_heads, dim, dt, page, n_pages, width, max_new, max_len, window,
