@@ -80,15 +80,16 @@ int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
 }
 
 // Arrival counters of the tiles whose keys are split, at the workspace's beginning whatever the call's shape, so that
-// no call's partial sums lie where another's counters are.  A split call has fewer tiles than this (attend_shape).
-constexpr int kCounters = 1024;
+// no call's partial sums lie where another's counters are.  A split call has at most kSplitWork tiles times splits, and
+// a tile 1 + (splits + 15) / 16 counters.
+constexpr int kSplitWork = 1024, kCounters = 4 * kSplitWork;
 // more query rows of a request and kv head than this go to the prompt kernel
 constexpr int kPromptFrom = 64;
 
 // How a call's work is dealt out, from its host-known sizes alone.
 struct AttendShape {
     bool prompt;             // attend_prompt_kernel, 128 query rows a workgroup; else attend_kernel, 16
-    int cols, tiles, chunk, splits;
+    int cols, tiles, chunk, splits, groups;
     int64_t part_bytes;
     int64_t bytes() const { return splits > 1 ? kCounters * 4 + part_bytes : 0; }
 };
@@ -101,9 +102,8 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t tiles = (rows + s.cols - 1) / s.cols;
     // keys of one tile: its rows span at most as many tokens
     const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + s.cols + 64) : d.max_len;
-    // split where the tiles leave the card's 256 CUs short of work (so fewer than kCounters tiles), into no less than
-    // 256 (512) keys
-    const int64_t want = s.prompt ? 512 : kCounters, least = s.prompt ? 512 : 256, each = std::max<int64_t>(pairs * tiles, 1);
+    // split where the tiles leave the card's 256 CUs short of work, into no less than 512 keys
+    const int64_t want = s.prompt ? 512 : kSplitWork, least = 512, each = std::max<int64_t>(pairs * tiles, 1);
     int64_t splits = std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
     const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
@@ -111,7 +111,8 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
         return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
                        (long long)rows);
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
-    s.part_bytes = pairs * tiles * splits * s.cols * (d.head_dim + 4) * 4;
+    s.groups = (int)((splits + kJoin - 1) / kJoin);
+    s.part_bytes = pairs * tiles * (splits + s.groups) * s.cols * (d.head_dim + 4) * 4;
     return PK_OK;
 }
 
@@ -271,7 +272,7 @@ PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
     p.n_rows = d->n_rows, p.requests = d->requests, p.heads = d->heads, p.kv_heads = d->kv_heads;
     p.page = d->page, p.page_shift = log2i(d->page), p.n_pages = d->n_pages, p.width = d->width;
     p.max_len = d->max_len, p.window = d->window, p.group = d->heads / d->kv_heads;
-    p.tiles = sh.tiles, p.splits = sh.splits, p.chunk = sh.chunk, p.scale = d->scale;
+    p.tiles = sh.tiles, p.splits = sh.splits, p.groups = sh.groups, p.chunk = sh.chunk, p.scale = d->scale;
     p.vec = aligned(d->q, 16) && d->q_row % 8 == 0 && d->q_head % 8 == 0;
     p.vec_out = aligned(d->out, 8) && d->out_row % 4 == 0 && d->out_head % 4 == 0;
     const unsigned grid = (unsigned)((int64_t)d->requests * d->kv_heads * sh.tiles * sh.splits);
