@@ -12,37 +12,42 @@ constexpr int kPlanTokens = 4;   // consecutive tokens of one thread: one 16-byt
 // Three running sums over the requests: new tokens (where a token's request is found), pages lacked (where its page
 // is in the ring), pages given up (where they go behind the ring's end).  Every workgroup makes all three in its LDS
 // from the two length arrays, at most 32 KB of reads, so that nothing is exchanged between workgroups and one launch
-// does it all; each then takes its share of the tokens and of the pages given up.
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, int wide) {
+// does it all; each then takes its share of the tokens and of the pages given up.  Latency alone counts: lengths are read
+// once, and a thread's four tokens, mostly of one request, take their pages in two loads together.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, int shift, int wide) {
     __shared__ int s_first[PK_LM_MAX_REQUESTS + 1], s_lack[PK_LM_MAX_REQUESTS + 1], s_free[PK_LM_MAX_REQUESTS + 1];
+    __shared__ int s_old[PK_LM_MAX_REQUESTS], s_new[PK_LM_MAX_REQUESTS];
     __shared__ int s_wave[3][kPlanThreads / 64], s_used;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int B = a.requests, most = a.width * a.page;
+    const int B = a.requests, page = 1 << shift, most = a.width << shift;
+    auto pages = [&](int n) { return (n + page - 1) >> shift; };
+    for (int b = tid; b < B; b += kPlanThreads) s_old[b] = a.old_len[b], s_new[b] = a.new_len[b];
     const int count = min(max(a.state[1], 0), a.n_pages);
     int head = a.state[0] % a.n_pages;
     if (head < 0) head += a.n_pages;
+    if (tid == 0) s_used = 0;
+    if (tid == 0 && B == 0) s_first[0] = s_free[0] = 0;   // no thread below has a last request
+    __syncthreads();
 
     // this thread's run of requests, their sums, and what lies before them
     const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, B), b1 = min(b0 + per, B);
     int tokens = 0, lack = 0;
     for (int b = b0; b < b1; ++b) {
-        const int o = a.old_len[b], n = a.new_len[b];
+        const int o = s_old[b], n = s_new[b];
         if (o < 0 || n < 0 || o > most || n > most) continue;
         tokens += max(n - o, 0);
-        lack += max((n + a.page - 1) / a.page - (o + a.page - 1) / a.page, 0);
+        lack += max(pages(n) - pages(o), 0);
     }
-    if (tid == 0) s_used = 0;
-    if (tid == 0 && B == 0) s_first[0] = s_free[0] = 0;   // no thread below has a last request
     const int st = wave_scan(tokens), sl = wave_scan(lack);
     if (lane == 63) s_wave[0][wave] = st, s_wave[1][wave] = sl;
     __syncthreads();
     int at = st - tokens, al = sl - lack, freed = 0, used = 0;
     for (int w = 0; w < wave; ++w) at += s_wave[0][w], al += s_wave[1][w];
     for (int b = b0; b < b1; ++b) {
-        const int o = a.old_len[b], n = a.new_len[b];
+        const int o = s_old[b], n = s_new[b];
         const bool ranged = !(o < 0 || n < 0 || o > most || n > most);
-        const int had = (o + a.page - 1) / a.page, want = (n + a.page - 1) / a.page;
-        const int need = ranged ? max(want - had, 0) : 0;
+        const int had = ranged ? pages(o) : 0, want = ranged ? pages(n) : 0;
+        const int need = max(want - had, 0);
         const bool ok = ranged && (need == 0 || al + need <= count);
         s_first[b] = at;
         s_lack[b] = ok ? al : -1;                       // -1: not served
@@ -78,38 +83,50 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, i
         a.state_out[1] = min(count - s_used + gone, a.n_pages);
     }
 
+    // page j of request b, which holds `had` pages and takes new ones from place `al` of the ring on
+    auto page_at = [&](int b, int j, int had, int al_b) {
+        const int64_t place = (int64_t)head + al_b + (j - had);
+        const int *p = j < had ? a.table + b * a.table_stride + j : a.ring + (place >= a.n_pages ? place - a.n_pages : place);
+        return *p;
+    };
     const int64_t stride = (int64_t)gridDim.x * kPlanThreads, me = (int64_t)blockIdx.x * kPlanThreads + tid;
     for (int64_t t0 = me * kPlanTokens; t0 < max(total, a.n_tokens); t0 += stride * kPlanTokens) {
-        int b = 0;
-        if (t0 < total) {                               // the last request that begins at or before t0
-            int hi = B;
+        v4i slot = {-1, -1, -1, -1}, pos = {-1, -1, -1, -1};
+        if (t0 < total) {
+            int b = 0, hi = B;                          // the last request that begins at or before t0
             while (hi - b > 1) {
                 const int mid = (b + hi) >> 1;
                 if (s_first[mid] <= t0) b = mid; else hi = mid;
             }
-        }
-        v4i slot, pos;
+            if (t0 + kPlanTokens <= s_first[b + 1]) {
+                const int al_b = s_lack[b];
+                if (al_b >= 0) {
+                    const int o = s_old[b], p = o + (int)(t0 - s_first[b]), had = pages(o);
+                    const int j0 = p >> shift, j1 = (p + kPlanTokens - 1) >> shift;
+                    const int id0 = page_at(b, j0, had, al_b), id1 = page_at(b, j1, had, al_b);
 #pragma unroll
-        for (int i = 0; i < kPlanTokens; ++i) {
-            const int64_t t = t0 + i;
-            slot[i] = pos[i] = -1;
-            if (t >= total) continue;
-            while (t >= s_first[b + 1]) ++b;
-            const int al_b = s_lack[b];
-            if (al_b < 0) continue;
-            const int o = a.old_len[b], p = o + (int)(t - s_first[b]), j = p / a.page, had = (o + a.page - 1) / a.page;
-            int id;
-            if (j < had) {
-                id = a.table[b * a.table_stride + j];
+                    for (int i = 0; i < kPlanTokens; ++i) {
+                        const int q = p + i, id = q >> shift == j0 ? id0 : id1;
+                        slot[i] = (id << shift) + (q & (page - 1));
+                        pos[i] = q;
+                        // a new page's first token is new: it enters the page into the table
+                        if ((q & (page - 1)) == 0) a.table[b * a.table_stride + (q >> shift)] = id;
+                    }
+                }
             } else {
-                int r = head + al_b + (j - had);
-                if (r >= a.n_pages) r -= a.n_pages;
-                id = a.ring[r];
-                // the page's first token is new: it enters the page into the table
-                if (p == j * a.page) a.table[b * a.table_stride + j] = id;
+                for (int i = 0; i < kPlanTokens; ++i) {
+                    const int64_t t = t0 + i;
+                    if (t >= total) break;
+                    while (t >= s_first[b + 1]) ++b;
+                    const int al_b = s_lack[b];
+                    if (al_b < 0) continue;
+                    const int o = s_old[b], q = o + (int)(t - s_first[b]);
+                    const int id = page_at(b, q >> shift, pages(o), al_b);
+                    slot[i] = (id << shift) + (q & (page - 1));
+                    pos[i] = q;
+                    if ((q & (page - 1)) == 0) a.table[b * a.table_stride + (q >> shift)] = id;
+                }
             }
-            slot[i] = id * a.page + (p - j * a.page);
-            pos[i] = p;
         }
         if (t0 + kPlanTokens <= a.n_tokens && wide) {
             *(v4i *)(a.slots + t0) = slot;
@@ -130,9 +147,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, i
             if (s_free[mid] <= f) b = mid; else hi = mid;
         }
         if (count + f >= a.n_pages) continue;           // a ring that says it holds more than there are
-        const int want = (a.new_len[b] + a.page - 1) / a.page;
         const int r = (int)(((int64_t)head + count + f) % a.n_pages);
-        a.ring[r] = a.table[b * a.table_stride + want + (f - s_free[b])];
+        a.ring[r] = a.table[b * a.table_stride + pages(s_new[b]) + (f - s_free[b])];
     }
 }
 
