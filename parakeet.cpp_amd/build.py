@@ -3,6 +3,8 @@
   libparakeet_hip.so      HIP kernels + C ABI      (csrc/pk_decode.hip: the decode loop,
                           csrc/pk_lm.hip: the language-model serving operators)
   libparakeet_decoder.so  C++ decoder API           (csrc/parakeet_decoder.cpp, csrc/gguf_reader.cpp)
+  _lm_torch.so            the serving operators' calls for torch tensors (csrc/lm_torch.cpp), built where
+                          torch is installed
   libpk_calib.so          copy kernel of known size (csrc/pk_calib.hip), used by bench.py to scale
                           hardware byte counters
   tests/cpp/decoder_api_main  test driver of the C++ API (tests/cpp/decoder_api_main.cpp)
@@ -24,6 +26,7 @@ from __future__ import annotations
 
 import os
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -51,6 +54,24 @@ def build_hip():
     extra = ["-DPK_TIMELINE"] if os.environ.get("PK_TIMELINE") else []
     srcs = [os.path.join(CSRC, f) for f in ("pk_decode.hip", "pk_lm.hip")]
     _run([HIPCC, *HIP_FLAGS, *extra, "-shared", *srcs, "-o", out + ".tmp"])
+    os.replace(out + ".tmp", out)
+    return out
+
+
+def build_lm_torch():
+    """parakeet.cpp_amd/_lm_torch.so: host code only (g++), against the installed torch's headers."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    root = os.path.dirname(torch.__file__)
+    out = os.path.join(HERE, "_lm_torch.so")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INC}", "-isystem", f"{root}/include",
+          "-isystem", f"{root}/include/torch/csrc/api/include", "-isystem", sysconfig.get_path("include"),
+          "-isystem", os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"), os.path.join(CSRC, "lm_torch.cpp"),
+          f"-L{root}/lib", f"-L{HERE}", "-lparakeet_hip", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
+          "-Wl,-rpath,$ORIGIN", "-o", out + ".tmp"])
     os.replace(out + ".tmp", out)
     return out
 
@@ -145,7 +166,7 @@ def build_sanitizers():
 
 
 def build_all():
-    return [build_hip(), build_decoder(), build_calib(), build_api_test("decoder_api_main", hip=True),
+    return [build_hip(), build_decoder(), build_lm_torch(), build_calib(), build_api_test("decoder_api_main", hip=True),
             build_api_test("loader_main"), build_dropin_test(), build_header_test("enc_proj_rule"),
             build_header_test("exchange_word"), *build_sanitizers()]
 

@@ -135,6 +135,13 @@ int attend_check(const pk_kv4_attend_desc *d) {
                        d->max_new, d->max_len, d->window, d->width);
     if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, d->head_dim);
+    if ((int64_t)std::max(d->n_rows, d->max_new) * (d->heads / d->kv_heads) > INT32_MAX - 4096)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows, max_new %d, %d query heads a kv head: row numbers are 32 bits", what, d->n_rows, d->max_new,
+                       d->heads / d->kv_heads);
+    // positions are 32 bits, some steps past the last key included
+    if ((int64_t)d->width * d->page > INT32_MAX - 4096 || d->max_len > INT32_MAX - 4096)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: a table of %d pages of %d tokens, max_len %d: positions are 32 bits", what, d->width, d->page,
+                       d->max_len);
     return PK_OK;
 }
 

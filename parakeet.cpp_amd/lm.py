@@ -21,12 +21,15 @@ Workspaces (``kv4_attend``, ``sample``) are kept per operator, device and stream
 ever grow; one that has been handed out is never freed, since a captured graph
 may hold it.  Give ``workspace=`` (zeroed uint8) to keep your own.
 
-torch and this library have to share one HIP runtime: where torch tensors are
-used, import torch before the library is first loaded.
+torch tensors are read by an extension of their own (csrc/lm_torch.cpp), others
+here, through ctypes.  torch and this library have to share one HIP runtime:
+where torch tensors are used, import torch before the library is first loaded.
 """
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
+import os
 import struct
 import sys
 
@@ -39,11 +42,19 @@ MAX_REQUESTS, MAX_VOCAB = 4096, 1048576
 
 EXPORTED = ["pk_kv_plan", "pk_kv4_store", "pk_kv4_load", "pk_kv4_attend", "pk_kv4_attend_workspace", "pk_sample",
             "pk_sample_workspace"]
+TORCH_PATH = os.path.join(pk.HERE, "_lm_torch.so")
 
 _FLOATS = {"f32": F32, "f16": F16, "bf16": BF16}
-_I32, _U8 = {"i32"}, {"u8"}
-_calls = None
+_calls: dict = {}
 _workspaces: dict = {}
+
+
+class _NoTorch:
+    """Stands for torch.Tensor until a torch tensor is met."""
+
+
+_Tensor = _NoTorch
+_torch_calls = None
 
 # the descriptors of parakeet_lm.h, in their order (native alignment)
 _PLAN = struct.Struct("11Pq5i0P")
@@ -52,36 +63,40 @@ _ATTEND = struct.Struct("8P7q12if0P")
 _SAMPLE = struct.Struct("10P2q4i0P")
 
 
-def _one_runtime():
-    """torch's HIP runtime and the library's have to be the same file."""
-    seen = set()
-    with open("/proc/self/maps") as f:
-        for line in f:
-            if "libamdhip64" in line:
-                seen.add(line.split(None, 5)[5].strip())
-    if len(seen) > 1:
-        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(sorted(seen))}): import torch before the parakeet library")
-
-
 def _load():
-    global _calls
     L = pk.lib()
-    found = {}
     for name in EXPORTED:
         f = getattr(L, name)
         f.argtypes = [C.c_char_p, C.c_void_p]
-        found[name] = f
+        _calls[name] = f
+
+
+def _new_torch(t):
+    """Whether t is a torch tensor, the first one to come: loads the extension that reads them."""
+    global _Tensor, _torch_calls
     torch = sys.modules.get("torch")
-    if torch is not None:
-        _one_runtime()
-        _FLOATS.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-        _I32.add(torch.int32)
-        _U8.add(torch.uint8)
-    _calls = found
-    return found
+    if _Tensor is not _NoTorch or torch is None or not isinstance(t, torch.Tensor):
+        return False
+    pk.lib()
+    runtimes = set()
+    with open("/proc/self/maps") as f:
+        for line in f:
+            if "libamdhip64" in line:
+                runtimes.add(line.split(None, 5)[5].strip())
+    if len(runtimes) > 1:
+        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(sorted(runtimes))}): import torch before the parakeet library")
+    if not os.path.exists(TORCH_PATH):
+        raise RuntimeError(f"{TORCH_PATH} is not built: run __graft_entry__.build()")
+    spec = importlib.util.spec_from_file_location("_lm_torch", TORCH_PATH)
+    _torch_calls = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(_torch_calls)
+    _Tensor = torch.Tensor
+    return True
 
 
 def _call(name, packed, stream):
+    if not _calls:
+        _load()
     rc = _calls[name](packed, stream)
     if rc:
         pk.check(rc)
@@ -90,24 +105,13 @@ def _call(name, packed, stream):
 def _dtype(t, what):
     d = _FLOATS.get(t.dtype)
     if d is None:
-        if _late_torch(t):
-            return _dtype(t, what)
         raise TypeError(f"{what}: {t.dtype} (f32, f16 or bf16)")
     return d
 
 
-def _late_torch(t):
-    """torch came after the first call with other arrays: take its types in (and see that the runtimes agree)."""
-    torch = sys.modules.get("torch")
-    if torch is None or torch.int32 in _I32 or not isinstance(t, torch.Tensor):
-        return False
-    _load()
-    return True
-
-
 def _i32(t, shape, what):
     """Pointer of a contiguous int32 array of this shape."""
-    if t.dtype not in _I32 and not (_late_torch(t) and t.dtype in _I32):
+    if t.dtype != "i32":
         raise TypeError(f"{what}: {t.dtype} (int32)")
     if tuple(t.shape) != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
@@ -126,7 +130,7 @@ def _f32(t, shape, what):
     return t.data_ptr()
 
 
-def _rows(t, dim, what, ndim=2):
+def _rows(t, what):
     """(pointer, row stride) of a 2-d array whose last axis is adjacent."""
     s = t.stride()
     if s[1] != 1 and t.shape[1] > 1:
@@ -146,7 +150,7 @@ def _heads(t, what):
 
 def _cache(cache, page, what):
     """(pointer, page stride, pages, heads, head_dim) of cache [n_pages, kv_heads, page (D + D/16)] bytes."""
-    if cache.dtype not in _U8 and not (_late_torch(cache) and cache.dtype in _U8):
+    if cache.dtype != "u8":
         raise TypeError(f"{what}: cache of {cache.dtype} (uint8)")
     n, heads, size = cache.shape
     s = cache.stride()
@@ -164,58 +168,17 @@ def kv4_shape(n_pages: int, kv_heads: int, head_dim: int, page: int):
     return n_pages, kv_heads, page * (head_dim + head_dim // 16)
 
 
-class _Here:
-    """The stream to use and, where needed, its tensors' device made current."""
-
-    def __init__(self, t, stream):
-        self.back = None
-        d = getattr(t, "device", None)
-        if d is None:
-            self.stream = stream
-            return
-        torch = sys.modules["torch"]
-        if d.type != "cuda":
-            raise ValueError("tensors have to be on the GPU")
-        now = torch._C._cuda_getDevice()
-        if d.index != now:
-            self.back = now
-            torch.cuda.set_device(d)
-        self.stream = torch._C._cuda_getCurrentRawStream(d.index) if stream is None else stream
-
-    def __enter__(self):
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            sys.modules["torch"].cuda.set_device(self.back)
-
-
-def _same_device(first, *others):
-    d = getattr(first, "device", None)
-    for t in others:
-        if t is not None and getattr(t, "device", None) != d:
-            raise ValueError(f"arrays on {d} and on {getattr(t, 'device', None)}")
-
-
-def _workspace(kind, like, stream, wanted, given):
+def _workspace(kind, stream, wanted, given):
     """(pointer, bytes) of at least `wanted` bytes, zeroed before the first use; each kind of call has its own."""
     if given is not None:
         return given.data_ptr(), given.numel()
     if wanted == 0:
         return 0, 0
-    d = getattr(like, "device", None)
-    kept = _workspaces.setdefault((kind, d, stream), [])
+    kept = _workspaces.setdefault((kind, stream), [])
     if not kept or kept[-1].numel() < wanted:
-        size = max(1 << 20, 1 << (wanted - 1).bit_length())
-        if d is None:
-            t = hipmem.Tensor((size,), "u8")
-            t.zero()
-            hipmem.synchronize()
-        else:
-            torch = sys.modules["torch"]
-            t = torch.zeros(size, dtype=torch.uint8, device=d)
-            if stream != torch._C._cuda_getCurrentRawStream(d.index):
-                torch.cuda.current_stream(d).synchronize()      # zeroed on torch's stream, used on another
+        t = hipmem.Tensor((max(1 << 20, 1 << (wanted - 1).bit_length()),), "u8")
+        t.zero()
+        hipmem.synchronize()
         kept.append(t)
     return kept[-1].data_ptr(), kept[-1].numel()
 
@@ -227,26 +190,24 @@ def kv_plan(old_len, new_len, table, ring, state, page: int, *, state_out, lens,
     free page ids, state [2] its {head, count}.  Written: state_out [2], lens and
     ok [requests], first [requests + 1], slots and pos [n_tokens].
     """
-    if _calls is None:
-        _load()
-    _same_device(old_len, new_len, table, ring, state, state_out, lens, ok, first, slots, pos)
+    if isinstance(table, _Tensor) or _new_torch(table):
+        rc = _torch_calls.kv_plan(old_len, new_len, table, ring, state, page, state_out, lens, ok, first, slots, pos, stream)
+        if rc:
+            pk.check(rc)
+        return
     B, width = table.shape
-    if table.dtype not in _I32 and not (_late_torch(table) and table.dtype in _I32):
+    if table.dtype != "i32":
         raise TypeError(f"table: {table.dtype} (int32)")
-    tp, ts = _rows(table, width, "table")
+    tp, ts = _rows(table, "table")
     n, cap = ring.shape[0], slots.shape[0]
     packed = _PLAN.pack(_i32(old_len, (B,), "old_len"), _i32(new_len, (B,), "new_len"), tp, _i32(ring, (n,), "ring"),
                         _i32(state, (2,), "state"), _i32(state_out, (2,), "state_out"), _i32(lens, (B,), "lens"),
                         _i32(ok, (B,), "ok"), _i32(first, (B + 1,), "first"), _i32(slots, (cap,), "slots"),
                         0 if pos is None else _i32(pos, (cap,), "pos"), ts, B, width, n, page, cap)
-    with _Here(table, stream) as s:
-        _call("pk_kv_plan", packed, s)
+    _call("pk_kv_plan", packed, stream)
 
 
 def _kv4_rows(name, k, v, slots, cache, page, stream):
-    if _calls is None:
-        _load()
-    _same_device(cache, k, v, slots)
     dt = _dtype(k, "k")
     if v.dtype != k.dtype or tuple(v.shape) != tuple(k.shape):
         raise ValueError(f"k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}")
@@ -257,19 +218,28 @@ def _kv4_rows(name, k, v, slots, cache, page, stream):
     if k.shape[1] != heads or k.shape[2] != dim:
         raise ValueError(f"rows of {k.shape[1]} heads of {k.shape[2]}, a cache of {heads} heads of {dim}")
     packed = _ROWS.pack(kp, vp, _i32(slots, (n,), "slots"), cp, kr, kh, vr, vh, ps, n, heads, dim, dt, page, n_pages)
-    with _Here(cache, stream) as s:
-        _call(name, packed, s)
+    _call(name, packed, stream)
 
 
 def kv4_store(k, v, slots, cache, page: int, stream=None):
     """pk_kv4_store: rows k, v [n, kv_heads, head_dim] into cache at slots [n]; rows with a slot outside it (-1) are
     skipped."""
+    if isinstance(cache, _Tensor) or _new_torch(cache):
+        rc = _torch_calls.kv4_store(k, v, slots, cache, page, stream)
+        if rc:
+            pk.check(rc)
+        return
     _kv4_rows("pk_kv4_store", k, v, slots, cache, page, stream)
 
 
 def kv4_load(cache, slots, k, v, page: int, stream=None):
     """pk_kv4_load: what the cache holds at slots [n], into k, v [n, kv_heads, head_dim]; rows with a slot outside it
     are left as they are."""
+    if isinstance(cache, _Tensor) or _new_torch(cache):
+        rc = _torch_calls.kv4_load(cache, slots, k, v, page, stream)
+        if rc:
+            pk.check(rc)
+        return
     _kv4_rows("pk_kv4_load", k, v, slots, cache, page, stream)
 
 
@@ -283,9 +253,11 @@ def kv4_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: in
     tokens of any request (max_len defaults to what the table can name); window
     > 0 limits every query to its last `window` keys; lse [n_rows, heads] f32.
     """
-    if _calls is None:
-        _load()
-    _same_device(q, cache, table, lens, out, first, lse, workspace)
+    if isinstance(q, _Tensor) or _new_torch(q):
+        rc = _torch_calls.kv4_attend(q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream)
+        if rc:
+            pk.check(rc)
+        return
     dt = _dtype(q, "q")
     if out.dtype != q.dtype or tuple(out.shape) != tuple(q.shape):
         raise ValueError(f"q {q.dtype} {tuple(q.shape)}, out {out.dtype} {tuple(out.shape)}")
@@ -298,20 +270,19 @@ def kv4_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: in
         raise ValueError(f"{heads} query heads of {d}, a cache of {kv_heads} heads of {dim}")
     if (heads > 1 and oh < dim) or (n > 1 and our < dim):
         raise ValueError(f"out: rows overlap (strides {our}, {oh})")
-    if table.dtype not in _I32 and not (_late_torch(table) and table.dtype in _I32):
+    if table.dtype != "i32":
         raise TypeError(f"table: {table.dtype} (int32)")
-    tp, ts = _rows(table, width, "table")
+    tp, ts = _rows(table, "table")
     if max_len is None:
         max_len = min(width * page, 2 ** 31 - 4097)
     head = (qp, op, 0 if lse is None else _f32(lse, (n, heads), "lse"), cp, tp, _i32(lens, (B,), "lens"),
             0 if first is None else _i32(first, (B + 1,), "first"))
     tail = (qr, qh, our, oh, ps, ts, n, B, heads, kv_heads, dim, dt, page, n_pages, width, max_new, max_len, window,
             dim ** -0.5 if scale is None else scale)
-    with _Here(q, stream) as s:
-        wanted = C.c_int64()
-        _call("pk_kv4_attend_workspace", _ATTEND.pack(*head, 0, 0, *tail), C.addressof(wanted))
-        wp, wb = _workspace("attend", q, s, wanted.value, workspace)
-        _call("pk_kv4_attend", _ATTEND.pack(*head, wp, wb, *tail), s)
+    wanted = C.c_int64()
+    _call("pk_kv4_attend_workspace", _ATTEND.pack(*head, 0, 0, *tail), C.addressof(wanted))
+    wp, wb = _workspace("attend", stream, wanted.value, workspace)
+    _call("pk_kv4_attend", _ATTEND.pack(*head, wp, wb, *tail), stream)
 
 
 def sample(logits, u, token, *, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, kept=None, workspace=None,
@@ -322,19 +293,20 @@ def sample(logits, u, token, *, temperature=None, top_k=None, top_p=None, min_p=
     token [rows] int32, prob [rows] f32 (its share of the kept weight) and kept
     [rows] int32 (how many tokens were kept) are written.
     """
-    if _calls is None:
-        _load()
-    _same_device(logits, u, token, temperature, top_k, top_p, min_p, prob, kept, workspace)
+    if isinstance(logits, _Tensor) or _new_torch(logits):
+        rc = _torch_calls.sample(logits, u, token, temperature, top_k, top_p, min_p, prob, kept, workspace, stream)
+        if rc:
+            pk.check(rc)
+        return
     dt = _dtype(logits, "logits")
     B, V = logits.shape
-    lp, lr = _rows(logits, V, "logits")
+    lp, lr = _rows(logits, "logits")
     shape = (B,)
     opt = lambda f, t, what: 0 if t is None else f(t, shape, what)  # noqa: E731
     head = (lp, _f32(u, shape, "u"), opt(_f32, temperature, "temperature"), opt(_i32, top_k, "top_k"),
             opt(_f32, top_p, "top_p"), opt(_f32, min_p, "min_p"), _i32(token, shape, "token"), opt(_f32, prob, "prob"),
             opt(_i32, kept, "kept"))
-    with _Here(logits, stream) as s:
-        wanted = C.c_int64()
-        _call("pk_sample_workspace", _SAMPLE.pack(*head, 0, 0, lr, B, V, dt, 0), C.addressof(wanted))
-        wp, wb = _workspace("sample", logits, s, wanted.value, workspace)
-        _call("pk_sample", _SAMPLE.pack(*head, wp, wb, lr, B, V, dt, 0), s)
+    wanted = C.c_int64()
+    _call("pk_sample_workspace", _SAMPLE.pack(*head, 0, 0, lr, B, V, dt, 0), C.addressof(wanted))
+    wp, wb = _workspace("sample", stream, wanted.value, workspace)
+    _call("pk_sample", _SAMPLE.pack(*head, wp, wb, lr, B, V, dt, 0), stream)

@@ -132,7 +132,7 @@ def test_store_and_load_refuse(pkg, kw, err):
     (dict(window=-1), "window"), (dict(max_new=-1), "max_new"), (dict(max_len=-1), "max_len"), (dict(max_new=2), "without first"),
     (dict(q=Arr((4, 4, 128), "bf16"), out=Arr((4, 4, 128), "bf16")), "without first"), (dict(cache=cache(ptr=4104)), "aligned"),
     (dict(table=Arr((3, 5), "i32", strides=(3, 1))), "table rows"), (dict(q=Arr((3, 4, 128), "bf16", ptr=0)), "NULL"),
-    (dict(max_len=2 ** 31 - 5000, workspace=Arr((4096,), "u8")), "workspace"), (dict(max_len=2 ** 31 - 1), "32 bits"),
+    (dict(max_len=2 ** 31 - 5000, workspace=Arr((4096,), "u8")), "workspace"), (dict(max_len=2 ** 31 - 1), "32 bits"), (dict(max_new=2 ** 30), "32 bits"),
     (dict(table=Arr((3, 2 ** 26), "i32")), "32 bits"), (dict(table=Arr((3, 0), "i32")), "width"),
     (dict(q=Arr((3, 4, 128), "bf16", strides=(1024, 1, 4))), "adjacent")])
 def test_attend_refuses(pkg, kw, err):
