@@ -19,7 +19,8 @@ namespace pklm {
 typedef unsigned long long u64;
 
 constexpr float kReach = 22.0f;            // distance that the bins cover
-constexpr int kWholeMost = 64;            // a list with all kept tokens has at most so many: they are compared each with each
+constexpr float kWeighed = -21.6f;         // a distance beyond this has no weight: exp(-21.6) < 2^-31
+constexpr int kWholeMost = 64;             // of a cut by weight: tokens up to which the list holds all before the cut too
 constexpr int kCountShift = 46;            // (count, weight) of up to 2^15 tokens in one word: 2^15 2^30 < 2^46
 constexpr u64 kMassMask = (1ull << kCountShift) - 1;
 
@@ -96,7 +97,7 @@ struct CutScratch {
 
     // before the barrier that precedes everything below
     __device__ void clear() {
-        for (int i = threadIdx.x; i < Bins; i += BS) mass[i] = 0;
+        for (int i = threadIdx.x; i < Bins; i += BS) mass[i] = 0, count[i] = 0;
         if (threadIdx.x < 2) n[threadIdx.x] = 0, bin[threadIdx.x] = -1;
     }
     __device__ u64 mass_to(int b) const { return b < 0 ? 0 : mass[b]; }
@@ -129,6 +130,25 @@ struct CutScratch {
             if (w < wave) bc += wave_count[w];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) mass[tid * kPer + i] = bm + m[i], count[tid * kPer + i] = bc + c[i];
+        __syncthreads();
+    }
+
+    // Running sums of count (in place) alone.
+    __device__ void scan_counts() {
+        constexpr int kPer = Bins / BS;
+        const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+        unsigned c[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) c[i] = count[tid * kPer + i] + (i ? c[i - 1] : 0);
+        const unsigned ic = wave_scan(c[kPer - 1]);
+        if (lane == 63) wave_count[wave] = ic;
+        __syncthreads();
+        unsigned bc = ic - c[kPer - 1];
+#pragma unroll
+        for (int w = 0; w < BS / 64; ++w)
+            if (w < wave) bc += wave_count[w];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) count[tid * kPer + i] = bc + c[i];
         __syncthreads();
     }
 
@@ -294,11 +314,12 @@ __device__ inline u64 drawn(const pk_sample_desc &a, int b, u64 total) {
     return share(total, u > 0x7FFFFFFFull ? 0x7FFFFFFFull : u);
 }
 
-// The drawn token of the first `kept` of a sorted list.
+// The drawn token of the first `kept` of a sorted list, at most kCounted: each is compared with each.
 template <class Scratch>
 __device__ inline void answer_from_list(Scratch &s, const pk_sample_desc &a, int b, const RowRule &rule, int kept) {
     const int tid = threadIdx.x;
-    if (tid < kept && s.list_w[tid] >= rule.least && (tid == kept - 1 || s.list_w[tid + 1] < rule.least)) s.found[0] = tid + 1;
+    const unsigned least = max(rule.least, 1u);
+    if (tid < kept && s.list_w[tid] >= least && (tid == kept - 1 || s.list_w[tid + 1] < least)) s.found[0] = tid + 1;
     __syncthreads();
     kept = s.found[0];
     const u64 total = s.list_mass[kept - 1], t = drawn(a, b, total);
@@ -327,12 +348,12 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
     __shared__ float s_max[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab, b = blockIdx.x;
     const auto *row = (const typename T::Raw *)a.logits + (int64_t)b * a.logits_row;
-    const int n = (V + BS - 1) / BS, base = wave * n * 64 + lane;
+    const int n = (V + BS - 1) / BS, base = wave * n * 64 + lane, end = min((wave + 1) * n * 64, V);
     float x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int i = base + e * 64;
-        x[e] = e < n && i < V ? logit<T>(row, i) : -INFINITY;
+        x[e] = i < end ? logit<T>(row, i) : -INFINITY;
     }
     RowRule rule;
     rule.settings(a, b);
@@ -350,17 +371,52 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
         if (tid == 0) answer(a, b, -1, 0, 0, 0);
         return;
     }
-    unsigned w[E];
+    // groups of four tokens a thread: the last one's may lie behind the row, as -inf
+    auto tokens = [&](auto f) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = e < n ? rule.weight(x[e]) : 0;
+        for (int g = 0; g < E; g += 4)
+            if (g < n)
+#pragma unroll
+                for (int e = g; e < g + 4; ++e) f(e);
+    };
+    if (rule.k_on && rule.k <= s.kCounted) {
+        // Few by count: the bins only count, and only the listed tokens' weights are worked out.  (Token by token, the
+        // exponentials and the weights' 64-bit sums take as long as all the rest.)
+        int bin[E];
+        tokens([&](int e) {
+            bin[e] = rule.distance(x[e]) > kWeighed ? rule.bin<kBins>(x[e]) : kBins;
+            if (bin[e] < kBins) atomicAdd(&s.count[bin[e]], 1u);
+        });
+        __syncthreads();
+        s.scan_counts();
+        const int at = s.reach(0, (u64)rule.k), last = at < 0 ? kBins - 1 : at, listed = s.count[last];
+        if (listed <= BS) {
+            tokens([&](int e) {
+                if (bin[e] <= last) s.list[atomicAdd(&s.n[0], 1)] = rank_of(x[e], base + e * 64);
+            });
+            __syncthreads();
+            s.sort(listed, rule);
+            int left = min(rule.k, listed);
+            if (rule.p_on) {
+                const u64 need = share(s.list_mass[left - 1], rule.p);
+                left = s.place(left, 0, need ? need : 1) + 1;
+            }
+            answer_from_list(s, a, b, rule, left);
+            return;
+        }
+        __syncthreads();
+        s.clear();
+        __syncthreads();
+    }
+    unsigned w[E];
+    tokens([&](int e) { w[e] = rule.weight(x[e]); });
     u64 cut = 0;
     if (rule.k_on || rule.p_on) {
         int bin[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            bin[e] = e < n && w[e] ? rule.bin<kBins>(x[e]) : kBins;
-            if (e < n && w[e]) atomicAdd(&s.mass[bin[e]], (1ull << kCountShift) | w[e]);
-        }
+        tokens([&](int e) {
+            bin[e] = w[e] ? rule.bin<kBins>(x[e]) : kBins;
+            if (w[e]) atomicAdd(&s.mass[bin[e]], (1ull << kCountShift) | w[e]);
+        });
         __syncthreads();
         constexpr int kPer = kBins / BS;
         u64 bm[kPer];
@@ -379,13 +435,13 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
             }
         };
         auto list = [&](int kind, int first, int last) {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < n && bin[e] >= first && bin[e] <= last) s.list[atomicAdd(&s.n[kind], 1)] = rank_of(x[e], base + e * 64);
+            tokens([&](int e) {
+                if (bin[e] >= first && bin[e] <= last) s.list[atomicAdd(&s.n[kind], 1)] = rank_of(x[e], base + e * 64);
+            });
             __syncthreads();
         };
         const int left = find_cut(s, rule, cut, list, each);
-        if (left > 0 && left <= kWholeMost) {
+        if (left > 0) {
             answer_from_list(s, a, b, rule, left);
             return;
         }
@@ -395,13 +451,11 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
     const int cut_i = cut ? index_of(cut) : 0;
     u64 mass = 0;
     unsigned kept = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (e < n) {
-            const bool in = w[e] && w[e] >= rule.least && (x[e] > cut_x || (x[e] == cut_x && base + e * 64 <= cut_i));
-            w[e] = in ? w[e] : 0;
-            mass += w[e], kept += in;
-        }
+    tokens([&](int e) {
+        const bool in = w[e] && w[e] >= rule.least && (x[e] > cut_x || (x[e] == cut_x && base + e * 64 <= cut_i));
+        w[e] = in ? w[e] : 0;
+        mass += w[e], kept += in;
+    });
     mass = wave_sum(mass), kept = wave_sum(kept);
     __syncthreads();                         // wave_mass may still be read
     if (lane == 0) s.wave_mass[wave] = mass, s.wave_count[wave] = kept;
@@ -416,16 +470,14 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
     const u64 t = drawn(a, b, total);
     if (lead > t || lead + mass <= t) return;
     u64 sum[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] = e < n ? wave_sum((u64)w[e]) : 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
+    tokens([&](int e) { sum[e] = wave_sum((u64)w[e]); });
+    tokens([&](int e) {
         if (lead <= t && t < lead + sum[e]) {
             const u64 hit = __ballot(lead + wave_scan((u64)w[e]) > t);
             if (lane == __ffsll(hit) - 1) answer(a, b, base + e * 64, w[e], total, all);
         }
         lead += sum[e];
-    }
+    });
 }
 
 // ---- rows too long for one workgroup's registers ----
@@ -442,6 +494,9 @@ struct RowPick {
     u64 total, mass_first, mass_k;  // weight of the row; before first; before bin_k less what first .. last hold
     unsigned count_k, unused;       // tokens before bin_k, likewise
 };
+
+// Whether a row is cut by a count so small that its bins only count: weights are worked out for the listed tokens alone.
+__device__ inline bool few_by_count(const RowRule &rule) { return rule.k_on && rule.k <= kSplitThreads / 4; }
 
 struct SplitRows {
     float *chunk_max;               // [rows][chunks]
@@ -529,11 +584,18 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_hist_kernel(pk_sample
     s.clear();
     if ((!rule.k_on && !rule.p_on) || rule.top == -INFINITY) return;
     __syncthreads();
+    const bool few = few_by_count(rule);
     for (int i = i0 + tid;;) {
+        if (few) {
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            const unsigned wt = rule.weight(x[e]);
-            if (wt) atomicAdd(&s.mass[rule.bin<kSplitBins>(x[e])], (1ull << kCountShift) | wt);
+            for (int e = 0; e < kBatch; ++e)
+                if (rule.distance(x[e]) > kWeighed) atomicAdd(&s.mass[rule.bin<kSplitBins>(x[e])], 1ull << kCountShift);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const unsigned wt = rule.weight(x[e]);
+                if (wt) atomicAdd(&s.mass[rule.bin<kSplitBins>(x[e])], (1ull << kCountShift) | wt);
+            }
         }
         i += kBatch * kSplitThreads;
         if (i - tid >= i1) break;
@@ -570,6 +632,13 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_hist_kernel(pk_sample
     auto mass_to = [&](int bin) { return s.mass_to(bin); };
     auto count_to = [&](int bin) { return s.count_to(bin); };
     RowPick p{kSplitBins, kSplitBins - 1, -1, 0, 0, 0, 0, 0, 0};
+    if (few) {
+        p.bin_k = s.reach(0, (u64)rule.k);
+        p.first = 0, p.last = p.bin_k < 0 ? kSplitBins - 1 : p.bin_k;
+        p.n = (int)count_to(p.last);
+        if (tid == 0) w.pick[r] = p;
+        return;
+    }
     u64 low = s.mass[kSplitBins - 1], high = low;          // between which the kept total after top_k lies
     if (rule.k_on) {
         p.bin_k = s.reach(0, (u64)rule.k);
@@ -618,7 +687,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
         return;
     }
     if (!rule.k_on && !rule.p_on) p = RowPick{kSplitBins, kSplitBins - 1, -1, 0, 0, 0, 0, 0, 0};
-    const bool crowded = p.n > kSplitCap;
+    const bool crowded = p.n > kSplitCap, few = few_by_count(rule);
     if (!crowded) {
         if (tid == 0) s.n[0] = 0;
         __syncthreads();
@@ -631,7 +700,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
             for (int e = 0; e < kBatch; ++e) {
                 const int bin = rule.bin<kSplitBins>(x[e]);
                 if (bin > p.last && bin != p.bin_k) continue;      // most tokens: no weight is worked out
-                const unsigned wt = rule.weight(x[e]);
+                const unsigned wt = few ? rule.distance(x[e]) > kWeighed : rule.weight(x[e]);
                 if (wt && bin < p.first) {
                     if (wt >= rule.least) mass += wt, ++kept;
                 } else if (wt) {
@@ -669,12 +738,13 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
             s.sort(n, rule);
             u64 total = p.total;
             int left = n;                    // of the list
-            if (p.bin_k >= 0) left = rule.k - (int)p.count_k, total = p.mass_k + s.list_mass[left - 1];
+            if (p.bin_k >= 0) left = rule.k - (int)p.count_k;
+            if (p.bin_k >= 0 || few) total = p.mass_k + s.list_mass[left - 1];
             if (rule.p_on) {
                 const u64 need = share(total, rule.p);
                 left = min(left, s.place(n, p.mass_first, need ? need : 1) + 1);
             }
-            if (p.first == 0 && left <= kWholeMost) {
+            if (p.first == 0 && left <= s.kCounted) {
                 answer_from_list(s, a, b, rule, left);
                 return;
             }

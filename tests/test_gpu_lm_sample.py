@@ -166,3 +166,34 @@ def test_frequencies():
     assert (np.abs(np.bincount(token, minlength=V) - B * w) <= 1.001).all()
     assert np.allclose(prob, w[token], rtol=1e-5)
     assert (np.diff(token) >= 0).all()
+
+
+@pytest.mark.parametrize("V", [300, 5000, 70000])
+def test_few_of_many_equal_logits(V):
+    """A small top_k inside more equal logits than any list holds; with fewer logits of any weight than top_k; beside
+    logits so far below that they have no weight."""
+    g = np.random.default_rng(V)
+    B = 8
+    x = np.full((B, V), -1.0, f32)
+    x[4:, g.permutation(V)[:3]] = 0.25
+    u = g.random(B)
+    for k in (1, 2, 5, 60, 200, 256, 257):
+        token, prob, kept = run(x, u, top_k=np.full(B, k))
+        assert (kept == min(k, V)).all()
+        for b in range(B):
+            assert token[b] in np.lexsort((np.arange(V), -x[b]))[:k]
+        check(x, u, np.full(B, 0.6), np.full(B, k), np.full(B, 0.8), np.zeros(B))
+    x[:] = -50.0
+    x[:, g.permutation(V)[:40]] = (g.standard_normal(40)).astype(f32)
+    x[:, 7] = x.max() - 21.52          # as good as none
+    token, prob, kept = check(x, u, np.full(B, 1.0), np.full(B, 100), np.full(B, 1.0), np.zeros(B))
+    check(x, u, np.full(B, 1.0), np.full(B, 100), np.full(B, 0.7), np.full(B, 0.01))
+    assert (x[np.arange(B), token] > -40).all()
+
+
+def test_every_row_length_up_to_a_few_thousand():
+    """Lengths around every number of tokens a thread takes."""
+    g = np.random.default_rng(12)
+    for V in sorted({64 * i + d for i in (1, 3, 4, 5, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 128, 129, 193, 255, 256, 257) for d in (-1, 0, 1)}):
+        x = (g.standard_normal((3, V)) * 3).astype(f32)
+        check(x, g.random(3), np.full(3, 0.9), np.array([0, 5, 0]), np.array([0.9, 0.9, 1.0]), np.zeros(3))
