@@ -2,13 +2,15 @@
 //
 // Weights are whole numbers, so sums are exact and the same in any order, and atomics may build them.  In the order
 // (falling logit, rising index) the kept tokens are a prefix, so the filters come down to one cut: the last kept token.
-// Every token has a rank word of 64 bits, its logit's ordered bits over its inverted index; kept is rank >= cut.
+// Every token has a rank word, its logit's ordered bits (those that its type has) over its inverted index; kept is
+// rank >= cut.
 //
 // To find the cut, tokens are binned by their distance from the largest logit, (max - x) / T in bins of 22/1,024
 // (weights round to none at 21.5), and the bins' (count, weight) sums are scanned.  That names the bin in which
 // the count reaches top_k or the weight reaches top_p's share.  The tokens up to that bin, or where they are too many
-// those of that bin alone, are listed and sorted, one a thread: the cut is a place in the list, and of a whole list the
-// token too.  A bin with more tokens than that (many equal logits) is split by the rank words' digits instead.
+// those of that bin alone, are listed.  A short list is sorted, each word's place the number of larger ones: the cut is a
+// place in it, and of a list with all kept tokens the token too.  In a longer one, and where a bin has more tokens than a
+// list holds (many equal logits), the cut's rank word is found eight bits at a time.
 #pragma once
 
 #include "lm_common.h"
@@ -29,7 +31,7 @@ __device__ inline unsigned order_key(float x) {
     const unsigned b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ inline u64 rank_of(float x, int i) { return (u64)order_key(x) << 32 | (0xFFFFFFFFu - (unsigned)i); }
+constexpr int kIndexBits = 20;             // PK_LM_MAX_VOCAB
 // floor(total * part / 2^31), part <= 2^31
 __device__ inline u64 share(u64 total, u64 part) { return (total >> 31) * part + (((total & 0x7FFFFFFFull) * part) >> 31); }
 __device__ inline u64 part31(float p) { return (u64)(fminf(fmaxf(p, 0.0f), 1.0f) * 2147483648.0f); }
@@ -41,8 +43,19 @@ struct RowRule {
     int k;               // how many at most
     u64 p;               // top_p in 2^-31
     bool k_on, p_on;
+    int spare;           // low bits that no logit of this type has in f32
 
+    __device__ u64 rank(float x, int i) const {
+        return (u64)(order_key(x) >> spare) << kIndexBits | (unsigned)((1 << kIndexBits) - 1 - i);
+    }
+    __device__ float logit_of(u64 rank) const {
+        const unsigned k = (unsigned)(rank >> kIndexBits) << spare;
+        return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~(k | ((1u << spare) - 1)));
+    }
+
+    template <class T>
     __device__ void settings(const pk_sample_desc &a, int b) {
+        spare = __is_same(T, F32) ? 0 : __is_same(T, F16) ? 13 : 16;
         const float t = a.temperature ? a.temperature[b] : 1.0f;
         const bool greedy = !(t > 0);
         inv = greedy ? 1.0f : fminf(1.0f / t, 3e38f);
@@ -73,11 +86,7 @@ struct Cut {
     u64 rank, mass;
 };
 
-__device__ inline float logit_of(u64 rank) {
-    const unsigned k = (unsigned)(rank >> 32);
-    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
-}
-__device__ inline int index_of(u64 rank) { return (int)(0xFFFFFFFFu - (unsigned)rank); }
+__device__ inline int index_of(u64 rank) { return (1 << kIndexBits) - 1 - (int)(rank & ((1 << kIndexBits) - 1)); }
 
 // What a workgroup of BS threads keeps in LDS to find a cut.
 template <int BS, int Bins>
@@ -91,7 +100,8 @@ struct CutScratch {
     unsigned wave_count[BS / 64];
     u64 digit_mass[256];
     unsigned digit_count[256];
-    u64 digit_at[3];
+    u64 digit_at[4];                 // tokens and weight before the digit reached, its weight, its tokens
+    unsigned differ[2];
     int n[2], bin[2], found[2];      // by count, by weight: tokens listed, bin reached, place in the list
     int digit;
 
@@ -163,49 +173,30 @@ struct CutScratch {
         return bin[kind];
     }
 
-    // list[0 .. n), n <= BS, into falling order, and its running weights.  Short lists: each word's place is the number
-    // of larger ones, some lanes a word.  Longer ones: a bitonic network, one word a thread, steps within a wave by lane
-    // exchanges.
+    // list[0 .. n), n <= kCounted, into falling order, its weights and running weights: each word's place is the number of
+    // larger ones, some lanes a word.
     __device__ void sort(int n_list, const RowRule &rule) {
-        const int tid = threadIdx.x;
-        if (n_list <= kCounted) {
-            constexpr int kLanes = BS / kCounted;
-            const int j = tid / kLanes;
-            const u64 v = j < n_list ? list[j] : 0;
-            int larger = 0;
+        constexpr int kLanes = BS / kCounted;
+        const int tid = threadIdx.x, j = tid / kLanes;
+        const u64 v = j < n_list ? list[j] : 0;
+        int larger = 0;
 #pragma unroll 4
-            for (int i = tid % kLanes; i < n_list; i += kLanes) larger += list[i] > v;
+        for (int i = tid % kLanes; i < n_list; i += kLanes) larger += list[i] > v;
 #pragma unroll
-            for (int d = kLanes / 2; d; d >>= 1) larger += __shfl_xor(larger, d);
-            __syncthreads();
-            if (j < n_list && tid % kLanes == 0) list[larger] = v;
-            __syncthreads();
-            const u64 u = tid < n_list ? list[tid] : 0;
-            const u64 w = tid < n_list ? rule.weight(logit_of(u)) : 0;
-            const u64 run = before(wave_scan(w), w) + w;
-            if (tid < n_list) list_mass[tid] = run, list_w[tid] = (unsigned)w;
-        } else {
-            int size = 64;
-            while (size < n_list) size <<= 1;
-            u64 v = tid < n_list ? list[tid] : 0;
-            for (int k = 2; k <= size; k <<= 1)
-                for (int j = k >> 1; j; j >>= 1) {
-                    u64 o = 0;
-                    if (j >= 64) {
-                        __syncthreads();
-                        list[tid] = v;
-                        __syncthreads();
-                        o = list[tid ^ j];
-                    } else if ((tid & ~63) < size) {
-                        o = __shfl_xor(v, j);
-                    }
-                    const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
-                    v = (o > v) == larger ? o : v;
-                }
-            const u64 w = tid < n_list ? rule.weight(logit_of(v)) : 0;
-            const u64 run = before(wave_scan(w), w) + w;      // the barrier in it: list has been read
-            list[tid] = v, list_mass[tid] = run, list_w[tid] = (unsigned)w;
-        }
+        for (int d = kLanes / 2; d; d >>= 1) larger += __shfl_xor(larger, d);
+        __syncthreads();
+        if (j < n_list && tid % kLanes == 0) list[larger] = v;
+        __syncthreads();
+        const u64 w = tid < n_list ? rule.weight(rule.logit_of(list[tid])) : 0;
+        const u64 run = before(wave_scan(w), w) + w;
+        if (tid < n_list) list_mass[tid] = run, list_w[tid] = (unsigned)w;
+        __syncthreads();
+    }
+
+    // Weights of an unsorted list, n <= BS.
+    __device__ void weigh(int n_list, const RowRule &rule) {
+        const int tid = threadIdx.x;
+        if (tid < n_list) list_w[tid] = rule.weight(rule.logit_of(list[tid]));
         __syncthreads();
     }
 
@@ -219,66 +210,124 @@ struct CutScratch {
 };
 
 // The token at which the count (kind 0) or the weight (kind 1) reaches `want`, among all that `each` gives (each(f) calls
-// f(rank, weight) for this thread's ones), without a list: eight bits of the rank words at a time.
-template <class Scratch, class Each>
-__device__ inline Cut cut_by_digits(Scratch &s, int kind, u64 want, Each each) {
-    u64 prefix = 0, c0 = 0, m0 = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < 256; i += Scratch::kThreads) s.digit_mass[i] = 0, s.digit_count[i] = 0;
+// f(rank, weight) for this thread's ones; some has one of the ranks): eight bits of the rank words at a time, from the
+// highest in which any two differ, until one token is left.
+// Packed: at most 2^15 tokens, counts and weights in one word.
+template <bool Packed = false, class Scratch, class Each>
+__device__ inline Cut cut_by_digits(Scratch &s, int kind, u64 want, u64 some, Each each) {
+    if (threadIdx.x < 2) s.differ[threadIdx.x] = 0;
+    __syncthreads();
+    {
+        u64 d = 0;
+        each([&](u64 r, unsigned) { d |= r ^ some; });
+        const unsigned lo = (unsigned)d, hi = (unsigned)(d >> 32);
+        if (lo) atomicOr(&s.differ[0], lo);
+        if (hi) atomicOr(&s.differ[1], hi);
+    }
+    __syncthreads();
+    const u64 differ = (u64)s.differ[1] << 32 | s.differ[0];
+    // not yet known, from the lowest.  (Without a choice on differ == 0: the compiler makes it a scalar select on a condition
+    // that it has in a vector compare's result.)
+    int bits = 63 - __builtin_clzll(differ << 1 | 1);
+    u64 prefix = some >> bits, c0 = 0, m0 = 0;       // rank words have at most 52 bits
+    while (bits > 0) {
+        const int width = min(bits, 8), shift = bits - width;
+        for (int i = threadIdx.x; i < 256; i += Scratch::kThreads) {
+            s.digit_mass[i] = 0;
+            if (!Packed) s.digit_count[i] = 0;
+        }
         __syncthreads();
         each([&](u64 r, unsigned w) {
-            if (shift == 56 || (r >> (shift + 8)) == prefix) {
-                atomicAdd(&s.digit_count[r >> shift & 255u], 1u);
-                atomicAdd(&s.digit_mass[r >> shift & 255u], (u64)w);
+            if (r >> bits == prefix) {
+                const int d = (int)(r >> shift) & ((1 << width) - 1);
+                if (!Packed) atomicAdd(&s.digit_count[d], 1u);
+                atomicAdd(&s.digit_mass[d], Packed ? (1ull << kCountShift) | w : (u64)w);
             }
         });
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int d = 255;
-            for (; d > 0; --d) {
-                if ((kind ? m0 + s.digit_mass[d] : c0 + s.digit_count[d]) >= want) break;
-                c0 += s.digit_count[d], m0 += s.digit_mass[d];
+        if (threadIdx.x < 64) {
+            // four digits a lane, the largest first
+            u64 m[4];
+            unsigned c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 255 - (4 * threadIdx.x + i);
+                m[i] = s.digit_mass[d] + (i ? m[i - 1] : 0);
+                c[i] = Packed ? 0 : s.digit_count[d] + (i ? c[i - 1] : 0);
             }
-            s.digit_at[0] = c0, s.digit_at[1] = m0, s.digit_at[2] = s.digit_mass[d], s.digit = d;
+            u64 bm = wave_scan(m[3]) - m[3], bc = 0;
+            if (Packed) {
+                bc = bm >> kCountShift, bm &= kMassMask;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[i] = (unsigned)(m[i] >> kCountShift), m[i] &= kMassMask;
+            } else {
+                bc = wave_scan(c[3]) - c[3];
+            }
+            bm += m0, bc += c0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u64 pm = bm + (i ? m[i - 1] : 0), pc = bc + (i ? c[i - 1] : 0);
+                if (kind ? pm < want && want <= bm + m[i] : pc < want && want <= bc + c[i]) {
+                    s.digit = 255 - (4 * (int)threadIdx.x + i);
+                    s.digit_at[0] = pc, s.digit_at[1] = pm, s.digit_at[2] = bm + m[i] - pm, s.digit_at[3] = bc + c[i] - pc;
+                }
+            }
         }
         __syncthreads();
-        c0 = s.digit_at[0], m0 = s.digit_at[1], prefix = prefix << 8 | (unsigned)s.digit;
+        c0 = s.digit_at[0], m0 = s.digit_at[1], prefix = prefix << width | (unsigned)s.digit, bits = shift;
+        if (s.digit_at[3] == 1) break;
+        __syncthreads();
     }
-    const Cut cut{prefix, m0 + s.digit_at[2]};
+    // the one token with this prefix
+    each([&](u64 r, unsigned w) {
+        if (r >> bits == prefix) s.digit_mass[0] = r, s.digit_mass[1] = w;
+    });
+    __syncthreads();
+    const Cut cut{s.digit_mass[0], m0 + s.digit_mass[1]};
     __syncthreads();
     return cut;
 }
 
-// The cut of a row whose bins are scanned.  list(kind, first, last) lists the tokens of some bins; each(f) is as above.
-// Returns how many tokens the cut leaves where the list holds all of them, else -1.
+// The same of an unsorted list with weights.
+template <class Scratch>
+__device__ inline Cut cut_in_list(Scratch &s, int n, int kind, u64 want) {
+    const int tid = threadIdx.x;
+    return cut_by_digits<true>(s, kind, want, s.list[0], [&](auto f) {
+        if (tid < n) f(s.list[tid], s.list_w[tid]);
+    });
+}
+
+// The cut of a row whose bins are scanned.  list(kind, first, last) lists the tokens of some bins; each(f) and some are
+// as above.  Returns how many tokens the cut leaves where the sorted list holds all of them, else -1.
 template <class Scratch, class List, class Each>
-__device__ inline int find_cut(Scratch &s, const RowRule &rule, u64 &cut, List list, Each each) {
+__device__ inline int find_cut(Scratch &s, const RowRule &rule, u64 &cut, u64 some, List list, Each each) {
     u64 total = s.mass[Scratch::kBins - 1];
     int kept = -1, n = 0;
     bool whole = false;
-    // lists the bins up to b, or b alone
-    auto listed = [&](int kind, int b) {
+    // the token in bin b at which the count or the weight reaches `want`, from a list of the bins up to b, or of b alone
+    auto cut_at = [&](int kind, int b, u64 want) {
         whole = s.count_to(b) <= kWholeMost;
         n = s.count_to(b) - (whole ? 0 : s.count_to(b - 1));
-        if (n > Scratch::kThreads) return false;
+        if (n > Scratch::kThreads) return cut_by_digits(s, kind, want, some, each);
         list(kind, whole ? 0 : b, b);
-        s.sort(n, rule);
-        return true;
+        if (whole) {
+            s.sort(n, rule);
+            const int at = kind ? s.place(n, 0, want) : (int)want - 1;
+            kept = at + 1;
+            return Cut{s.list[at], s.list_mass[at]};
+        }
+        s.weigh(n, rule);
+        const u64 c0 = s.count_to(b - 1), m0 = s.mass_to(b - 1);
+        Cut c = cut_in_list(s, n, kind, want - (kind ? m0 : c0));
+        c.mass += m0;
+        return c;
     };
-    bool have = false;       // a list with every token that may be kept
+    bool have = false;       // a sorted list with every token that may be kept
     if (rule.k_on) {
         const int b = s.reach(0, (u64)rule.k);
         if (b >= 0) {
-            if (listed(0, b)) {
-                const int at = rule.k - 1 - (whole ? 0 : (int)s.count_to(b - 1));
-                cut = s.list[at], total = s.list_mass[at] + (whole ? 0 : s.mass_to(b - 1));
-                have = whole;
-                if (whole) kept = at + 1;
-            } else {
-                const Cut c = cut_by_digits(s, 0, (u64)rule.k, each);
-                cut = c.rank, total = c.mass;
-            }
+            const Cut c = cut_at(0, b, (u64)rule.k);
+            cut = c.rank, total = c.mass, have = whole;
         }
     }
     if (rule.p_on) {
@@ -289,14 +338,8 @@ __device__ inline int find_cut(Scratch &s, const RowRule &rule, u64 &cut, List l
             const int at = s.place(n, 0, need);
             c = s.list[at], kept = at + 1;
         } else {
-            const int b = s.reach(1, need);
-            if (listed(1, b)) {
-                const int at = s.place(n, whole ? 0 : s.mass_to(b - 1), need);
-                c = s.list[at];
-                if (whole) kept = at + 1;    // a whole list by weight ends before any cut by count that had none
-            } else {
-                c = cut_by_digits(s, 1, need, each).rank;
-            }
+            kept = -1;
+            c = cut_at(1, s.reach(1, need), need).rank;
         }
         cut = cut > c ? cut : c;
     }
@@ -326,18 +369,37 @@ __device__ inline void answer_from_list(Scratch &s, const pk_sample_desc &a, int
     int lanes = 64;
     while (lanes > 1 && kept * lanes > Scratch::kThreads) lanes >>= 1;
     const int j = tid / lanes;
-    const unsigned own = j < kept ? (unsigned)s.list[j] : 0;       // inverted indices
+    const int own = j < kept ? index_of(s.list[j]) : 0;
     u64 before = 0;
 #pragma unroll 4
     for (int i = tid & (lanes - 1); i < kept; i += lanes) {
-        const unsigned other = (unsigned)s.list[i], w = s.list_w[i];
-        before += other > own ? w : 0;
+        const unsigned w = s.list_w[i];
+        before += index_of(s.list[i]) < own ? w : 0;
     }
     for (int d = lanes >> 1; d; d >>= 1) before += __shfl_xor(before, d);
     if (j < kept && (tid & (lanes - 1)) == 0) {
         const unsigned w = s.list_w[j];
         if (before <= t && t < before + w) answer(a, b, index_of(s.list[j]), w, total, kept);
     }
+}
+
+// Sorts an unsorted list, n <= BS, whose first rule.k <= kCounted tokens are wanted; of more than kCounted those alone are
+// kept.  Returns how many are.
+template <class Scratch>
+__device__ inline int shorten(Scratch &s, const RowRule &rule, int n) {
+    if (n > Scratch::kCounted) {
+        const int tid = threadIdx.x;
+        s.weigh(n, rule);
+        const Cut c = cut_in_list(s, n, 0, (u64)rule.k);
+        const u64 v = tid < n ? s.list[tid] : 0;
+        if (tid == 0) s.n[1] = 0;
+        __syncthreads();
+        if (v >= c.rank && tid < n) s.list[atomicAdd(&s.n[1], 1)] = v;
+        __syncthreads();
+        n = rule.k;
+    }
+    s.sort(n, rule);
+    return n;
 }
 
 // A row on one workgroup, its tokens in registers: wave w has tokens (w n + e) 64 + lane, e < n <= E.
@@ -356,7 +418,7 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
         x[e] = i < end ? logit<T>(row, i) : -INFINITY;
     }
     RowRule rule;
-    rule.settings(a, b);
+    rule.settings<T>(a, b);
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
@@ -392,11 +454,11 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
         const int at = s.reach(0, (u64)rule.k), last = at < 0 ? kBins - 1 : at, listed = s.count[last];
         if (listed <= BS) {
             tokens([&](int e) {
-                if (bin[e] <= last) s.list[atomicAdd(&s.n[0], 1)] = rank_of(x[e], base + e * 64);
+                if (bin[e] <= last) s.list[atomicAdd(&s.n[0], 1)] = rule.rank(x[e], base + e * 64);
             });
             __syncthreads();
-            s.sort(listed, rule);
-            int left = min(rule.k, listed);
+            const int left0 = shorten(s, rule, listed);
+            int left = min(rule.k, left0);
             if (rule.p_on) {
                 const u64 need = share(s.list_mass[left - 1], rule.p);
                 left = s.place(left, 0, need ? need : 1) + 1;
@@ -431,23 +493,23 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
             for (int i = tid; i < V; i += BS) {
                 const float y = logit<T>(row, i);
                 const unsigned wt = rule.weight(y);
-                if (wt) f(rank_of(y, i), wt);
+                if (wt) f(rule.rank(y, i), wt);
             }
         };
         auto list = [&](int kind, int first, int last) {
             tokens([&](int e) {
-                if (bin[e] >= first && bin[e] <= last) s.list[atomicAdd(&s.n[kind], 1)] = rank_of(x[e], base + e * 64);
+                if (bin[e] >= first && bin[e] <= last) s.list[atomicAdd(&s.n[kind], 1)] = rule.rank(x[e], base + e * 64);
             });
             __syncthreads();
         };
-        const int left = find_cut(s, rule, cut, list, each);
+        const int left = find_cut(s, rule, cut, rule.rank(top, 0), list, each);
         if (left > 0) {
             answer_from_list(s, a, b, rule, left);
             return;
         }
     }
     // kept weights; each wave's sum, then the token in the wave that the drawn weight falls to
-    const float cut_x = cut ? logit_of(cut) : -INFINITY;
+    const float cut_x = cut ? rule.logit_of(cut) : -INFINITY;
     const int cut_i = cut ? index_of(cut) : 0;
     u64 mass = 0;
     unsigned kept = 0;
@@ -579,7 +641,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_hist_kernel(pk_sample
     float x[kBatch];
     load_batch<T>(row, i0 + tid, kSplitThreads, i1, x);       // on its way while the settings are read
     RowRule rule;
-    rule.settings(a, w.row0 + r);
+    rule.settings<T>(a, w.row0 + r);
     rule.top = row_max(w, r);
     s.clear();
     if ((!rule.k_on && !rule.p_on) || rule.top == -INFINITY) return;
@@ -680,7 +742,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
     if (from - lane < end) load_batch<T>(row, from, 64, end, x);      // on its way while the settings are read
     RowPick p = w.pick[r];
     RowRule rule;
-    rule.settings(a, b);
+    rule.settings<T>(a, b);
     rule.top = row_max(w, r);
     if (rule.top == -INFINITY) {
         if (chunk == 0 && tid == 0) answer(a, b, -1, 0, 0, 0);
@@ -705,7 +767,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
                     if (wt >= rule.least) mass += wt, ++kept;
                 } else if (wt) {
                     const int at = atomicAdd(&s.n[0], 1);
-                    if (at < kSplitCap) s.list[at] = rank_of(x[e], i0 + e * 64);
+                    if (at < kSplitCap) s.list[at] = rule.rank(x[e], i0 + e * 64);
                 }
             }
         }
@@ -735,23 +797,38 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
         if (tid == 0) put_shared(&w.listed[r], 0);
         __syncthreads();
         if (n) {
-            s.sort(n, rule);
-            u64 total = p.total;
-            int left = n;                    // of the list
-            if (p.bin_k >= 0) left = rule.k - (int)p.count_k;
-            if (p.bin_k >= 0 || few) total = p.mass_k + s.list_mass[left - 1];
-            if (rule.p_on) {
-                const u64 need = share(total, rule.p);
-                left = min(left, s.place(n, p.mass_first, need ? need : 1) + 1);
+            if (few || n <= s.kCounted) {
+                const int sorted = few ? shorten(s, rule, n) : n;
+                if (!few) s.sort(n, rule);
+                u64 total = p.total;
+                int left = sorted;                   // of the list
+                if (p.bin_k >= 0) left = rule.k - (int)p.count_k;
+                if (p.bin_k >= 0 || few) total = p.mass_k + s.list_mass[left - 1];
+                if (rule.p_on) {
+                    const u64 need = share(total, rule.p);
+                    left = min(left, s.place(left, p.mass_first, need ? need : 1) + 1);
+                }
+                if (p.first == 0) {
+                    answer_from_list(s, a, b, rule, left);
+                    return;
+                }
+                cut = s.list[left - 1];
+            } else {
+                s.weigh(n, rule);
+                u64 total = p.total;
+                if (p.bin_k >= 0) {
+                    const Cut c = cut_in_list(s, n, 0, (u64)rule.k - p.count_k);
+                    cut = c.rank, total = p.mass_k + c.mass;
+                }
+                if (rule.p_on) {
+                    const u64 need = share(total, rule.p);
+                    const Cut c = cut_in_list(s, n, 1, (need ? need : 1) - p.mass_first);
+                    cut = cut > c.rank ? cut : c.rank;
+                }
             }
-            if (p.first == 0 && left <= s.kCounted) {
-                answer_from_list(s, a, b, rule, left);
-                return;
-            }
-            cut = s.list[left - 1];
-            if (tid < left) {
-                const unsigned wt = s.list_w[tid];
-                if (wt >= rule.least) atomicAdd(&s_run[index_of(s.list[tid]) / run_size], (u64)wt), ++kept;
+            if (tid < n && s.list[tid] >= cut && s.list_w[tid] >= rule.least) {
+                atomicAdd(&s_run[index_of(s.list[tid]) / run_size], (u64)s.list_w[tid]);
+                ++kept;
             }
         }
     } else {
@@ -760,17 +837,17 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
             for (int i = tid; i < V; i += kSplitThreads) {
                 const float x = logit<T>(row, i);
                 const unsigned wt = rule.weight(x);
-                if (wt) f(rank_of(x, i), wt);
+                if (wt) f(rule.rank(x, i), wt);
             }
         };
         u64 total = p.total;
         if (p.bin_k >= 0) {
-            const Cut c = cut_by_digits(s, 0, (u64)rule.k, each);
+            const Cut c = cut_by_digits(s, 0, (u64)rule.k, rule.rank(rule.top, 0), each);
             cut = c.rank, total = c.mass;
         }
         if (rule.p_on) {
             const u64 need = share(total, rule.p);
-            const Cut c = cut_by_digits(s, 1, need ? need : 1, each);
+            const Cut c = cut_by_digits(s, 1, need ? need : 1, rule.rank(rule.top, 0), each);
             cut = cut > c.rank ? cut : c.rank;
         }
         for (int q = wave; q < runs; q += kRuns) {
@@ -780,7 +857,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
                 if (i >= V) break;
                 const float x = logit<T>(row, i);
                 const unsigned wt = rule.weight(x);
-                if (wt && wt >= rule.least && rank_of(x, i) >= cut) mass += wt, ++kept;
+                if (wt && wt >= rule.least && rule.rank(x, i) >= cut) mass += wt, ++kept;
             }
             mass = wave_sum(mass);
             if (lane == 0) s_run[q] = mass;
@@ -816,7 +893,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
             if (e < w.per && i < V) {
                 const float x = logit<T>(row, i);
                 const unsigned v = rule.weight(x);
-                if (v && v >= rule.least && rank_of(x, i) >= cut) wt[h] = v;
+                if (v && v >= rule.least && rule.rank(x, i) >= cut) wt[h] = v;
             }
             const u64 sum = wave_sum((u64)wt[h]);
             if (lane == 0 && e < w.per) s_row[e] = sum;

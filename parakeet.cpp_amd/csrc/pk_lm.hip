@@ -158,8 +158,9 @@ struct SampleShape {
 SampleShape sample_shape(int rows, int vocab) {
     SampleShape s{};
     if (vocab <= kRowVocab) return s;
-    // about 16 chunks a row: fewer leave one session's row on few workgroups, more are slow to add up
-    s.per = std::min(std::max((vocab + 16 * kSplitThreads - 1) / (16 * kSplitThreads), 4), kMaxChunks);
+    // about 16 chunks a row, 32 of few rows: fewer leave them on few workgroups, more are slow to add up
+    const int aim = rows <= 8 ? 32 : 16;
+    s.per = std::min(std::max((vocab + aim * kSplitThreads - 1) / (aim * kSplitThreads), 4), kMaxChunks);
     s.chunks = (vocab + s.per * kSplitThreads - 1) / (s.per * kSplitThreads);
     s.rows = std::min({rows, kSplitRowsMost, std::max(kSplitGroups / s.chunks, 1)});
     int64_t at = SampleShape::kCounterBytes;
