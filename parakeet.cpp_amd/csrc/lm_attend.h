@@ -30,7 +30,7 @@ struct AttendParams {
     const uint8_t *cache;
     const int *table, *lens, *first;
     int *arrived;       // [tiles][1 + groups] how many groups of a tile are done, how many splits of each group
-    float *part;        // [tiles][splits + groups][columns][D sums, maximum, total, 2 unused]
+    float *part;        // [tiles][splits + groups][16][D sums, maximum, total, 2 unused]
     int64_t q_row, q_head, out_row, out_head, page_stride, table_stride;
     int n_rows, requests, heads, kv_heads, page, page_shift, n_pages, width, max_len, window, group;
     int tiles, splits, groups, chunk, vec, vec_out;
@@ -113,6 +113,19 @@ __device__ inline v4f load_shared(const float *base, unsigned at) {
     return __builtin_bit_cast(v4f, load_shared4((const unsigned *)base, at));
 }
 
+// Where a lane's codes of 32 keys lie in their record, which does not change from step to step.  A step's keys are on
+// one page, or with pages of 16 (Small) on two; on one page the rest of an address is the same in the whole wave.
+template <int D, bool Small>
+struct KeyOffsets {
+    unsigned k, v;
+
+    __device__ KeyOffsets(const Record &rec) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+        k = ((8 * (c >> 2) + (c & 3)) & (Small ? 15 : 31)) * (D / 2) + g * (D / 8);
+        v = rec.v_codes() + (Small ? g & 1 : g) * (4 * D) + c * (D / 4);
+    }
+};
+
 // One step's operands of a lane: 32 keys, of K two rows' D/4 channels, of V 8 keys' D/16 channels.
 template <int D>
 struct KeyTile {
@@ -121,27 +134,38 @@ struct KeyTile {
     unsigned ks[2];
     u2 vs;
 
-    // id0, id1: pages of the tile's two 16-key halves (the same page where pages are larger), -1: none
-    __device__ void load(const AttendParams &a, const Record &rec, int64_t head_at, int kb, int id0, int id1) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-        const uint8_t *rec0 = a.cache + max(id0, 0) * a.page_stride + head_at;
-        const uint8_t *rec1 = a.cache + max(id1, 0) * a.page_stride + head_at;
-        const int koff = (kb + 8 * (c >> 2) + (c & 3)) & (a.page - 1), voff = (kb + 8 * g) & (a.page - 1);
-        const uint8_t *krec = c < 8 ? rec0 : rec1, *vrec = g < 2 ? rec0 : rec1;
+    // id0, id1: pages of the tile's two 16-key halves (the same where pages are larger), -1: none
+    template <bool Small>
+    __device__ void load_k(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0, int id1) {
+        const uint8_t *p = a.cache + head_at + max(id0, 0) * a.page_stride;
+        if (Small) p = (threadIdx.x & 8) ? a.cache + head_at + max(id1, 0) * a.page_stride : p;
+        const int off = Small ? 0 : kb & (a.page - 1);
+        const uint8_t *kp = p + off * (D / 2), *sp = p + off * (D / 32);
+        unsigned kat = at.k;
+        asm volatile("" : "+v"(kat));       // the scales' offset is worked out anew: registers are scarcer than that
+        const unsigned ksat = rec.k_scales() + (kat >> 4);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const uint8_t *code = krec + (koff + 4 * t) * (D / 2) + g * (D / 8);
-            if (D == 64) *(u2 *)k[t] = *(const u2 *)code;
+            if (D == 64) *(u2 *)k[t] = *(const u2 *)(kp + kat + 4 * t * (D / 2));
             else
 #pragma unroll
-                for (int i = 0; i < D / 128; ++i) *(u4 *)&k[t][4 * i] = *(const u4 *)(code + 16 * i);
-            const uint8_t *sc = krec + rec.k_scales() + (koff + 4 * t) * (D / 32) + g * (D / 4) / 32;
-            ks[t] = D == 256 ? *(const uint16_t *)sc : *sc;
+                for (int i = 0; i < D / 128; ++i) *(u4 *)&k[t][4 * i] = *(const u4 *)(kp + kat + 4 * t * (D / 2) + 16 * i);
+            ks[t] = D == 256 ? *(const uint16_t *)(sp + ksat + 4 * t * (D / 32)) : sp[ksat + 4 * t * (D / 32)];
         }
-        const uint8_t *code = vrec + rec.v_codes() + (voff >> 3) * (4 * D) + c * (D / 4);
+    }
+    template <bool Small>
+    __device__ void load_v(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0, int id1) {
+        const uint8_t *p = a.cache + head_at + max(id0, 0) * a.page_stride;
+        if (Small) p = (threadIdx.x & 32) ? a.cache + head_at + max(id1, 0) * a.page_stride : p;
+        const int off = Small ? 0 : kb & (a.page - 1);
+        const uint8_t *vp = p + (off >> 3) * (4 * D), *sp = p + off;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int g = lane >> 4, c = lane & 15;
+        const unsigned vsat = rec.v_scales() + (c * (D / 16) / 32) * a.page + (Small ? g & 1 : g) * 8;
 #pragma unroll
-        for (int i = 0; i < kVWords / 4; ++i) *(u4 *)&v[4 * i] = *(const u4 *)(code + 16 * i);
-        vs = *(const u2 *)(vrec + rec.v_scales() + (c * (D / 16) / 32) * a.page + voff);
+        for (int i = 0; i < kVWords / 4; ++i) *(u4 *)&v[4 * i] = *(const u4 *)(vp + at.v + 16 * i);
+        vs = *(const u2 *)(sp + vsat);
     }
     // key j's word w of V codes (D = 64: its 16 bits, in the low half)
     __device__ unsigned v_word(int j, int w) const {
@@ -282,11 +306,11 @@ __device__ inline bool last_to_come(int *counter, int of, int *s_last) {
     return *s_last;
 }
 
-// base: [n][Cols][D sums, maximum, total, 2 unused]; finish(column, quad, sums of its 4 channels, maximum, total)
-template <int D, int Cols, int Threads, class Finish>
+// base: [n][16][D sums, maximum, total, 2 unused]; finish(column, quad, sums of its 4 channels, maximum, total)
+template <int D, class Finish>
 __device__ inline void join_some(const float *base, int n, int live, float to_log2, Finish finish) {
     constexpr int kQuads = D / 4, kRow = D + 4;
-    for (int u = threadIdx.x; u < live * kQuads; u += Threads) {
+    for (int u = threadIdx.x; u < live * kQuads; u += kAttendThreads) {
         const int col = u / kQuads, quad = u % kQuads;
         v4f o = {0, 0, 0, 0};
         float top = -INFINITY, total = 0;
@@ -295,7 +319,7 @@ __device__ inline void join_some(const float *base, int n, int live, float to_lo
             v4f x[8], ml[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const unsigned p = (min(i0 + i, n - 1) * Cols + col) * kRow;
+                const unsigned p = (min(i0 + i, n - 1) * 16 + col) * kRow;
                 x[i] = load_shared(base, p + 4 * quad), ml[i] = load_shared(base, p + D);
             }
             float t2 = top;
@@ -314,29 +338,29 @@ __device__ inline void join_some(const float *base, int n, int live, float to_lo
 }
 
 // This split's sums are in its place of tile `at`; `mine` splits have keys.
-template <int D, int Cols, int Threads, class Finish>
+template <int D, class Finish>
 __device__ inline void join(const AttendParams &a, int64_t at, int split, int mine, int live, float to_log2, int *s_last, Finish finish) {
-    constexpr int kPlace = Cols * (D + 4);
+    constexpr int kPlace = 16 * (D + 4);
     float *all = a.part + at * (a.splits + a.groups) * kPlace, *joined = all + (int64_t)a.splits * kPlace;
     int *arrived = a.arrived + at * (1 + a.groups);
     const int group = split / kJoin, groups = (mine + kJoin - 1) / kJoin, n = min(kJoin, mine - group * kJoin);
     if (!last_to_come(arrived + 1 + group, n, s_last)) return;
     const float *base = all + (int64_t)group * kJoin * kPlace;
     if (groups == 1) {
-        join_some<D, Cols, Threads>(base, n, live, to_log2, finish);
+        join_some<D>(base, n, live, to_log2, finish);
         return;
     }
-    join_some<D, Cols, Threads>(base, n, live, to_log2, [&](int col, int quad, v4f o, float top, float total) {
-        const unsigned p = (group * Cols + col) * (D + 4);
+    join_some<D>(base, n, live, to_log2, [&](int col, int quad, v4f o, float top, float total) {
+        const unsigned p = (group * 16 + col) * (D + 4);
         store_shared(joined, p + 4 * quad, o);
         if (quad == 0) store_shared(joined, p + D, v4f{top, total, 0, 0});
     });
     if (!last_to_come(arrived, groups, s_last)) return;
-    join_some<D, Cols, Threads>(joined, groups, live, to_log2, finish);
+    join_some<D>(joined, groups, live, to_log2, finish);
 }
 
 // One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.
-template <class T, int D>
+template <class T, int D, bool Small>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
     constexpr int kTiles = D / 16, kRow = D + 4;
@@ -390,24 +414,32 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
     constexpr int kStride = 32 * kAttendWaves;
     int kb = k0 + 32 * wave;
     if (kb < k1) {
-        // the next step's operands are on their way while this one's are worked on, the pages after that looked up
-        KeyTile<D> cur, next;
-        int id0 = page_of(kb), id1 = page_of(kb + 16);
-        int n0 = page_of(kb + kStride), n1 = page_of(kb + kStride + 16);
-        cur.load(a, rec, head_at, kb, id0, id1);
+        // The next step's K is read into this one's registers as soon as the scores are formed, V after the sums; pages are
+        // looked up a step ahead.  (A second set of registers, read a whole step ahead, spills where two planes of Q and P
+        // are held, and takes longer elsewhere too: 64 sessions of up to 4,097 keys 37.5 us against 35.1, 200,003 and
+        // 100,001 keys in f16 48.5 against 29.4.)
+        const KeyOffsets<D, Small> at(rec);
+        KeyTile<D> x;
+        auto second = [&](int first, int key) { return Small ? page_of(key + 16) : first; };
+        int id0 = page_of(kb), id1 = second(id0, kb);
+        int n0 = page_of(kb + kStride), n1 = second(n0, kb + kStride);
+        x.load_k(a, rec, at, head_at, kb, id0, id1);
+        x.load_v(a, rec, at, head_at, kb, id0, id1);
         for (;;) {
             const int nb = kb + kStride < k1 ? kb + kStride : kb;
             const int l0 = nb == kb ? id0 : n0, l1 = nb == kb ? id1 : n1;
-            next.load(a, rec, head_at, nb, l0, l1);
-            n0 = page_of(nb + kStride), n1 = page_of(nb + kStride + 16);
+            n0 = page_of(nb + kStride), n1 = second(n0, nb + kStride);
             v4f s[2];
-            sm.scores(cur, q, s);
-            u2 vs = cur.vs;
+            sm.scores(x, q, s);
+            __builtin_amdgcn_sched_barrier(0);
+            x.load_k(a, rec, at, head_at, nb, l0, l1);
+            u2 vs = x.vs;
             if (kb + 32 > hi_min || kb < lo_max || id0 < 0 || id1 < 0)
                 sm.mask(s, vs, kb + 8 * g, (g < 2 ? id0 : id1) >= 0, lo, hi, lo_min, hi_max);
-            sm.add(s, cur, vs, to_log2);
+            sm.add(s, x, vs, to_log2);
+            __builtin_amdgcn_sched_barrier(0);
+            x.load_v(a, rec, at, head_at, nb, l0, l1);
             if (nb == kb) break;
-            cur = next;
             kb = nb, id0 = l0, id1 = l1;
         }
     }
@@ -472,7 +504,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
             if (quad == 0) store_shared(all, p + D, v4f{top, total, 0, 0});
         }
     }
-    if (mine > 1) join<D, 16, kAttendThreads>(a, at, split, mine, live, to_log2, &s_last, finish);
+    if (mine > 1) join<D>(a, at, split, mine, live, to_log2, &s_last, finish);
 }
 
 // ---- many query rows: prompts ----
@@ -492,6 +524,21 @@ __device__ inline v16f mfma32(u4 a, u4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
+// As KeyOffsets, for a thread's share of 64 keys.  Small: they may be on pages of their own, of 16 or 32 tokens.
+template <int D, bool Small>
+struct PromptOffsets {
+    unsigned k, ks, v, vs;
+
+    __device__ PromptOffsets(const AttendParams &a, const Record &rec) {
+        const int t = threadIdx.x, quarter = t & 3, r = (t >> 1) & 15, half = t & 1;
+        const int tokens = Small ? min(a.page, 64) : 64, kkey = (t >> 2) & (tokens - 1), vkey = ((t >> 5) * 8) & (tokens - 1);
+        k = kkey * (D / 2) + quarter * (D / 8);
+        ks = rec.k_scales() + kkey * (D / 32) + quarter * (D / 4) / 32;
+        v = rec.v_codes() + (vkey >> 3) * (4 * D) + r * (D / 4) + (D == 256 ? 4 * half : 0);
+        vs = rec.v_scales() + (r * (D / 16) / 32) * a.page + vkey;
+    }
+};
+
 // One thread's share of 64 keys' bytes: of K a quarter of a key's channels, of V half the channels of an entry of 8 keys.
 template <int D>
 struct PromptBytes {
@@ -509,30 +556,29 @@ struct PromptBytes {
         vs = u2{a, b};
     }
 
-    __device__ void load(const AttendParams &a, const Record &rec, int64_t head_at, int kb, int kid, int vid) {
-        const int t = threadIdx.x, kkey = kb + (t >> 2), quarter = t & 3;
-        const int vkey = kb + (t >> 5) * 8, r = (t >> 1) & 15, half = t & 1;
-        const uint8_t *krec = a.cache + max(kid, 0) * a.page_stride + head_at, *vrec = a.cache + max(vid, 0) * a.page_stride + head_at;
-        const int koff = kkey & (a.page - 1), voff = vkey & (a.page - 1);
-        const uint8_t *code = krec + koff * (D / 2) + quarter * (D / 8);
-        if (D == 64) *(u2 *)k = *(const u2 *)code;
+    // kid, vid: pages of this thread's keys, the same for all threads where pages hold 64 tokens or more (not Small)
+    template <bool Small>
+    __device__ void load(const AttendParams &a, const PromptOffsets<D, Small> &at, int64_t head_at, int kb, int kid, int vid) {
+        const int half = threadIdx.x & 1, off = kb & (a.page - 1);
+        const uint8_t *krec = a.cache + max(kid, 0) * a.page_stride + head_at;
+        const uint8_t *vrec = Small ? a.cache + max(vid, 0) * a.page_stride + head_at : krec;
+        const uint8_t *kp = krec + off * (D / 2), *ksp = krec + off * (D / 32), *vp = vrec + (off >> 3) * (4 * D), *vsp = vrec + off;
+        if (D == 64) *(u2 *)k = *(const u2 *)(kp + at.k);
         else
 #pragma unroll
-            for (int i = 0; i < D / 128; ++i) *(u4 *)&k[4 * i] = *(const u4 *)(code + 16 * i);
-        const uint8_t *sc = krec + rec.k_scales() + koff * (D / 32) + quarter * (D / 4) / 32;
-        ks = D == 256 ? *(const uint16_t *)sc : *sc;
-        const uint8_t *vcode = vrec + rec.v_codes() + (voff >> 3) * (4 * D) + r * (D / 4);
+            for (int i = 0; i < D / 128; ++i) *(u4 *)&k[4 * i] = *(const u4 *)(kp + at.k + 16 * i);
+        ks = D == 256 ? *(const uint16_t *)(ksp + at.ks) : ksp[at.ks];
         if (D == 64) {
-            const u4 w = *(const u4 *)vcode;
+            const u4 w = *(const u4 *)(vp + at.v);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[2 * i] = w[i] >> (8 * half), v[2 * i + 1] = w[i] >> (16 + 8 * half);
         } else if (D == 128) {
-            *(u4 *)&v[0] = *(const u4 *)vcode, *(u4 *)&v[4] = *(const u4 *)(vcode + 16);
+            *(u4 *)&v[0] = *(const u4 *)(vp + at.v), *(u4 *)&v[4] = *(const u4 *)(vp + at.v + 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = *(const unsigned *)(vcode + 8 * i + 4 * half);
+            for (int i = 0; i < 8; ++i) v[i] = *(const unsigned *)(vp + at.v + 8 * i);
         }
-        vs = *(const u2 *)(vrec + rec.v_scales() + (r * (D / 16) / 32) * a.page + voff);
+        vs = *(const u2 *)(vsp + at.vs);
     }
 };
 
@@ -596,13 +642,13 @@ struct alignas(16) PromptTile {
     }
 };
 
-template <class T, int D>
+template <class T, int D, bool Small>
 __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_prompt_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
-    constexpr int kSteps = D / 16, kTiles = D / 32, kRow = D + 4;
+    constexpr int kSteps = D / 16, kTiles = D / 32;
     using Raw = typename T::Raw;
     __shared__ PromptTile<D> s_tile[2];
-    __shared__ int s_missing[2], s_last;
+    __shared__ int s_missing[2];
 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, c = lane & 31;
     // the last tiles of a prompt see the most keys: they go first
@@ -610,7 +656,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
     const int hk = id % a.kv_heads;
     id /= a.kv_heads;
     const int turn = id / a.requests, b = (id + turn) % a.requests;       // turned on: see attend_kernel
-    const int split = turn % a.splits, tile = a.tiles - 1 - turn / a.splits;
+    const int tile = a.tiles - 1 - turn;
 
     const int f0 = a.first ? a.first[b] : b, f1 = a.first ? a.first[b + 1] : b + 1;
     const int q0 = max(f0, 0), q1 = min(f1, a.n_rows), rows = (q1 - q0) * a.group, row0 = tile * kPromptCols;
@@ -621,10 +667,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
     auto begin_of = [&](int r) { return a.window ? max(place0 + r / a.group + 1 - a.window, 0) : 0; };
     const int row_last = min(row0 + kPromptCols, rows) - 1;
     const int hi_min = end_of(row0), hi_max = end_of(row_last), lo_min = begin_of(row0), lo_max = begin_of(row_last);
-    const int start = lo_min & ~(kPromptKeys - 1);
-    const int mine = max((hi_max - start + a.chunk - 1) / a.chunk, 1);
-    if (split >= mine) return;
-    const int k0 = start + split * a.chunk, k1 = min(k0 + a.chunk, hi_max);
+    const int k0 = lo_min & ~(kPromptKeys - 1), k1 = hi_max;
 
     // this wave's columns
     const int wrow0 = row0 + wave * 32, row = min(wrow0 + c, rows - 1), tok = row / a.group, head = hk * a.group + row % a.group;
@@ -680,17 +723,20 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
     const int kkey = t >> 2, vkey = (t >> 5) * 8;        // of 64, in this thread's staging
     auto edge_at = [&](int kb) { return kb + kPromptKeys > hi_min || kb < lo_max; };
     if (k0 < k1) {
+        const PromptOffsets<D, Small> offsets(a, rec);
         PromptBytes<D> bytes;
-        int kid = page_of(k0 + kkey), vid = page_of(k0 + vkey);
-        bytes.load(a, rec, head_at, k0, kid, vid);
+        auto page_k = [&](int key) { return page_of(Small ? key + kkey : key); };
+        auto page_v = [&](int key, int k_page) { return Small ? page_of(key + vkey) : k_page; };
+        int kid = page_k(k0), vid = page_v(k0, kid);
+        bytes.load(a, offsets, head_at, k0, kid, vid);
         if (t < 2) s_missing[t] = -1;
         __syncthreads();
         if (kid < 0 || vid < 0) s_missing[0] = k0;       // which tile of this buffer lacks a page
         s_tile[0].clean(bytes, k0, edge_at(k0), vid >= 0, lo_min, hi_max);
         s_tile[0].stage(bytes);
-        kid = page_of(k0 + kPromptKeys + kkey), vid = page_of(k0 + kPromptKeys + vkey);
-        bytes.load(a, rec, head_at, k0 + kPromptKeys, kid, vid);
-        int kid2 = page_of(k0 + 2 * kPromptKeys + kkey), vid2 = page_of(k0 + 2 * kPromptKeys + vkey);
+        kid = page_k(k0 + kPromptKeys), vid = page_v(k0 + kPromptKeys, kid);
+        bytes.load(a, offsets, head_at, k0 + kPromptKeys, kid, vid);
+        int kid2 = page_k(k0 + 2 * kPromptKeys), vid2 = page_v(k0 + 2 * kPromptKeys, kid2);
         __syncthreads();
         int buf = 0;
         // While a tile is worked on, the next one is unpacked (between the products of Q and K, which leave the vector
@@ -740,8 +786,8 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
                 }
             }
             kid = kid2, vid = vid2;
-            bytes.load(a, rec, head_at, kb + 2 * kPromptKeys, kid, vid);
-            kid2 = page_of(kb + 3 * kPromptKeys + kkey), vid2 = page_of(kb + 3 * kPromptKeys + vkey);
+            bytes.load(a, offsets, head_at, kb + 2 * kPromptKeys, kid, vid);
+            kid2 = page_k(kb + 3 * kPromptKeys), vid2 = page_v(kb + 3 * kPromptKeys, kid2);
             if (active) {
                 const bool missing = s_missing[buf] == kb;
                 if (kb + kPromptKeys > whi_min || kb < wlo_max || missing) {
@@ -852,55 +898,27 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
         for (int n = 0; n < kTiles; ++n) v[2 * n] = acc[n][4 * half + i], v[2 * n + 1] = acc[n][8 + 4 * half + i];
         return 8 * half + 4 * h + i;
     };
-    auto lse_of = [&](float top, float total) { return total == 0.0f ? -INFINITY : top * to_log2 * kLn2 + logf(total); };
-    if (mine == 1) {
-        if (!live) return;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        Raw *out = (Raw *)a.out + (int64_t)(q0 + tok) * a.out_row + head * a.out_head;
+    if (!live) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    Raw *out = (Raw *)a.out + (int64_t)(q0 + tok) * a.out_row + head * a.out_head;
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[D / 16];
-                const int r = entry(half, i, v);
-                alignas(8) Raw w[D / 16];
+        for (int i = 0; i < 4; ++i) {
+            float v[D / 16];
+            const int r = entry(half, i, v);
+            alignas(8) Raw w[D / 16];
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) w[j] = T::put(v[j] * inv);
-                Raw *o = out + r * (D / 16);
-                if (a.vec_out)
+            for (int j = 0; j < D / 16; ++j) w[j] = T::put(v[j] * inv);
+            Raw *o = out + r * (D / 16);
+            if (a.vec_out)
 #pragma unroll
-                    for (int j = 0; j < D / 64; ++j) ((u2 *)o)[j] = ((u2 *)w)[j];
-                else
+                for (int j = 0; j < D / 64; ++j) ((u2 *)o)[j] = ((u2 *)w)[j];
+            else
 #pragma unroll
-                    for (int j = 0; j < D / 16; ++j) o[j] = w[j];
-            }
-        if (a.lse && h == 0) a.lse[(int64_t)(q0 + tok) * a.heads + head] = lse_of(m, l);
-        return;
-    }
-    const int64_t at = ((int64_t)b * a.kv_heads + hk) * a.tiles + tile;
-    float *all = a.part + at * (a.splits + a.groups) * kPromptCols * kRow;
-    if (live) {
-        const unsigned p = (split * kPromptCols + wave * 32 + c) * kRow;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[D / 16];
-                const int r = entry(half, i, v);
-#pragma unroll
-                for (int j = 0; j < D / 16; j += 4) store_shared(all, p + r * (D / 16) + j, v4f{v[j], v[j + 1], v[j + 2], v[j + 3]});
-            }
-        if (h == 0) store_shared(all, p + D, v4f{m, l, 0, 0});
-    }
-    join<D, kPromptCols, kPromptThreads>(a, at, split, mine, min(rows - row0, kPromptCols), to_log2, &s_last,
-                                         [&](int col, int quad, v4f o, float top, float total) {
-        const int r = row0 + col, tk = r / a.group, hd = hk * a.group + r % a.group;
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        Raw *out = (Raw *)a.out + (int64_t)(q0 + tk) * a.out_row + hd * a.out_head + 4 * quad;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = T::put(o[i] * inv);
-        if (a.lse && quad == 0) a.lse[(int64_t)(q0 + tk) * a.heads + hd] = lse_of(top, total);
-    });
+                for (int j = 0; j < D / 16; ++j) o[j] = w[j];
+        }
+    if (a.lse && h == 0) a.lse[(int64_t)(q0 + tok) * a.heads + head] = l == 0.0f ? -INFINITY : m * to_log2 * kLn2 + logf(l);
 }
 
 }  // namespace pklm

@@ -89,30 +89,33 @@ int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
 // no call's partial sums lie where another's counters are.  A split call has at most kSplitWork tiles times splits, and
 // a tile 1 + (splits + 15) / 16 counters.
 constexpr int kSplitWork = 512, kCounters = 4 * kSplitWork;
-// more query rows of a request and kv head than this go to the prompt kernel
-constexpr int kPromptFrom = 64;
+// attend_prompt_kernel takes calls of more than kPromptRows query rows to a request and kv head that give it kPromptGroups
+// workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  Requests of
+// uneven length up to 8,191, 32 heads on 8, D = 128, microseconds of the prompt kernel and of the other: 16 requests of up
+// to 64 new tokens (256 workgroups) 169 and 117, 128 (512) 251 and 196, 256 (1,024) 296 and 349; one request of 512 (128)
+// 118 and 124, 2,048 (512) 271 and 429.
+constexpr int kPromptRows = 64, kPromptGroups = 512;
 
 // How a call's work is dealt out, from its host-known sizes alone.
 struct AttendShape {
     bool prompt;             // attend_prompt_kernel, 128 query rows a workgroup; else attend_kernel, 16
-    int cols, tiles, chunk, splits, groups;
+    int tiles, chunk, splits, groups;
     int64_t part_bytes;
     int64_t bytes() const { return splits > 1 ? kCounters * 4 + part_bytes : 0; }
 };
 
 int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
-    s.prompt = rows > kPromptFrom;
-    s.cols = s.prompt ? kPromptCols : 16;
-    const int step = s.prompt ? kPromptKeys : 32 * kAttendWaves;
-    const int64_t tiles = (rows + s.cols - 1) / s.cols;
+    const int64_t prompt_tiles = (rows + kPromptCols - 1) / kPromptCols;
+    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= kPromptGroups;
+    const int64_t tiles = s.prompt ? prompt_tiles : (rows + 15) / 16, step = 32 * kAttendWaves;
     // keys of one tile: its rows span at most as many tokens
-    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + s.cols + 64) : d.max_len;
+    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 64) : d.max_len;
     // Split where the tiles leave the card short of work (512 workgroups are resident), into no less than 512 keys.
     // 200,003 and 100,001 keys on 2 kv heads, 64 sessions of up to 4,097 keys on 8: 35.0 and 37.9 us; for twice as many
     // splits 42.7 and 39.0, for four times 50.0 and 41.1.
     const int64_t want = kSplitWork, least = 512, each = std::max<int64_t>(pairs * tiles, 1);
-    int64_t splits = std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
+    int64_t splits = s.prompt ? 1 : std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
     const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
     if (pairs * tiles * splits > INT32_MAX)
@@ -120,7 +123,7 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
                        (long long)rows);
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
     s.groups = (int)((splits + kJoin - 1) / kJoin);
-    s.part_bytes = pairs * tiles * (splits + s.groups) * s.cols * (d.head_dim + 4) * 4;
+    s.part_bytes = pairs * tiles * (splits + s.groups) * 16 * (d.head_dim + 4) * 4;
     return PK_OK;
 }
 
@@ -206,8 +209,12 @@ void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s
 
 template <class T, int D>
 void launch_attend(const AttendParams &p, bool prompt, unsigned grid, hipStream_t s) {
-    if (prompt) attend_prompt_kernel<T, D><<<grid, kPromptThreads, 0, s>>>(p);
-    else attend_kernel<T, D><<<grid, kAttendThreads, 0, s>>>(p);
+    // pages of whole key tiles: addresses are worked out a wave at a time.  A prompt of 512 tokens x 4 on up to 8,191 keys
+    // takes 431 us with f16 rows of 128 then, 443 otherwise; of D = 256, whose registers are full, 664 and 521.
+    if (prompt && (D == 256 || p.page < kPromptKeys)) attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+    else if (prompt) attend_prompt_kernel<T, D, D == 256><<<grid, kPromptThreads, 0, s>>>(p);
+    else if (p.page < 32) attend_kernel<T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
+    else attend_kernel<T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
 }
 
 template <class T>
