@@ -22,7 +22,6 @@ typedef unsigned long long u64;
 
 constexpr float kReach = 22.0f;            // distance that the bins cover
 constexpr float kWeighed = -21.6f;         // a distance beyond this has no weight: exp(-21.6) < 2^-31
-constexpr int kWholeMost = 64;             // of a cut by weight: tokens up to which the list holds all before the cut too
 constexpr int kCountShift = 46;            // (count, weight) of up to 2^15 tokens in one word: 2^15 2^30 < 2^46
 constexpr u64 kMassMask = (1ull << kCountShift) - 1;
 
@@ -88,14 +87,14 @@ struct Cut {
 
 __device__ inline int index_of(u64 rank) { return (1 << kIndexBits) - 1 - (int)(rank & ((1 << kIndexBits) - 1)); }
 
-// What a workgroup of BS threads keeps in LDS to find a cut.
-template <int BS, int Bins>
+// What a workgroup of BS threads keeps in LDS to find a cut: List, the most tokens that are listed.
+template <int BS, int Bins, int List = BS>
 struct CutScratch {
     static constexpr int kThreads = BS, kBins = Bins, kCounted = BS / 4;
     u64 mass[Bins];                  // (count, weight) of a bin in one word; then running weight
     unsigned count[Bins];            // running count of tokens
-    u64 list[BS], list_mass[BS];     // rank words, falling once sorted; running weight
-    unsigned list_w[BS];             // weight
+    u64 list[List], list_mass[BS];   // rank words, falling once sorted; running weight
+    unsigned list_w[List];           // weight
     u64 wave_mass[BS / 64];
     unsigned wave_count[BS / 64];
     u64 digit_mass[256];
@@ -193,10 +192,9 @@ struct CutScratch {
         __syncthreads();
     }
 
-    // Weights of an unsorted list, n <= BS.
+    // Weights of an unsorted list.
     __device__ void weigh(int n_list, const RowRule &rule) {
-        const int tid = threadIdx.x;
-        if (tid < n_list) list_w[tid] = rule.weight(rule.logit_of(list[tid]));
+        for (int i = threadIdx.x; i < n_list; i += BS) list_w[i] = rule.weight(rule.logit_of(list[i]));
         __syncthreads();
     }
 
@@ -291,59 +289,40 @@ __device__ inline Cut cut_by_digits(Scratch &s, int kind, u64 want, u64 some, Ea
 // The same of an unsorted list with weights.
 template <class Scratch>
 __device__ inline Cut cut_in_list(Scratch &s, int n, int kind, u64 want) {
-    const int tid = threadIdx.x;
     return cut_by_digits<true>(s, kind, want, s.list[0], [&](auto f) {
-        if (tid < n) f(s.list[tid], s.list_w[tid]);
+        for (int i = threadIdx.x; i < n; i += Scratch::kThreads) f(s.list[i], s.list_w[i]);
     });
 }
 
-// The cut of a row whose bins are scanned.  list(kind, first, last) lists the tokens of some bins; each(f) and some are
-// as above.  Returns how many tokens the cut leaves where the sorted list holds all of them, else -1.
+// The cut of a row whose bins are scanned.  list(kind, bin) lists a bin's tokens; each(f) and some are as above.
 template <class Scratch, class List, class Each>
-__device__ inline int find_cut(Scratch &s, const RowRule &rule, u64 &cut, u64 some, List list, Each each) {
-    u64 total = s.mass[Scratch::kBins - 1];
-    int kept = -1, n = 0;
-    bool whole = false;
-    // the token in bin b at which the count or the weight reaches `want`, from a list of the bins up to b, or of b alone
+__device__ inline u64 find_cut(Scratch &s, const RowRule &rule, u64 some, List list, Each each) {
+    // the token in bin b at which the count or the weight reaches `want`
     auto cut_at = [&](int kind, int b, u64 want) {
-        whole = s.count_to(b) <= kWholeMost;
-        n = s.count_to(b) - (whole ? 0 : s.count_to(b - 1));
+        const int n = s.count_to(b) - s.count_to(b - 1);
         if (n > Scratch::kThreads) return cut_by_digits(s, kind, want, some, each);
-        list(kind, whole ? 0 : b, b);
-        if (whole) {
-            s.sort(n, rule);
-            const int at = kind ? s.place(n, 0, want) : (int)want - 1;
-            kept = at + 1;
-            return Cut{s.list[at], s.list_mass[at]};
-        }
+        list(kind, b);
         s.weigh(n, rule);
         const u64 c0 = s.count_to(b - 1), m0 = s.mass_to(b - 1);
         Cut c = cut_in_list(s, n, kind, want - (kind ? m0 : c0));
         c.mass += m0;
         return c;
     };
-    bool have = false;       // a sorted list with every token that may be kept
+    u64 cut = 0, total = s.mass[Scratch::kBins - 1];
     if (rule.k_on) {
         const int b = s.reach(0, (u64)rule.k);
         if (b >= 0) {
             const Cut c = cut_at(0, b, (u64)rule.k);
-            cut = c.rank, total = c.mass, have = whole;
+            cut = c.rank, total = c.mass;
         }
     }
     if (rule.p_on) {
         u64 need = share(total, rule.p);
         need = need ? need : 1;              // the first token is kept whatever the share
-        u64 c;
-        if (have) {
-            const int at = s.place(n, 0, need);
-            c = s.list[at], kept = at + 1;
-        } else {
-            kept = -1;
-            c = cut_at(1, s.reach(1, need), need).rank;
-        }
+        const u64 c = cut_at(1, s.reach(1, need), need).rank;
         cut = cut > c ? cut : c;
     }
-    return kept;
+    return cut;
 }
 
 // Sets a row's results.
@@ -496,17 +475,13 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
                 if (wt) f(rule.rank(y, i), wt);
             }
         };
-        auto list = [&](int kind, int first, int last) {
+        auto list = [&](int kind, int at) {
             tokens([&](int e) {
-                if (bin[e] >= first && bin[e] <= last) s.list[atomicAdd(&s.n[kind], 1)] = rule.rank(x[e], base + e * 64);
+                if (bin[e] == at) s.list[atomicAdd(&s.n[kind], 1)] = rule.rank(x[e], base + e * 64);
             });
             __syncthreads();
         };
-        const int left = find_cut(s, rule, cut, rule.rank(top, 0), list, each);
-        if (left > 0) {
-            answer_from_list(s, a, b, rule, left);
-            return;
-        }
+        cut = find_cut(s, rule, rule.rank(top, 0), list, each);
     }
     // kept weights; each wave's sum, then the token in the wave that the drawn weight falls to
     const float cut_x = cut ? rule.logit_of(cut) : -INFINITY;
@@ -548,7 +523,7 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
 // chunk to arrive adds up and names the bins to list from; the kept weight of each chunk's 16 runs with the listed
 // tokens beside, from which the row's last chunk finds the cut, the run and the token.
 
-constexpr int kSplitThreads = 1024, kSplitBins = 1024, kSplitCap = kSplitThreads, kRuns = kSplitThreads / 64, kMaxChunks = 32;
+constexpr int kSplitThreads = 1024, kSplitBins = 1024, kSplitCap = 4096, kRuns = kSplitThreads / 64, kMaxChunks = 32;
 
 // What is listed of a row: the tokens of the bins first .. last, and of bin_k.
 struct RowPick {
@@ -713,7 +688,6 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_hist_kernel(pk_sample
         const int b1 = s.reach(1, need_high ? need_high : 1);
         p.first = p.bin_k >= 0 ? min(b0, p.bin_k) : b0, p.last = p.bin_k >= 0 ? min(b1, p.bin_k) : b1;
     }
-    if (p.first < kSplitBins && count_to(max(p.last, p.bin_k)) <= kWholeMost) p.first = 0, p.last = max(p.last, p.bin_k);     // all that may be kept
     if (tid == 0) {
         const unsigned ranged = count_to(p.last) - count_to(p.first - 1);
         const bool apart = p.bin_k > p.last;
@@ -730,7 +704,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_hist_kernel(pk_sample
 
 template <class T>
 __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample_desc a, SplitRows w) {
-    __shared__ CutScratch<kSplitThreads, kSplitBins> s;
+    __shared__ CutScratch<kSplitThreads, kSplitBins, kSplitCap> s;
     __shared__ u64 s_run[kMaxChunks * kRuns], s_row[kMaxChunks];
     __shared__ int s_flag, s_at;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -749,7 +723,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
         return;
     }
     if (!rule.k_on && !rule.p_on) p = RowPick{kSplitBins, kSplitBins - 1, -1, 0, 0, 0, 0, 0, 0};
-    const bool crowded = p.n > kSplitCap, few = few_by_count(rule);
+    const bool few = few_by_count(rule), crowded = p.n > (few ? kSplitThreads : kSplitCap);
     if (!crowded) {
         if (tid == 0) s.n[0] = 0;
         __syncthreads();
@@ -789,7 +763,7 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
     unsigned kept = 0;
     if (!crowded) {
         const int n = p.n;
-        if (tid < n) s.list[tid] = get_shared(&w.list_rank[(int64_t)r * kSplitCap + tid]);
+        for (int i = tid; i < n; i += kSplitThreads) s.list[i] = get_shared(&w.list_rank[(int64_t)r * kSplitCap + i]);
         if (tid < runs) {
             s_run[tid] = get_shared(&w.run_mass[(int64_t)r * runs + tid]);
             kept = get_shared(&w.run_kept[(int64_t)r * runs + tid]);
@@ -826,10 +800,11 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
                     cut = cut > c.rank ? cut : c.rank;
                 }
             }
-            if (tid < n && s.list[tid] >= cut && s.list_w[tid] >= rule.least) {
-                atomicAdd(&s_run[index_of(s.list[tid]) / run_size], (u64)s.list_w[tid]);
-                ++kept;
-            }
+            for (int i = tid; i < n; i += kSplitThreads)
+                if (s.list[i] >= cut && s.list_w[i] >= rule.least) {
+                    atomicAdd(&s_run[index_of(s.list[i]) / run_size], (u64)s.list_w[i]);
+                    ++kept;
+                }
         }
     } else {
         // more tokens at the cut than the list holds: this workgroup goes over the row by itself

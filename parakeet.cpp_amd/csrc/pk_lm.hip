@@ -47,7 +47,9 @@ int check_cache(const char *what, const void *cache, int64_t page_stride, int pa
 
 template <class T, int D, bool Store>
 void launch_rows(const pk_kv4_rows_desc &d, int wide, hipStream_t s) {
-    const int pass = kRowThreads * 8 / D, many = d.n_rows > 4096;
+    // Several passes a thread where there are values for it: 24,577 rows of 8 heads x 128 in bf16 take 53.4 us, 54.8 in single
+    // passes, 40,000 rows 93.3 and 98.0; 8,192 rows 19.7 and 18.3, 24,577 of 2 heads x 64 in f32 15.9 and 14.5.
+    const int pass = kRowThreads * 8 / D, many = (int64_t)d.n_rows * d.heads * D >= 1 << 24;
     const unsigned blocks = (unsigned)((d.n_rows + (many ? kRowPasses : 1) * pass - 1) / ((many ? kRowPasses : 1) * pass));
     const dim3 grid(blocks, 2 * d.heads);
     if (many) rows_kernel<T, D, Store, kRowPasses><<<grid, kRowThreads, 0, s>>>(d, log2i(d.page), wide);
@@ -148,7 +150,9 @@ int attend_check(const pk_kv4_attend_desc *d) {
     return PK_OK;
 }
 
-// Sampling.  A row of up to kRowVocab logits is one workgroup's, its tokens in registers; longer rows are cut in chunks.
+// Sampling.  A row of up to kRowVocab logits is one workgroup's, its tokens in registers, 16 a thread; longer rows are cut in
+// chunks, in three launches.  Rows of 16,384 in f32 with filters, microseconds on one workgroup and in chunks: 1 row 9.8 and
+// 18.4, 64 rows 21.6 and 23.8, 512 rows 48 and 96.
 constexpr int kRowVocab = 16384, kSplitRowsMost = 512, kSplitGroups = 2048;
 
 struct SampleShape {
@@ -161,8 +165,11 @@ struct SampleShape {
 SampleShape sample_shape(int rows, int vocab) {
     SampleShape s{};
     if (vocab <= kRowVocab) return s;
-    // about 16 chunks a row, 32 of few rows: fewer leave them on few workgroups, more are slow to add up
-    const int aim = rows <= 8 ? 32 : 16;
+    // As many chunks a row as give each of the card's 256 units one, 2 to 16: more are slow to add up.  128,001 logits in
+    // bf16, microseconds at 4, 8, 16 and 32 chunks: one row by top-p 43.8, 33.5, 28.3, 29.6; 8 rows 43.8, 33.4, 30.0,
+    // 34.5; 64 rows each with its own filters 45.7, 46.3, 60.9, 95.8; 256 rows 115, 144, 206 at 4, 8 and 16.  256 rows of
+    // 32,000 at 2 and 4: 43.1, 58.5.
+    const int aim = std::min(std::max(256 / std::max(rows, 1), 2), 16);
     s.per = std::min(std::max((vocab + aim * kSplitThreads - 1) / (aim * kSplitThreads), 4), kMaxChunks);
     s.chunks = (vocab + s.per * kSplitThreads - 1) / (s.per * kSplitThreads);
     s.rows = std::min({rows, kSplitRowsMost, std::max(kSplitGroups / s.chunks, 1)});
@@ -186,8 +193,11 @@ SampleShape sample_shape(int rows, int vocab) {
 template <class T>
 void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s) {
     const unsigned rows = (unsigned)d.rows;
+    // A workgroup of 256 or of 1,024 threads: the larger is quicker by itself, of the smaller four fit in its place.  Rows of
+    // 2,000 logits, microseconds: 256 rows 12.2 and 10.2, 384 rows 12.4 and 16.1; of 1,000: 64 rows 9.5 and 9.8, 512 rows
+    // 10.8 and 17.3; of 4,000: 64 rows 14.7 and 10.8, 512 rows 19.1 and 20.7 (without filters 12.2 and 10.9).
     if (d.vocab <= 1024) sample_row_kernel<T, 256, 4><<<rows, 256, 0, s>>>(d);
-    else if (d.vocab <= 2048) sample_row_kernel<T, 256, 8><<<rows, 256, 0, s>>>(d);
+    else if (d.vocab <= 2048 && d.rows > 256) sample_row_kernel<T, 256, 8><<<rows, 256, 0, s>>>(d);
     else if (d.vocab <= 4096) sample_row_kernel<T, 1024, 4><<<rows, 1024, 0, s>>>(d);
     else if (d.vocab <= kRowVocab) sample_row_kernel<T, 1024, 16><<<rows, 1024, 0, s>>>(d);
     else {
