@@ -136,7 +136,8 @@ struct KeyTile {
 
     // id0, id1: pages of the tile's two 16-key halves (the same where pages are larger), -1: none
     template <bool Small>
-    __device__ void load_k(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0, int id1) {
+    __device__ void load_k(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0,
+                           int id1) {
         const uint8_t *p = a.cache + head_at + max(id0, 0) * a.page_stride;
         if (Small) p = (threadIdx.x & 8) ? a.cache + head_at + max(id1, 0) * a.page_stride : p;
         const int off = Small ? 0 : kb & (a.page - 1);
@@ -154,7 +155,8 @@ struct KeyTile {
         }
     }
     template <bool Small>
-    __device__ void load_v(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0, int id1) {
+    __device__ void load_v(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0,
+                           int id1) {
         const uint8_t *p = a.cache + head_at + max(id0, 0) * a.page_stride;
         if (Small) p = (threadIdx.x & 32) ? a.cache + head_at + max(id1, 0) * a.page_stride : p;
         const int off = Small ? 0 : kb & (a.page - 1);
@@ -359,7 +361,12 @@ __device__ inline void join(const AttendParams &a, int64_t at, int split, int mi
     join_some<D>(joined, groups, live, to_log2, finish);
 }
 
-// One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.
+// One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.  Each wave
+// keeps its own maximum, sum and O of all columns, in registers, and they meet once at the end: keys are read and unpacked
+// once and no step waits for another wave.  What bounds it is memory where sessions are many: 64 of up to 4,097 keys, 32
+// heads on 8 of 128 channels, 146 MB in 34.8 us (4.2 TB/s, a large copy 4.9); then the unpacking, two bf16 planes and the
+// join: 200,003 and 100,001 keys on 2 kv heads in f16, 82 MB in 29.3 us (2.8 TB/s).  One session of 733 keys: 7.3 us, a
+// launch, four steps and one join.
 template <class T, int D, bool Small>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
@@ -515,6 +522,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
 // the maximum crosses lanes once per 64 keys; row 8b + 4h + i of a score tile stands for key 16 (b / 2) + 8h + 4 (b % 2) + i,
 // which makes a lane's scores its own operand of O^T as above.  V lies transposed, row 16j + r holding channel
 // (D/16) r + j: rows that 16 lanes write together are adjacent.
+//
+// Four prompts of up to 2,047 tokens on up to 4,095 keys, 32 heads on 8 of 128 channels in bf16: 225 us, 163 GFLOP at 0.72
+// PFLOP/s, where a large library product of bf16 reaches 1.22.  A wave and 64 keys take 1,024 cycles of matrix instructions
+// and about 1,400 of vector ones (the exponentials and the unpacking); of two waves a vector unit the one's seldom run
+// beside the other's for long.  Memory is not full (26 MB fetched).  Splitting the keys in two to shorten the tail took 342 us.
 
 constexpr int kPromptThreads = 256, kPromptCols = 128, kPromptKeys = 64;
 
@@ -744,6 +756,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
         for (int kb = k0; kb < k1; kb += kPromptKeys, buf ^= 1) {
             const int nb = kb + kPromptKeys;
             PromptTile<D> &next = s_tile[buf ^ 1];
+            if (D < 256) __builtin_amdgcn_s_setprio(0);
             if (kid < 0 || vid < 0) s_missing[buf ^ 1] = nb;
             next.clean(bytes, nb, edge_at(nb), vid >= 0, lo_min, hi_max);
             const bool active = kb < whi_max && nb > wlo_min;
@@ -862,6 +875,9 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
                     for (int n = 0; n < kTiles; ++n)
                         vv[g & 1][n] = *(const u4 *)(x.v + (32 * n + c) * PromptTile<D>::kVRow + 32 * g + 16 * h);
                 };
+                // Waves that sum go before the other workgroup's that unpack: 231 -> 225 us; in f16, 512 tokens x 4 on up to
+                // 8,191 keys, 408 -> 383.  (D = 256 is alone on its unit.)
+                if (D < 256) __builtin_amdgcn_s_setprio(1);
                 operands(0);
                 __builtin_amdgcn_sched_barrier(0);
                 exponentials(0);

@@ -114,8 +114,8 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     // keys of one tile: its rows span at most as many tokens
     const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 64) : d.max_len;
     // Split where the tiles leave the card short of work (512 workgroups are resident), into no less than 512 keys.
-    // 200,003 and 100,001 keys on 2 kv heads, 64 sessions of up to 4,097 keys on 8: 35.0 and 37.9 us; for twice as many
-    // splits 42.7 and 39.0, for four times 50.0 and 41.1.
+    // 200,003 and 100,001 keys on 2 kv heads, 64 sessions of up to 4,097 keys on 8, 8 of up to 32,000: 29.5, 35.8 and 40.6
+    // us; for twice as many splits 34.3, 37.2 and 43.3, for half as many 29.3, 36.1 and 46.0.
     const int64_t want = kSplitWork, least = 512, each = std::max<int64_t>(pairs * tiles, 1);
     int64_t splits = s.prompt ? 1 : std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
     const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
@@ -220,7 +220,7 @@ void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s
 template <class T, int D>
 void launch_attend(const AttendParams &p, bool prompt, unsigned grid, hipStream_t s) {
     // pages of whole key tiles: addresses are worked out a wave at a time.  A prompt of 512 tokens x 4 on up to 8,191 keys
-    // takes 431 us with f16 rows of 128 then, 443 otherwise; of D = 256, whose registers are full, 664 and 521.
+    // takes 431 us with f16 rows of 128 then, 443 otherwise; of D = 256, whose registers are full, 664 and 526.
     if (prompt && (D == 256 || p.page < kPromptKeys)) attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
     else if (prompt) attend_prompt_kernel<T, D, D == 256><<<grid, kPromptThreads, 0, s>>>(p);
     else if (p.page < 32) attend_kernel<T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
