@@ -95,7 +95,8 @@ constexpr int kSplitWork = 512, kCounters = 4 * kSplitWork;
 // workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  Requests of
 // uneven length up to 8,191, 32 heads on 8, D = 128, microseconds of the prompt kernel and of the other: 16 requests of up
 // to 64 new tokens (256 workgroups) 169 and 117, 128 (512) 251 and 196, 256 (1,024) 296 and 349; one request of 512 (128)
-// 118 and 124, 2,048 (512) 271 and 429.
+// 118 and 124, 2,048 (512) 271 and 429.  Not f16 rows of 256, which its registers do not hold: two requests of up to 1,024
+// new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
 constexpr int kPromptRows = 64, kPromptGroups = 512;
 
 // How a call's work is dealt out, from its host-known sizes alone.
@@ -109,7 +110,7 @@ struct AttendShape {
 int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
     const int64_t prompt_tiles = (rows + kPromptCols - 1) / kPromptCols;
-    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= kPromptGroups;
+    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= kPromptGroups && !(d.dtype == PK_DTYPE_F16 && d.head_dim == 256);
     const int64_t tiles = s.prompt ? prompt_tiles : (rows + 15) / 16, step = 32 * kAttendWaves;
     // keys of one tile: its rows span at most as many tokens
     const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 64) : d.max_len;
@@ -221,9 +222,13 @@ template <class T, int D>
 void launch_attend(const AttendParams &p, bool prompt, unsigned grid, hipStream_t s) {
     // pages of whole key tiles: addresses are worked out a wave at a time.  A prompt of 512 tokens x 4 on up to 8,191 keys
     // takes 431 us with f16 rows of 128 then, 443 otherwise; of D = 256, whose registers are full, 664 and 526.
-    if (prompt && (D == 256 || p.page < kPromptKeys)) attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
-    else if (prompt) attend_prompt_kernel<T, D, D == 256><<<grid, kPromptThreads, 0, s>>>(p);
-    else if (p.page < 32) attend_kernel<T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
+    if constexpr (D == 256 && __is_same(T, BF16)) {
+        if (prompt) return attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+    } else if constexpr (D < 256) {
+        if (prompt && p.page < kPromptKeys) return attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt) return attend_prompt_kernel<T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
+    }
+    if (p.page < 32) attend_kernel<T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
     else attend_kernel<T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
 }
 
