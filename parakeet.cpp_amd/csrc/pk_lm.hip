@@ -95,10 +95,11 @@ constexpr int kSplitWork = 512, kCounters = 4 * kSplitWork;
 // workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  Requests of
 // uneven length up to 8,191, 32 heads on 8, D = 128, microseconds of the prompt kernel and of the other: 16 requests of up
 // to 64 new tokens (256 workgroups) 169 and 117, 128 (512) 251 and 196, 256 (1,024) 296 and 349; one request of 512 (128)
-// 118 and 124, 2,048 (512) 271 and 429; bf16 rows of 256, four requests of up to 512 tokens on 6,000 keys (512) 398 and 365,
-// 1,024 (1,024) 645 and 674, 2,047 (2,048) 1,012 and 1,220.  Not f16 rows of 256, which its registers do not hold: two requests of up to 1,024
+// 118 and 124, 2,048 (512) 271 and 429; bf16 rows of 256, four requests of up to 512 tokens on 6,000 keys (512) 398 and
+// 365, 1,024 (1,024) 645 and 674, 2,047 (2,048) 1,012 and 1,220.  64 requests on up to 2,047 keys: 64 rows each 69 and 43,
+// 96 rows 69 and 55, 128 rows 70 and 70.  Not f16 rows of 256, which its registers do not hold: two requests of up to 1,024
 // new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
-constexpr int kPromptRows = 64, kPromptGroups = 512;
+constexpr int kPromptRows = 128, kPromptGroups = 512;
 
 // How a call's work is dealt out, from its host-known sizes alone.
 struct AttendShape {
