@@ -602,8 +602,8 @@ struct alignas(16) PromptTile {
     uint8_t nan[kPromptKeys][D / 32];       // of an edge tile: blocks of V that are NaN
 
     // What lies at keys without a page may be anything; so at an edge, where some column does not see some key, at keys
-    // outside [lo, hi), which no column sees.  NaN blocks of the others are taken out there and marked.
-    __device__ void clean(PromptBytes<D> &x, int kb, bool edge, bool vfine, int lo, int hi) {
+    // outside [lo, hi), which no column sees.  NaN blocks of the others are taken out there and marked; marked becomes kb.
+    __device__ void clean(PromptBytes<D> &x, int kb, bool edge, bool vfine, int lo, int hi, int &marked) {
         const int t = threadIdx.x, a8 = t >> 5, r = (t >> 1) & 15;
         if (edge || !vfine) {
 #pragma unroll
@@ -611,6 +611,7 @@ struct alignas(16) PromptTile {
                 const int at = 8 * (j & 3), kj = kb + 8 * a8 + j;
                 const bool dead = !vfine || kj >= hi || kj < lo, bad = (x.vs[j >> 2] >> at & 255u) == 255u;
                 if (edge) nan[8 * a8 + j][r * (D / 16) / 32] = bad && !dead;     // by all threads of the block alike
+                if (bad && !dead) marked = kb;
                 if (bad || dead) x.vs[j >> 2] = (x.vs[j >> 2] & ~(255u << at)) | 127u << at;
             }
         }
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
     constexpr int kSteps = D / 16, kTiles = D / 32;
     using Raw = typename T::Raw;
     __shared__ PromptTile<D> s_tile[2];
-    __shared__ int s_missing[2];
+    __shared__ int s_missing[2], s_marked[2];       // the tile of each buffer that lacks a page, has marked NaN blocks
 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, c = lane & 31;
     // the last tiles of a prompt see the most keys: they go first
@@ -741,10 +742,10 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
         auto page_v = [&](int key, int k_page) { return Small ? page_of(key + vkey) : k_page; };
         int kid = page_k(k0), vid = page_v(k0, kid);
         bytes.load(a, offsets, head_at, k0, kid, vid);
-        if (t < 2) s_missing[t] = -1;
+        if (t < 2) s_missing[t] = s_marked[t] = -1;
         __syncthreads();
-        if (kid < 0 || vid < 0) s_missing[0] = k0;       // which tile of this buffer lacks a page
-        s_tile[0].clean(bytes, k0, edge_at(k0), vid >= 0, lo_min, hi_max);
+        if (kid < 0 || vid < 0) s_missing[0] = k0;
+        s_tile[0].clean(bytes, k0, edge_at(k0), vid >= 0, lo_min, hi_max, s_marked[0]);
         s_tile[0].stage(bytes);
         kid = page_k(k0 + kPromptKeys), vid = page_v(k0 + kPromptKeys, kid);
         bytes.load(a, offsets, head_at, k0 + kPromptKeys, kid, vid);
@@ -758,7 +759,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
             PromptTile<D> &next = s_tile[buf ^ 1];
             if (D < 256) __builtin_amdgcn_s_setprio(0);
             if (kid < 0 || vid < 0) s_missing[buf ^ 1] = nb;
-            next.clean(bytes, nb, edge_at(nb), vid >= 0, lo_min, hi_max);
+            next.clean(bytes, nb, edge_at(nb), vid >= 0, lo_min, hi_max, s_marked[buf ^ 1]);
             const bool active = kb < whi_max && nb > wlo_min;
             v16f s[2];
             const PromptTile<D> &x = s_tile[buf];
@@ -802,16 +803,16 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
             bytes.load(a, offsets, head_at, kb + 2 * kPromptKeys, kid, vid);
             kid2 = page_k(kb + 3 * kPromptKeys), vid2 = page_v(kb + 3 * kPromptKeys, kid2);
             if (active) {
-                const bool missing = s_missing[buf] == kb;
-                if (kb + kPromptKeys > whi_min || kb < wlo_max || missing) {
-                    const bool edge = edge_at(kb);
+                // a tile can be an edge, its NaN blocks marked, for other waves' columns and whole for this one's
+                const bool missing = s_missing[buf] == kb, marked = s_marked[buf] == kb;
+                if (kb + kPromptKeys > whi_min || kb < wlo_max || missing || marked) {
                     unsigned bad = 0;             // channel blocks whose NaN this column sees
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int at = 32 * (i >> 4) + 16 * (i >> 3 & 1) + 8 * h + (i & 7), key = kb + at;
                         const bool see = key < hi && key >= lo && !(missing && page_of(key) < 0);
                         if (!see) s[i >> 4][i & 15] = -INFINITY;
-                        else if (edge)
+                        else if (marked)
 #pragma unroll
                             for (int j = 0; j < D / 32; ++j) bad |= (unsigned)x.nan[at][j] << j;
                     }
