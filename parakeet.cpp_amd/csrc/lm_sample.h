@@ -815,12 +815,13 @@ __global__ __launch_bounds__(kSplitThreads, 8) void sample_pick_kernel(pk_sample
                 }
         }
     } else {
-        // more tokens at the cut than the list holds: this workgroup goes over the row by itself
+        // more tokens at the cut than the list holds: this workgroup goes over the row by itself, over the tokens that the
+        // bins counted (a count by logits alone has some whose weight is none, so that it may reach k where weights do not)
         auto each = [&](auto f) {
             for (int i = tid; i < V; i += kSplitThreads) {
                 const float x = logit<T>(row, i);
                 const unsigned wt = rule.weight(x);
-                if (wt) f(rule.rank(x, i), wt);
+                if (few ? rule.distance(x) > kWeighed : wt != 0) f(rule.rank(x, i), wt);
             }
         };
         u64 total = p.total;
