@@ -130,11 +130,14 @@ int32_t narrow(int64_t v, const char *what) {
     return (int32_t)v;
 }
 
-// Workspaces by kind of call, device and stream.  They only grow, and one that was handed out is never freed: a captured
-// graph may hold it.
+// Workspaces by kind of call, device and stream, and by capture where a graph is being captured: a graph has its own and
+// zeroes it whenever it is replayed, so it may be replayed before, after and beside other graphs and eager calls.  They only
+// grow, and one that was handed out is never freed: a captured graph may hold it.
+constexpr int64_t kEager = -1;
 struct Workspace {
     int kind, device;
     void *stream;
+    int64_t capture;        // the capture's number, or kEager
     int64_t bytes;
     at::Tensor t;
 };
@@ -142,6 +145,23 @@ std::vector<Workspace> &workspaces() {
     static auto *all = new std::vector<Workspace>;      // not destroyed at exit: the runtime may be gone by then
     return *all;
 }
+
+int64_t capture_of(void *stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id);
+    if (e != hipSuccess) throw Refused{PyExc_RuntimeError, std::string("hipStreamGetCaptureInfo: ") + hipGetErrorString(e)};
+    return status == hipStreamCaptureStatusNone ? kEager : (int64_t)(id & 0x7FFFFFFFFFFFFFFFull);
+}
+
+// Makes a stream torch's current one.
+struct CurrentStream {
+    c10::hip::HIPStream before;
+    CurrentStream(void *stream, c10::DeviceIndex device) : before(c10::hip::getCurrentHIPStream(device)) {
+        if ((void *)before.stream() != stream) c10::hip::setCurrentHIPStream(c10::hip::getStreamFromExternal((hipStream_t)stream, device));
+    }
+    ~CurrentStream() { c10::hip::setCurrentHIPStream(before); }
+};
 
 void workspace(Call &c, int given, int kind, void *stream, int64_t wanted, void *&ptr, int64_t &bytes) {
     if (!c.none(given)) {
@@ -153,19 +173,19 @@ void workspace(Call &c, int given, int kind, void *stream, int64_t wanted, void 
     ptr = nullptr, bytes = 0;
     if (wanted == 0) return;
     auto &all = workspaces();
+    const int64_t capture = capture_of(stream);
     for (auto w = all.rbegin(); w != all.rend(); ++w)
-        if (w->kind == kind && w->device == c.device.index() && w->stream == stream) {
+        if (w->kind == kind && w->device == c.device.index() && w->stream == stream && w->capture == capture) {
             if (w->bytes < wanted) break;
             ptr = w->t.data_ptr(), bytes = w->bytes;
             return;
         }
     int64_t size = 1 << 20;
     while (size < wanted) size *= 2;
+    const CurrentStream here(stream, c.device.index());      // zeroed in the order of the calls that use it
     at::Tensor t = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(c.device));
-    const auto now = c10::hip::getCurrentHIPStream(c.device.index());
-    if ((void *)now.stream() != stream) now.synchronize();      // zeroed on torch's stream, used on another
     ptr = t.data_ptr(), bytes = size;
-    all.push_back({kind, (int)c.device.index(), stream, size, std::move(t)});
+    all.push_back({kind, (int)c.device.index(), stream, capture, size, std::move(t)});
 }
 
 // f(call) -> status, with its C++ exceptions turned into Python's

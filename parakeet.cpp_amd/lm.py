@@ -19,7 +19,9 @@ library's status.
 
 Workspaces (``kv4_attend``, ``sample``) are kept per operator, device and stream and only
 ever grow; one that has been handed out is never freed, since a captured graph
-may hold it.  Give ``workspace=`` (zeroed uint8) to keep your own.
+may hold it.  For torch tensors a graph's capture has its own, which the graph zeroes, so that
+graphs may be replayed in any order and beside each other.  Give ``workspace=`` (zeroed
+uint8) to keep your own.
 
 torch tensors are read by an extension of their own (csrc/lm_torch.cpp), others
 here, through ctypes.  torch and this library have to share one HIP runtime:
