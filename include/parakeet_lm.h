@@ -78,7 +78,8 @@ PK_API int pk_kv_plan(const pk_kv_plan_desc *desc, void *stream);
  * outside the cache are skipped.  Blocks are rounded to the nearest code, ties
  * to the even code, under the power of two that puts the largest of the 32
  * values between 3.5 and 7 (kept to 2^-120 .. 2^125, so that smaller blocks
- * vanish and the largest stay finite). */
+ * vanish and the largest stay finite; f16 rows over 57,344 are held as 65,536,
+ * which f16 results, of pk_kv4_attend too, give as 65,504). */
 typedef struct pk_kv4_rows_desc {
     void *k, *v;                        /* read by pk_kv4_store, written by pk_kv4_load */
     const int32_t *slots;

@@ -484,7 +484,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
         Raw *out = (Raw *)a.out + (int64_t)(q0 + t) * a.out_row + h * a.out_head + 4 * quad;
         Raw v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = T::put(o[i] * inv);
+        for (int i = 0; i < 4; ++i) v[i] = T::put(T::held(o[i] * inv));
         if (a.vec_out) *(u2 *)out = *(u2 *)v;
         else
 #pragma unroll
@@ -926,7 +926,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
             const int r = entry(half, i, v);
             alignas(8) Raw w[D / 16];
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) w[j] = T::put(v[j] * inv);
+            for (int j = 0; j < D / 16; ++j) w[j] = T::put(T::held(v[j] * inv));
             Raw *o = out + r * (D / 16);
             if (a.vec_out)
 #pragma unroll

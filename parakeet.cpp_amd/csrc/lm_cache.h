@@ -162,6 +162,9 @@ __device__ inline void some_rows(const pk_kv4_rows_desc &a, int page_shift, int 
     x[p][2 * i] = two[0], x[p][2 * i + 1] = two[1];
             PK_TWO(0) PK_TWO(1) PK_TWO(2) PK_TWO(3)
 #undef PK_TWO
+            if (scale[p] >= 127 + 14)                    // 4 x 2^14 is the first value past f16's largest
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[p][i] = T::held(x[p][i]);
             store8<T>(x_at + (row0 + p * kPass) * x_row, wide, x[p]);
         }
     }

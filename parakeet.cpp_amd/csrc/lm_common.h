@@ -21,21 +21,26 @@ __device__ inline float f16_f32(unsigned short h) { return (float)__builtin_bit_
 __device__ inline unsigned short f32_bf16(float x) { return __builtin_bit_cast(unsigned short, (__bf16)x); }
 __device__ inline unsigned short f32_f16(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
 
-// Element types: f32 and the two 16-bit ones.
+// Element types: f32 and the two 16-bit ones.  held: a value of the cache, or a mean of such, as the type is to have it.
 struct F32 {
     using Raw = float;
     __device__ static float get(Raw v) { return v; }
     __device__ static Raw put(float v) { return v; }
+    __device__ static float held(float v) { return v; }
 };
 struct F16 {
     using Raw = unsigned short;
     __device__ static float get(Raw v) { return f16_f32(v); }
     __device__ static Raw put(float v) { return f32_f16(v); }
+    // The cache holds f16 rows over 57,344 as 65,536, the step past f16's largest value: that, and means of it to their
+    // rounding, go back to 65,504, so that finite rows stay finite.  Beyond it there are infinities as in any conversion.
+    __device__ static float held(float v) { return fabsf(v) <= 0x1.002p16f ? fminf(fmaxf(v, -65504.0f), 65504.0f) : v; }
 };
 struct BF16 {
     using Raw = unsigned short;
     __device__ static float get(Raw v) { return bf16_f32(v); }
     __device__ static Raw put(float v) { return f32_bf16(v); }
+    __device__ static float held(float v) { return v; }
 };
 
 // 2^e of whole numbers -126 .. 127
