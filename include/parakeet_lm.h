@@ -65,9 +65,10 @@ typedef struct pk_kv_plan_desc {
     int32_t *lens;                      /* out [requests] lengths after the call; neither old_len nor new_len */
     int32_t *ok;                        /* out [requests] 1 = served */
     int32_t *first;                     /* out [requests + 1]: new tokens before request b (served or not) */
-    int32_t *slots;                     /* out [n_tokens]: slot of each new token, -1 for tokens of requests not served
-                                           and behind the last token */
-    int32_t *pos;                       /* out [n_tokens]: its position in its request, -1 likewise; nullable */
+    int32_t *slots;                     /* out [n_tokens]: slot of each new token, -1 for tokens of requests not served,
+                                           behind the last token, and on page ids that are negative or have no 32-bit slots */
+    int32_t *pos;                       /* out [n_tokens]: its position in its request, -1 for tokens of requests not served
+                                           and behind the last token; nullable */
     int64_t table_stride;
     int32_t requests, width, n_pages, page, n_tokens;
 } pk_kv_plan_desc;

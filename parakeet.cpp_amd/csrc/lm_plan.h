@@ -85,6 +85,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, i
         a.state_out[1] = min(count - s_used + gone, a.n_pages);
     }
 
+    // A slot, -1 where the id is no page: negative, or so large that its slots are past 32 bits and would wrap to others.
+    auto slot_at = [&](int id, int q) {
+        return (unsigned)id <= (unsigned)INT32_MAX >> shift ? (id << shift) + (q & (page - 1)) : -1;
+    };
     // page j of request b, which holds `had` pages and takes new ones from place `al` of the ring on
     auto page_at = [&](int b, int j, int had, int al_b) {
         const int64_t place = (int64_t)head + al_b + (j - had);
@@ -109,7 +113,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, i
 #pragma unroll
                     for (int i = 0; i < kPlanTokens; ++i) {
                         const int q = p + i, id = q >> shift == j0 ? id0 : id1;
-                        slot[i] = (id << shift) + (q & (page - 1));
+                        slot[i] = slot_at(id, q);
                         pos[i] = q;
                         // a new page's first token is new: it enters the page into the table
                         if ((q & (page - 1)) == 0) a.table[b * a.table_stride + (q >> shift)] = id;
@@ -124,7 +128,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, i
                     if (al_b < 0) continue;
                     const int o = s_old[b], q = o + (int)(t - s_first[b]);
                     const int id = page_at(b, q >> shift, pages(o), al_b);
-                    slot[i] = (id << shift) + (q & (page - 1));
+                    slot[i] = slot_at(id, q);
                     pos[i] = q;
                     if ((q & (page - 1)) == 0) a.table[b * a.table_stride + (q >> shift)] = id;
                 }
