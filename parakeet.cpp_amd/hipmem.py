@@ -23,6 +23,8 @@ def hip():
         L.hipFree.argtypes = [C.c_void_p]
         L.hipMemcpy.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]
         L.hipMemset.argtypes = [C.c_void_p, C.c_int, C.c_size_t]
+        L.hipGetDevice.argtypes = [C.POINTER(C.c_int)]
+        L.hipStreamIsCapturing.argtypes = [C.c_void_p, C.POINTER(C.c_int)]
         L.hipGetErrorString.restype = C.c_char_p
         _hip = L
     return _hip
@@ -128,6 +130,20 @@ class Tensor:
 
     def zero(self):
         self.buffer.zero()
+
+
+def device() -> int:
+    """The current device."""
+    d = C.c_int()
+    _check(hip().hipGetDevice(C.byref(d)), "hipGetDevice")
+    return d.value
+
+
+def capturing(stream) -> bool:
+    """Whether a graph is being captured on the stream."""
+    status = C.c_int()
+    _check(hip().hipStreamIsCapturing(stream, C.byref(status)), "hipStreamIsCapturing")
+    return status.value != 0
 
 
 def synchronize():

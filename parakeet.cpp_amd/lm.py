@@ -20,8 +20,9 @@ library's status.
 Workspaces (``kv4_attend``, ``sample``) are kept per operator, device and stream and only
 ever grow; one that has been handed out is never freed, since a captured graph
 may hold it.  For torch tensors a graph's capture has its own, which the graph zeroes, so that
-graphs may be replayed in any order and beside each other.  Give ``workspace=`` (zeroed
-uint8) to keep your own.
+graphs may be replayed in any order and beside each other.  Other graphs share their
+stream's: one that is to run beside calls on that stream, or beside another of its
+graphs, is given a ``workspace=`` (zeroed uint8) of its own.
 
 torch tensors are read by an extension of their own (csrc/lm_torch.cpp), others
 here, through ctypes.  torch and this library have to share one HIP runtime:
@@ -171,13 +172,19 @@ def kv4_shape(n_pages: int, kv_heads: int, head_dim: int, page: int):
 
 
 def _workspace(kind, stream, wanted, given):
-    """(pointer, bytes) of at least `wanted` bytes, zeroed before the first use; each kind of call has its own."""
+    """(pointer, bytes) of at least `wanted` bytes, zeroed before the first use; each kind of call has its own on each device
+    and stream."""
     if given is not None:
+        if given.dtype != "u8" or not given.is_contiguous():
+            raise TypeError("workspace: not contiguous uint8")
         return given.data_ptr(), given.numel()
     if wanted == 0:
         return 0, 0
-    kept = _workspaces.setdefault((kind, stream), [])
+    kept = _workspaces.setdefault((kind, hipmem.device(), stream), [])
     if not kept or kept[-1].numel() < wanted:
+        if hipmem.capturing(stream):
+            raise RuntimeError(f"{kind}: a workspace of {wanted} bytes cannot be made during a capture: give workspace=, "
+                               "or make one call of these sizes on the stream before")
         t = hipmem.Tensor((max(1 << 20, 1 << (wanted - 1).bit_length()),), "u8")
         t.zero()
         hipmem.synchronize()
