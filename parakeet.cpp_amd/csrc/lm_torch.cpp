@@ -11,6 +11,7 @@
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -56,6 +57,8 @@ struct Call {
         } else if (t.device() != device) {
             value_error("arrays on " + device.str() + " and on " + t.device().str());
         }
+        if (t.requires_grad() && c10::GradMode::is_enabled())
+            value_error(std::string(what) + " requires a gradient, and these operators have none: call them under torch.no_grad()");
         return t;
     }
     bool none(int i) const { return args[i] == Py_None; }

@@ -25,7 +25,10 @@ stream's: one that is to run beside calls on that stream, or beside another of i
 graphs, is given a ``workspace=`` (zeroed uint8) of its own.
 
 torch tensors are read by an extension of their own (csrc/lm_torch.cpp), others
-here, through ctypes.  torch and this library have to share one HIP runtime:
+here, through ctypes.  The operators have no backward pass: a tensor that requires a
+gradient is refused unless gradients are off (``torch.no_grad()``).  Tensors given with a
+``stream`` other than torch's current one have to stay until it has passed the call
+(``Tensor.record_stream``).  torch and this library have to share one HIP runtime:
 where torch tensors are used, import torch before the library is first loaded.
 """
 from __future__ import annotations
