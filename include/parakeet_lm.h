@@ -115,7 +115,7 @@ typedef struct pk_kv4_attend_desc {
     int32_t max_new;                    /* no request brings more queries */
     int32_t max_len;                    /* no request holds more tokens (longer ones are cut there) */
     int32_t window;                     /* 0 = none */
-    float scale;
+    float scale;                        /* finite */
 } pk_kv4_attend_desc;
 PK_API int pk_kv4_attend(const pk_kv4_attend_desc *desc, void *stream);
 /* Bytes of workspace that the call wants (host arithmetic; pointers are not looked at). */

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 
@@ -143,6 +144,7 @@ int attend_check(const pk_kv4_attend_desc *d) {
                        d->max_new, d->max_len, d->window, d->width);
     if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, d->head_dim);
+    if (!std::isfinite(d->scale)) return pk_fail(PK_ERR_ARG, "%s: a scale of %g", what, d->scale);
     if ((int64_t)std::max(d->n_rows, d->max_new) * (d->heads / d->kv_heads) > INT32_MAX - 4096)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows, max_new %d, %d query heads a kv head: row numbers are 32 bits", what, d->n_rows, d->max_new,
                        d->heads / d->kv_heads);
