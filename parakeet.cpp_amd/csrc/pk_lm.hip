@@ -25,6 +25,9 @@ bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0;
 bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
 int log2i(int v) { return 31 - __builtin_clz((unsigned)v); }
 
+// A launch has fewer than 2^32 threads.
+constexpr int64_t most_groups(int threads) { return UINT32_MAX / threads; }
+
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? PK_OK : pk_fail(PK_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
@@ -46,13 +49,18 @@ int check_cache(const char *what, const void *cache, int64_t page_stride, int pa
     return PK_OK;
 }
 
+// Several passes a thread where there are values for it: 24,577 rows of 8 heads x 128 in bf16 take 53.4 us, 54.8 in single
+// passes, 40,000 rows 93.3 and 98.0; 8,192 rows 19.7 and 18.3, 24,577 of 2 heads x 64 in f32 15.9 and 14.5.
+bool many_rows(const pk_kv4_rows_desc &d) { return (int64_t)d.n_rows * d.heads * d.head_dim >= 1 << 24; }
+int64_t row_groups(const pk_kv4_rows_desc &d) {
+    const int each = kRowThreads * 8 / d.head_dim * (many_rows(d) ? kRowPasses : 1);
+    return ((int64_t)d.n_rows + each - 1) / each;
+}
+
 template <class T, int D, bool Store>
 void launch_rows(const pk_kv4_rows_desc &d, int wide, hipStream_t s) {
-    // Several passes a thread where there are values for it: 24,577 rows of 8 heads x 128 in bf16 take 53.4 us, 54.8 in single
-    // passes, 40,000 rows 93.3 and 98.0; 8,192 rows 19.7 and 18.3, 24,577 of 2 heads x 64 in f32 15.9 and 14.5.
-    const int pass = kRowThreads * 8 / D, many = (int64_t)d.n_rows * d.heads * D >= 1 << 24;
-    const unsigned blocks = (unsigned)((d.n_rows + (many ? kRowPasses : 1) * pass - 1) / ((many ? kRowPasses : 1) * pass));
-    const dim3 grid(blocks, 2 * d.heads);
+    const bool many = many_rows(d);
+    const dim3 grid((unsigned)row_groups(d), 2 * d.heads);
     if (many) rows_kernel<T, D, Store, kRowPasses><<<grid, kRowThreads, 0, s>>>(d, log2i(d.page), wide);
     else rows_kernel<T, D, Store, 1><<<grid, kRowThreads, 0, s>>>(d, log2i(d.page), wide);
 }
@@ -78,6 +86,8 @@ int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
     if (!aligned(d->k, size) || !aligned(d->v, size) || !aligned(d->slots, 4))
         return pk_fail(PK_ERR_ARG, "%s: rows or slots not aligned to their type", what);
     if (d->heads > 32767) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d heads (at most 32767)", what, d->heads);
+    if (row_groups(*d) > most_groups(kRowThreads))
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d channels in one call", what, d->n_rows, d->head_dim);
     const int per = 16 / size;
     const int wide = aligned(d->k, 16) && aligned(d->v, 16) && d->k_row % per == 0 && d->k_head % per == 0 &&
                      d->v_row % per == 0 && d->v_head % per == 0;
@@ -113,6 +123,11 @@ struct AttendShape {
 int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
     const int64_t prompt_tiles = (rows + kPromptCols - 1) / kPromptCols;
+    auto too_many = [&] {
+        return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
+                       (long long)rows);
+    };
+    if (pairs > most_groups(kPromptThreads)) return too_many();
     s.prompt = rows > kPromptRows && pairs * prompt_tiles >= kPromptGroups && !(d.dtype == PK_DTYPE_F16 && d.head_dim == 256);
     const int64_t tiles = s.prompt ? prompt_tiles : (rows + 15) / 16, step = 32 * kAttendWaves;
     // keys of one tile: its rows span at most as many tokens
@@ -124,9 +139,7 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     int64_t splits = s.prompt ? 1 : std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
     const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
-    if (pairs * tiles * splits > INT32_MAX)
-        return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
-                       (long long)rows);
+    if (pairs * tiles * splits > most_groups(s.prompt ? kPromptThreads : kAttendThreads)) return too_many();
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
     s.groups = (int)((splits + kJoin - 1) / kJoin);
     s.part_bytes = pairs * tiles * (splits + s.groups) * 16 * (d.head_dim + 4) * 4;
@@ -195,14 +208,16 @@ SampleShape sample_shape(int rows, int vocab) {
     return s;
 }
 
+// A workgroup of 256 or of 1,024 threads a row: the larger is quicker by itself, of the smaller four fit in its place.  Rows of
+// 2,000 logits, microseconds: 256 rows 12.2 and 10.2, 384 rows 12.4 and 16.1; of 1,000: 64 rows 9.5 and 9.8, 512 rows
+// 10.8 and 17.3; of 4,000: 64 rows 14.7 and 10.8, 512 rows 19.1 and 20.7 (without filters 12.2 and 10.9).
+int row_threads(const pk_sample_desc &d) { return d.vocab <= 1024 || (d.vocab <= 2048 && d.rows > 256) ? 256 : 1024; }
+
 template <class T>
 void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s) {
     const unsigned rows = (unsigned)d.rows;
-    // A workgroup of 256 or of 1,024 threads: the larger is quicker by itself, of the smaller four fit in its place.  Rows of
-    // 2,000 logits, microseconds: 256 rows 12.2 and 10.2, 384 rows 12.4 and 16.1; of 1,000: 64 rows 9.5 and 9.8, 512 rows
-    // 10.8 and 17.3; of 4,000: 64 rows 14.7 and 10.8, 512 rows 19.1 and 20.7 (without filters 12.2 and 10.9).
     if (d.vocab <= 1024) sample_row_kernel<T, 256, 4><<<rows, 256, 0, s>>>(d);
-    else if (d.vocab <= 2048 && d.rows > 256) sample_row_kernel<T, 256, 8><<<rows, 256, 0, s>>>(d);
+    else if (row_threads(d) == 256) sample_row_kernel<T, 256, 8><<<rows, 256, 0, s>>>(d);
     else if (d.vocab <= 4096) sample_row_kernel<T, 1024, 4><<<rows, 1024, 0, s>>>(d);
     else if (d.vocab <= kRowVocab) sample_row_kernel<T, 1024, 16><<<rows, 1024, 0, s>>>(d);
     else {
@@ -347,6 +362,8 @@ PK_API int pk_sample(const pk_sample_desc *d, void *stream) {
     if (d->dtype != PK_DTYPE_F32 && d->dtype != PK_DTYPE_F16 && d->dtype != PK_DTYPE_BF16)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
     if (!aligned(d->logits, d->dtype == PK_DTYPE_F32 ? 4 : 2)) return pk_fail(PK_ERR_ARG, "%s: logits not aligned to their type", what);
+    if (d->vocab <= kRowVocab && d->rows > most_groups(row_threads(*d)))
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d logits in one call", what, d->rows, d->vocab);
     const SampleShape sh = sample_shape(d->rows, d->vocab);
     if (sh.bytes > 0 && (!d->workspace || !aligned(d->workspace, 16) || d->workspace_bytes < sh.bytes))
         return pk_fail(PK_ERR_ARG, "%s: a workspace of %lld bytes is wanted, aligned to 16 (%lld given)", what, (long long)sh.bytes,
