@@ -477,7 +477,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
     }
     constexpr int kQuads = D / 4;       // 4 channels a thread from here on
     const int64_t at = ((int64_t)b * a.kv_heads + hk) * a.tiles + tile;
-    float *all = a.part + at * (a.splits + a.groups) * 16 * kRow;      // under 2^31 bytes: at most 1,024 splits
+    float *all = a.part + at * (a.splits + a.groups) * 16 * kRow;      // 32-bit offsets: see attend_shape
     auto finish = [&](int col, int quad, v4f o, float top, float total) {
         const int r = tile * 16 + col, t = r / a.group, h = hk * a.group + r % a.group;
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;

@@ -103,13 +103,19 @@ int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
 // a tile 1 + (splits + 15) / 16 counters.
 constexpr int kSplitWork = 512, kCounters = 4 * kSplitWork;
 // attend_prompt_kernel takes calls of more than kPromptRows query rows to a request and kv head that give it kPromptGroups
-// workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  Requests of
-// uneven length up to 8,191, 32 heads on 8, D = 128, microseconds of the prompt kernel and of the other: 16 requests of up
-// to 64 new tokens (256 workgroups) 169 and 117, 128 (512) 251 and 196, 256 (1,024) 296 and 349; one request of 512 (128)
-// 118 and 124, 2,048 (512) 271 and 429; bf16 rows of 256, four requests of up to 512 tokens on 6,000 keys (512) 398 and
-// 365, 1,024 (1,024) 645 and 674, 2,047 (2,048) 1,012 and 1,220.  64 requests on up to 2,047 keys: 64 rows each 69 and 43,
-// 96 rows 69 and 55, 128 rows 70 and 70.  Not f16 rows of 256, which its registers do not hold: two requests of up to 1,024
-// new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
+// workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  The host has
+// bounds alone: where requests stay below them, workgroups stay empty and the others' keys make a tail.  32 heads on 8 of 128
+// channels in bf16, requests x new tokens on up to 8,191 keys, microseconds of the prompt kernel and of the other:
+//   workgroups             256                           512                                      1,024
+//   requests all alike     2 x 512: 226, 231             4 x 512: 278, 462; 16 x 128: 307, 512
+//   lengths spread evenly  4 x 256: 225, 132             4 x 512: 244, 224; 16 x 128: 233, 186    4 x 1,024: 314, 400
+//   one request            1 x 1,024: 224, 223           1 x 2,048: 269, 412                      1 x 4,096: 435, 709
+//   without keys held      4 x 256: 18, 21               4 x 512: 25, 42; 16 x 128: 17, 31
+// f16 at 512, 16 x 128: alike 486, 660; spread, on 6,000 keys 264, 175.  bf16 rows of 256 channels at 512, 4 x 512: alike 803,
+// 952; spread, on 6,000 keys 399, 365.  So 512 costs up to half where lengths are spread on long axes, and a higher
+// bound would cost as much or more where they are not.  64 requests of spread lengths on up to 2,047 keys: 64 rows each 69
+// and 43, 96 rows 69 and 55, 128 rows 70 and 70.  Not f16 rows of 256, which its registers do not hold: two requests of up
+// to 1,024 new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
 constexpr int kPromptRows = 128, kPromptGroups = 512;
 
 // How a call's work is dealt out, from its host-known sizes alone.
@@ -140,6 +146,8 @@ int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
     if (pairs * tiles * splits > most_groups(s.prompt ? kPromptThreads : kAttendThreads)) return too_many();
+    // a tile's partial sums are reached by 32-bit byte offsets
+    static_assert((kSplitWork + (kSplitWork + kJoin - 1) / kJoin) * 16 * (256 + 4) * 4ll < 1ll << 31, "at most kSplitWork splits");
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
     s.groups = (int)((splits + kJoin - 1) / kJoin);
     s.part_bytes = pairs * tiles * (splits + s.groups) * 16 * (d.head_dim + 4) * 4;
