@@ -76,7 +76,8 @@ PK_API int pk_kv_plan(const pk_kv_plan_desc *desc, void *stream);
 
 /* Rows k, v [n_rows][heads][head_dim] (strides per row and per head, channels
  * adjacent) into the cache at slots[n_rows], or from there.  Rows whose slot is
- * outside the cache are skipped.  Blocks are rounded to the nearest code, ties
+ * outside the cache are skipped; of rows stored to one slot in one call any mix
+ * may be left there.  Blocks are rounded to the nearest code, ties
  * to the even code, under the power of two that puts the largest of the 32
  * values between 3.5 and 7 (kept to 2^-120 .. 2^125, so that smaller blocks
  * vanish and the largest stay finite; f16 rows over 57,344 are held as 65,536,
@@ -96,8 +97,12 @@ PK_API int pk_kv4_load(const pk_kv4_rows_desc *desc, void *stream);
  * brings queries first[b] .. first[b + 1] of q, its last tokens: query i stands
  * at position p = lens[b] - (first[b + 1] - first[b]) + i and sees the keys at
  * positions 0 .. p, with a window the last `window` of them (its own included).
- * A query that sees no key gives zeros and an lse of -inf.  Query head h reads
- * kv head h / (heads / kv_heads). */
+ * A query that sees no key gives zeros and an lse of -inf, as does one whose
+ * scores overflow to -inf all.  Query head h reads kv head
+ * h / (heads / kv_heads).  Scores, sums and O are f32; probabilities are rounded
+ * before the product with V, for bf16 results to bf16, which adds to the error
+ * of a result's own rounding (0.0022 of the results' norm instead of 0.0016 over
+ * prompts of 2,047), for f16 results to two bf16, 16 bits, which does not. */
 typedef struct pk_kv4_attend_desc {
     const void *q;                      /* f16 or bf16 [n_rows][heads][head_dim] */
     void *out;                          /* as q */

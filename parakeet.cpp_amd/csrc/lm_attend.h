@@ -364,9 +364,10 @@ __device__ inline void join(const AttendParams &a, int64_t at, int split, int mi
 // One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.  Each wave
 // keeps its own maximum, sum and O of all columns, in registers, and they meet once at the end: keys are read and unpacked
 // once and no step waits for another wave.  What bounds it is memory where sessions are many: 64 of up to 4,097 keys, 32
-// heads on 8 of 128 channels, 146 MB in 34.8 us (4.2 TB/s, a large copy 4.9); then the unpacking, two bf16 planes and the
-// join: 200,003 and 100,001 keys on 2 kv heads in f16, 82 MB in 29.3 us (2.8 TB/s).  One session of 733 keys: 7.3 us, a
-// launch, four steps and one join.
+// heads on 8 of 128 channels, 144 MB in 35 to 39 us (4.1 to 3.7 TB/s, a large copy 4.9).  200,003 and up to 100,001 keys on
+// 2 kv heads in f16, 77 MB in 29.4 us (2.6 TB/s): the unpacking, two bf16 planes and the join, and the split, which goes by the
+// longest request: up to 336 workgroups have keys, two on some units and one on most.  One session of 733 keys: 7.3 us, a launch,
+// two steps of the first of its two splits, and their join.
 template <class T, int D, bool Small>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
@@ -523,10 +524,12 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kerne
 // which makes a lane's scores its own operand of O^T as above.  V lies transposed, row 16j + r holding channel
 // (D/16) r + j: rows that 16 lanes write together are adjacent.
 //
-// Four prompts of up to 2,047 tokens on up to 4,095 keys, 32 heads on 8 of 128 channels in bf16: 225 us, 163 GFLOP at 0.72
+// Four prompts of up to 2,047 tokens on up to 4,095 keys, 32 heads on 8 of 128 channels in bf16: 225 us, 162 GFLOP at 0.72
 // PFLOP/s, where a large library product of bf16 reaches 1.22.  A wave and 64 keys take 1,024 cycles of matrix instructions
 // and about 1,400 of vector ones (the exponentials and the unpacking); of two waves a vector unit the one's seldom run
-// beside the other's for long.  Memory is not full (26 MB fetched).  Splitting the keys in two to shorten the tail took 342 us.
+// beside the other's for long.  LDS is as full as the matrix cores: eight waves a unit read 32 KB of K and V each, 256 KB in
+// the 2,048 cycles of their matrix instructions, 128 bytes a cycle, since each operand read serves 32 columns only.  Memory is
+// not (54 MB fetched).  Splitting the keys in two to shorten the tail took 342 us.
 
 constexpr int kPromptThreads = 256, kPromptCols = 128, kPromptKeys = 64;
 

@@ -98,9 +98,8 @@ __device__ inline void get_codes(const Place<D> &at, int c, unsigned &code, unsi
 // threads take the same channels of 8 rows of V: where these go to the 8 slots of one group, as a prompt's do, they write
 // 32 adjacent bytes, 512 with the channels beside.  A block of workgroups is one head's K or V, so that no thread divides
 // by the number of heads; four passes a thread where there are many rows, their loads together.  24,577 rows of 8 x 128
-// bf16: 32.9 us in (101 MB read, 27 written: 3.9 TB/s), 21.0 us back out (6.1 TB/s, half of it read where it was just
-// written); with threads along the channels of V, one pass and 64-bit divisions 52 and 38.  64 rows: 2.6 and 2.4 us, a
-// launch each.
+// bf16: 32.8 us in (101 MB read, 27 written: 3.9 TB/s), 21.0 us back out (27 MB read, 101 written: 6.1 TB/s); with threads
+// along the channels of V, one pass and 64-bit divisions 52 and 38.  64 rows: 2.7 and 2.5 us, a launch each.
 template <class T, int D, bool Store, bool V, int Passes>
 __device__ inline void some_rows(const pk_kv4_rows_desc &a, int page_shift, int wide, int h) {
     constexpr int kPer = D / 8, kPass = kRowThreads / kPer;

@@ -15,7 +15,7 @@ constexpr int kPlanTokens = 4;   // consecutive tokens of one thread: one 16-byt
 // does it all; each then takes its share of the tokens and of the pages given up.  Latency alone counts: lengths are read
 // once, and a thread's four tokens, mostly of one request, take their pages in two loads together.  One request with one new
 // token: 3.0 us, which is a launch and four loads that wait for each other.  512 requests of up to 8,191 tokens, 254,000
-// slots and positions (2.2 MB): 7.2 us, most of it the three sums.
+// slots and positions (2.2 MB): 7.8 us, most of it the three sums.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(pk_kv_plan_desc a, int shift, int wide) {
     __shared__ int s_first[PK_LM_MAX_REQUESTS + 1], s_lack[PK_LM_MAX_REQUESTS + 1], s_free[PK_LM_MAX_REQUESTS + 1];
     __shared__ int s_old[PK_LM_MAX_REQUESTS], s_new[PK_LM_MAX_REQUESTS];

@@ -382,8 +382,8 @@ __device__ inline int shorten(Scratch &s, const RowRule &rule, int n) {
 }
 
 // A row on one workgroup, its tokens in registers: wave w has tokens (w n + e) 64 + lane, e < n <= E.  The logits are read
-// once and the rest is a chain of barriers, so latency bounds it: one row of 8,193 logits with top-k and top-p 8.0 us, 512
-// rows of 1,027 with filters of their own 11.0 us.
+// once and the rest is a chain of barriers, so latency bounds it: one row of 8,193 logits with top-k and top-p 8.1 us, 512
+// rows of 1,027 with filters of their own 11.5 us.
 template <class T, int BS, int E>
 __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
     constexpr int kWaves = BS / 64, kBins = 1024;
@@ -523,9 +523,9 @@ __global__ __launch_bounds__(BS) void sample_row_kernel(pk_sample_desc a) {
 //
 // Three launches over chunks of rows: the largest logit of each chunk; the bins' sums of each chunk, which the row's last
 // chunk to arrive adds up and names the bins to list from; the kept weight of each chunk's 16 runs with the listed
-// tokens beside, from which the row's last chunk finds the cut, the run and the token.  A row is read three times, from the
-// second time on out of the cache.  One row of 128,001 bf16 logits by top_p: 4.6 + 10.0 + 16.5 us under a profiler, 27 us
-// one call after another; 64 rows each with its own filters 5.1 + 15.2 + 27.0 and 46 us.  The chain at a row's end bounds
+// tokens beside, from which the row's last chunk finds the cut, the run and the token.  A row is read three times (64 rows
+// of 128,001 in bf16 past the L2 each time: 16 MB a launch).  One such row by top_p: 4.6 + 9.9 + 17.0 us under a profiler, 27 us
+// one call after another; 64 rows each with its own filters 5.2 + 15.4 + 27.2 and 46 us.  The chain at a row's end bounds
 // it: bins and lists that meet in memory, scans and digits, a barrier after each.  Two workgroups a unit (64 registers): 256
 // rows 116 us, one with 128 registers 157; 64 rows 46.6 and 45.2.  A list of 4,096: at 1,024, 64 rows of 262,144 often had
 // more than that in the bin of the cut and took 772 us, not 70.
