@@ -10,6 +10,11 @@
  *   pk_kv4_load     rows back out of it
  *   pk_kv4_attend   attention over that cache: single tokens and whole prompts
  *   pk_sample       the next token from logits and given uniform numbers
+ *   pk_qk_rope      norms of queries and keys for each head, with the position rotation
+ *   pk_kv8_append   key and value rows into a paged cache held in 8 bits, keys normed and rotated on the way
+ *   pk_kv8_load     rows back out of it
+ *   pk_kv8_attend   attention over that cache
+ *   pk_verify       drafted tokens against the target's probabilities, from given uniform numbers
  *
  * Conventions.  Every call checks its descriptor on the host, enqueues its
  * kernels on the caller's stream (a hipStream_t, NULL = the default stream)
@@ -152,6 +157,99 @@ typedef struct pk_sample_desc {
 } pk_sample_desc;
 PK_API int pk_sample(const pk_sample_desc *desc, void *stream);
 PK_API int pk_sample_workspace(const pk_sample_desc *desc, int64_t *bytes);
+
+/* Norms and rotation.  Every row of queries q [n_rows][heads][head_dim] and of keys k is normed,
+ * x / sqrt(mean(x^2) + eps) * weight (where norm is set), and its first rot_dim channels are turned in pairs by the
+ * angles t = pos * inv_freq[j]: (a, b) -> (a cos t - b sin t, a sin t + b cos t).  Pair j is channels j and rot_dim / 2 + j,
+ * or 2j and 2j + 1 where interleaved is set.  Angles are f64, the rest f32, rounded once.  Rows at positions below 0 are
+ * left out: their outputs stay as they are. */
+typedef struct pk_qk_rope_desc {
+    const void *q, *k;                  /* k nullable where kv_heads is 0 */
+    void *q_out, *k_out;                /* may be q and k themselves */
+    const float *q_weight, *k_weight;   /* [head_dim], NULL = 1; read where norm is set */
+    const float *inv_freq;              /* [rot_dim / 2]; nullable where rot_dim is 0 */
+    const int32_t *pos;                 /* [n_rows]; nullable where rot_dim is 0 */
+    int64_t q_row, q_head, k_row, k_head, q_out_row, q_out_head, k_out_row, k_out_head;     /* strides */
+    int32_t n_rows, heads, kv_heads, head_dim, dtype;
+    int32_t rot_dim;                    /* a multiple of 16 up to head_dim; 0 = no rotation */
+    int32_t norm, interleaved;
+    float eps;                          /* 0 or more */
+} pk_qk_rope_desc;
+PK_API int pk_qk_rope(const pk_qk_rope_desc *desc, void *stream);
+
+/* The 8-bit cache.  Values are 8-bit floating point codes (sign, 4 exponent bits, 3 of fraction, largest 448; 0x7F is
+ * NaN) under one power of two 2^e for the 32 tokens of a block and one head, of K and of V; e is the smallest, -100 .. 119,
+ * that puts the block's largest magnitude at 448 2^e or below.  A page holds `page` tokens (32, 64, 128 or 256).  The
+ * record of one (page, kv head) is
+ *
+ *   K codes [page][D] | V codes [page/8][32][8][D/32] | scales [page/32][4]
+ *
+ * page * 2 D + page / 2 bytes; V entry [a][r][i] holds channels r*D/32 .. (r+1)*D/32 of token 8a + i.  The scales are f32:
+ * K's, V's and two zeros; a negative one stands for its magnitude and marks a block that holds a NaN.  A record lies at
+ *   cache + id * page_stride + head * (page * 2 D + page / 2).
+ *
+ * pk_kv8_append puts rows k, v into the cache at slots[n_rows], keys normed and rotated as by pk_qk_rope before they
+ * are rounded, and norms and rotates queries into q_out where they are given (heads > 0).  Infinities become NaN.  Rows
+ * whose slot is outside the cache, or at positions below 0, are skipped (a query's row goes by its position alone).  Tokens are
+ * appended: of a block, a call's rows lie one after the other in the call, their slots rising by one; the block's rows
+ * before them are held already (none where they begin it, and then its scale begins anew), those behind them are not held
+ * any more.  Held rows are rounded again where the block's scale grows with a new one, which loses at most the last bits
+ * of values below 2^-6 of the scale.  Rows in another order leave the block's rows undefined (not other blocks). */
+typedef struct pk_kv8_append_desc {
+    const void *k, *v, *q;              /* q nullable where heads is 0 */
+    void *q_out;                        /* may be q itself */
+    const int32_t *slots;
+    const int32_t *pos;                 /* [n_rows]; nullable where rot_dim is 0 */
+    const float *q_weight, *k_weight;   /* [head_dim], NULL = 1; read where norm is set */
+    const float *inv_freq;              /* [rot_dim / 2]; nullable where rot_dim is 0 */
+    void *cache;
+    int64_t k_row, k_head, v_row, v_head, q_row, q_head, q_out_row, q_out_head;             /* strides */
+    int64_t page_stride;                /* bytes between pages */
+    int32_t n_rows, heads, kv_heads, head_dim, dtype, page, n_pages, rot_dim, norm, interleaved;
+    float eps;
+} pk_kv8_append_desc;
+PK_API int pk_kv8_append(const pk_kv8_append_desc *desc, void *stream);
+
+/* As pk_kv4_load and pk_kv4_attend, over the 8-bit cache.  Values at NaN codes are NaN; f16 results give held values of
+ * 65,536, to which rows over 63,488 may be rounded, as 65,504. */
+PK_API int pk_kv8_load(const pk_kv4_rows_desc *desc, void *stream);
+PK_API int pk_kv8_attend(const pk_kv4_attend_desc *desc, void *stream);
+PK_API int pk_kv8_attend_workspace(const pk_kv4_attend_desc *desc, int64_t *bytes);
+
+/* Drafted tokens.  Request b brought the tokens tokens[first[b] .. first[b + 1]) to the target: the last one that it had and
+ * the drafts behind it.  Row r of logits is what the target says behind tokens[r]; its draft is tokens[r + 1], the last row
+ * has none.  With the weights w of pk_sample (whole numbers, at the request's temperature) p = w / sum w; of draft logits,
+ * at draft_temperature, likewise q; without draft logits q is 1 at the draft.  Drafts are accepted, first to last, while
+ * u[r] q < p at the draft.  The token behind the accepted ones is drawn with u_draw[b] by rising index as pk_sample does:
+ * behind the last draft from p; where a draft was refused from max(p - q, 0) in steps of 2^-52 (without draft logits from p
+ * less the draft), or from p where that leaves nothing.  So the tokens are distributed as if drawn from p one by one.  Tokens
+ * that a filter bars are given as -inf.  All in whole numbers and single f64 steps: no result depends on the order of a sum.
+ * A draft outside the vocabulary is refused, and the token then drawn from p; a row of -inf accepts nothing and gives -1. */
+typedef struct pk_verify_desc {
+    const void *logits;                 /* [n_rows][vocab], rows logits_row apart */
+    const void *draft;                  /* [n_rows][vocab], rows draft_row apart, of the same type: what draft tokens[r + 1] was drawn
+                                           from is row r, last rows are not read; nullable */
+    const int32_t *tokens;              /* [n_rows] */
+    const int32_t *first;               /* [requests + 1] */
+    const float *temperature, *draft_temperature;       /* [requests], NULL = 1; 0 or less = the largest alone */
+    const float *u;                     /* [n_rows] uniform in [0, 1) */
+    const float *u_draw;                /* [requests] */
+    const int32_t *lens;                /* [requests] tokens held, those of this call included; nullable */
+    int32_t *out;                       /* out [n_rows]: the accepted drafts, the token drawn behind them, then -1; rows of no
+                                           request stay as they are */
+    int32_t *accepted;                  /* out [requests]: how many drafts were accepted */
+    int32_t *lens_out;                  /* out [requests]: lens less the refused drafts, not lens itself; nullable */
+    float *prob;                        /* out [n_rows]: p of the token in out, 0 at -1; nullable */
+    void *workspace;                    /* pk_verify_workspace() bytes, zeroed once before its first use.  One call at a time may
+                                           use it. */
+    int64_t workspace_bytes;
+    int64_t logits_row, draft_row;
+    int32_t n_rows, requests, vocab, dtype;
+    int32_t max_new;                    /* no request brings more rows (those behind are left out) */
+    int32_t reserved;
+} pk_verify_desc;
+PK_API int pk_verify(const pk_verify_desc *desc, void *stream);
+PK_API int pk_verify_workspace(const pk_verify_desc *desc, int64_t *bytes);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,7 @@
 """Build recipe for the native libraries (gfx950 only, built in-tree).
 
   libparakeet_hip.so      HIP kernels + C ABI      (csrc/pk_decode.hip: the decode loop,
-                          csrc/pk_lm.hip: the language-model serving operators)
+                          csrc/pk_lm.hip, csrc/pk_lm_step.hip: the language-model serving operators)
   libparakeet_decoder.so  C++ decoder API           (csrc/parakeet_decoder.cpp, csrc/gguf_reader.cpp)
   _lm_torch.so            the serving operators' calls for torch tensors (csrc/lm_torch.cpp), built where
                           torch is installed
@@ -52,7 +52,7 @@ def build_hip():
     out = os.path.join(HERE, "libparakeet_hip.so")
     # PK_TIMELINE=1 compiles the decode loop's per-wave checkpoint timeline (profiling builds only)
     extra = ["-DPK_TIMELINE"] if os.environ.get("PK_TIMELINE") else []
-    srcs = [os.path.join(CSRC, f) for f in ("pk_decode.hip", "pk_lm.hip")]
+    srcs = [os.path.join(CSRC, f) for f in ("pk_decode.hip", "pk_lm.hip", "pk_lm_step.hip")]
     _run([HIPCC, *HIP_FLAGS, *extra, "-shared", *srcs, "-o", out + ".tmp"])
     os.replace(out + ".tmp", out)
     return out

@@ -1,0 +1,144 @@
+// lm_rope.h -- norms of queries and keys for each head and the position rotation (pk_qk_rope, and on the way into the
+// 8-bit cache pk_kv8_append).
+//
+// A row of D channels of one head is D/8 lanes' 8 adjacent channels, so that a wave holds 512 / D rows and the norm's
+// sum stays within a row's lanes.  The angles of a token are the same for all its heads: a workgroup works out the sines
+// and cosines of its rows once, into LDS, and its waves go over the heads.  An angle is pos * inv_freq in f64, in turns
+// less the whole ones: in f32 a position of 200,000 has lost 2^-7 of a radian.
+#pragma once
+
+#include "lm_cache.h"
+#include "lm_common.h"
+#include "parakeet_lm.h"
+
+namespace pklm {
+
+constexpr int kTurnThreads = 256, kTurnWaves = kTurnThreads / 64, kTurnRows = 32;
+
+// Sum over the D/8 lanes of a row.
+template <int Lanes>
+__device__ inline float row_sum(float v) {
+    v += from_lane<0xB1, 0xF>(v, 0.0f);                 // lane ^ 1
+    v += from_lane<0x4E, 0xF>(v, 0.0f);                 // lane ^ 2
+    v += from_lane<0x141, 0xF>(v, 0.0f);                // the other four of eight
+    if (Lanes > 8) v += from_lane<0x140, 0xF>(v, 0.0f); // the other eight of sixteen
+    if (Lanes > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+// How rows are normed and turned.
+struct Turn {
+    const float *inv_freq;
+    const int *pos;              // nullable where nothing is turned
+    int rot, norm, interleaved;
+    float eps;
+
+    __device__ bool live(int64_t row) const { return !pos || pos[row] >= 0; }
+};
+
+template <int D>
+struct TurnTable {
+    float c[kTurnRows * D / 2], s[kTurnRows * D / 2];
+
+    // the angles of the n rows from row0; a barrier on either side
+    __device__ void fill(const Turn &turn, int64_t row0, int n) {
+        const int half = turn.rot / 2;
+        for (int i = threadIdx.x; i < n * half; i += kTurnThreads) {
+            const int r = i / half, j = i - r * half;
+            double t = (double)turn.pos[row0 + r] * (double)turn.inv_freq[j] * 0.15915494309189533577;
+            t -= rint(t);
+            sincospif(2.0f * (float)t, &s[r * half + j], &c[r * half + j]);
+        }
+    }
+};
+
+// A lane's 8 channels from 8 lane_c of a row: normed with the weights w, turned by the angles of the table's row r.
+template <int D>
+__device__ inline void norm_and_turn(float (&x)[8], int lane_c, const Turn &turn, const TurnTable<D> &table, int r, const float (&w)[8]) {
+    if (turn.norm) {
+        float sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
+        const float inv = 1.0f / sqrtf(row_sum<D / 8>(sum) * (1.0f / D) + turn.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= inv * w[i];
+    }
+    if (turn.rot == 0) return;
+    const int half = turn.rot / 2;
+    if (turn.interleaved) {
+        if (8 * lane_c < turn.rot) {
+            const v4f c = *(const v4f *)&table.c[r * half + 4 * lane_c], s = *(const v4f *)&table.s[r * half + 4 * lane_c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = x[2 * i], b = x[2 * i + 1];
+                x[2 * i] = a * c[i] - b * s[i], x[2 * i + 1] = a * s[i] + b * c[i];
+            }
+        }
+    } else {
+        // the other channel of a pair is half channels, whole lanes, away
+        const int lanes = half / 8, lane = threadIdx.x & 63;
+        const bool low = lane_c < lanes, in = lane_c < 2 * lanes;
+        const int from = in ? (low ? lane + lanes : lane - lanes) : lane;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], from);
+        if (in) {
+            const int at = r * half + 8 * (low ? lane_c : lane_c - lanes);
+#pragma unroll
+            for (int i4 = 0; i4 < 8; i4 += 4) {
+                const v4f c = *(const v4f *)&table.c[at + i4], s = *(const v4f *)&table.s[at + i4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i4 + i] = x[i4 + i] * c[i] + (low ? -y[i4 + i] : y[i4 + i]) * s[i];
+            }
+        }
+    }
+}
+
+__device__ inline void load_weights(const float *weight, int lane_c, float (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = weight ? weight[8 * lane_c + i] : 1.0f;
+}
+
+// One head's rows row0 .. row0 + n, n <= kTurnRows, from x into y, on one wave.
+template <class T, int D>
+__device__ inline void turn_rows(const typename T::Raw *x, int64_t x_row, bool wide, typename T::Raw *y, int64_t y_row, bool y_wide,
+                                 const float *weight, const Turn &turn, const TurnTable<D> &table, int64_t row0, int n) {
+    constexpr int kLanes = D / 8, kRows = 64 / kLanes;
+    const int lane = threadIdx.x & 63, c = lane % kLanes;
+    float w[8];
+    load_weights(weight, c, w);
+    for (int r0 = 0; r0 < n; r0 += kRows) {
+        const int r = min(r0 + lane / kLanes, n - 1);
+        const int64_t row = row0 + r;
+        float v[8];
+        load8<T>(x + row * x_row + 8 * c, wide, v);
+        norm_and_turn<D>(v, c, turn, table, r, w);
+        if (r0 + lane / kLanes < n && turn.live(row)) store8<T>(y + row * y_row + 8 * c, y_wide, v);
+    }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(kTurnThreads) void rope_kernel(pk_qk_rope_desc a, int rows, int wide_q, int wide_k) {
+    using Raw = typename T::Raw;
+    __shared__ TurnTable<D> s_table;
+    const Turn turn{a.inv_freq, a.pos, a.rot_dim, a.norm, a.interleaved, a.eps};
+    const int64_t row0 = (int64_t)blockIdx.x * rows;
+    const int n = (int)min((int64_t)rows, a.n_rows - row0), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (a.rot_dim) {
+        s_table.fill(turn, row0, n);
+        __syncthreads();
+    }
+    for (int u = blockIdx.y * kTurnWaves + wave; u < a.heads + a.kv_heads; u += gridDim.y * kTurnWaves) {
+        if (u < a.heads)
+            turn_rows<T, D>((const Raw *)a.q + u * a.q_head, a.q_row, wide_q & 1, (Raw *)a.q_out + u * a.q_out_head, a.q_out_row, wide_q & 2,
+                            a.q_weight, turn, s_table, row0, n);
+        else
+            turn_rows<T, D>((const Raw *)a.k + (u - a.heads) * a.k_head, a.k_row, wide_k & 1, (Raw *)a.k_out + (u - a.heads) * a.k_out_head,
+                            a.k_out_row, wide_k & 2, a.k_weight, turn, s_table, row0, n);
+    }
+}
+
+}  // namespace pklm

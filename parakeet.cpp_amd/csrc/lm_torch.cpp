@@ -126,6 +126,58 @@ struct Call {
                         " tokens, the records of a page adjacent");
         return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2), t.size(0), t.size(1), t.size(2) * 16 / (page * 17)};
     }
+    Cache cache8(int i, int64_t page) {
+        const at::Tensor &t = tensor(i, "cache");
+        if (t.scalar_type() != at::kByte) type_error(std::string("cache of ") + c10::toString(t.scalar_type()) + " (uint8)");
+        if (t.dim() != 3 || page <= 0 || t.size(2) * 2 <= page || (t.size(2) * 2 - page) % (4 * page) || t.stride(2) != 1 ||
+            (t.size(1) > 1 && t.stride(1) != t.size(2)))
+            value_error("cache of shape " + shape_text(t.sizes()) + ": expected kv8_shape(...) for pages of " + std::to_string(page) +
+                        " tokens, the records of a page adjacent");
+        return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2), t.size(0), t.size(1), (t.size(2) * 2 - page) / (4 * page)};
+    }
+    bool flag(int i) const {
+        const int v = PyObject_IsTrue(args[i]);
+        if (v < 0) throw Refused{nullptr, ""};
+        return v != 0;
+    }
+    float real(int i) const {
+        const double v = PyFloat_AsDouble(args[i]);
+        if (PyErr_Occurred()) throw Refused{nullptr, ""};
+        return (float)v;
+    }
+    // rows that are normed and rotated, their results and weights
+    struct Turned {
+        const void *x;
+        void *y;
+        const float *weight;
+        int64_t x_row, x_head, y_row, y_head, n, heads, dim;
+        at::ScalarType type;
+    };
+    Turned turned(int ix, int iy, int iw, const char *what) {
+        const std::string out = std::string(what) + "_out", w = std::string(what) + "_weight";
+        const at::Tensor &x = heads(ix, what);
+        if (none(iy)) value_error(out + ": missing");
+        const at::Tensor &y = heads(iy, out.c_str());
+        if (x.scalar_type() != y.scalar_type() || x.sizes() != y.sizes())
+            value_error(std::string(what) + " " + shape_text(x.sizes()) + " " + c10::toString(x.scalar_type()) + ", " + out + " " + shape_text(y.sizes()) +
+                        " " + c10::toString(y.scalar_type()));
+        if ((x.size(1) > 1 && y.stride(1) < x.size(2)) || (x.size(0) > 1 && y.stride(0) < x.size(2))) value_error(out + ": rows overlap");
+        return {x.data_ptr(), y.data_ptr(), f32_or(iw, w.c_str(), {x.size(2)}), x.stride(0), x.stride(1), y.stride(0), y.stride(1),
+                x.size(0), x.size(1), x.size(2), x.scalar_type()};
+    }
+    // the norm's and the rotation's settings of a descriptor
+    template <class Desc>
+    void turn(Desc &d, int ipos, int iinv, int ieps, int iinterleaved, int64_t n) {
+        d.pos = i32_or(ipos, "pos", {n});
+        if (!none(iinv)) {
+            const at::Tensor &t = tensor(iinv, "inv_freq");
+            if (t.dim() != 1) value_error("inv_freq has one axis");
+            d.inv_freq = f32(iinv, "inv_freq", {t.size(0)});
+            if (t.size(0) > 4096) value_error("inv_freq: out of range");
+            d.rot_dim = (int32_t)(2 * t.size(0));
+        }
+        d.norm = !none(ieps), d.eps = none(ieps) ? 0.0f : real(ieps), d.interleaved = flag(iinterleaved);
+    }
 };
 
 int32_t narrow(int64_t v, const char *what) {
@@ -229,12 +281,12 @@ PyObject *kv_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
-template <int (*Entry)(const pk_kv4_rows_desc *, void *)>
+template <int (*Entry)(const pk_kv4_rows_desc *, void *), Call::Cache (Call::*Layout)(int, int64_t) = &Call::cache>
 int rows(Call &c, int ik, int iv, int islots, int icache) {
     pk_kv4_rows_desc d{};
     d.page = c.whole32(4, "page");
     const at::Tensor &k = c.heads(ik, "k"), &v = c.heads(iv, "v");
-    const auto cache = c.cache(icache, d.page);
+    const auto cache = (c.*Layout)(icache, d.page);
     if (k.scalar_type() != v.scalar_type() || k.sizes() != v.sizes())
         value_error("k " + shape_text(k.sizes()) + " " + c10::toString(k.scalar_type()) + ", v " + shape_text(v.sizes()) + " " + c10::toString(v.scalar_type()));
     if (k.size(1) != cache.heads || k.size(2) != cache.dim)
@@ -255,12 +307,13 @@ PyObject *kv4_load(PyObject *, PyObject *const *args, Py_ssize_t n) {       // c
     return guarded(args, n, 6, [](Call &c) { return rows<pk_kv4_load>(c, 2, 3, 1, 0); });
 }
 
-PyObject *kv4_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded(args, n, 14, [](Call &c) {
+template <int (*Entry)(const pk_kv4_attend_desc *, void *), int (*Wanted)(const pk_kv4_attend_desc *, int64_t *), Call::Cache (Call::*Layout)(int, int64_t)>
+PyObject *attend(PyObject *const *args, Py_ssize_t n, int kind) {
+    return guarded(args, n, 14, [kind](Call &c) {
         pk_kv4_attend_desc d{};
         const at::Tensor &q = c.heads(0, "q"), &out = c.heads(4, "out");
         d.page = c.whole32(5, "page");
-        const auto cache = c.cache(1, d.page);
+        const auto cache = (c.*Layout)(1, d.page);
         const at::Tensor &table = c.table(2, d.table_stride);
         if (out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes())
             value_error("q " + shape_text(q.sizes()) + ", out " + shape_text(out.sizes()) + " " + c10::toString(out.scalar_type()));
@@ -289,11 +342,13 @@ PyObject *kv4_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const c10::DeviceGuard guard(c.device);
         void *stream = c.stream(13);
         int64_t wanted = 0;
-        if (const int rc = pk_kv4_attend_workspace(&d, &wanted)) return rc;
-        workspace(c, 12, 0, stream, wanted, d.workspace, d.workspace_bytes);
-        return pk_kv4_attend(&d, stream);
+        if (const int rc = Wanted(&d, &wanted)) return rc;
+        workspace(c, 12, kind, stream, wanted, d.workspace, d.workspace_bytes);
+        return Entry(&d, stream);
     });
 }
+PyObject *kv4_attend(PyObject *, PyObject *const *args, Py_ssize_t n) { return attend<pk_kv4_attend, pk_kv4_attend_workspace, &Call::cache>(args, n, 0); }
+PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) { return attend<pk_kv8_attend, pk_kv8_attend_workspace, &Call::cache8>(args, n, 2); }
 
 PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded(args, n, 11, [](Call &c) {
@@ -316,11 +371,102 @@ PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+PyObject *kv8_load(PyObject *, PyObject *const *args, Py_ssize_t n) {       // cache, slots, k, v, page, stream
+    return guarded(args, n, 6, [](Call &c) { return rows<pk_kv8_load, &Call::cache8>(c, 2, 3, 1, 0); });
+}
+
+PyObject *qk_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded(args, n, 11, [](Call &c) {
+        pk_qk_rope_desc d{};
+        const auto q = c.turned(0, 1, 7, "q");
+        d.q = q.x, d.q_out = q.y, d.q_weight = q.weight, d.q_row = q.x_row, d.q_head = q.x_head, d.q_out_row = q.y_row, d.q_out_head = q.y_head;
+        d.dtype = c.dtype(c.tensor(0, "q"), "q");
+        if (!c.none(4)) {
+            const auto k = c.turned(4, 5, 8, "k");
+            if (k.type != q.type || k.n != q.n || k.dim != q.dim) value_error("k: rows of another number, size or type than q's");
+            d.k = k.x, d.k_out = k.y, d.k_weight = k.weight, d.k_row = k.x_row, d.k_head = k.x_head, d.k_out_row = k.y_row, d.k_out_head = k.y_head;
+            d.kv_heads = narrow(k.heads, "heads");
+        }
+        c.turn(d, 2, 3, 6, 9, q.n);
+        d.n_rows = narrow(q.n, "rows"), d.heads = narrow(q.heads, "heads"), d.head_dim = narrow(q.dim, "head_dim");
+        const c10::DeviceGuard guard(c.device);
+        return pk_qk_rope(&d, c.stream(10));
+    });
+}
+
+PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded(args, n, 14, [](Call &c) {
+        pk_kv8_append_desc d{};
+        d.page = c.whole32(4, "page");
+        const at::Tensor &k = c.heads(0, "k"), &v = c.heads(1, "v");
+        const auto cache = c.cache8(3, d.page);
+        if (k.scalar_type() != v.scalar_type() || k.sizes() != v.sizes())
+            value_error("k " + shape_text(k.sizes()) + " " + c10::toString(k.scalar_type()) + ", v " + shape_text(v.sizes()) + " " + c10::toString(v.scalar_type()));
+        if (k.size(1) != cache.heads || k.size(2) != cache.dim)
+            value_error("rows of " + std::to_string(k.size(1)) + " heads of " + std::to_string(k.size(2)) + ", a cache of " +
+                        std::to_string(cache.heads) + " heads of " + std::to_string(cache.dim));
+        d.dtype = c.dtype(k, "k");
+        d.k = k.data_ptr(), d.v = v.data_ptr(), d.slots = c.i32(2, "slots", {k.size(0)}), d.cache = cache.ptr;
+        d.k_row = k.stride(0), d.k_head = k.stride(1), d.v_row = v.stride(0), d.v_head = v.stride(1), d.page_stride = cache.page_stride;
+        d.k_weight = c.f32_or(8, "k_weight", {k.size(2)});
+        if (!c.none(9)) {
+            const auto q = c.turned(9, 10, 11, "q");
+            if (q.type != k.scalar_type() || q.n != k.size(0) || q.dim != k.size(2)) value_error("q: rows of another number, size or type than k's");
+            d.q = q.x, d.q_out = q.y, d.q_weight = q.weight, d.q_row = q.x_row, d.q_head = q.x_head, d.q_out_row = q.y_row, d.q_out_head = q.y_head;
+            d.heads = narrow(q.heads, "heads");
+        }
+        c.turn(d, 5, 6, 7, 12, k.size(0));
+        d.n_rows = narrow(k.size(0), "rows"), d.kv_heads = narrow(cache.heads, "heads"), d.head_dim = narrow(cache.dim, "head_dim");
+        d.n_pages = narrow(cache.pages, "pages");
+        const c10::DeviceGuard guard(c.device);
+        return pk_kv8_append(&d, c.stream(13));
+    });
+}
+
+PyObject *verify(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded(args, n, 16, [](Call &c) {
+        pk_verify_desc d{};
+        const at::Tensor &x = c.tensor(0, "logits"), &first = c.tensor(2, "first");
+        auto rows2 = [](const at::Tensor &t, const char *what) {
+            if (t.dim() != 2) value_error(std::string(what) + ": shape " + shape_text(t.sizes()) + ", expected [rows, vocab]");
+            if (t.size(1) > 1 && t.stride(1) != 1) value_error(std::string(what) + ": the last axis is not adjacent");
+        };
+        rows2(x, "logits");
+        if (first.dim() != 1 || first.size(0) < 1) value_error("first: shape " + shape_text(first.sizes()) + ", expected [requests + 1]");
+        const int64_t N = x.size(0), B = first.size(0) - 1;
+        d.logits = x.data_ptr(), d.logits_row = x.stride(0), d.dtype = c.dtype(x, "logits");
+        if (!c.none(8)) {
+            const at::Tensor &y = c.tensor(8, "draft");
+            rows2(y, "draft");
+            if (y.scalar_type() != x.scalar_type() || y.sizes() != x.sizes())
+                value_error("logits " + shape_text(x.sizes()) + ", draft " + shape_text(y.sizes()) + " " + c10::toString(y.scalar_type()));
+            d.draft = y.data_ptr(), d.draft_row = y.stride(0);
+        }
+        d.tokens = c.i32(1, "tokens", {N}), d.first = c.i32(2, "first", {B + 1}), d.u = c.f32(3, "u", {N}), d.u_draw = c.f32(4, "u_draw", {B});
+        d.out = c.i32(5, "out", {N}), d.accepted = c.i32(6, "accepted", {B});
+        d.n_rows = narrow(N, "rows"), d.requests = narrow(B, "requests"), d.vocab = narrow(x.size(1), "vocab");
+        d.max_new = c.none(7) ? d.n_rows : c.whole32(7, "max_new");
+        d.temperature = c.f32_or(9, "temperature", {B}), d.draft_temperature = c.f32_or(10, "draft_temperature", {B});
+        d.lens = c.i32_or(11, "lens", {B}), d.lens_out = c.i32_or(12, "lens_out", {B}), d.prob = c.f32_or(13, "prob", {N});
+        const c10::DeviceGuard guard(c.device);
+        void *stream = c.stream(15);
+        int64_t wanted = 0;
+        if (const int rc = pk_verify_workspace(&d, &wanted)) return rc;
+        workspace(c, 14, 3, stream, wanted, d.workspace, d.workspace_bytes);
+        return pk_verify(&d, stream);
+    });
+}
+
 PyMethodDef methods[] = {{"kv_plan", (PyCFunction)(void (*)(void))kv_plan, METH_FASTCALL, nullptr},
                          {"kv4_store", (PyCFunction)(void (*)(void))kv4_store, METH_FASTCALL, nullptr},
                          {"kv4_load", (PyCFunction)(void (*)(void))kv4_load, METH_FASTCALL, nullptr},
                          {"kv4_attend", (PyCFunction)(void (*)(void))kv4_attend, METH_FASTCALL, nullptr},
                          {"sample", (PyCFunction)(void (*)(void))sample, METH_FASTCALL, nullptr},
+                         {"qk_rope", (PyCFunction)(void (*)(void))qk_rope, METH_FASTCALL, nullptr},
+                         {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
+                         {"kv8_load", (PyCFunction)(void (*)(void))kv8_load, METH_FASTCALL, nullptr},
+                         {"kv8_attend", (PyCFunction)(void (*)(void))kv8_attend, METH_FASTCALL, nullptr},
+                         {"verify", (PyCFunction)(void (*)(void))verify, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module{PyModuleDef_HEAD_INIT, "_lm_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

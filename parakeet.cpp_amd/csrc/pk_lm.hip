@@ -11,8 +11,10 @@
 #include <cstring>
 
 #include "last_error.h"
-#include "lm_attend.h"
+#include "lm_attend4.h"
+#include "lm_attend_host.h"
 #include "lm_cache.h"
+#include "lm_host.h"
 #include "lm_plan.h"
 #include "lm_sample.h"
 #include "parakeet_lm.h"
@@ -21,17 +23,7 @@ namespace {
 
 using namespace pklm;
 
-bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
-int log2i(int v) { return 31 - __builtin_clz((unsigned)v); }
-
-// A launch has fewer than 2^32 threads.
-constexpr int64_t most_groups(int threads) { return UINT32_MAX / threads; }
-
-int launched(const char *what) {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? PK_OK : pk_fail(PK_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
-}
 
 // What pk_kv4_store, _load and _attend ask of the cache; 0 = fine.
 int check_cache(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
@@ -96,84 +88,6 @@ int rows_call(const char *what, const pk_kv4_rows_desc *d, void *stream) {
     else if (d->dtype == PK_DTYPE_F16) launch_rows<F16, Store>(*d, wide, s);
     else launch_rows<BF16, Store>(*d, wide, s);
     return launched(what);
-}
-
-// Arrival counters of the tiles whose keys are split, at the workspace's beginning whatever the call's shape, so that
-// no call's partial sums lie where another's counters are.  A split call has at most kSplitWork tiles times splits, and
-// a tile 1 + (splits + 15) / 16 counters.
-constexpr int kSplitWork = 512, kCounters = 4 * kSplitWork;
-// attend_prompt_kernel takes calls of more than kPromptRows query rows to a request and kv head that give it kPromptGroups
-// workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  The host has
-// bounds alone: where requests stay below them, workgroups stay empty and the others' keys make a tail.  32 heads on 8 of 128
-// channels in bf16, requests x new tokens on up to 8,191 keys, microseconds of the prompt kernel and of the other:
-//   workgroups             256                           512                                      1,024
-//   requests all alike     2 x 512: 226, 231             4 x 512: 278, 462; 16 x 128: 307, 512
-//   lengths spread evenly  4 x 256: 225, 132             4 x 512: 244, 224; 16 x 128: 233, 186    4 x 1,024: 314, 400
-//   one request            1 x 1,024: 224, 223           1 x 2,048: 269, 412                      1 x 4,096: 435, 709
-//   without keys held      4 x 256: 18, 21               4 x 512: 25, 42; 16 x 128: 17, 31
-// f16 at 512, 16 x 128: alike 486, 660; spread, on 6,000 keys 264, 175.  bf16 rows of 256 channels at 512, 4 x 512: alike 803,
-// 952; spread, on 6,000 keys 399, 365.  So 512 costs up to half where lengths are spread on long axes, and a higher
-// bound would cost as much or more where they are not.  64 requests of spread lengths on up to 2,047 keys: 64 rows each 69
-// and 43, 96 rows 69 and 55, 128 rows 70 and 70.  Not f16 rows of 256, which its registers do not hold: two requests of up
-// to 1,024 new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
-constexpr int kPromptRows = 128, kPromptGroups = 512;
-
-// How a call's work is dealt out, from its host-known sizes alone.
-struct AttendShape {
-    bool prompt;             // attend_prompt_kernel, 128 query rows a workgroup; else attend_kernel, 16
-    int tiles, chunk, splits, groups;
-    int64_t part_bytes;
-    int64_t bytes() const { return splits > 1 ? kCounters * 4 + part_bytes : 0; }
-};
-
-int attend_shape(const pk_kv4_attend_desc &d, AttendShape &s) {
-    const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
-    const int64_t prompt_tiles = (rows + kPromptCols - 1) / kPromptCols;
-    auto too_many = [&] {
-        return pk_fail(PK_ERR_UNSUPPORTED, "pk_kv4_attend: %lld requests x kv heads of %lld query rows in one call", (long long)pairs,
-                       (long long)rows);
-    };
-    if (pairs > most_groups(kPromptThreads)) return too_many();
-    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= kPromptGroups && !(d.dtype == PK_DTYPE_F16 && d.head_dim == 256);
-    const int64_t tiles = s.prompt ? prompt_tiles : (rows + 15) / 16, step = 32 * kAttendWaves;
-    // keys of one tile: its rows span at most as many tokens
-    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 64) : d.max_len;
-    // Split where the tiles leave the card short of work (512 workgroups are resident), into no less than 512 keys.
-    // 200,003 and 100,001 keys on 2 kv heads, 64 sessions of up to 4,097 keys on 8, 8 of up to 32,000: 29.5, 35.8 and 40.6
-    // us; for twice as many splits 34.3, 37.2 and 43.3, for half as many 29.3, 36.1 and 46.0.
-    const int64_t want = kSplitWork, least = 512, each = std::max<int64_t>(pairs * tiles, 1);
-    int64_t splits = s.prompt ? 1 : std::max<int64_t>(std::min<int64_t>(want / each, (keys + least - 1) / least), 1);
-    const int64_t chunk = std::max<int64_t>(((keys + splits - 1) / splits + step - 1) / step * step, step);
-    splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
-    if (pairs * tiles * splits > most_groups(s.prompt ? kPromptThreads : kAttendThreads)) return too_many();
-    // a tile's partial sums are reached by 32-bit byte offsets
-    static_assert((kSplitWork + (kSplitWork + kJoin - 1) / kJoin) * 16 * (256 + 4) * 4ll < 1ll << 31, "at most kSplitWork splits");
-    s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
-    s.groups = (int)((splits + kJoin - 1) / kJoin);
-    s.part_bytes = pairs * tiles * (splits + s.groups) * 16 * (d.head_dim + 4) * 4;
-    return PK_OK;
-}
-
-int attend_check(const pk_kv4_attend_desc *d) {
-    const char *what = "pk_kv4_attend";
-    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
-    if (d->dtype != PK_DTYPE_F16 && d->dtype != PK_DTYPE_BF16) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d (f16 or bf16)", what, d->dtype);
-    if (d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads)
-        return pk_fail(PK_ERR_ARG, "%s: %d query heads on %d kv heads", what, d->heads, d->kv_heads);
-    if (d->requests < 0 || d->n_rows < 0 || d->max_new < 0 || d->max_len < 0 || d->window < 0 || d->width <= 0)
-        return pk_fail(PK_ERR_ARG, "%s: %d requests, %d rows, max_new %d, max_len %d, window %d, table width %d", what, d->requests, d->n_rows,
-                       d->max_new, d->max_len, d->window, d->width);
-    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
-        return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, d->head_dim);
-    if (!std::isfinite(d->scale)) return pk_fail(PK_ERR_ARG, "%s: a scale of %g", what, d->scale);
-    if ((int64_t)std::max(d->n_rows, d->max_new) * (d->heads / d->kv_heads) > INT32_MAX - 4096)
-        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows, max_new %d, %d query heads a kv head: row numbers are 32 bits", what, d->n_rows, d->max_new,
-                       d->heads / d->kv_heads);
-    // positions are 32 bits, some steps past the last key included
-    if ((int64_t)d->width * d->page > INT32_MAX - 4096 || d->max_len > INT32_MAX - 4096)
-        return pk_fail(PK_ERR_UNSUPPORTED, "%s: a table of %d pages of %d tokens, max_len %d: positions are 32 bits", what, d->width, d->page,
-                       d->max_len);
-    return PK_OK;
 }
 
 // Sampling.  A row of up to kRowVocab logits is one workgroup's, its tokens in registers, 16 a thread; longer rows are cut in
@@ -245,18 +159,25 @@ void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s
     }
 }
 
+struct HostKv4 {
+    static int check(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
+        return check_cache(what, cache, page_stride, page, n_pages, heads, dim);
+    }
+    static bool has_prompt(int dtype, int dim) { return !(dtype == PK_DTYPE_F16 && dim == 256); }
+};
+
 template <class T, int D>
 void launch_attend(const AttendParams &p, bool prompt, unsigned grid, hipStream_t s) {
     // pages of whole key tiles: addresses are worked out a wave at a time.  A prompt of 512 tokens x 4 on up to 8,191 keys
     // takes 431 us with f16 rows of 128 then, 443 otherwise; of D = 256, whose registers are full, 664 and 526.
     if constexpr (D == 256 && __is_same(T, BF16)) {
-        if (prompt) return attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt) return attend_prompt_kernel<Kv4, T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
     } else if constexpr (D < 256) {
-        if (prompt && p.page < kPromptKeys) return attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
-        if (prompt) return attend_prompt_kernel<T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt && p.page < kPromptKeys) return attend_prompt_kernel<Kv4, T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt) return attend_prompt_kernel<Kv4, T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
     }
-    if (p.page < 32) attend_kernel<T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
-    else attend_kernel<T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
+    if (p.page < 32) attend_kernel<Kv4, T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
+    else attend_kernel<Kv4, T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
 }
 
 template <class T>
@@ -300,50 +221,14 @@ PK_API int pk_kv4_store(const pk_kv4_rows_desc *d, void *stream) { return rows_c
 PK_API int pk_kv4_load(const pk_kv4_rows_desc *d, void *stream) { return rows_call<false>("pk_kv4_load", d, stream); }
 
 PK_API int pk_kv4_attend_workspace(const pk_kv4_attend_desc *d, int64_t *bytes) {
-    pk_fail_clear();
-    if (int rc = attend_check(d)) return rc;
-    if (!bytes) return pk_fail(PK_ERR_ARG, "pk_kv4_attend_workspace: NULL result");
-    AttendShape s;
-    if (int rc = attend_shape(*d, s)) return rc;
-    *bytes = s.bytes();
-    return PK_OK;
+    return attend_workspace<HostKv4>("pk_kv4_attend", d, bytes);
 }
 
 PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
-    pk_fail_clear();
-    const char *what = "pk_kv4_attend";
-    if (int rc = attend_check(d)) return rc;
-    if (int rc = check_cache(what, d->cache, d->page_stride, d->page, d->n_pages, d->kv_heads, d->head_dim)) return rc;
-    if (d->n_rows == 0 || d->requests == 0 || d->max_new == 0) return PK_OK;
-    if (!d->q || !d->out || !d->table || !d->lens) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
-    if (!aligned(d->q, 2) || !aligned(d->out, 2) || !aligned(d->lse, 4))
-        return pk_fail(PK_ERR_ARG, "%s: q, out or lse not aligned to its type", what);
-    if (!d->first && (d->n_rows != d->requests || d->max_new != 1))
-        return pk_fail(PK_ERR_ARG, "%s: without first, one query per request: %d rows, %d requests, max_new %d", what, d->n_rows, d->requests, d->max_new);
-    if (d->requests > 1 && d->table_stride < d->width)
-        return pk_fail(PK_ERR_ARG, "%s: table rows %lld apart, %d wide", what, (long long)d->table_stride, d->width);
-    AttendShape sh;
-    if (int rc = attend_shape(*d, sh)) return rc;
-    if (sh.bytes() > 0 && (!d->workspace || !aligned(d->workspace, 16) || d->workspace_bytes < sh.bytes()))
-        return pk_fail(PK_ERR_ARG, "%s: a workspace of %lld bytes is wanted, aligned to 16 (%lld given)", what, (long long)sh.bytes(),
-                       (long long)(d->workspace ? d->workspace_bytes : 0));
-    AttendParams p;
-    p.q = d->q, p.out = d->out, p.lse = d->lse, p.cache = (const uint8_t *)d->cache;
-    p.table = d->table, p.lens = d->lens, p.first = d->first;
-    p.arrived = (int *)d->workspace;
-    p.part = (float *)((char *)d->workspace + kCounters * 4);
-    p.q_row = d->q_row, p.q_head = d->q_head, p.out_row = d->out_row, p.out_head = d->out_head;
-    p.page_stride = d->page_stride, p.table_stride = d->table_stride;
-    p.n_rows = d->n_rows, p.requests = d->requests, p.heads = d->heads, p.kv_heads = d->kv_heads;
-    p.page = d->page, p.page_shift = log2i(d->page), p.n_pages = d->n_pages, p.width = d->width;
-    p.max_len = d->max_len, p.window = d->window, p.group = d->heads / d->kv_heads;
-    p.tiles = sh.tiles, p.splits = sh.splits, p.groups = sh.groups, p.chunk = sh.chunk, p.scale = d->scale;
-    p.vec = aligned(d->q, 16) && d->q_row % 8 == 0 && d->q_head % 8 == 0;
-    p.vec_out = aligned(d->out, 8) && d->out_row % 4 == 0 && d->out_head % 4 == 0;
-    const unsigned grid = (unsigned)((int64_t)d->requests * d->kv_heads * sh.tiles * sh.splits);
-    if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, sh.prompt, d->head_dim, grid, (hipStream_t)stream);
-    else launch_attend<BF16>(p, sh.prompt, d->head_dim, grid, (hipStream_t)stream);
-    return launched(what);
+    return attend_call<HostKv4>("pk_kv4_attend", d, [&](const AttendParams &p, bool prompt, unsigned grid) {
+        if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
+        else launch_attend<BF16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
+    });
 }
 
 static int sample_check(const char *what, const pk_sample_desc *d) {

@@ -1,0 +1,296 @@
+// pk_lm_step.hip -- host side + C ABI of parakeet_lm.h's operators of a step with drafted tokens: norms and rotation, the
+// 8-bit cache, attention over it, verification.  The kernels are in lm_rope.h, lm_cache8.h, lm_attend.h and lm_verify.h.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "lm_attend8.h"
+#include "lm_attend_host.h"
+#include "lm_cache8.h"
+#include "lm_host.h"
+#include "lm_rope.h"
+#include "lm_verify.h"
+#include "parakeet_lm.h"
+
+namespace {
+
+using namespace pklm;
+
+// What pk_kv8_append, _load and _attend ask of the cache; 0 = fine.
+int check_cache8(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
+    if (page != 32 && page != 64 && page != 128 && page != 256)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: pages of %d tokens (32, 64, 128 or 256)", what, page);
+    if (dim != 64 && dim != 128 && dim != 256) return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, dim);
+    if (heads <= 0 || n_pages <= 0) return pk_fail(PK_ERR_ARG, "%s: %d heads, %d pages", what, heads, n_pages);
+    if ((int64_t)n_pages * page > INT32_MAX)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d pages of %d tokens: slots are 32 bits", what, n_pages, page);
+    if (!cache || !aligned(cache, 16)) return pk_fail(PK_ERR_ARG, "%s: the cache is NULL or not aligned to 16 bytes", what);
+    const Record8 rec{page, dim};
+    if (page_stride % 16 || page_stride < heads * rec.bytes())
+        return pk_fail(PK_ERR_ARG, "%s: page_stride %lld bytes (a multiple of 16, at least %lld)", what, (long long)page_stride,
+                       (long long)(heads * rec.bytes()));
+    return PK_OK;
+}
+
+// What pk_qk_rope and pk_kv8_append ask of the norm and the rotation.
+int check_turn(const char *what, int dim, int rot, const float *inv_freq, const int32_t *pos, int norm, float eps, const float *qw, const float *kw) {
+    if (rot < 0 || rot > dim || rot % 16) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d of %d channels turned (a multiple of 16)", what, rot, dim);
+    if (rot && (!inv_freq || !pos)) return pk_fail(PK_ERR_ARG, "%s: NULL positions or inv_freq", what);
+    if (norm && !(eps >= 0 && std::isfinite(eps))) return pk_fail(PK_ERR_ARG, "%s: an eps of %g", what, eps);
+    if (!aligned(inv_freq, 4) || !aligned(pos, 4) || !aligned(qw, 4) || !aligned(kw, 4))
+        return pk_fail(PK_ERR_ARG, "%s: positions, inv_freq or weights not aligned to their type", what);
+    return PK_OK;
+}
+
+// Whether 8 channels of any row are 16-byte aligned.
+bool wide_rows(const void *p, int64_t row, int64_t head, int size) {
+    const int per = 16 / size;
+    return aligned(p, 16) && row % per == 0 && head % per == 0;
+}
+
+// Rows of a workgroup, workgroups beside it on the same rows.
+struct TurnGrid {
+    int rows, parts;
+    int64_t groups;
+};
+// As many rows as leave 1,024 workgroups, then a head a wave as long as there are fewer.
+TurnGrid turn_grid(int n_rows, int units, int least) {
+    TurnGrid g;
+    g.rows = (int)std::min<int64_t>(std::max<int64_t>(n_rows / 1024, least), kTurnRows);
+    g.groups = ((int64_t)n_rows + g.rows - 1) / g.rows;
+    const int64_t most = (units + kTurnWaves - 1) / kTurnWaves;
+    g.parts = (int)std::min<int64_t>(std::max<int64_t>((1024 + g.groups - 1) / g.groups, 1), most);
+    return g;
+}
+
+template <class F>
+void by_type(int dtype, F f) {
+    if (dtype == PK_DTYPE_F32) f(F32{});
+    else if (dtype == PK_DTYPE_F16) f(F16{});
+    else f(BF16{});
+}
+template <class F>
+void by_dim(int dim, F f) {
+    if (dim == 64) f(std::integral_constant<int, 64>{});
+    else if (dim == 128) f(std::integral_constant<int, 128>{});
+    else f(std::integral_constant<int, 256>{});
+}
+
+struct HostKv8 {
+    static int check(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
+        return check_cache8(what, cache, page_stride, page, n_pages, heads, dim);
+    }
+    static bool has_prompt(int dtype, int dim) { return !(dtype == PK_DTYPE_F16 && dim == 256); }
+};
+
+template <class T>
+void launch_attend8(const AttendParams &p, bool prompt, int dim, unsigned grid, hipStream_t s) {
+    by_dim(dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if constexpr (D < 256 || __is_same(T, BF16)) {
+            if (prompt) return attend_prompt_kernel<Kv8, T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
+        }
+        attend_kernel<Kv8, T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
+    });
+}
+
+// Verification.  Rows of up to kVerifyVocab logits are a workgroup's each, in one launch; longer ones are cut in chunks.
+constexpr int kVerifyVocab = 16384;
+
+struct VerifyShape {
+    int per, chunks;             // tokens a thread takes of a chunk, chunks of a row
+    // counters first, the same place for every shape: they are zero between calls
+    static constexpr int64_t kCounterBytes = PK_LM_MAX_REQUESTS * 4;
+    int64_t max_at, at_at, sum_at, left_at, bytes;
+};
+
+VerifyShape verify_shape(const pk_verify_desc &d) {
+    VerifyShape s{};
+    const int64_t rows = (int64_t)d.requests * d.max_new;
+    if (d.vocab <= kVerifyVocab) {
+        s.bytes = VerifyShape::kCounterBytes + rows * (int64_t)sizeof(RowVerdict);
+        return s;
+    }
+    const int aim = (int)std::min<int64_t>(std::max<int64_t>(512 / std::max<int64_t>(rows, 1), 2), 16);
+    s.per = std::min(std::max((d.vocab + aim * kSplitThreads - 1) / (aim * kSplitThreads), 4), kMaxChunks);
+    s.chunks = (d.vocab + s.per * kSplitThreads - 1) / (s.per * kSplitThreads);
+    int64_t at = VerifyShape::kCounterBytes;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    s.max_at = take(rows * 2 * s.chunks * 4), s.at_at = take(rows * 2 * s.chunks * 4), s.sum_at = take(rows * 2 * s.chunks * 8);
+    s.left_at = take((int64_t)d.requests * s.chunks * 8);
+    s.bytes = at;
+    return s;
+}
+static_assert(PK_LM_MAX_VOCAB <= 64 * kMaxChunks * kSplitThreads, "a chunk a lane");
+
+int verify_check(const char *what, const pk_verify_desc *d) {
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (d->requests < 0 || d->requests > PK_LM_MAX_REQUESTS)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests (at most %d)", what, d->requests, PK_LM_MAX_REQUESTS);
+    if (d->n_rows < 0 || d->max_new < 0 || d->vocab <= 0 || d->vocab > PK_LM_MAX_VOCAB)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows, max_new %d, %d logits (1 .. %d)", what, d->n_rows, d->max_new, d->vocab, PK_LM_MAX_VOCAB);
+    // with 16 chunks a row at most of two sources
+    if ((int64_t)d->requests * d->max_new > most_groups(kSplitThreads) / 128)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests of up to %d rows in one call", what, d->requests, d->max_new);
+    return PK_OK;
+}
+
+template <class T, int BS, int E>
+void launch_verify_rows(const pk_verify_desc &d, hipStream_t s) {
+    int *arrived = (int *)d.workspace;
+    auto *verdicts = (RowVerdict *)((char *)d.workspace + VerifyShape::kCounterBytes);
+    const unsigned grid = (unsigned)(d.requests * d.max_new);
+    if (d.draft) verify_row_kernel<T, BS, E, true><<<grid, BS, 0, s>>>(d, arrived, verdicts);
+    else verify_row_kernel<T, BS, E, false><<<grid, BS, 0, s>>>(d, arrived, verdicts);
+}
+
+template <class T>
+void launch_verify(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s) {
+    if (d.vocab <= 1024) return launch_verify_rows<T, 256, 4>(d, s);
+    if (d.vocab <= 2048) return launch_verify_rows<T, 256, 8>(d, s);
+    if (d.vocab <= 4096) return launch_verify_rows<T, 1024, 4>(d, s);
+    if (d.vocab <= kVerifyVocab) return launch_verify_rows<T, 1024, 16>(d, s);
+    char *w = (char *)d.workspace;
+    SplitVerify p;
+    p.arrived = (int *)w, p.chunk_max = (float *)(w + sh.max_at), p.chunk_at = (int *)(w + sh.at_at), p.chunk_sum = (u64 *)(w + sh.sum_at);
+    p.left = (u64 *)(w + sh.left_at);
+    p.chunks = sh.chunks, p.per = sh.per, p.sources = d.draft ? 2 : 1;
+    const unsigned grid = (unsigned)(d.requests * d.max_new * p.sources * p.chunks);
+    verify_max_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
+    verify_sum_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
+    verify_draw_kernel<T><<<(unsigned)(d.requests * p.chunks), kSplitThreads, 0, s>>>(d, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+PK_API int pk_qk_rope(const pk_qk_rope_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_qk_rope";
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 or 256)", what, d->head_dim);
+    if (!float_type(d->dtype)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
+    if (d->n_rows < 0 || d->heads < 0 || d->kv_heads < 0 || d->heads + (int64_t)d->kv_heads > 65535)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d and %d heads (at most 65535)", what, d->n_rows, d->heads, d->kv_heads);
+    if (int rc = check_turn(what, d->head_dim, d->rot_dim, d->inv_freq, d->pos, d->norm, d->eps, d->q_weight, d->k_weight)) return rc;
+    if (d->n_rows == 0 || d->heads + d->kv_heads == 0) return PK_OK;
+    const int size = type_size(d->dtype);
+    if ((d->heads && (!d->q || !d->q_out)) || (d->kv_heads && (!d->k || !d->k_out))) return pk_fail(PK_ERR_ARG, "%s: NULL rows", what);
+    if (!aligned(d->q, size) || !aligned(d->k, size) || !aligned(d->q_out, size) || !aligned(d->k_out, size))
+        return pk_fail(PK_ERR_ARG, "%s: rows not aligned to their type", what);
+    const TurnGrid g = turn_grid(d->n_rows, d->heads + d->kv_heads, 512 / d->head_dim);
+    if (g.groups * g.parts > most_groups(kTurnThreads)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows in one call", what, d->n_rows);
+    const int wide_q = wide_rows(d->q, d->q_row, d->q_head, size) | wide_rows(d->q_out, d->q_out_row, d->q_out_head, size) << 1;
+    const int wide_k = wide_rows(d->k, d->k_row, d->k_head, size) | wide_rows(d->k_out, d->k_out_row, d->k_out_head, size) << 1;
+    by_type(d->dtype, [&](auto t) {
+        by_dim(d->head_dim, [&](auto dim) {
+            rope_kernel<decltype(t), dim.value><<<dim3((unsigned)g.groups, g.parts), kTurnThreads, 0, (hipStream_t)stream>>>(*d, g.rows, wide_q, wide_k);
+        });
+    });
+    return launched(what);
+}
+
+PK_API int pk_kv8_append(const pk_kv8_append_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_kv8_append";
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (int rc = check_cache8(what, d->cache, d->page_stride, d->page, d->n_pages, d->kv_heads, d->head_dim)) return rc;
+    if (!float_type(d->dtype)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
+    if (d->n_rows < 0 || d->heads < 0 || d->heads + 2 * (int64_t)d->kv_heads > 65535)
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d and 2 x %d heads (at most 65535)", what, d->n_rows, d->heads, d->kv_heads);
+    if (int rc = check_turn(what, d->head_dim, d->rot_dim, d->inv_freq, d->pos, d->norm, d->eps, d->q_weight, d->k_weight)) return rc;
+    if (d->n_rows == 0) return PK_OK;
+    const int size = type_size(d->dtype);
+    if (!d->k || !d->v || !d->slots || (d->heads && (!d->q || !d->q_out))) return pk_fail(PK_ERR_ARG, "%s: NULL rows or slots", what);
+    if (!aligned(d->k, size) || !aligned(d->v, size) || !aligned(d->q, size) || !aligned(d->q_out, size) || !aligned(d->slots, 4))
+        return pk_fail(PK_ERR_ARG, "%s: rows or slots not aligned to their type", what);
+    const TurnGrid g = turn_grid(d->n_rows, 2 * d->kv_heads + d->heads, 1);
+    if (g.groups * g.parts > most_groups(kTurnThreads)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows in one call", what, d->n_rows);
+    const int wide_q = wide_rows(d->q, d->q_row, d->q_head, size) | wide_rows(d->q_out, d->q_out_row, d->q_out_head, size) << 1;
+    const int wide_kv = wide_rows(d->k, d->k_row, d->k_head, size) && wide_rows(d->v, d->v_row, d->v_head, size);
+    by_type(d->dtype, [&](auto t) {
+        by_dim(d->head_dim, [&](auto dim) {
+            append_kernel<decltype(t), dim.value><<<dim3((unsigned)g.groups, g.parts), kTurnThreads, 0, (hipStream_t)stream>>>(
+                *d, g.rows, log2i(d->page), wide_q, wide_kv);
+        });
+    });
+    return launched(what);
+}
+
+PK_API int pk_kv8_load(const pk_kv4_rows_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_kv8_load";
+    if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
+    if (int rc = check_cache8(what, d->cache, d->page_stride, d->page, d->n_pages, d->heads, d->head_dim)) return rc;
+    if (d->n_rows < 0) return pk_fail(PK_ERR_ARG, "%s: %d rows", what, d->n_rows);
+    if (d->n_rows == 0) return PK_OK;
+    if (!float_type(d->dtype)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
+    const int size = type_size(d->dtype);
+    if (!d->k || !d->v || !d->slots) return pk_fail(PK_ERR_ARG, "%s: NULL rows or slots", what);
+    if (!aligned(d->k, size) || !aligned(d->v, size) || !aligned(d->slots, 4))
+        return pk_fail(PK_ERR_ARG, "%s: rows or slots not aligned to their type", what);
+    if (d->heads > 32767) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d heads (at most 32767)", what, d->heads);
+    const int each = kRowThreads * 8 / d->head_dim;
+    const int64_t groups = ((int64_t)d->n_rows + each - 1) / each;
+    if (groups * 2 * d->heads > most_groups(kRowThreads))
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d channels in one call", what, d->n_rows, d->head_dim);
+    const int wide = wide_rows(d->k, d->k_row, d->k_head, size) && wide_rows(d->v, d->v_row, d->v_head, size);
+    by_type(d->dtype, [&](auto t) {
+        by_dim(d->head_dim, [&](auto dim) {
+            load8_kernel<decltype(t), dim.value><<<dim3((unsigned)groups, 2 * d->heads), kRowThreads, 0, (hipStream_t)stream>>>(*d, log2i(d->page), wide);
+        });
+    });
+    return launched(what);
+}
+
+PK_API int pk_kv8_attend_workspace(const pk_kv4_attend_desc *d, int64_t *bytes) {
+    return attend_workspace<HostKv8>("pk_kv8_attend", d, bytes);
+}
+
+PK_API int pk_kv8_attend(const pk_kv4_attend_desc *d, void *stream) {
+    return attend_call<HostKv8>("pk_kv8_attend", d, [&](const AttendParams &p, bool prompt, unsigned grid) {
+        if (d->dtype == PK_DTYPE_F16) launch_attend8<F16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
+        else launch_attend8<BF16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
+    });
+}
+
+PK_API int pk_verify_workspace(const pk_verify_desc *d, int64_t *bytes) {
+    pk_fail_clear();
+    if (int rc = verify_check("pk_verify_workspace", d)) return rc;
+    if (!bytes) return pk_fail(PK_ERR_ARG, "pk_verify_workspace: NULL result");
+    *bytes = verify_shape(*d).bytes;
+    return PK_OK;
+}
+
+PK_API int pk_verify(const pk_verify_desc *d, void *stream) {
+    pk_fail_clear();
+    const char *what = "pk_verify";
+    if (int rc = verify_check(what, d)) return rc;
+    if (!float_type(d->dtype)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
+    if (d->requests == 0) return PK_OK;
+    if (d->max_new == 0) return pk_fail(PK_ERR_ARG, "%s: max_new 0", what);
+    if (!d->logits || !d->tokens || !d->first || !d->u || !d->u_draw || !d->out || !d->accepted) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
+    if ((d->lens_out && !d->lens) || d->lens_out == d->lens) {
+        if (d->lens_out) return pk_fail(PK_ERR_ARG, "%s: lens_out without lens, or lens itself", what);
+    }
+    if (d->out == d->tokens) return pk_fail(PK_ERR_ARG, "%s: out is written while tokens are read", what);
+    const int size = type_size(d->dtype);
+    if (!aligned(d->logits, size) || !aligned(d->draft, size)) return pk_fail(PK_ERR_ARG, "%s: logits not aligned to their type", what);
+    const VerifyShape sh = verify_shape(*d);
+    if (!d->workspace || !aligned(d->workspace, 16) || d->workspace_bytes < sh.bytes)
+        return pk_fail(PK_ERR_ARG, "%s: a workspace of %lld bytes is wanted, aligned to 16 (%lld given)", what, (long long)sh.bytes,
+                       (long long)(d->workspace ? d->workspace_bytes : 0));
+    by_type(d->dtype, [&](auto t) { launch_verify<decltype(t)>(*d, sh, (hipStream_t)stream); });
+    return launched(what);
+}
+
+}  // extern "C"

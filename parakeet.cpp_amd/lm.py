@@ -9,6 +9,14 @@ products, over sessions that share one paged cache held in 4 bits:
     lm.sample(logits, u, ...)       the next token of every session
     lm.kv4_load(...)                rows back out of the cache
 
+and, for models that norm and rotate queries and keys, a cache held in 8 bits and steps with drafted tokens:
+
+    lm.qk_rope(q, q_out, ...)       norms of queries and keys for each head, and the position rotation
+    lm.kv8_append(k, v, ...)        rows into a paged cache held in 8 bits, normed and rotated on the way
+    lm.kv8_attend(q, ...)           attention over it
+    lm.kv8_load(...)                rows back out of it
+    lm.verify(logits, tokens, ...)  which drafted tokens stand, and the token behind them
+
 Arrays are ``torch`` tensors on the GPU or ``hipmem.Tensor``s, inputs and
 outputs alike: outputs are given by the caller and written in place.  Calls are
 enqueued on ``stream`` (a hipStream_t as an integer; by default torch's current
@@ -17,7 +25,7 @@ the workspaces below, wait for nothing and can be captured into a graph.
 Arguments are checked here and in the library; ``pk.PkError`` carries the
 library's status.
 
-Workspaces (``kv4_attend``, ``sample``) are kept per operator, device and stream and only
+Workspaces (``kv4_attend``, ``kv8_attend``, ``sample``, ``verify``) are kept per operator, device and stream and only
 ever grow; one that has been handed out is never freed, since a captured graph
 may hold it.  For torch tensors a graph's capture has its own, which the graph zeroes, so that
 graphs may be replayed in any order and beside each other.  Other graphs share their
@@ -43,11 +51,13 @@ from . import hipmem, pk
 
 F32, F16, BF16 = 0, 1, 2                 # parakeet_lm.h PK_DTYPE_*
 PAGES = (16, 32, 64, 128, 256)
+KV8_PAGES = (32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 MAX_REQUESTS, MAX_VOCAB = 4096, 1048576
 
 EXPORTED = ["pk_kv_plan", "pk_kv4_store", "pk_kv4_load", "pk_kv4_attend", "pk_kv4_attend_workspace", "pk_sample",
-            "pk_sample_workspace"]
+            "pk_sample_workspace", "pk_qk_rope", "pk_kv8_append", "pk_kv8_load", "pk_kv8_attend", "pk_kv8_attend_workspace", "pk_verify",
+            "pk_verify_workspace"]
 TORCH_PATH = os.path.join(pk.HERE, "_lm_torch.so")
 
 _FLOATS = {"f32": F32, "f16": F16, "bf16": BF16}
@@ -67,6 +77,9 @@ _PLAN = struct.Struct("11Pq5i0P")
 _ROWS = struct.Struct("4P5q6i0P")
 _ATTEND = struct.Struct("8P7q12if0P")
 _SAMPLE = struct.Struct("10P2q4i0P")
+_ROPE = struct.Struct("8P8q8if0P")
+_APPEND = struct.Struct("10P9q10if0P")
+_VERIFY = struct.Struct("14P3q6i0P")
 
 
 def _load():
@@ -174,6 +187,51 @@ def kv4_shape(n_pages: int, kv_heads: int, head_dim: int, page: int):
     return n_pages, kv_heads, page * (head_dim + head_dim // 16)
 
 
+def _cache8(cache, page, what):
+    """(pointer, page stride, pages, heads, head_dim) of cache [n_pages, kv_heads, page (2 D + 1/2)] bytes."""
+    if cache.dtype != "u8":
+        raise TypeError(f"{what}: cache of {cache.dtype} (uint8)")
+    n, heads, size = cache.shape
+    s = cache.stride()
+    dim, odd = divmod(2 * size - page, 4 * page) if page > 0 else (0, 1)
+    if odd or dim <= 0 or s[2] != 1 or (heads > 1 and s[1] != size):
+        raise ValueError(f"{what}: cache of shape {tuple(cache.shape)}, strides {tuple(s)}: expected kv8_shape(...) "
+                         f"for pages of {page} tokens, the records of a page adjacent")
+    return cache.data_ptr(), s[0] if n > 1 else heads * size, n, heads, dim
+
+
+def kv8_shape(n_pages: int, kv_heads: int, head_dim: int, page: int):
+    """Shape of a cache (uint8) of n_pages pages of `page` tokens: a byte a value of K and of V, 16 bytes for 32 tokens."""
+    if page not in KV8_PAGES or head_dim not in HEAD_DIMS:
+        raise ValueError(f"pages of {page} tokens (one of {KV8_PAGES}), head_dim {head_dim} (one of {HEAD_DIMS})")
+    return n_pages, kv_heads, page * 2 * head_dim + page // 2
+
+
+def _apart(t, what):
+    """Refuses outputs whose rows or heads lie over each other."""
+    s = t.stride()
+    n, heads, dim = t.shape
+    if (heads > 1 and s[1] < dim) or (n > 1 and s[0] < dim):
+        raise ValueError(f"{what}: rows overlap (strides {s[0]}, {s[1]})")
+
+
+def _turned(x, y, weight, what):
+    """(pointers of rows and of their result and weights, their strides) of one of the two that are normed and rotated."""
+    if y is None or y.dtype != x.dtype or tuple(y.shape) != tuple(x.shape):
+        raise ValueError(f"{what} {x.dtype} {tuple(x.shape)}, {what}_out {y and (y.dtype, tuple(y.shape))}")
+    xp, xr, xh = _heads(x, what)
+    yp, yr, yh = _heads(y, what + "_out")
+    _apart(y, what + "_out")
+    return (xp, yp, 0 if weight is None else _f32(weight, (x.shape[2],), what + "_weight")), (xr, xh, yr, yh)
+
+
+def _inv(inv_freq):
+    """(pointer, channels turned)"""
+    if inv_freq is None:
+        return 0, 0
+    return _f32(inv_freq, (inv_freq.shape[0],), "inv_freq"), 2 * inv_freq.shape[0]
+
+
 def _workspace(kind, stream, wanted, given):
     """(pointer, bytes) of at least `wanted` bytes, zeroed before the first use; each kind of call has its own on each device
     and stream."""
@@ -219,13 +277,13 @@ def kv_plan(old_len, new_len, table, ring, state, page: int, *, state_out, lens,
     _call("pk_kv_plan", packed, stream)
 
 
-def _kv4_rows(name, k, v, slots, cache, page, stream):
+def _kv4_rows(name, k, v, slots, cache, page, stream, layout=_cache):
     dt = _dtype(k, "k")
     if v.dtype != k.dtype or tuple(v.shape) != tuple(k.shape):
         raise ValueError(f"k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}")
     kp, kr, kh = _heads(k, "k")
     vp, vr, vh = _heads(v, "v")
-    cp, ps, n_pages, heads, dim = _cache(cache, page, name)
+    cp, ps, n_pages, heads, dim = layout(cache, page, name)
     n = k.shape[0]
     if k.shape[1] != heads or k.shape[2] != dim:
         raise ValueError(f"rows of {k.shape[1]} heads of {k.shape[2]}, a cache of {heads} heads of {dim}")
@@ -255,27 +313,13 @@ def kv4_load(cache, slots, k, v, page: int, stream=None):
     _kv4_rows("pk_kv4_load", k, v, slots, cache, page, stream)
 
 
-def kv4_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: int = 1, max_len: int | None = None,
-               scale: float | None = None, window: int = 0, lse=None, workspace=None, stream=None):
-    """pk_kv4_attend: out = softmax(scale q K^T) V, causal.
-
-    q, out [n_rows, heads, head_dim]; table [requests, width]; lens [requests]
-    tokens held, q's included; first [requests + 1] where each request's queries
-    begin (None: one query each); max_new and max_len bound the queries and the
-    tokens of any request (max_len defaults to what the table can name); window
-    > 0 limits every query to its last `window` keys; lse [n_rows, heads] f32.
-    """
-    if isinstance(q, _Tensor) or _new_torch(q):
-        rc = _torch_calls.kv4_attend(q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream)
-        if rc:
-            pk.check(rc)
-        return
+def _attend(name, layout, kind, q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream):
     dt = _dtype(q, "q")
     if out.dtype != q.dtype or tuple(out.shape) != tuple(q.shape):
         raise ValueError(f"q {q.dtype} {tuple(q.shape)}, out {out.dtype} {tuple(out.shape)}")
     qp, qr, qh = _heads(q, "q")
     op, our, oh = _heads(out, "out")
-    cp, ps, n_pages, kv_heads, dim = _cache(cache, page, "kv4_attend")
+    cp, ps, n_pages, kv_heads, dim = layout(cache, page, name)
     n, heads, d = q.shape
     B, width = table.shape
     if d != dim or heads % kv_heads:
@@ -292,9 +336,27 @@ def kv4_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: in
     tail = (qr, qh, our, oh, ps, ts, n, B, heads, kv_heads, dim, dt, page, n_pages, width, max_new, max_len, window,
             dim ** -0.5 if scale is None else scale)
     wanted = C.c_int64()
-    _call("pk_kv4_attend_workspace", _ATTEND.pack(*head, 0, 0, *tail), C.addressof(wanted))
-    wp, wb = _workspace("attend", stream, wanted.value, workspace)
-    _call("pk_kv4_attend", _ATTEND.pack(*head, wp, wb, *tail), stream)
+    _call(name + "_workspace", _ATTEND.pack(*head, 0, 0, *tail), C.addressof(wanted))
+    wp, wb = _workspace(kind, stream, wanted.value, workspace)
+    _call(name, _ATTEND.pack(*head, wp, wb, *tail), stream)
+
+
+def kv4_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: int = 1, max_len: int | None = None,
+               scale: float | None = None, window: int = 0, lse=None, workspace=None, stream=None):
+    """pk_kv4_attend: out = softmax(scale q K^T) V, causal.
+
+    q, out [n_rows, heads, head_dim]; table [requests, width]; lens [requests]
+    tokens held, q's included; first [requests + 1] where each request's queries
+    begin (None: one query each); max_new and max_len bound the queries and the
+    tokens of any request (max_len defaults to what the table can name); window
+    > 0 limits every query to its last `window` keys; lse [n_rows, heads] f32.
+    """
+    if isinstance(q, _Tensor) or _new_torch(q):
+        rc = _torch_calls.kv4_attend(q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream)
+        if rc:
+            pk.check(rc)
+        return
+    _attend("pk_kv4_attend", _cache, "attend", q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream)
 
 
 def sample(logits, u, token, *, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, kept=None, workspace=None,
@@ -322,3 +384,128 @@ def sample(logits, u, token, *, temperature=None, top_k=None, top_p=None, min_p=
     _call("pk_sample_workspace", _SAMPLE.pack(*head, 0, 0, lr, B, V, dt, 0), C.addressof(wanted))
     wp, wb = _workspace("sample", stream, wanted.value, workspace)
     _call("pk_sample", _SAMPLE.pack(*head, wp, wb, lr, B, V, dt, 0), stream)
+
+
+def qk_rope(q, q_out, pos, inv_freq, *, k=None, k_out=None, eps: float | None = None, q_weight=None, k_weight=None,
+            interleaved: bool = False, stream=None):
+    """pk_qk_rope: rows q [n, heads, head_dim], and k [n, kv_heads, head_dim], normed where eps is given (weights [head_dim] f32,
+    None = 1) and turned by the angles pos [n] * inv_freq (f32, None: not turned), into q_out and k_out, which may be q and k.
+
+    The first 2 * len(inv_freq) channels are turned, pair j being channels j and len(inv_freq) + j, or 2j and 2j + 1 with
+    `interleaved`.  Rows at positions below 0 are left as they are in the outputs.
+    """
+    if isinstance(q, _Tensor) or _new_torch(q):
+        rc = _torch_calls.qk_rope(q, q_out, pos, inv_freq, k, k_out, eps, q_weight, k_weight, interleaved, stream)
+        if rc:
+            pk.check(rc)
+        return
+    (qp, qo, qw), qs = _turned(q, q_out, q_weight, "q")
+    n, heads, dim = q.shape
+    kp = ko = kw = kv_heads = 0
+    ks = (0, 0, 0, 0)
+    if k is not None:
+        if k.dtype != q.dtype or k.shape[0] != n or k.shape[2] != dim:
+            raise ValueError(f"q {q.dtype} {tuple(q.shape)}, k {k.dtype} {tuple(k.shape)}")
+        (kp, ko, kw), ks = _turned(k, k_out, k_weight, "k")
+        kv_heads = k.shape[1]
+    ip, rot = _inv(inv_freq)
+    packed = _ROPE.pack(qp, kp, qo, ko, qw, kw, ip, 0 if pos is None else _i32(pos, (n,), "pos"), *qs[:2], *ks[:2], *qs[2:], *ks[2:],
+                        n, heads, kv_heads, dim, _dtype(q, "q"), rot, eps is not None, bool(interleaved), 0.0 if eps is None else eps)
+    _call("pk_qk_rope", packed, stream)
+
+
+def kv8_append(k, v, slots, cache, page: int, *, pos=None, inv_freq=None, eps: float | None = None, k_weight=None, q=None, q_out=None,
+               q_weight=None, interleaved: bool = False, stream=None):
+    """pk_kv8_append: rows k, v [n, kv_heads, head_dim] into cache (kv8_shape) at slots [n], k normed and turned before as by
+    qk_rope; where q [n, heads, head_dim] is given it is normed and turned into q_out in the same launch.
+
+    Rows with a slot outside the cache (-1), or a position below 0, are skipped.  A request's rows lie one after the other in
+    the call, their slots rising, behind what the cache holds of it already, as kv_plan deals them out.
+    """
+    if isinstance(cache, _Tensor) or _new_torch(cache):
+        rc = _torch_calls.kv8_append(k, v, slots, cache, page, pos, inv_freq, eps, k_weight, q, q_out, q_weight, interleaved, stream)
+        if rc:
+            pk.check(rc)
+        return
+    dt = _dtype(k, "k")
+    if v.dtype != k.dtype or tuple(v.shape) != tuple(k.shape):
+        raise ValueError(f"k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}")
+    kp, kr, kh = _heads(k, "k")
+    vp, vr, vh = _heads(v, "v")
+    cp, ps, n_pages, kv_heads, dim = _cache8(cache, page, "kv8_append")
+    n = k.shape[0]
+    if k.shape[1] != kv_heads or k.shape[2] != dim:
+        raise ValueError(f"rows of {k.shape[1]} heads of {k.shape[2]}, a cache of {kv_heads} heads of {dim}")
+    qp = qo = qw = heads = 0
+    qs = (0, 0, 0, 0)
+    if q is not None:
+        if q.dtype != k.dtype or q.shape[0] != n or q.shape[2] != dim:
+            raise ValueError(f"k {k.dtype} {tuple(k.shape)}, q {q.dtype} {tuple(q.shape)}")
+        (qp, qo, qw), qs = _turned(q, q_out, q_weight, "q")
+        heads = q.shape[1]
+    ip, rot = _inv(inv_freq)
+    packed = _APPEND.pack(kp, vp, qp, qo, _i32(slots, (n,), "slots"), 0 if pos is None else _i32(pos, (n,), "pos"), qw,
+                          0 if k_weight is None else _f32(k_weight, (dim,), "k_weight"), ip, cp, kr, kh, vr, vh, *qs, ps, n, heads, kv_heads,
+                          dim, dt, page, n_pages, rot, eps is not None, bool(interleaved), 0.0 if eps is None else eps)
+    _call("pk_kv8_append", packed, stream)
+
+
+def kv8_load(cache, slots, k, v, page: int, stream=None):
+    """pk_kv8_load: as kv4_load, out of an 8-bit cache."""
+    if isinstance(cache, _Tensor) or _new_torch(cache):
+        rc = _torch_calls.kv8_load(cache, slots, k, v, page, stream)
+        if rc:
+            pk.check(rc)
+        return
+    _kv4_rows("pk_kv8_load", k, v, slots, cache, page, stream, _cache8)
+
+
+def kv8_attend(q, cache, table, lens, out, page: int, *, first=None, max_new: int = 1, max_len: int | None = None,
+               scale: float | None = None, window: int = 0, lse=None, workspace=None, stream=None):
+    """pk_kv8_attend: as kv4_attend, over an 8-bit cache (kv8_shape)."""
+    if isinstance(q, _Tensor) or _new_torch(q):
+        rc = _torch_calls.kv8_attend(q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream)
+        if rc:
+            pk.check(rc)
+        return
+    _attend("pk_kv8_attend", _cache8, "attend8", q, cache, table, lens, out, page, first, max_new, max_len, scale, window, lse, workspace, stream)
+
+
+def verify(logits, tokens, first, u, u_draw, out, accepted, *, max_new: int | None = None, draft=None, temperature=None,
+           draft_temperature=None, lens=None, lens_out=None, prob=None, workspace=None, stream=None):
+    """pk_verify: request b brought tokens[first[b] .. first[b + 1]), its last token and the drafts behind it; row r of logits
+    [n, vocab] is what the target says behind tokens[r], row r of `draft` [n, vocab] what tokens[r + 1] was drawn from (None:
+    drafts that were not drawn).
+
+    Uniform numbers u [n] decide on the drafts, u_draw [requests] on the token behind those accepted.  Written: out [n] int32
+    (the accepted drafts, that token, then -1), accepted [requests], lens_out [requests] (lens less the refused drafts, what
+    kv_plan is to cut the cache back to) and prob [n] f32.  max_new bounds the rows of any request (None: n).
+    temperature and draft_temperature [requests] f32 (None = 1).
+    """
+    if isinstance(logits, _Tensor) or _new_torch(logits):
+        rc = _torch_calls.verify(logits, tokens, first, u, u_draw, out, accepted, max_new, draft, temperature, draft_temperature, lens, lens_out,
+                                 prob, workspace, stream)
+        if rc:
+            pk.check(rc)
+        return
+    dt = _dtype(logits, "logits")
+    n, V = logits.shape
+    lp, lr = _rows(logits, "logits")
+    dp = dr = 0
+    if draft is not None:
+        if draft.dtype != logits.dtype or tuple(draft.shape) != (n, V):
+            raise ValueError(f"logits {logits.dtype} {(n, V)}, draft {draft.dtype} {tuple(draft.shape)}")
+        dp, dr = _rows(draft, "draft")
+    if len(first.shape) != 1 or first.shape[0] < 1:
+        raise ValueError(f"first: shape {tuple(first.shape)}, expected [requests + 1]")
+    B = first.shape[0] - 1
+    opt = lambda f, t, shape, what: 0 if t is None else f(t, shape, what)  # noqa: E731
+    head = (lp, dp, _i32(tokens, (n,), "tokens"), _i32(first, (B + 1,), "first"), opt(_f32, temperature, (B,), "temperature"),
+            opt(_f32, draft_temperature, (B,), "draft_temperature"), _f32(u, (n,), "u"), _f32(u_draw, (B,), "u_draw"),
+            opt(_i32, lens, (B,), "lens"), _i32(out, (n,), "out"), _i32(accepted, (B,), "accepted"), opt(_i32, lens_out, (B,), "lens_out"),
+            opt(_f32, prob, (n,), "prob"))
+    tail = (lr, dr, n, B, V, dt, n if max_new is None else max_new, 0)
+    wanted = C.c_int64()
+    _call("pk_verify_workspace", _VERIFY.pack(*head, 0, 0, *tail), C.addressof(wanted))
+    wp, wb = _workspace("verify", stream, wanted.value, workspace)
+    _call("pk_verify", _VERIFY.pack(*head, wp, wb, *tail), stream)

@@ -11,8 +11,8 @@ joint QKV product and its next tokens, over a paged cache held in 8 bits.
 The cache.  Values are 8-bit floating point (sign, 4 exponent bits, 3 of fraction, largest 448, one NaN) under one power
 of two 2^e for the 32 tokens of a block and one head, K and V each; e is the smallest, -100 .. 119, that puts the block's
 largest magnitude at 448 2^e or below.  A page holds `page` tokens; a (page, kv head) record is K codes [page][D] | V codes
-[page/8][16][8][D/16] | [page/32] entries of 16 bytes: the K scale and the V scale in f32, negative where the block
-holds a NaN, and 8 bytes of zeros.  In the V codes, entry [a][r][i] has the D/16 channels from r D/16 of token 8a + i.
+[page/8][32][8][D/32] | [page/32] entries of 16 bytes: the K scale and the V scale in f32, negative where the block
+holds a NaN, and 8 bytes of zeros.  In the V codes, entry [a][r][i] has the D/32 channels from r D/32 of token 8a + i.
 """
 import math
 
@@ -360,7 +360,7 @@ def _records(k, v, page):
         bad = (~torch.isfinite(x)).any(-1).any(2)
         scales.append(torch.where(bad, -_pow2(e), _pow2(e)))
     kc = parts[0].permute(0, 2, 1, 3).reshape(n, H, -1)
-    vc = parts[1].view(n, page // 8, 8, H, 16, D // 16).permute(0, 3, 1, 4, 2, 5).reshape(n, H, -1)
+    vc = parts[1].view(n, page // 8, 8, H, 32, D // 32).permute(0, 3, 1, 4, 2, 5).reshape(n, H, -1)
     sc = torch.stack(scales + [torch.zeros_like(scales[0])] * 2, -1).transpose(1, 2).reshape(n, H, -1).contiguous()
     return torch.cat([kc, vc, sc.view(torch.uint8)], -1)
 
@@ -372,9 +372,9 @@ def _scales(cache, page, D):
 
 def _code_places(off, page, D):
     """Byte places [rows, D] of K and of V codes at these offsets of their pages."""
-    d, per = torch.arange(D, device=off.device), D // 16
+    d, per = torch.arange(D, device=off.device), D // 32
     return (off[:, None] * D + d,
-            page * D + ((off[:, None] // 8 * 16 + d // per) * 8 + off[:, None] % 8) * per + d % per)
+            page * D + ((off[:, None] // 8 * 32 + d // per) * 8 + off[:, None] % 8) * per + d % per)
 
 
 def _plain_append(s):
@@ -419,7 +419,7 @@ def _rows(records, page, D):
     """The values k, v [..., H, page, D] that records [..., H, bytes] stand for."""
     sc = _scales(records, page, D)
     kc = records[..., :page * D].contiguous().unflatten(-1, (page // BLOCK, BLOCK, D))
-    vc = records[..., page * D:2 * page * D].contiguous().unflatten(-1, (page // 8, 16, 8, D // 16)).transpose(-3, -2)
+    vc = records[..., page * D:2 * page * D].contiguous().unflatten(-1, (page // 8, 32, 8, D // 32)).transpose(-3, -2)
     vc = vc.flatten(-4).unflatten(-1, (page // BLOCK, BLOCK, D))
     return (_values(kc, sc[..., 0, None, None]).flatten(-3, -2), _values(vc, sc[..., 1, None, None]).flatten(-3, -2))
 
@@ -621,7 +621,7 @@ def _exact_append(case, s):
         old = back[:s["older"]]
         d = torch.arange(D, device="cuda")
         off = old % page
-        width = D // 16
+        width = D // 32
         place = off[:, None] * D + d if name == "k" else (
             page * D + off[:, None] // 8 * (8 * D) + d // width * (8 * width) + off[:, None] % 8 * width + d % width)
         code = s["cache"][(old // page)[:, None, None], torch.arange(H, device="cuda")[:, None], place[:, None]].int()
@@ -645,7 +645,7 @@ def _exact_attend(case, s):
     out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device="cuda")
     d = torch.arange(D, device="cuda")
-    width = D // 16
+    width = D // 32
     for b in range(B):
         n, new = lens[b], first[b + 1] - first[b]
         if n == 0:
