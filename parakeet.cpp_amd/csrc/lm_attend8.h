@@ -236,10 +236,13 @@ struct alignas(16) PromptTile8 {
     // NaNs is put into their channels.
     template <class Paged>
     __device__ void mask(v16f (&s)[2], v16f (&acc)[D / 32], int kb, int h, int lo, int hi, bool marked, Paged paged) const {
+        // A block of keys has a page or has none, so that its keys' bounds say it all.  (A look at the page of each key in the condition
+        // is compiled so that scores keep their values where the look alone is false.)
+        const int ends[2] = {paged(kb) ? hi : kb, paged(kb + kBlock) ? hi : kb};
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const int key = kb + 32 * (i >> 4) + 16 * (i >> 3 & 1) + 8 * h + (i & 7);
-            if (!(key < hi && key >= lo && paged(key))) s[i >> 4][i & 15] = -INFINITY;
+            s[i >> 4][i & 15] = ((key < ends[i >> 4]) & (key >= lo)) ? s[i >> 4][i & 15] : -INFINITY;
         }
         if (!marked) return;
         const int from = min(max(lo - kb, 0), 64), to = min(max(hi - kb, 0), 64);

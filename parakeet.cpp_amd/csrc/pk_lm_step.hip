@@ -279,9 +279,7 @@ PK_API int pk_verify(const pk_verify_desc *d, void *stream) {
     if (d->requests == 0) return PK_OK;
     if (d->max_new == 0) return pk_fail(PK_ERR_ARG, "%s: max_new 0", what);
     if (!d->logits || !d->tokens || !d->first || !d->u || !d->u_draw || !d->out || !d->accepted) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
-    if ((d->lens_out && !d->lens) || d->lens_out == d->lens) {
-        if (d->lens_out) return pk_fail(PK_ERR_ARG, "%s: lens_out without lens, or lens itself", what);
-    }
+    if (d->lens_out && (!d->lens || d->lens_out == d->lens)) return pk_fail(PK_ERR_ARG, "%s: lens_out without lens, or lens itself", what);
     if (d->out == d->tokens) return pk_fail(PK_ERR_ARG, "%s: out is written while tokens are read", what);
     const int size = type_size(d->dtype);
     if (!aligned(d->logits, size) || !aligned(d->draft, size)) return pk_fail(PK_ERR_ARG, "%s: logits not aligned to their type", what);
