@@ -1,8 +1,10 @@
 // lm_rope.h -- norms of queries and keys for each head and the position rotation (pk_qk_rope, and on the way into the
 // 8-bit cache pk_kv8_append).
 //
-// A row of D channels of one head is D/8 lanes' 8 adjacent channels, so that a wave holds 512 / D rows and the norm's
-// sum stays within a row's lanes.  The angles of a token are the same for all its heads: a workgroup works out the sines
+// A row of D channels of one head is D/8 lanes' 8 channels, so that a wave holds 512 / D rows and the norm's sum stays within a
+// row's lanes.  Where all channels are turned, in halves, a lane has 4 channels of the lower half and their partners in the upper one;
+// with partners beside each other, 8 adjacent channels; so no value crosses lanes.  (Partners through shuffles: 16,385 rows of
+// 32 + 8 heads x 128 took 88 us.)  Only a part's rotation in halves needs shuffles.  The angles of a token are the same for all its heads: a workgroup works out the sines
 // and cosines of its rows once, into LDS, and its waves go over the heads.  An angle is pos * inv_freq in f64, in turns
 // less the whole ones: in f32 a position of 200,000 has lost 2^-7 of a radian.
 #pragma once
@@ -29,8 +31,11 @@ __device__ inline float row_sum(float v) {
     return v;
 }
 
-// How rows are normed and turned.
+// How rows are normed and turned.  Halves: all channels are, in halves, and rows are aligned to four channels; a lane's 8 are
+// 4 of each half.
+template <bool Halves>
 struct Turn {
+    static constexpr bool halves = Halves;
     const float *inv_freq;
     const int *pos;              // nullable where nothing is turned
     int rot, norm, interleaved;
@@ -39,11 +44,49 @@ struct Turn {
     __device__ bool live(int64_t row) const { return !pos || pos[row] >= 0; }
 };
 
+// A lane's 8 channels of a row: 4 from lo, 4 from hi.
+template <int D>
+struct LaneChannels {
+    int lo, hi;
+    __device__ LaneChannels(int c, bool halves) : lo(halves ? 4 * c : 8 * c), hi(halves ? D / 2 + 4 * c : 8 * c + 4) {}
+};
+template <class Raw>
+struct alignas(4 * sizeof(Raw)) Four {
+    Raw v[4];
+};
+template <class T, int D>
+__device__ inline void load_channels(const typename T::Raw *row, const LaneChannels<D> &at, bool wide, float (&x)[8]) {
+    using Raw = typename T::Raw;
+    Four<Raw> lo, hi;
+    if (wide) {
+        lo = *(const Four<Raw> *)(row + at.lo), hi = *(const Four<Raw> *)(row + at.hi);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lo.v[i] = row[at.lo + i], hi.v[i] = row[at.hi + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = T::get(lo.v[i]), x[4 + i] = T::get(hi.v[i]);
+}
+template <class T, int D>
+__device__ inline void store_channels(typename T::Raw *row, const LaneChannels<D> &at, bool wide, const float (&x)[8]) {
+    using Raw = typename T::Raw;
+    Four<Raw> lo, hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lo.v[i] = T::put(x[i]), hi.v[i] = T::put(x[4 + i]);
+    if (wide) {
+        *(Four<Raw> *)(row + at.lo) = lo, *(Four<Raw> *)(row + at.hi) = hi;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row[at.lo + i] = lo.v[i], row[at.hi + i] = hi.v[i];
+    }
+}
+
 template <int D>
 struct TurnTable {
     float c[kTurnRows * D / 2], s[kTurnRows * D / 2];
 
     // the angles of the n rows from row0; a barrier on either side
+    template <class Turn>
     __device__ void fill(const Turn &turn, int64_t row0, int n) {
         const int half = turn.rot / 2;
         for (int i = threadIdx.x; i < n * half; i += kTurnThreads) {
@@ -55,8 +98,8 @@ struct TurnTable {
     }
 };
 
-// A lane's 8 channels from 8 lane_c of a row: normed with the weights w, turned by the angles of the table's row r.
-template <int D>
+// A lane's 8 channels of a row, the lane_c'th of its lanes: normed with the weights w, turned by the angles of the table's row r.
+template <int D, class Turn>
 __device__ inline void norm_and_turn(float (&x)[8], int lane_c, const Turn &turn, const TurnTable<D> &table, int r, const float (&w)[8]) {
     if (turn.norm) {
         float sum = 0;
@@ -66,9 +109,16 @@ __device__ inline void norm_and_turn(float (&x)[8], int lane_c, const Turn &turn
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= inv * w[i];
     }
-    if (turn.rot == 0) return;
-    const int half = turn.rot / 2;
-    if (turn.interleaved) {
+    if (!Turn::halves && turn.rot == 0) return;
+    const int half = Turn::halves ? D / 2 : turn.rot / 2;
+    if (Turn::halves) {
+        const v4f c = *(const v4f *)&table.c[r * half + 4 * lane_c], s = *(const v4f *)&table.s[r * half + 4 * lane_c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = x[i], b = x[4 + i];
+            x[i] = a * c[i] - b * s[i], x[4 + i] = a * s[i] + b * c[i];
+        }
+    } else if (turn.interleaved) {
         if (8 * lane_c < turn.rot) {
             const v4f c = *(const v4f *)&table.c[r * half + 4 * lane_c], s = *(const v4f *)&table.s[r * half + 4 * lane_c];
 #pragma unroll
@@ -97,34 +147,56 @@ __device__ inline void norm_and_turn(float (&x)[8], int lane_c, const Turn &turn
     }
 }
 
-__device__ inline void load_weights(const float *weight, int lane_c, float (&w)[8]) {
+template <int D>
+__device__ inline void load_weights(const float *weight, const LaneChannels<D> &at, float (&w)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = weight ? weight[8 * lane_c + i] : 1.0f;
+    for (int i = 0; i < 8; ++i) w[i] = weight ? weight[i < 4 ? at.lo + i : at.hi + i - 4] : 1.0f;
 }
 
-// One head's rows row0 .. row0 + n, n <= kTurnRows, from x into y, on one wave.
-template <class T, int D>
-__device__ inline void turn_rows(const typename T::Raw *x, int64_t x_row, bool wide, typename T::Raw *y, int64_t y_row, bool y_wide,
-                                 const float *weight, const Turn &turn, const TurnTable<D> &table, int64_t row0, int n) {
+// One head's rows row0 .. row0 + n, n <= kTurnRows, from x into y, on one wave: Batch passes' loads together.  (One pass at
+// a time leaves too little on its way: 16,385 rows of 32 + 8 heads x 128, 8-byte partners through shuffles, took 104 us, 4 at a time 88.)
+template <class T, int D, int Batch, class Turn>
+__device__ inline void turn_some(const typename T::Raw *x, int64_t x_row, bool wide, typename T::Raw *y, int64_t y_row, bool y_wide,
+                                 const float (&w)[8], const Turn &turn, const TurnTable<D> &table, int64_t row0, int n) {
     constexpr int kLanes = D / 8, kRows = 64 / kLanes;
     const int lane = threadIdx.x & 63, c = lane % kLanes;
-    float w[8];
-    load_weights(weight, c, w);
-    for (int r0 = 0; r0 < n; r0 += kRows) {
-        const int r = min(r0 + lane / kLanes, n - 1);
-        const int64_t row = row0 + r;
-        float v[8];
-        load8<T>(x + row * x_row + 8 * c, wide, v);
-        norm_and_turn<D>(v, c, turn, table, r, w);
-        if (r0 + lane / kLanes < n && turn.live(row)) store8<T>(y + row * y_row + 8 * c, y_wide, v);
+    const LaneChannels<D> at(c, Turn::halves);
+    for (int r0 = 0; r0 < n; r0 += kRows * Batch) {
+        float v[Batch][8];
+        bool live[Batch];
+#pragma unroll
+        for (int p = 0; p < Batch; ++p) {
+            const int r = r0 + p * kRows + lane / kLanes;
+            const int64_t row = row0 + min(r, n - 1);
+            load_channels<T, D>(x + row * x_row, at, Turn::halves || wide, v[p]);
+            live[p] = r < n && turn.live(row);
+        }
+#pragma unroll
+        for (int p = 0; p < Batch; ++p) {
+            const int r = r0 + p * kRows + lane / kLanes;
+            if (Batch > 1 && r0 + p * kRows >= n) break;
+            norm_and_turn<D>(v[p], c, turn, table, min(r, n - 1), w);
+            if (live[p]) store_channels<T, D>(y + (row0 + r) * y_row, at, Turn::halves || y_wide, v[p]);
+        }
     }
 }
+template <class T, int D, int Batch, class Turn>
+__device__ inline void turn_rows(const typename T::Raw *x, int64_t x_row, bool wide, typename T::Raw *y, int64_t y_row, bool y_wide,
+                                 const float *weight, const Turn &turn, const TurnTable<D> &table, int64_t row0, int n) {
+    float w[8];
+    load_weights(weight, LaneChannels<D>((threadIdx.x & 63) % (D / 8), Turn::halves), w);
+    if (n <= 512 / D) turn_some<T, D, 1>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n);
+    else turn_some<T, D, Batch>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n);
+}
 
-template <class T, int D>
-__global__ __launch_bounds__(kTurnThreads) void rope_kernel(pk_qk_rope_desc a, int rows, int wide_q, int wide_k) {
+// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms take 74.6 us, 3.9 TB/s, where a
+// large copy reaches 5.2: 2 passes' loads a wave, 8 waves a vector unit (4 passes, of which 5 fit, 82.5).  One row of 16 heads takes 3.0 us,
+// a launch and the sines.
+template <class T, int D, bool Halves>
+__global__ __launch_bounds__(kTurnThreads, !Halves ? 4 : D == 256 ? 5 : 8) void rope_kernel(pk_qk_rope_desc a, int rows, int wide_q, int wide_k) {
     using Raw = typename T::Raw;
     __shared__ TurnTable<D> s_table;
-    const Turn turn{a.inv_freq, a.pos, a.rot_dim, a.norm, a.interleaved, a.eps};
+    const Turn<Halves> turn{a.inv_freq, a.pos, a.rot_dim, a.norm, a.interleaved, a.eps};
     const int64_t row0 = (int64_t)blockIdx.x * rows;
     const int n = (int)min((int64_t)rows, a.n_rows - row0), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (a.rot_dim) {
@@ -133,10 +205,10 @@ __global__ __launch_bounds__(kTurnThreads) void rope_kernel(pk_qk_rope_desc a, i
     }
     for (int u = blockIdx.y * kTurnWaves + wave; u < a.heads + a.kv_heads; u += gridDim.y * kTurnWaves) {
         if (u < a.heads)
-            turn_rows<T, D>((const Raw *)a.q + u * a.q_head, a.q_row, wide_q & 1, (Raw *)a.q_out + u * a.q_out_head, a.q_out_row, wide_q & 2,
+            turn_rows<T, D, 2>((const Raw *)a.q + u * a.q_head, a.q_row, wide_q & 1, (Raw *)a.q_out + u * a.q_out_head, a.q_out_row, wide_q & 2,
                             a.q_weight, turn, s_table, row0, n);
         else
-            turn_rows<T, D>((const Raw *)a.k + (u - a.heads) * a.k_head, a.k_row, wide_k & 1, (Raw *)a.k_out + (u - a.heads) * a.k_out_head,
+            turn_rows<T, D, 2>((const Raw *)a.k + (u - a.heads) * a.k_head, a.k_row, wide_k & 1, (Raw *)a.k_out + (u - a.heads) * a.k_out_head,
                             a.k_out_row, wide_k & 2, a.k_weight, turn, s_table, row0, n);
     }
 }

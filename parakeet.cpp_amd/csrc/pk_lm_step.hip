@@ -45,10 +45,9 @@ int check_turn(const char *what, int dim, int rot, const float *inv_freq, const 
     return PK_OK;
 }
 
-// Whether 8 channels of any row are 16-byte aligned.
-bool wide_rows(const void *p, int64_t row, int64_t head, int size) {
-    const int per = 16 / size;
-    return aligned(p, 16) && row % per == 0 && head % per == 0;
+// Whether `each` channels of any row are aligned to their bytes.
+bool wide_rows(const void *p, int64_t row, int64_t head, int size, int each = 4) {
+    return aligned(p, each * size) && row % each == 0 && head % each == 0;
 }
 
 // Rows of a workgroup, workgroups beside it on the same rows.
@@ -56,13 +55,14 @@ struct TurnGrid {
     int rows, parts;
     int64_t groups;
 };
-// As many rows as leave 1,024 workgroups, then a head a wave as long as there are fewer.
-TurnGrid turn_grid(int n_rows, int units, int least) {
+// As many rows as leave 1,024 workgroups, whole blocks where there are many, then parts of the heads as long as that gives more than
+// 2,048 workgroups or a part for each.
+TurnGrid turn_grid(int n_rows, int parts, int least) {
     TurnGrid g;
     g.rows = (int)std::min<int64_t>(std::max<int64_t>(n_rows / 1024, least), kTurnRows);
+    if (g.rows > kTurnRows / 2) g.rows = kTurnRows;
     g.groups = ((int64_t)n_rows + g.rows - 1) / g.rows;
-    const int64_t most = (units + kTurnWaves - 1) / kTurnWaves;
-    g.parts = (int)std::min<int64_t>(std::max<int64_t>((1024 + g.groups - 1) / g.groups, 1), most);
+    g.parts = (int)std::min<int64_t>(std::max<int64_t>((2048 + g.groups - 1) / g.groups, 1), std::max(parts, 1));
     return g;
 }
 
@@ -187,13 +187,16 @@ PK_API int pk_qk_rope(const pk_qk_rope_desc *d, void *stream) {
     if ((d->heads && (!d->q || !d->q_out)) || (d->kv_heads && (!d->k || !d->k_out))) return pk_fail(PK_ERR_ARG, "%s: NULL rows", what);
     if (!aligned(d->q, size) || !aligned(d->k, size) || !aligned(d->q_out, size) || !aligned(d->k_out, size))
         return pk_fail(PK_ERR_ARG, "%s: rows not aligned to their type", what);
-    const TurnGrid g = turn_grid(d->n_rows, d->heads + d->kv_heads, 512 / d->head_dim);
+    const TurnGrid g = turn_grid(d->n_rows, (d->heads + d->kv_heads + kTurnWaves - 1) / kTurnWaves, 512 / d->head_dim);
     if (g.groups * g.parts > most_groups(kTurnThreads)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows in one call", what, d->n_rows);
     const int wide_q = wide_rows(d->q, d->q_row, d->q_head, size) | wide_rows(d->q_out, d->q_out_row, d->q_out_head, size) << 1;
     const int wide_k = wide_rows(d->k, d->k_row, d->k_head, size) | wide_rows(d->k_out, d->k_out_row, d->k_out_head, size) << 1;
+    const bool halves = d->rot_dim == d->head_dim && !d->interleaved && (wide_q == 3 || !d->heads) && (wide_k == 3 || !d->kv_heads);
     by_type(d->dtype, [&](auto t) {
         by_dim(d->head_dim, [&](auto dim) {
-            rope_kernel<decltype(t), dim.value><<<dim3((unsigned)g.groups, g.parts), kTurnThreads, 0, (hipStream_t)stream>>>(*d, g.rows, wide_q, wide_k);
+            const dim3 grid((unsigned)g.groups, g.parts);
+            if (halves) rope_kernel<decltype(t), dim.value, true><<<grid, kTurnThreads, 0, (hipStream_t)stream>>>(*d, g.rows, wide_q, wide_k);
+            else rope_kernel<decltype(t), dim.value, false><<<grid, kTurnThreads, 0, (hipStream_t)stream>>>(*d, g.rows, wide_q, wide_k);
         });
     });
     return launched(what);
@@ -213,14 +216,17 @@ PK_API int pk_kv8_append(const pk_kv8_append_desc *d, void *stream) {
     if (!d->k || !d->v || !d->slots || (d->heads && (!d->q || !d->q_out))) return pk_fail(PK_ERR_ARG, "%s: NULL rows or slots", what);
     if (!aligned(d->k, size) || !aligned(d->v, size) || !aligned(d->q, size) || !aligned(d->q_out, size) || !aligned(d->slots, 4))
         return pk_fail(PK_ERR_ARG, "%s: rows or slots not aligned to their type", what);
-    const TurnGrid g = turn_grid(d->n_rows, 2 * d->kv_heads + d->heads, 1);
+    const TurnGrid g = turn_grid(d->n_rows, std::max(2 * d->kv_heads, (d->heads + kTurnWaves - 1) / kTurnWaves), 1);
     if (g.groups * g.parts > most_groups(kTurnThreads)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows in one call", what, d->n_rows);
     const int wide_q = wide_rows(d->q, d->q_row, d->q_head, size) | wide_rows(d->q_out, d->q_out_row, d->q_out_head, size) << 1;
     const int wide_kv = wide_rows(d->k, d->k_row, d->k_head, size) && wide_rows(d->v, d->v_row, d->v_head, size);
+    const bool halves = d->rot_dim == d->head_dim && !d->interleaved && (wide_q == 3 || !d->heads) && wide_kv;
     by_type(d->dtype, [&](auto t) {
         by_dim(d->head_dim, [&](auto dim) {
-            append_kernel<decltype(t), dim.value><<<dim3((unsigned)g.groups, g.parts), kTurnThreads, 0, (hipStream_t)stream>>>(
-                *d, g.rows, log2i(d->page), wide_q, wide_kv);
+            const dim3 grid((unsigned)g.groups, g.parts);
+            const int shift = log2i(d->page);
+            if (halves) append_kernel<decltype(t), dim.value, true><<<grid, kTurnThreads, 0, (hipStream_t)stream>>>(*d, g.rows, shift, wide_q, wide_kv);
+            else append_kernel<decltype(t), dim.value, false><<<grid, kTurnThreads, 0, (hipStream_t)stream>>>(*d, g.rows, shift, wide_q, wide_kv);
         });
     });
     return launched(what);
@@ -243,7 +249,7 @@ PK_API int pk_kv8_load(const pk_kv4_rows_desc *d, void *stream) {
     const int64_t groups = ((int64_t)d->n_rows + each - 1) / each;
     if (groups * 2 * d->heads > most_groups(kRowThreads))
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows of %d channels in one call", what, d->n_rows, d->head_dim);
-    const int wide = wide_rows(d->k, d->k_row, d->k_head, size) && wide_rows(d->v, d->v_row, d->v_head, size);
+    const int wide = wide_rows(d->k, d->k_row, d->k_head, size, 16 / size) && wide_rows(d->v, d->v_row, d->v_head, size, 16 / size);
     by_type(d->dtype, [&](auto t) {
         by_dim(d->head_dim, [&](auto dim) {
             load8_kernel<decltype(t), dim.value><<<dim3((unsigned)groups, 2 * d->heads), kRowThreads, 0, (hipStream_t)stream>>>(*d, log2i(d->page), wide);
