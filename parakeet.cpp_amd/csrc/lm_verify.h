@@ -1,9 +1,9 @@
 // lm_verify.h -- drafted tokens against the target's probabilities (pk_verify).
 //
-// Weights are pk_sample's whole numbers, w = round(2^30 exp((x - max) / T)), so that their sums are exact in any order.  What is
-// compared and drawn from follows from them in single f64 steps, p = w (1 / sum w): the same wherever it is worked out.  A
-// refused draft's successor is drawn from max(p - q, 0) in steps of 2^-52, whole numbers again, whose sum is at most 2^52 and a
-// half step for each token.
+// Weights are whole numbers, w = round(2^30 exp((x - max) / T)), as pk_sample's but for the last bits of the exponential, so that
+// their sums are exact in any order.  What is compared and drawn from follows from them in single f64 steps, p = w (1 / sum w):
+// the same wherever it is worked out.  A refused draft's successor is drawn from max(p - q, 0) in steps of 2^-52, whole
+// numbers again, whose sum is at most 2^52 and a half step for each token.
 #pragma once
 
 #include "lm_common.h"
@@ -14,9 +14,9 @@ namespace pklm {
 
 constexpr int kNever = 0x7FFFFFFF;
 
-// One row's weights: the logits' largest, 1 / T, and where the largest alone counts its place.
+// One row's weights: the logits' largest, log2(e) / T, and where the largest alone counts its place.
 struct RowWeights {
-    RowRule rule;
+    float top, to_log2;
     bool greedy;
     int top_at;
     double inv_sum;
@@ -24,21 +24,50 @@ struct RowWeights {
     __device__ void settings(const float *temperature, int b) {
         const float t = temperature ? temperature[b] : 1.0f;
         greedy = !(t > 0);
-        rule.inv = greedy ? 1.0f : fminf(1.0f / t, 3e38f);
+        to_log2 = fminf(fmaxf(1.4426950408889634f / (greedy ? 1.0f : t), 1e-38f), 3e38f);
     }
+    __device__ void largest(float x) { top = x == -INFINITY ? 0.0f : x; }      // a row of -inf has no weight
+    // exp2 of one rounded product: off by 2^-23 and 2^-24 of the exponent, 2^-19 of itself where weights end.  (The library's expf takes
+    // half as long again: weights are what bounds long rows.)
     __device__ unsigned weight(float x, int i) const {
-        if (greedy) return i == top_at && x != -INFINITY ? 1u << 30 : 0u;
-        return rule.weight(x);
+        if (greedy) return i == top_at ? 1u << 30 : 0u;
+        const float d = x == top ? 0.0f : x - top;
+        return (unsigned)rintf(__builtin_amdgcn_exp2f(d * to_log2) * 1073741824.0f);
     }
     __device__ void total(u64 sum) { inv_sum = sum ? 1.0 / (double)sum : 0.0; }
     __device__ double share_of(unsigned w) const { return __dmul_rn((double)w, inv_sum); }
 };
 
+// 8 adjacent logits of a row, from i on, as they come from memory; rows need not be aligned.
+template <class T>
+struct Tokens8 {
+    typename T::Raw raw[8];
+
+    __device__ void load(const typename T::Raw *row, int i, int end) {
+        if (i + 8 <= end) {
+            __builtin_memcpy(raw, row + i, sizeof(raw));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) raw[e] = i < end ? row[min(i + e, end - 1)] : (typename T::Raw)0;
+        }
+    }
+    // -inf behind the row's end and for NaN
+    __device__ float get(int e, int i, int end) const {
+        const float x = T::get(raw[e]);
+        return x != x || i + e >= end ? -INFINITY : x;
+    }
+};
+__device__ inline int wave_min(int v) { return lane_value(wave_scan(v, kNever, [](int a, int b) { return min(a, b); }), 63); }
+
 __device__ inline double uniform(float u) {
     const u64 v = part31(u);
     return (double)(v > 0x7FFFFFFFull ? 0x7FFFFFFFull : v) * 0x1p-31;
 }
-__device__ inline u64 left_of(double p, double q) { return p > q ? (u64)(__dadd_rn(p, -q) * 0x1p52) : 0; }
+// In steps of 2^-52, cut to whole ones: at most 2^52, so that added to 2^52 they are the low bits.
+__device__ inline u64 left_of(double p, double q) {
+    const double d = __dadd_rn(p, -q);
+    return d > 0 ? __double_as_longlong(__dadd_rn(trunc(d * 0x1p52), 0x1p52)) - __double_as_longlong(0x1p52) : 0;
+}
 
 // Rows of a request: [begin, begin + n) of the call's.
 struct RequestRows {
@@ -66,15 +95,15 @@ struct alignas(16) RowVerdict {
     int unused;
 };
 
-// A request's rows on a workgroup each, tokens in registers as sample_row_kernel has them.  Every row that refuses its
-// draft draws its own token, whether or not an earlier row has refused; the request's last workgroup to arrive has the rows'
-// verdicts and writes them up to the first refusal.
-template <class T, int BS, int E, bool Draft>
+// A request's rows on a workgroup each, tokens in registers: wave w has tokens ((w n + g) 64 + lane) 8 + e of a row, g < n <= G.  Every
+// row that refuses its draft draws its own token, whether or not an earlier row has refused; the request's last workgroup to
+// arrive has the rows' verdicts and writes them up to the first refusal.
+template <class T, int BS, int G, bool Draft>
 __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *arrived, RowVerdict *verdicts) {
-    constexpr int kWaves = BS / 64;
+    constexpr int kWaves = BS / 64, E = 8 * G, kSources = Draft ? 2 : 1;
     __shared__ float s_max[2][kWaves];
     __shared__ int s_at[2][kWaves];
-    __shared__ u64 s_sum[2][kWaves];
+    __shared__ u64 s_sum[2][kWaves], s_left[kWaves];
     __shared__ RowVerdict s_verdict;
     __shared__ int s_flag;
     using Raw = typename T::Raw;
@@ -84,30 +113,31 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
     if (rows.n == 0 && j == 0 && tid == 0) verify_counts(a, b, 0, 0);
     if (j >= rows.n) return;
     const int r = rows.begin + j, d = rows.draft(a, j);
-    constexpr int kSources = Draft ? 2 : 1;
     const bool drafted = d >= 0;
-    const int n = (V + BS - 1) / BS, base = wave * n * 64 + lane, end = min((wave + 1) * n * 64, V);
+    const int n = (V + 8 * BS - 1) / (8 * BS);
+    auto index = [&](int g) { return ((wave * n + g) * 64 + lane) * 8; };
     const Raw *row[2] = {(const Raw *)a.logits + (int64_t)r * a.logits_row, Draft ? (const Raw *)a.draft + (int64_t)r * a.draft_row : nullptr};
-    float x[kSources][E], at_draft[2];
+    Tokens8<T> raw[kSources][G];
+    float at_draft[2];
     RowWeights rw[2];
-    rw[0].settings(a.temperature, b);
-    if (Draft) rw[1].settings(a.draft_temperature, b);
 #pragma unroll
     for (int q = 0; q < kSources; ++q) {
-        const bool on = q == 0 || drafted;      // without a draft its row is not read
+        const int end = q == 0 || drafted ? V : 0;      // without a draft its row is not read
+#pragma unroll
+        for (int g = 0; g < G; ++g) raw[q][g].load(row[q], g < n ? index(g) : end, end);
+        at_draft[q] = drafted ? logit<T>(row[q], d) : -INFINITY;
+        rw[q].settings(q ? a.draft_temperature : a.temperature, b);
+    }
+    float x[kSources][E];
+#pragma unroll
+    for (int q = 0; q < kSources; ++q) {
+        const int end = q == 0 || drafted ? V : 0;
+        float top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int i = base + e * 64;
-            x[q][e] = on && i < end ? logit<T>(row[q], i) : -INFINITY;
+            x[q][e] = raw[q][e / 8].get(e % 8, e / 8 < n ? index(e / 8) : end, end);
+            top = fmaxf(top, x[q][e]);
         }
-        at_draft[q] = drafted ? logit<T>(row[q], d) : -INFINITY;
-    }
-    // the largest, and its first place
-#pragma unroll
-    for (int q = 0; q < kSources; ++q) {
-        float top = x[q][0];
-#pragma unroll
-        for (int e = 1; e < E; ++e) top = fmaxf(top, x[q][e]);
         top = wave_max(top);
         if (lane == 0) s_max[q][wave] = top;
     }
@@ -117,28 +147,38 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         float top = s_max[q][0];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_max[q][w]);
-        rw[q].rule.top = top;
-        int at = kNever;
-        if (rw[q].greedy)
-#pragma unroll
-            for (int e = 0; e < E; ++e) at = min(at, x[q][e] == top ? base + e * 64 : kNever);
-        at = lane_value(wave_scan(at, kNever, [](int u, int v) { return min(u, v); }), 63);
-        if (lane == 0) s_at[q][wave] = at;
+        rw[q].largest(top), rw[q].top_at = kNever;
     }
-    __syncthreads();
+    if (rw[0].greedy || (Draft && rw[1].greedy)) {       // the first place of the largest
+#pragma unroll
+        for (int q = 0; q < kSources; ++q) {
+            int at = kNever;
+#pragma unroll
+            for (int e = E - 1; e >= 0; --e) at = x[q][e] == rw[q].top ? index(e / 8) + e % 8 : at;
+            at = wave_min(at);
+            if (lane == 0) s_at[q][wave] = at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < kSources; ++q)
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) rw[q].top_at = min(rw[q].top_at, s_at[q][v]);
+    }
     unsigned w[kSources][E];
 #pragma unroll
     for (int q = 0; q < kSources; ++q) {
-        int at = s_at[q][0];
-#pragma unroll
-        for (int v = 1; v < kWaves; ++v) at = min(at, s_at[q][v]);
-        rw[q].top_at = at;
         u64 sum = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            w[q][e] = rw[q].weight(x[q][e], base + e * 64);
-            sum += w[q][e];
-        }
+        for (int g = 0; g < G; ++g)
+            if (g < n)
+#pragma unroll
+                for (int e = 8 * g; e < 8 * g + 8; ++e) {
+                    w[q][e] = rw[q].weight(x[q][e], index(g) + e % 8);
+                    sum += w[q][e];
+                }
+            else
+#pragma unroll
+                for (int e = 8 * g; e < 8 * g + 8; ++e) w[q][e] = 0;
         sum = wave_sum(sum);
         if (lane == 0) s_sum[q][wave] = sum;
     }
@@ -161,18 +201,17 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             left[e] = w[0][e];
-            if (drafted) left[e] = Draft ? left_of(rw[0].share_of(w[0][e]), rw[1].share_of(w[kSources - 1][e])) : base + e * 64 == d ? 0 : left[e];
+            if (drafted) left[e] = Draft ? left_of(rw[0].share_of(w[0][e]), rw[1].share_of(w[kSources - 1][e])) : index(e / 8) + e % 8 == d ? 0 : left[e];
             mass += left[e];
         }
         mass = wave_sum(mass);
-        __syncthreads();                         // s_sum may still be read
-        if (lane == 0) s_sum[1][wave] = mass;
+        if (lane == 0) s_left[wave] = mass;
         __syncthreads();
         u64 all = 0, lead = 0;
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) {
-            if (v < wave) lead += s_sum[1][v];
-            all += s_sum[1][v];
+            if (v < wave) lead += s_left[v];
+            all += s_left[v];
         }
         if (all == 0) {                          // nothing: from the target itself
 #pragma unroll
@@ -185,16 +224,31 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         const u64 u = part31(a.u_draw[b]), t = share(all, u > 0x7FFFFFFFull ? 0x7FFFFFFFull : u);
         if (lead <= t && t < lead + mass)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const u64 run = wave_scan(left[e]), sum = lane_value(run, 63);
-                if (lead <= t && t < lead + sum) {
-                    const u64 hit = __ballot(lead + run > t);
-                    if (lane == __ffsll(hit) - 1) s_verdict = RowVerdict{0, base + e * 64, (float)rw[0].share_of(w[0][e]), 0};
-                }
-                lead += sum;
+            for (int g = 0; g < G; ++g) {
+                u64 own = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) own += left[8 * g + e];
+                const u64 run = wave_scan(own);
+                u64 at = lead + run - own;
+                if (at <= t && t < at + own)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (at <= t && t < at + left[8 * g + e])
+                            s_verdict = RowVerdict{0, index(g) + e, (float)rw[0].share_of(w[0][8 * g + e]), 0};
+                        at += left[8 * g + e];
+                    }
+                lead += lane_value(run, 63);
             }
     }
     __syncthreads();
+    auto write = [&](int at, const RowVerdict &v, bool kept) {
+        a.out[rows.begin + at] = kept ? v.token : -1;
+        if (a.prob) a.prob[rows.begin + at] = kept ? v.prob : 0.0f;
+    };
+    if (rows.n == 1) {
+        if (tid == 0) write(0, s_verdict, true), verify_counts(a, b, 1, 0);
+        return;
+    }
     RowVerdict *mine = verdicts + (int64_t)b * a.max_new;
     if (tid == 0) store_shared4((unsigned *)(mine + j), 0, __builtin_bit_cast(u4, s_verdict));
     if (!last_to_arrive(&arrived[b], rows.n, &s_flag) || wave != 0) return;
@@ -204,11 +258,7 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         if (j0 + lane < rows.n) v = __builtin_bit_cast(RowVerdict, load_shared4((const unsigned *)(mine + j0), 4 * lane));
         const u64 refused = __ballot(!v.ok);
         if (stop == kNever && refused) stop = j0 + __ffsll(refused) - 1;
-        if (j0 + lane < rows.n) {
-            const bool kept = j0 + lane <= stop;
-            a.out[rows.begin + j0 + lane] = kept ? v.token : -1;
-            if (a.prob) a.prob[rows.begin + j0 + lane] = kept ? v.prob : 0.0f;
-        }
+        if (j0 + lane < rows.n) write(j0 + lane, v, j0 + lane <= stop);
     }
     if (lane == 0) verify_counts(a, b, rows.n, stop);
 }
@@ -219,23 +269,26 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
 // that refuses its draft alone, what each chunk has left to draw from, of which the request's last chunk to arrive draws.
 // A launch's workgroups work out for themselves what follows from the launch before.
 
+constexpr int kVerifyThreads = 512, kVerifyWaves = kVerifyThreads / 64, kVerifyPass = 8 * kVerifyThreads;
+
 struct SplitVerify {
     float *chunk_max;       // [rows][2][chunks], of the target and of the draft
-    int *chunk_at;          // likewise
+    int *chunk_at;          // likewise; where the largest alone counts
     u64 *chunk_sum;         // likewise
     u64 *left;              // [requests][chunks]
     int *arrived;           // [requests], zero between calls
-    int chunks, per, sources;
+    int chunks, passes, sources;        // a chunk is passes * kVerifyPass tokens, a wave's part of it in one run
+    int draw_chunks, draw_passes;       // likewise, of the one row of a request that is drawn from
 };
 
-// A workgroup's chunk of a row: (request, row of it, source) and the tokens [i0, i1).
+// A workgroup's chunk of a row: (request, row of it, source).
 struct VerifyChunk {
     int b, j, q, chunk;
     __device__ VerifyChunk(const pk_verify_desc &a, const SplitVerify &w) {
-        int64_t id = blockIdx.x;
-        chunk = (int)(id % w.chunks), id /= w.chunks;
-        q = (int)(id % w.sources), id /= w.sources;
-        j = (int)(id % a.max_new), b = (int)(id / a.max_new);
+        unsigned id = blockIdx.x;
+        chunk = id % w.chunks, id /= w.chunks;
+        q = id % w.sources, id /= w.sources;
+        j = id % a.max_new, b = id / a.max_new;
     }
 };
 
@@ -244,45 +297,62 @@ __device__ inline const typename T::Raw *verify_row(const pk_verify_desc &a, int
     using Raw = typename T::Raw;
     return q ? (const Raw *)a.draft + (int64_t)r * a.draft_row : (const Raw *)a.logits + (int64_t)r * a.logits_row;
 }
+// The first token of this lane in a pass of a chunk.
+__device__ inline int verify_token(int passes, int chunk, int pass) {
+    return ((chunk * kVerifyWaves + (int)(threadIdx.x >> 6)) * passes + pass) * 512 + (int)(threadIdx.x & 63) * 8;
+}
 
-// The weights' rule of a row, from its chunks' maxima.
-__device__ inline void row_rule(const pk_verify_desc &a, const SplitVerify &w, int b, int64_t place, int q, RowWeights &rw) {
+// A row's rule, from its chunks' maxima, and its weight where the chunks have theirs: by a whole wave.
+__device__ inline u64 row_rule(const pk_verify_desc &a, const SplitVerify &w, int b, int64_t place, int q, RowWeights &rw, bool summed) {
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (place * 2 + q) * w.chunks + lane;
     rw.settings(q ? a.draft_temperature : a.temperature, b);
-    const float *m = w.chunk_max + (place * 2 + q) * w.chunks;
-    const int *at = w.chunk_at + (place * 2 + q) * w.chunks;
-    float top = m[0];
-    int top_at = at[0];
-    for (int c = 1; c < w.chunks; ++c)
-        if (m[c] > top) top = m[c], top_at = at[c];
-    rw.rule.top = top, rw.top_at = top_at;
+    const bool in = lane < w.chunks;
+    const float m = in ? w.chunk_max[at] : -INFINITY;
+    const u64 sum = summed && in ? w.chunk_sum[at] : 0;
+    const int p = rw.greedy && in ? w.chunk_at[at] : kNever;
+    rw.largest(wave_max(m));
+    rw.top_at = rw.greedy ? wave_min(m == rw.top ? p : kNever) : kNever;
+    const u64 total = summed ? wave_sum(sum) : 0;
+    rw.total(total);
+    return total;
 }
 
 template <class T>
-__global__ __launch_bounds__(kSplitThreads) void verify_max_kernel(pk_verify_desc a, SplitVerify w) {
-    __shared__ float s_max[kRuns];
-    __shared__ int s_at[kRuns];
+__global__ __launch_bounds__(kVerifyThreads) void verify_max_kernel(pk_verify_desc a, SplitVerify w) {
+    __shared__ float s_max[kVerifyWaves];
+    __shared__ int s_at[kVerifyWaves];
     const VerifyChunk c(a, w);
     const RequestRows rows(a, c.b);
     if (c.j >= rows.n || (c.q && rows.draft(a, c.j) < 0)) return;
     const auto *row = verify_row<T>(a, c.q, rows.begin + c.j);
-    const int tid = threadIdx.x, size = w.per * kSplitThreads, i0 = c.chunk * size, i1 = min(i0 + size, a.vocab);
+    const int tid = threadIdx.x, V = a.vocab;
+    RowWeights rw;
+    rw.settings(c.q ? a.draft_temperature : a.temperature, c.b);
     float top = -INFINITY;
     int at = kNever;
-    for (int i = i0 + tid; i < i1; i += kBatch * kSplitThreads) {
-        float x[kBatch];
-        load_batch<T>(row, i, kSplitThreads, i1, x);
+    for (int p0 = 0; p0 < w.passes; p0 += 2) {
+        Tokens8<T> x[2];
+        int i[2];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-            if (x[e] > top) top = x[e], at = i + e * kSplitThreads;
+        for (int p = 0; p < 2; ++p) i[p] = p0 + p < w.passes ? verify_token(w.passes, c.chunk, p0 + p) : V, x[p].load(row, i[p], V);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = x[p].get(e, i[p], V);
+                if (rw.greedy && v > top) at = i[p] + e;
+                top = fmaxf(top, v);
+            }
     }
     const float wave_top = wave_max(top);
-    at = lane_value(wave_scan(top == wave_top ? at : kNever, kNever, [](int u, int v) { return min(u, v); }), 63);
+    at = rw.greedy ? wave_min(top == wave_top ? at : kNever) : kNever;
     if ((tid & 63) == 0) s_max[tid >> 6] = wave_top, s_at[tid >> 6] = at;
     __syncthreads();
     if (tid == 0) {
         float m = s_max[0];
         int p = s_at[0];
-        for (int v = 1; v < kRuns; ++v)
+        for (int v = 1; v < kVerifyWaves; ++v)
             if (s_max[v] > m || (s_max[v] == m && s_at[v] < p)) m = s_max[v], p = s_at[v];
         const int64_t place = (((int64_t)c.b * a.max_new + c.j) * 2 + c.q) * w.chunks + c.chunk;
         w.chunk_max[place] = m, w.chunk_at[place] = p;
@@ -290,141 +360,130 @@ __global__ __launch_bounds__(kSplitThreads) void verify_max_kernel(pk_verify_des
 }
 
 template <class T>
-__global__ __launch_bounds__(kSplitThreads) void verify_sum_kernel(pk_verify_desc a, SplitVerify w) {
-    __shared__ u64 s_sum[kRuns];
+__global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(pk_verify_desc a, SplitVerify w) {
+    __shared__ u64 s_sum[kVerifyWaves];
     const VerifyChunk c(a, w);
     const RequestRows rows(a, c.b);
     if (c.j >= rows.n || (c.q && rows.draft(a, c.j) < 0)) return;
     const auto *row = verify_row<T>(a, c.q, rows.begin + c.j);
-    const int tid = threadIdx.x, size = w.per * kSplitThreads, i0 = c.chunk * size, i1 = min(i0 + size, a.vocab);
+    const int tid = threadIdx.x, V = a.vocab;
     const int64_t place = (int64_t)c.b * a.max_new + c.j;
-    float x[kBatch];
-    load_batch<T>(row, i0 + tid, kSplitThreads, i1, x);       // on its way while the rule is worked out
+    Tokens8<T> x;
+    x.load(row, verify_token(w.passes, c.chunk, 0), V);       // on its way while the rule is worked out
     RowWeights rw;
-    row_rule(a, w, c.b, place, c.q, rw);
+    row_rule(a, w, c.b, place, c.q, rw, false);
     u64 sum = 0;
-    for (int i = i0 + tid;;) {
+    for (int p = 0; p < w.passes; ++p) {
+        const int i = verify_token(w.passes, c.chunk, p);
+        Tokens8<T> y;
+        y.load(row, p + 1 < w.passes ? verify_token(w.passes, c.chunk, p + 1) : V, V);
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) sum += rw.weight(x[e], i + e * kSplitThreads);
-        i += kBatch * kSplitThreads;
-        if (i - tid >= i1) break;
-        load_batch<T>(row, i, kSplitThreads, i1, x);
+        for (int e = 0; e < 8; e += 2) sum += rw.weight(x.get(e, i, V), i + e) + rw.weight(x.get(e + 1, i, V), i + e + 1);
+        x = y;
     }
     sum = wave_sum(sum);
     if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
     __syncthreads();
     if (tid < 64) {
-        sum = wave_sum(tid < kRuns ? s_sum[tid] : 0);
+        sum = wave_sum(tid < kVerifyWaves ? s_sum[tid] : 0);
         if (tid == 0) w.chunk_sum[(place * 2 + c.q) * w.chunks + c.chunk] = sum;
     }
 }
 
 template <class T>
-__global__ __launch_bounds__(kSplitThreads) void verify_draw_kernel(pk_verify_desc a, SplitVerify w) {
-    __shared__ u64 s_sum[kRuns], s_base;
-    __shared__ int s_stop, s_flag, s_chunk;
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_desc a, SplitVerify w) {
+    __shared__ u64 s_sum[kVerifyWaves], s_base;
+    __shared__ int s_stop[2], s_flag, s_chunk;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab;
-    const int b = blockIdx.x / w.chunks, chunk = blockIdx.x % w.chunks;
+    const int b = blockIdx.x / w.draw_chunks, chunk = blockIdx.x % w.draw_chunks;
     const RequestRows rows(a, b);
     if (rows.n == 0) {
         if (chunk == 0 && tid == 0) verify_counts(a, b, 0, 0);
         return;
     }
-    // a row's rules with their sums; by a whole wave
-    auto rules = [&](int j, int d, RowWeights (&rw)[2]) {
+    const bool two_sources = w.sources > 1;
+    RowWeights target, draft;
+    // p and q of a row's draft; by a whole wave
+    auto shares = [&](int j, int d, double &q) {
+        const float x = logit<T>(verify_row<T>(a, 0, rows.begin + j), d), y = two_sources ? logit<T>(verify_row<T>(a, 1, rows.begin + j), d) : 0.0f;
         const int64_t place = (int64_t)b * a.max_new + j;
-        u64 sum = 0;
-        for (int q = 0; q < (d >= 0 ? w.sources : 1); ++q) {
-            row_rule(a, w, b, place, q, rw[q]);
-            const u64 s = wave_sum(lane < w.chunks ? w.chunk_sum[(place * 2 + q) * w.chunks + lane] : 0);
-            rw[q].total(s);
-            if (q == 0) sum = s;
+        row_rule(a, w, b, place, 0, target, true);
+        q = 1.0;
+        if (two_sources) {
+            row_rule(a, w, b, place, 1, draft, true);
+            q = draft.share_of(draft.weight(y, d));
         }
-        return sum;
+        return target.share_of(target.weight(x, d));
     };
-    auto draft_share = [&](int j, int d, const RowWeights (&rw)[2], double &q) {
-        q = w.sources > 1 ? rw[1].share_of(rw[1].weight(logit<T>(verify_row<T>(a, 1, rows.begin + j), d), d)) : 1.0;
-        return rw[0].share_of(rw[0].weight(logit<T>(verify_row<T>(a, 0, rows.begin + j), d), d));
-    };
-    // the first row that refuses its draft, a row a wave
-    if (tid == 0) s_stop = kNever;
+    // The first row that refuses its draft, a row a wave; those in front of it stay.  Rounds of rows have two places in turn, since a
+    // wave may look at a round's after another has begun the next.
+    if (tid < 2) s_stop[tid] = kNever;
     __syncthreads();
-    for (int j0 = 0;; j0 += kRuns) {
-        const int j = j0 + wave;
-        if (j < rows.n) {
-            const int d = rows.draft(a, j);
-            bool ok = false;
-            if (d >= 0) {
-                RowWeights rw[2];
-                rules(j, d, rw);
-                double q;
-                const double p = draft_share(j, d, rw, q);
-                ok = __dmul_rn(uniform(a.u[rows.begin + j]), q) < p;
-            }
-            if (!ok && lane == 0) atomicMin(&s_stop, j);
-        }
+    int stop = kNever;
+    for (int j0 = 0, round = 0; stop == kNever; j0 += kVerifyWaves, round ^= 1) {      // ends: the last row has no draft
+        const int j = j0 + wave, d = j < rows.n ? rows.draft(a, j) : -1;
+        double p = 0, q = 1;
+        if (d >= 0) p = shares(j, d, q);
+        const bool ok = d >= 0 && __dmul_rn(uniform(a.u[rows.begin + j]), q) < p;
+        if (!ok && lane == 0 && j < rows.n) atomicMin(&s_stop[round], j);
         __syncthreads();
-        if (s_stop != kNever) break;             // the last row has no draft
+        stop = s_stop[round];
+        if (chunk == 0 && lane == 0 && j < min(rows.n, stop)) {
+            a.out[rows.begin + j] = d;
+            if (a.prob) a.prob[rows.begin + j] = (float)p;
+        }
     }
-    const int stop = s_stop;
     if (chunk == 0) {
-        for (int j = wave; j < rows.n; j += kRuns) {
-            if (j == stop) continue;
-            int token = -1;
-            float prob = 0;
-            if (j < stop) {
-                token = rows.draft(a, j);
-                RowWeights rw[2];
-                rules(j, token, rw);
-                double q;
-                prob = (float)draft_share(j, token, rw, q);
-            }
-            if (lane == 0) {
-                a.out[rows.begin + j] = token;
-                if (a.prob) a.prob[rows.begin + j] = prob;
-            }
+        for (int j = stop + 1 + tid; j < rows.n; j += kVerifyThreads) {
+            a.out[rows.begin + j] = -1;
+            if (a.prob) a.prob[rows.begin + j] = 0.0f;
         }
         if (tid == 0) verify_counts(a, b, rows.n, stop);
     }
     const int d = rows.draft(a, stop), r = rows.begin + stop;
-    RowWeights rw[2];
-    const u64 total = rules(stop, d, rw);
-    const bool drafted = d >= 0, two = drafted && w.sources > 1;
+    const int64_t place = (int64_t)b * a.max_new + stop;
+    const bool drafted = d >= 0, two = drafted && two_sources;
     const auto *x_row = verify_row<T>(a, 0, r), *y_row = two ? verify_row<T>(a, 1, r) : x_row;
-    auto left = [&](int i, bool any) -> u64 {
-        if (i >= V) return 0;
-        const unsigned wt = rw[0].weight(logit<T>(x_row, i), i);
-        if (any || !drafted) return wt;
-        if (!two) return i == d ? 0 : wt;
-        return left_of(rw[0].share_of(wt), rw[1].share_of(rw[1].weight(logit<T>(y_row, i), i)));
+    const u64 total = row_rule(a, w, b, place, 0, target, true);
+    if (two) row_rule(a, w, b, place, 1, draft, true);
+    // what is left of a lane's 8 tokens of a pass
+    auto left_of_pass = [&](int ch, int pass, bool any, u64 (&left)[8]) {
+        const int i = verify_token(w.draw_passes, ch, pass);
+        Tokens8<T> x, y;
+        x.load(x_row, i, V);
+        if (two && !any) y.load(y_row, i, V);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned wt = target.weight(x.get(e, i, V), i + e);
+            left[e] = wt;
+            if (!any && drafted) left[e] = two ? left_of(target.share_of(wt), draft.share_of(draft.weight(y.get(e, i, V), i + e))) : i + e == d ? 0 : left[e];
+        }
     };
-    // a chunk is kRuns runs of 64 per tokens, a wave each
     auto run_sum = [&](int ch, bool any) {
         u64 mass = 0;
-        const int i0 = (ch * kRuns + wave) * 64 * w.per + lane;
-#pragma unroll 4
-        for (int e = 0; e < w.per; ++e) mass += left(i0 + e * 64, any);
+        for (int p = 0; p < w.draw_passes; ++p) {
+            u64 left[8];
+            left_of_pass(ch, p, any, left);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mass += left[e];
+        }
         return wave_sum(mass);
-    };
-    auto chunk_total = [&]() {
-        u64 s = 0;
-        for (int v = 0; v < kRuns; ++v) s += s_sum[v];
-        return s;
     };
     {
         const u64 mass = run_sum(chunk, false);
         if (lane == 0) s_sum[wave] = mass;
         __syncthreads();
-        if (tid == 0) put_shared(&w.left[(int64_t)b * w.chunks + chunk], chunk_total());
+        if (tid == 0) {
+            u64 s = 0;
+            for (int v = 0; v < kVerifyWaves; ++v) s += s_sum[v];
+            put_shared(&w.left[(int64_t)b * w.draw_chunks + chunk], s);
+        }
     }
-    if (!last_to_arrive(&w.arrived[b], w.chunks, &s_flag)) return;
-    const u64 of_chunk = lane < w.chunks ? get_shared(&w.left[(int64_t)b * w.chunks + lane]) : 0;
-    u64 all = wave_sum(of_chunk), mine = of_chunk;
+    if (!last_to_arrive(&w.arrived[b], w.draw_chunks, &s_flag)) return;
+    const u64 mine = lane < w.draw_chunks ? get_shared(&w.left[(int64_t)b * w.draw_chunks + lane]) : 0;
+    u64 all = wave_sum(mine);
     const bool any = all == 0;                   // nothing: from the target itself
-    if (any) {
-        all = total;
-        mine = lane < w.chunks ? w.chunk_sum[((int64_t)b * a.max_new + stop) * 2 * w.chunks + lane] : 0;
-    }
+    if (any) all = total;
     if (all == 0) {
         if (tid == 0) {
             a.out[r] = -1;
@@ -433,29 +492,43 @@ __global__ __launch_bounds__(kSplitThreads) void verify_draw_kernel(pk_verify_de
         return;
     }
     const u64 u = part31(a.u_draw[b]), t = share(all, u > 0x7FFFFFFFull ? 0x7FFFFFFFull : u);
-    if (wave == 0) {
+    // the chunk in which the drawn weight falls: from the chunks' sums, or (seldom) chunk by chunk
+    if (wave == 0 && !any) {
         const u64 before = wave_scan(mine) - mine;
         if (before <= t && t < before + mine) s_chunk = lane, s_base = before;
     }
     __syncthreads();
-    const int ch = s_chunk;
-    const u64 mass = run_sum(ch, any);
-    if (lane == 0) s_sum[wave] = mass;
-    __syncthreads();
-    u64 lead = s_base;
+    int ch = any ? 0 : s_chunk;
+    u64 lead = any ? 0 : s_base, mass = 0;
+    for (;; ++ch) {                              // ends: t is below the sum over all chunks
+        mass = run_sum(ch, any);
+        if (lane == 0) s_sum[wave] = mass;
+        __syncthreads();
+        u64 of_chunk = 0;
+        for (int v = 0; v < kVerifyWaves; ++v) of_chunk += s_sum[v];
+        if (t < lead + of_chunk || ch + 1 >= w.draw_chunks) break;
+        lead += of_chunk;
+        __syncthreads();
+    }
     for (int v = 0; v < wave; ++v) lead += s_sum[v];
     if (lead > t || lead + mass <= t) return;
-    const int i0 = (ch * kRuns + wave) * 64 * w.per + lane;
-    for (int e = 0; e < w.per; ++e) {
-        const int i = i0 + e * 64;
-        const u64 run = wave_scan(left(i, any)), sum = lane_value(run, 63);
-        if (lead <= t && t < lead + sum) {
-            const u64 hit = __ballot(lead + run > t);
-            if (lane == __ffsll(hit) - 1) {
-                a.out[r] = i;
-                if (a.prob) a.prob[r] = (float)rw[0].share_of(rw[0].weight(logit<T>(x_row, i), i));
+    for (int p = 0; p < w.draw_passes; ++p) {
+        u64 left[8], own = 0;
+        left_of_pass(ch, p, any, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own += left[e];
+        const u64 run = wave_scan(own), sum = lane_value(run, 63);
+        u64 at = lead + run - own;
+        if (at <= t && t < at + own) {
+            const int i0 = verify_token(w.draw_passes, ch, p);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (at <= t && t < at + left[e]) {
+                    a.out[r] = i0 + e;
+                    if (a.prob) a.prob[r] = (float)target.share_of(target.weight(logit<T>(x_row, i0 + e), i0 + e));
+                }
+                at += left[e];
             }
-            break;
         }
         lead += sum;
     }

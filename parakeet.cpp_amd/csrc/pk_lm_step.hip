@@ -101,7 +101,7 @@ void launch_attend8(const AttendParams &p, bool prompt, int dim, unsigned grid, 
 constexpr int kVerifyVocab = 16384;
 
 struct VerifyShape {
-    int per, chunks;             // tokens a thread takes of a chunk, chunks of a row
+    int passes, chunks, draw_passes, draw_chunks;        // see SplitVerify
     // counters first, the same place for every shape: they are zero between calls
     static constexpr int64_t kCounterBytes = PK_LM_MAX_REQUESTS * 4;
     int64_t max_at, at_at, sum_at, left_at, bytes;
@@ -114,9 +114,14 @@ VerifyShape verify_shape(const pk_verify_desc &d) {
         s.bytes = VerifyShape::kCounterBytes + rows * (int64_t)sizeof(RowVerdict);
         return s;
     }
-    const int aim = (int)std::min<int64_t>(std::max<int64_t>(512 / std::max<int64_t>(rows, 1), 2), 16);
-    s.per = std::min(std::max((d.vocab + aim * kSplitThreads - 1) / (aim * kSplitThreads), 4), kMaxChunks);
-    s.chunks = (d.vocab + s.per * kSplitThreads - 1) / (s.per * kSplitThreads);
+    // As many chunks as make 4,096 workgroups, 64 of a row at most (a lane has one each), of two passes at least.
+    auto cut = [&](int64_t each, int &chunks, int &passes) {
+        const int64_t aim = std::min<int64_t>(std::max<int64_t>(4096 / std::max<int64_t>(each, 1), 1), 64);
+        passes = (int)std::max<int64_t>(2, (d.vocab + aim * kVerifyPass - 1) / (aim * kVerifyPass));
+        chunks = (d.vocab + passes * kVerifyPass - 1) / (passes * kVerifyPass);
+    };
+    cut(rows * (d.draft ? 2 : 1), s.chunks, s.passes);
+    cut(d.requests, s.draw_chunks, s.draw_passes);
     int64_t at = VerifyShape::kCounterBytes;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -124,11 +129,10 @@ VerifyShape verify_shape(const pk_verify_desc &d) {
         return here;
     };
     s.max_at = take(rows * 2 * s.chunks * 4), s.at_at = take(rows * 2 * s.chunks * 4), s.sum_at = take(rows * 2 * s.chunks * 8);
-    s.left_at = take((int64_t)d.requests * s.chunks * 8);
+    s.left_at = take((int64_t)d.requests * s.draw_chunks * 8);
     s.bytes = at;
     return s;
 }
-static_assert(PK_LM_MAX_VOCAB <= 64 * kMaxChunks * kSplitThreads, "a chunk a lane");
 
 int verify_check(const char *what, const pk_verify_desc *d) {
     if (!d) return pk_fail(PK_ERR_ARG, "%s: no descriptor", what);
@@ -136,36 +140,36 @@ int verify_check(const char *what, const pk_verify_desc *d) {
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests (at most %d)", what, d->requests, PK_LM_MAX_REQUESTS);
     if (d->n_rows < 0 || d->max_new < 0 || d->vocab <= 0 || d->vocab > PK_LM_MAX_VOCAB)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows, max_new %d, %d logits (1 .. %d)", what, d->n_rows, d->max_new, d->vocab, PK_LM_MAX_VOCAB);
-    // with 16 chunks a row at most of two sources
-    if ((int64_t)d->requests * d->max_new > most_groups(kSplitThreads) / 128)
+    // with 64 chunks a row at most of two sources
+    if ((int64_t)d->requests * d->max_new > most_groups(kVerifyThreads) / 128)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests of up to %d rows in one call", what, d->requests, d->max_new);
     return PK_OK;
 }
 
-template <class T, int BS, int E>
+template <class T, int BS, int G>
 void launch_verify_rows(const pk_verify_desc &d, hipStream_t s) {
     int *arrived = (int *)d.workspace;
     auto *verdicts = (RowVerdict *)((char *)d.workspace + VerifyShape::kCounterBytes);
     const unsigned grid = (unsigned)(d.requests * d.max_new);
-    if (d.draft) verify_row_kernel<T, BS, E, true><<<grid, BS, 0, s>>>(d, arrived, verdicts);
-    else verify_row_kernel<T, BS, E, false><<<grid, BS, 0, s>>>(d, arrived, verdicts);
+    if (d.draft) verify_row_kernel<T, BS, G, true><<<grid, BS, 0, s>>>(d, arrived, verdicts);
+    else verify_row_kernel<T, BS, G, false><<<grid, BS, 0, s>>>(d, arrived, verdicts);
 }
 
 template <class T>
 void launch_verify(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s) {
-    if (d.vocab <= 1024) return launch_verify_rows<T, 256, 4>(d, s);
-    if (d.vocab <= 2048) return launch_verify_rows<T, 256, 8>(d, s);
-    if (d.vocab <= 4096) return launch_verify_rows<T, 1024, 4>(d, s);
-    if (d.vocab <= kVerifyVocab) return launch_verify_rows<T, 1024, 16>(d, s);
+    if (d.vocab <= 2048) return launch_verify_rows<T, 256, 1>(d, s);
+    if (d.vocab <= 8192) return launch_verify_rows<T, 1024, 1>(d, s);
+    if (d.vocab <= kVerifyVocab) return launch_verify_rows<T, 1024, 2>(d, s);
     char *w = (char *)d.workspace;
     SplitVerify p;
     p.arrived = (int *)w, p.chunk_max = (float *)(w + sh.max_at), p.chunk_at = (int *)(w + sh.at_at), p.chunk_sum = (u64 *)(w + sh.sum_at);
     p.left = (u64 *)(w + sh.left_at);
-    p.chunks = sh.chunks, p.per = sh.per, p.sources = d.draft ? 2 : 1;
+    p.chunks = sh.chunks, p.passes = sh.passes, p.sources = d.draft ? 2 : 1;
+    p.draw_chunks = sh.draw_chunks, p.draw_passes = sh.draw_passes;
     const unsigned grid = (unsigned)(d.requests * d.max_new * p.sources * p.chunks);
-    verify_max_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
-    verify_sum_kernel<T><<<grid, kSplitThreads, 0, s>>>(d, p);
-    verify_draw_kernel<T><<<(unsigned)(d.requests * p.chunks), kSplitThreads, 0, s>>>(d, p);
+    verify_max_kernel<T><<<grid, kVerifyThreads, 0, s>>>(d, p);
+    verify_sum_kernel<T><<<grid, kVerifyThreads, 0, s>>>(d, p);
+    verify_draw_kernel<T><<<(unsigned)(d.requests * p.draw_chunks), kVerifyThreads, 0, s>>>(d, p);
 }
 
 }  // namespace
