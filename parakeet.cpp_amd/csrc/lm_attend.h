@@ -1,11 +1,10 @@
-// lm_attend.h -- attention over a paged cache (pk_kv4_attend, pk_kv8_attend): what does not depend on how the cache holds its
-// values.  How it does is the template parameter C: Kv4 (lm_attend4.h) or Kv8 (lm_attend8.h).
+// lm_attend.h -- attention over the 4-bit paged cache (pk_kv4_attend).
 //
 // With columns c for the 16 query rows of a tile (a row is a (token, query head of one kv head) pair), S = K Q^T and
 // O^T = V^T P both run on v_mfma_f32_16x16x32_bf16.  K's and V's codes become bf16 with their block's scale applied in
-// one conversion of two (exact: a 4-bit level has two significant bits, an 8-bit one four).  A bf16 query is its own operand,
-// an f16 one the sum of two bf16 (exact: 11 bits in 8 + 8).  So scores are f32 sums of exact products; P is rounded to bf16, or
-// for an f16 result to a pair of them (16 bits).  The matrix core could multiply the codes as they are
+// one conversion of two (exact: a level has two significant bits).  A bf16 query is its own operand, an f16 one the sum
+// of two bf16 (exact: 11 bits in 8 + 8).  So scores are f32 sums of exact products; P is rounded to bf16, or for an f16
+// result to a pair of them (16 bits).  The matrix core could multiply the 4-bit codes as they are
 // (v_mfma_scale_f32_16x16x128_f8f6f4, queries as sums of 8-bit floats), at the same rate for exact bf16 queries and with
 // no conversion of K, but its sums keep too little: errors of up to 2^-16 of the sum of magnitudes were measured, 2^-22
 // for the bf16 products.
@@ -15,8 +14,6 @@
 // value crosses lanes.  The cache's V order gives a lane its 8 keys x D/16 channels in one run of bytes; of a K row it
 // takes D/4 adjacent channels, the order of channels being free as long as the queries have the same.
 #pragma once
-
-#include <utility>
 
 #include "lm_common.h"
 #include "parakeet_lm.h"
@@ -81,6 +78,16 @@ struct Queries {
     }
 };
 
+// 8 codes as 8 bf16
+__device__ inline u4 unpack8(unsigned w, float scale) {
+    u4 r;
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+    return r;
+}
+
 __device__ inline v4f mfma(u4 a, u4 b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
@@ -106,11 +113,67 @@ __device__ inline v4f load_shared(const float *base, unsigned at) {
     return __builtin_bit_cast(v4f, load_shared4((const unsigned *)base, at));
 }
 
-// f(0), f(1) .. f(N - 1), each a constant.
-template <class F, int... I>
-__device__ inline void unrolled(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
-template <int N, class F>
-__device__ inline void unrolled(F f) { unrolled(f, std::make_integer_sequence<int, N>{}); }
+// Where a lane's codes of 32 keys lie in their record, which does not change from step to step.  A step's keys are on
+// one page, or with pages of 16 (Small) on two; on one page the rest of an address is the same in the whole wave.
+template <int D, bool Small>
+struct KeyOffsets {
+    unsigned k, v;
+
+    __device__ KeyOffsets(const Record &rec) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+        k = ((8 * (c >> 2) + (c & 3)) & (Small ? 15 : 31)) * (D / 2) + g * (D / 8);
+        v = rec.v_codes() + (Small ? g & 1 : g) * (4 * D) + c * (D / 4);
+    }
+};
+
+// One step's operands of a lane: 32 keys, of K two rows' D/4 channels, of V 8 keys' D/16 channels.
+template <int D>
+struct KeyTile {
+    static constexpr int kKWords = D / 32, kVWords = D == 64 ? 4 : D / 16;
+    unsigned k[2][kKWords], v[kVWords];
+    unsigned ks[2];
+    u2 vs;
+
+    // id0, id1: pages of the tile's two 16-key halves (the same where pages are larger), -1: none
+    template <bool Small>
+    __device__ void load_k(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0,
+                           int id1) {
+        const uint8_t *p = a.cache + head_at + max(id0, 0) * a.page_stride;
+        if (Small) p = (threadIdx.x & 8) ? a.cache + head_at + max(id1, 0) * a.page_stride : p;
+        const int off = Small ? 0 : kb & (a.page - 1);
+        const uint8_t *kp = p + off * (D / 2), *sp = p + off * (D / 32);
+        unsigned kat = at.k;
+        asm volatile("" : "+v"(kat));       // the scales' offset is worked out anew: registers are scarcer than that
+        const unsigned ksat = rec.k_scales() + (kat >> 4);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (D == 64) *(u2 *)k[t] = *(const u2 *)(kp + kat + 4 * t * (D / 2));
+            else
+#pragma unroll
+                for (int i = 0; i < D / 128; ++i) *(u4 *)&k[t][4 * i] = *(const u4 *)(kp + kat + 4 * t * (D / 2) + 16 * i);
+            ks[t] = D == 256 ? *(const uint16_t *)(sp + ksat + 4 * t * (D / 32)) : sp[ksat + 4 * t * (D / 32)];
+        }
+    }
+    template <bool Small>
+    __device__ void load_v(const AttendParams &a, const Record &rec, const KeyOffsets<D, Small> &at, int64_t head_at, int kb, int id0,
+                           int id1) {
+        const uint8_t *p = a.cache + head_at + max(id0, 0) * a.page_stride;
+        if (Small) p = (threadIdx.x & 32) ? a.cache + head_at + max(id1, 0) * a.page_stride : p;
+        const int off = Small ? 0 : kb & (a.page - 1);
+        const uint8_t *vp = p + (off >> 3) * (4 * D), *sp = p + off;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int g = lane >> 4, c = lane & 15;
+        const unsigned vsat = rec.v_scales() + (c * (D / 16) / 32) * a.page + (Small ? g & 1 : g) * 8;
+#pragma unroll
+        for (int i = 0; i < kVWords / 4; ++i) *(u4 *)&v[4 * i] = *(const u4 *)(vp + at.v + 16 * i);
+        vs = *(const u2 *)(sp + vsat);
+    }
+    // key j's word w of V codes (D = 64: its 16 bits, in the low half)
+    __device__ unsigned v_word(int j, int w) const {
+        return D == 64 ? (j & 1 ? v[j >> 1] >> 16 : v[j >> 1]) : v[j * (D / 128 > 0 ? D / 128 : 1) + w];
+    }
+};
 
 // Online softmax of 16 columns over 32 keys a step, on one wave.
 template <int D, int Planes>
@@ -125,22 +188,52 @@ struct Softmax {
         m = -INFINITY, l = 0;
     }
 
-    template <class Tile>
-    __device__ void scores(const Tile &x, const Queries<D, Planes> &q, v4f (&s)[2]) const {
+    __device__ void scores(const KeyTile<D> &x, const Queries<D, Planes> &q, v4f (&s)[2]) const {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             s[t] = v4f{0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < D / 32; ++ks) {
-                const u4 k8 = x.k8(t, ks);
+                const unsigned sb = D == 256 ? x.ks[t] >> (8 * (ks / 4)) & 255u : x.ks[t];
+                const u4 k8 = unpack8(x.k[t][ks], __uint_as_float(sb << 23));
 #pragma unroll
                 for (int n = 0; n < Planes; ++n) s[t] = mfma(k8, q.b[n][ks], s[t]);
             }
         }
     }
 
-    template <class Tile>
-    __device__ void add(const v4f (&s)[2], const Tile &x, typename Tile::VScales vs, float to_log2) {
+    // Keys vk .. vk + 7 of this lane: [lo, hi) is what its column sees, [lo_all, hi_all) what any column sees.  Scores
+    // of keys not seen become -inf.  What lies at keys that no column sees may be anything: their V scale becomes 1.  A
+    // NaN block of V that only some columns see is taken out, and those columns are made NaN.
+    __device__ void mask(v4f (&s)[2], u2 &vs, int vk, bool fine, int lo, int hi, int lo_all, int hi_all) {
+        unsigned nan_keys = 0, seen = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = vk + j, at = 8 * (j & 3);
+            if (fine && key < hi && key >= lo) seen |= 1u << j;
+            else s[j >> 2][j & 3] = -INFINITY;
+            const bool dead = !fine || key >= hi_all || key < lo_all;
+            const bool nan = (vs[j >> 2] >> at & 255u) == 255u;
+            if (!dead && nan) nan_keys |= 1u << j;
+            if (dead || nan) vs[j >> 2] = (vs[j >> 2] & ~(255u << at)) | 127u << at;
+        }
+        if (__any(nan_keys != 0)) {
+            u4 va, pa;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                va[j] = (nan_keys >> (2 * j) & 1 ? 0x3F80u : 0) | (nan_keys >> (2 * j + 1) & 1 ? 0x3F800000u : 0);
+                pa[j] = (seen >> (2 * j) & 1 ? 0x3F80u : 0) | (seen >> (2 * j + 1) & 1 ? 0x3F800000u : 0);
+            }
+            const v4f n = mfma(va, pa, v4f{0, 0, 0, 0});      // how many such keys each column sees, by channel entry
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n[i] > 0)
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) acc[t][i] = __builtin_nanf("");
+        }
+    }
+
+    __device__ void add(const v4f (&s)[2], const KeyTile<D> &x, u2 vs, float to_log2) {
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         top = column_max(top);
@@ -168,16 +261,16 @@ struct Softmax {
         }
         float vscale[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vscale[j] = Tile::v_scale(vs, j);
-        // two channels at a time
-        unrolled<D / 32>([&](auto pair) {
-            constexpr int kPair = decltype(pair)::value;
-            v4f &even = acc[2 * kPair], &odd = acc[2 * kPair + 1];
+        for (int j = 0; j < 8; ++j) vscale[j] = __uint_as_float((vs[j >> 2] >> (8 * (j & 3)) & 255u) << 23);
+        // two channels at a time: a byte of each key's codes
+        auto two = [&](auto sel, int word, v4f &even, v4f &odd) {
+            constexpr int kSel = decltype(sel)::value;
             u4 ve, vo;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const unsigned au = x.template v_pair<kPair>(2 * j, vscale[2 * j]);
-                const unsigned bu = x.template v_pair<kPair>(2 * j + 1, vscale[2 * j + 1]);
+                const bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v_word(2 * j, word), vscale[2 * j], kSel);
+                const bf2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v_word(2 * j + 1, word), vscale[2 * j + 1], kSel);
+                const unsigned au = __builtin_bit_cast(unsigned, a), bu = __builtin_bit_cast(unsigned, b);
                 ve[j] = __builtin_amdgcn_perm(bu, au, 0x05040100u);
                 vo[j] = __builtin_amdgcn_perm(bu, au, 0x07060302u);
             }
@@ -187,7 +280,16 @@ struct Softmax {
                 even = mfma(ve, pl, even);
                 odd = mfma(vo, pl, odd);
             }
-        });
+        };
+#pragma unroll
+        for (int w = 0; w < (D == 64 ? 1 : D / 128); ++w) {
+            two(std::integral_constant<int, 0>{}, w, acc[8 * w + 0], acc[8 * w + 1]);
+            two(std::integral_constant<int, 1>{}, w, acc[8 * w + 2], acc[8 * w + 3]);
+            if constexpr (D > 64) {
+                two(std::integral_constant<int, 2>{}, w, acc[8 * w + 4], acc[8 * w + 5]);
+                two(std::integral_constant<int, 3>{}, w, acc[8 * w + 6], acc[8 * w + 7]);
+            }
+        }
     }
 };
 
@@ -206,8 +308,8 @@ __device__ inline bool last_to_come(int *counter, int of, int *s_last) {
     return *s_last;
 }
 
-// base: [n][16][D sums, maximum, total, 2 unused]; finish(column, quad, sums of its 4 channels, maximum, total)
-template <int D, class Finish>
+// base: [n][Cols][D sums, maximum, total, 2 unused]; finish(column, quad, sums of its 4 channels, maximum, total)
+template <int D, int Cols, class Finish>
 __device__ inline void join_some(const float *base, int n, int live, float to_log2, Finish finish) {
     constexpr int kQuads = D / 4, kRow = D + 4;
     for (int u = threadIdx.x; u < live * kQuads; u += kAttendThreads) {
@@ -219,7 +321,7 @@ __device__ inline void join_some(const float *base, int n, int live, float to_lo
             v4f x[8], ml[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const unsigned p = (min(i0 + i, n - 1) * 16 + col) * kRow;
+                const unsigned p = (min(i0 + i, n - 1) * Cols + col) * kRow;
                 x[i] = load_shared(base, p + 4 * quad), ml[i] = load_shared(base, p + D);
             }
             float t2 = top;
@@ -238,25 +340,25 @@ __device__ inline void join_some(const float *base, int n, int live, float to_lo
 }
 
 // This split's sums are in its place of tile `at`; `mine` splits have keys.
-template <int D, class Finish>
+template <int D, int Cols = 16, class Finish>
 __device__ inline void join(const AttendParams &a, int64_t at, int split, int mine, int live, float to_log2, int *s_last, Finish finish) {
-    constexpr int kPlace = 16 * (D + 4);
+    constexpr int kPlace = Cols * (D + 4);
     float *all = a.part + at * (a.splits + a.groups) * kPlace, *joined = all + (int64_t)a.splits * kPlace;
     int *arrived = a.arrived + at * (1 + a.groups);
     const int group = split / kJoin, groups = (mine + kJoin - 1) / kJoin, n = min(kJoin, mine - group * kJoin);
     if (!last_to_come(arrived + 1 + group, n, s_last)) return;
     const float *base = all + (int64_t)group * kJoin * kPlace;
     if (groups == 1) {
-        join_some<D>(base, n, live, to_log2, finish);
+        join_some<D, Cols>(base, n, live, to_log2, finish);
         return;
     }
-    join_some<D>(base, n, live, to_log2, [&](int col, int quad, v4f o, float top, float total) {
-        const unsigned p = (group * 16 + col) * (D + 4);
+    join_some<D, Cols>(base, n, live, to_log2, [&](int col, int quad, v4f o, float top, float total) {
+        const unsigned p = (group * Cols + col) * (D + 4);
         store_shared(joined, p + 4 * quad, o);
         if (quad == 0) store_shared(joined, p + D, v4f{top, total, 0, 0});
     });
     if (!last_to_come(arrived, groups, s_last)) return;
-    join_some<D>(joined, groups, live, to_log2, finish);
+    join_some<D, Cols>(joined, groups, live, to_log2, finish);
 }
 
 // One 16-column tile, its keys dealt to the eight waves 32 at a time; `splits` workgroups share a tile's keys.  Each wave
@@ -266,8 +368,8 @@ __device__ inline void join(const AttendParams &a, int64_t at, int split, int mi
 // 2 kv heads in f16, 77 MB in 29.4 us (2.6 TB/s): the unpacking, two bf16 planes and the join, and the split, which goes by the
 // longest request: up to 336 workgroups have keys, two on some units and one on most.  One session of 733 keys: 7.3 us, a launch,
 // two steps of the first of its two splits, and their join.
-template <class C, class T, int D, bool Small>
-__global__ __launch_bounds__(kAttendThreads, (C::template kWaves<T, D>)) void attend_kernel(AttendParams a) {
+template <class T, int D, bool Small>
+__global__ __launch_bounds__(kAttendThreads, D == 256 ? 2 : 4) void attend_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
     constexpr int kTiles = D / 16, kRow = D + 4;
     using Raw = typename T::Raw;
@@ -306,7 +408,7 @@ __global__ __launch_bounds__(kAttendThreads, (C::template kWaves<T, D>)) void at
     // the scale's sign is in the queries; a scale of zero would make 0 * -inf of a key not seen
     const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
 
-    const typename C::Rec rec{a.page, D};
+    const Record rec{a.page, D};
     const int64_t head_at = hk * rec.bytes();
     const int *table = a.table + b * a.table_stride;
     const int last_page = max(held - 1, 0) >> a.page_shift;
@@ -324,8 +426,8 @@ __global__ __launch_bounds__(kAttendThreads, (C::template kWaves<T, D>)) void at
         // looked up a step ahead.  (A second set of registers, read a whole step ahead, spills where two planes of Q and P
         // are held, and takes longer elsewhere too: 64 sessions of up to 4,097 keys 37.5 us against 35.1, 200,003 and
         // 100,001 keys in f16 48.5 against 29.4.)
-        const typename C::template Offsets<D, Small> at(rec);
-        typename C::template Tile<D> x;
+        const KeyOffsets<D, Small> at(rec);
+        KeyTile<D> x;
         auto second = [&](int first, int key) { return Small ? page_of(key + 16) : first; };
         int id0 = page_of(kb), id1 = second(id0, kb);
         int n0 = page_of(kb + kStride), n1 = second(n0, kb + kStride);
@@ -339,9 +441,9 @@ __global__ __launch_bounds__(kAttendThreads, (C::template kWaves<T, D>)) void at
             sm.scores(x, q, s);
             __builtin_amdgcn_sched_barrier(0);
             x.load_k(a, rec, at, head_at, nb, l0, l1);
-            auto vs = x.vs;
+            u2 vs = x.vs;
             if (kb + 32 > hi_min || kb < lo_max || id0 < 0 || id1 < 0)
-                x.mask(sm, s, vs, kb + 8 * g, (g < 2 ? id0 : id1) >= 0, lo, hi, lo_min, hi_max);
+                sm.mask(s, vs, kb + 8 * g, (g < 2 ? id0 : id1) >= 0, lo, hi, lo_min, hi_max);
             sm.add(s, x, vs, to_log2);
             __builtin_amdgcn_sched_barrier(0);
             x.load_v(a, rec, at, head_at, nb, l0, l1);
@@ -437,13 +539,131 @@ __device__ inline v16f mfma32(u4 a, u4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
-template <class C, class T, int D, bool Small>
+// As KeyOffsets, for a thread's share of 64 keys.  Small: they may be on pages of their own, of 16 or 32 tokens.
+template <int D, bool Small>
+struct PromptOffsets {
+    unsigned k, ks, v, vs;
+
+    __device__ PromptOffsets(const AttendParams &a, const Record &rec) {
+        const int t = threadIdx.x, quarter = t & 3, r = (t >> 1) & 15, half = t & 1;
+        const int tokens = Small ? min(a.page, 64) : 64, kkey = (t >> 2) & (tokens - 1), vkey = ((t >> 5) * 8) & (tokens - 1);
+        k = kkey * (D / 2) + quarter * (D / 8);
+        ks = rec.k_scales() + kkey * (D / 32) + quarter * (D / 4) / 32;
+        v = rec.v_codes() + (vkey >> 3) * (4 * D) + r * (D / 4) + (D == 256 ? 4 * half : 0);
+        vs = rec.v_scales() + (r * (D / 16) / 32) * a.page + vkey;
+    }
+};
+
+// One thread's share of 64 keys' bytes: of K a quarter of a key's channels, of V half the channels of an entry of 8 keys.
+template <int D>
+struct PromptBytes {
+    unsigned k[D / 32], v[8], ks;
+    u2 vs;
+
+    // What is made of the bytes is made after this point, not before (the compiler would).
+    __device__ void pin() {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) asm volatile("" : "+v"(k[i]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(v[i]));
+        unsigned a = vs[0], b = vs[1];
+        asm volatile("" : "+v"(ks), "+v"(a), "+v"(b));
+        vs = u2{a, b};
+    }
+
+    // kid, vid: pages of this thread's keys, the same for all threads where pages hold 64 tokens or more (not Small)
+    template <bool Small>
+    __device__ void load(const AttendParams &a, const PromptOffsets<D, Small> &at, int64_t head_at, int kb, int kid, int vid) {
+        const int half = threadIdx.x & 1, off = kb & (a.page - 1);
+        const uint8_t *krec = a.cache + max(kid, 0) * a.page_stride + head_at;
+        const uint8_t *vrec = Small ? a.cache + max(vid, 0) * a.page_stride + head_at : krec;
+        const uint8_t *kp = krec + off * (D / 2), *ksp = krec + off * (D / 32), *vp = vrec + (off >> 3) * (4 * D), *vsp = vrec + off;
+        if (D == 64) *(u2 *)k = *(const u2 *)(kp + at.k);
+        else
+#pragma unroll
+            for (int i = 0; i < D / 128; ++i) *(u4 *)&k[4 * i] = *(const u4 *)(kp + at.k + 16 * i);
+        ks = D == 256 ? *(const uint16_t *)(ksp + at.ks) : ksp[at.ks];
+        if (D == 64) {
+            const u4 w = *(const u4 *)(vp + at.v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[2 * i] = w[i] >> (8 * half), v[2 * i + 1] = w[i] >> (16 + 8 * half);
+        } else if (D == 128) {
+            *(u4 *)&v[0] = *(const u4 *)(vp + at.v), *(u4 *)&v[4] = *(const u4 *)(vp + at.v + 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = *(const unsigned *)(vp + at.v + 8 * i);
+        }
+        vs = *(const u2 *)(vsp + at.vs);
+    }
+};
+
+template <int D>
+struct alignas(16) PromptTile {
+    static constexpr int kKRow = D * 2 + 16, kVRow = kPromptKeys * 2 + 16;     // bytes; the pads spread rows over banks
+    uint8_t k[kPromptKeys * kKRow], v[D * kVRow];
+
+    uint8_t nan[kPromptKeys][D / 32];       // of an edge tile: blocks of V that are NaN
+
+    // What lies at keys without a page may be anything; so at an edge, where some column does not see some key, at keys
+    // outside [lo, hi), which no column sees.  NaN blocks of the others are taken out there and marked; marked becomes kb.
+    __device__ void clean(PromptBytes<D> &x, int kb, bool edge, bool vfine, int lo, int hi, int &marked) {
+        const int t = threadIdx.x, a8 = t >> 5, r = (t >> 1) & 15;
+        if (edge || !vfine) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = 8 * (j & 3), kj = kb + 8 * a8 + j;
+                const bool dead = !vfine || kj >= hi || kj < lo, bad = (x.vs[j >> 2] >> at & 255u) == 255u;
+                if (edge) nan[8 * a8 + j][r * (D / 16) / 32] = bad && !dead;     // by all threads of the block alike
+                if (bad && !dead) marked = kb;
+                if (bad || dead) x.vs[j >> 2] = (x.vs[j >> 2] & ~(255u << at)) | 127u << at;
+            }
+        }
+    }
+    __device__ void stage(const PromptBytes<D> &x) {
+        const int t = threadIdx.x, key = t >> 2, quarter = t & 3;
+        uint8_t *krow = k + key * kKRow + quarter * (D / 2);
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+            const unsigned sb = D == 256 ? x.ks >> (8 * (w / 4)) & 255u : x.ks;
+            *(u4 *)(krow + 16 * w) = unpack8(x.k[w], __uint_as_float(sb << 23));
+        }
+        const int a8 = t >> 5, r = (t >> 1) & 15, half = t & 1;
+        const u2 vs = x.vs;
+        float scale[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) scale[j] = __uint_as_float((vs[j >> 2] >> (8 * (j & 3)) & 255u) << 23);
+        constexpr int kEach = D / 32;                  // channels of this thread, two a byte
+        auto two = [&](auto sel, int shift) {
+            constexpr int kSel = decltype(sel)::value;
+            u4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bf2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v[2 * j] >> shift, scale[2 * j], kSel);
+                const bf2 q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x.v[2 * j + 1] >> shift, scale[2 * j + 1], kSel);
+                const unsigned pu = __builtin_bit_cast(unsigned, p), qu = __builtin_bit_cast(unsigned, q);
+                even[j] = __builtin_amdgcn_perm(qu, pu, 0x05040100u);
+                odd[j] = __builtin_amdgcn_perm(qu, pu, 0x07060302u);
+            }
+            const int n = half * kEach + 2 * kSel;
+            *(u4 *)(v + (n * 16 + r) * kVRow + a8 * 16) = even;
+            *(u4 *)(v + ((n + 1) * 16 + r) * kVRow + a8 * 16) = odd;
+        };
+        const int shift = D == 128 ? 16 * half : 0;
+        two(std::integral_constant<int, 0>{}, shift);
+        if constexpr (D >= 128) two(std::integral_constant<int, 1>{}, shift);
+        if constexpr (D == 256) {
+            two(std::integral_constant<int, 2>{}, shift);
+            two(std::integral_constant<int, 3>{}, shift);
+        }
+    }
+};
+
+template <class T, int D, bool Small>
 __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_prompt_kernel(AttendParams a) {
     constexpr int Planes = __is_same(T, F16) ? 2 : 1;
     constexpr int kSteps = D / 16, kTiles = D / 32;
     using Raw = typename T::Raw;
-    using Tile = typename C::template PromptTile<D>;
-    __shared__ Tile s_tile[2];
+    __shared__ PromptTile<D> s_tile[2];
     __shared__ int s_missing[2], s_marked[2];       // the tile of each buffer that lacks a page, has marked NaN blocks
 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, c = lane & 31;
@@ -500,7 +720,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
     }
     const float to_log2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
 
-    const typename C::Rec rec{a.page, D};
+    const Record rec{a.page, D};
     const int64_t head_at = hk * rec.bytes();
     const int *table = a.table + b * a.table_stride;
     const int last_page = max(held - 1, 0) >> a.page_shift;
@@ -516,12 +736,13 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
         for (int i = 0; i < 16; ++i) acc[n][i] = 0;
     float m = -INFINITY, l = 0;
 
+    const int kkey = t >> 2, vkey = (t >> 5) * 8;        // of 64, in this thread's staging
     auto edge_at = [&](int kb) { return kb + kPromptKeys > hi_min || kb < lo_max; };
     if (k0 < k1) {
-        const typename C::template PromptOffsets<D, Small> offsets(a, rec);
-        typename C::template PromptBytes<D> bytes;
-        auto page_k = [&](int key) { return page_of(key + offsets.k_key()); };
-        auto page_v = [&](int key, int k_page) { return offsets.kTwoPages ? page_of(key + offsets.v_key()) : k_page; };
+        const PromptOffsets<D, Small> offsets(a, rec);
+        PromptBytes<D> bytes;
+        auto page_k = [&](int key) { return page_of(Small ? key + kkey : key); };
+        auto page_v = [&](int key, int k_page) { return Small ? page_of(key + vkey) : k_page; };
         int kid = page_k(k0), vid = page_v(k0, kid);
         bytes.load(a, offsets, head_at, k0, kid, vid);
         if (t < 2) s_missing[t] = s_marked[t] = -1;
@@ -538,13 +759,13 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
         // unit free) and the one after that is on its way from memory; behind the last one the last page is read again.
         for (int kb = k0; kb < k1; kb += kPromptKeys, buf ^= 1) {
             const int nb = kb + kPromptKeys;
-            Tile &next = s_tile[buf ^ 1];
+            PromptTile<D> &next = s_tile[buf ^ 1];
             if (D < 256) __builtin_amdgcn_s_setprio(0);
             if (kid < 0 || vid < 0) s_missing[buf ^ 1] = nb;
             next.clean(bytes, nb, edge_at(nb), vid >= 0, lo_min, hi_max, s_marked[buf ^ 1]);
             const bool active = kb < whi_max && nb > wlo_min;
             v16f s[2];
-            const Tile &x = s_tile[buf];
+            const PromptTile<D> &x = s_tile[buf];
             {
                 // all operands first, so that no product waits for its own; the two halves' products in turn, the next
                 // tile's unpacking between them
@@ -561,7 +782,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
                     for (int ks = 0; ks < kAhead; ++ks)
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
-                            kk[u][ks] = *(const u4 *)(x.k + (32 * u + krow) * Tile::kKRow + 32 * (k8 + ks) + 16 * h);
+                            kk[u][ks] = *(const u4 *)(x.k + (32 * u + krow) * PromptTile<D>::kKRow + 32 * (k8 + ks) + 16 * h);
                     __builtin_amdgcn_sched_barrier(0);
                     if (k8 + kAhead >= kSteps) bytes.pin();
 #pragma unroll
@@ -587,8 +808,27 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
             if (active) {
                 // a tile can be an edge, its NaN blocks marked, for other waves' columns and whole for this one's
                 const bool missing = s_missing[buf] == kb, marked = s_marked[buf] == kb;
-                if (kb + kPromptKeys > whi_min || kb < wlo_max || missing || marked)
-                    x.mask(s, acc, kb, h, lo, hi, marked, [&](int key) { return !(missing && page_of(key) < 0); });
+                if (kb + kPromptKeys > whi_min || kb < wlo_max || missing || marked) {
+                    unsigned bad = 0;             // channel blocks whose NaN this column sees
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int at = 32 * (i >> 4) + 16 * (i >> 3 & 1) + 8 * h + (i & 7), key = kb + at;
+                        const bool see = key < hi && key >= lo && !(missing && page_of(key) < 0);
+                        if (!see) s[i >> 4][i & 15] = -INFINITY;
+                        else if (marked)
+#pragma unroll
+                            for (int j = 0; j < D / 32; ++j) bad |= (unsigned)x.nan[at][j] << j;
+                    }
+                    bad |= (unsigned)__shfl_xor((int)bad, 32);
+                    if (__any(bad != 0))
+#pragma unroll
+                        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int r = (8 * (i >> 2) + 4 * h + (i & 3)) & 15;
+                                if (bad >> (r * (D / 16) / 32) & 1) acc[n][i] = __builtin_nanf("");
+                            }
+                }
                 float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
@@ -637,7 +877,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend_promp
                 auto operands = [&](int g) {
 #pragma unroll
                     for (int n = 0; n < kTiles; ++n)
-                        vv[g & 1][n] = *(const u4 *)(x.v + (32 * n + c) * Tile::kVRow + 32 * g + 16 * h);
+                        vv[g & 1][n] = *(const u4 *)(x.v + (32 * n + c) * PromptTile<D>::kVRow + 32 * g + 16 * h);
                 };
                 // Waves that sum go before the other workgroup's that unpack: 231 -> 225 us; in f16, 512 tokens x 4 on up to
                 // 8,191 keys, 408 -> 383.  (D = 256 is alone on its unit.)

@@ -1,7 +1,9 @@
 // lm_attend_host.h -- host side of attention over a paged cache (pk_kv4_attend, pk_kv8_attend): checks, the choice of kernel and
 // how a call's work is dealt out.  C is the cache's kind, as in lm_attend.h, with what the host asks of it:
 //   check(...)            of a call's cache
-//   has_prompt(dtype, D)  whether attend_prompt_kernel takes it
+//   has_prompt(dtype, D)  whether its kernel for prompts takes it
+//   prompt_cols(D), prompt_groups(D)   query rows of that kernel's workgroup; as many of them are worth it
+//   tile_cols(rows, D)    query rows of the other kernel's workgroup, of `rows` of a request and kv head
 #pragma once
 
 #include <algorithm>
@@ -35,7 +37,8 @@ constexpr int kPromptRows = 128, kPromptGroups = 512;
 
 // How a call's work is dealt out, from its host-known sizes alone.
 struct AttendShape {
-    bool prompt;             // attend_prompt_kernel, 128 query rows a workgroup; else attend_kernel, 16
+    bool prompt;             // the kernel for prompts; else the one that splits a long axis
+    int cols;                // query rows a workgroup
     int tiles, chunk, splits, groups;
     int64_t part_bytes;
     int64_t bytes() const { return splits > 1 ? kCounters * 4 + part_bytes : 0; }
@@ -44,16 +47,17 @@ struct AttendShape {
 template <class C>
 int attend_shape(const char *what, const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
-    const int64_t prompt_tiles = (rows + kPromptCols - 1) / kPromptCols;
+    const int64_t prompt_tiles = (rows + C::prompt_cols(d.head_dim) - 1) / C::prompt_cols(d.head_dim);
     auto too_many = [&] {
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %lld requests x kv heads of %lld query rows in one call", what, (long long)pairs,
                        (long long)rows);
     };
     if (pairs > most_groups(kPromptThreads)) return too_many();
-    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= kPromptGroups && C::has_prompt(d.dtype, d.head_dim);
-    const int64_t tiles = s.prompt ? prompt_tiles : (rows + 15) / 16, step = 32 * kAttendWaves;
+    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= C::prompt_groups(d.head_dim) && C::has_prompt(d.dtype, d.head_dim);
+    s.cols = s.prompt ? C::prompt_cols(d.head_dim) : C::tile_cols(rows, d.head_dim);
+    const int64_t tiles = (rows + s.cols - 1) / s.cols, step = 32 * kAttendWaves;
     // keys of one tile: its rows span at most as many tokens
-    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + 16 + 64) : d.max_len;
+    const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + s.cols + 64) : d.max_len;
     // Split where the tiles leave the card short of work (512 workgroups are resident), into no less than 512 keys.
     // 200,003 and 100,001 keys on 2 kv heads, 64 sessions of up to 4,097 keys on 8, 8 of up to 32,000: 29.5, 35.8 and 40.6
     // us; for twice as many splits 34.3, 37.2 and 43.3, for half as many 29.3, 36.1 and 46.0.
@@ -63,10 +67,10 @@ int attend_shape(const char *what, const pk_kv4_attend_desc &d, AttendShape &s) 
     splits = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
     if (pairs * tiles * splits > most_groups(s.prompt ? kPromptThreads : kAttendThreads)) return too_many();
     // a tile's partial sums are reached by 32-bit byte offsets
-    static_assert((kSplitWork + (kSplitWork + kJoin - 1) / kJoin) * 16 * (256 + 4) * 4ll < 1ll << 31, "at most kSplitWork splits");
+    static_assert((kSplitWork + (kSplitWork + kJoin - 1) / kJoin) * 32 * (256 + 4) * 4ll < 1ll << 31, "at most kSplitWork splits");
     s.tiles = (int)tiles, s.chunk = (int)chunk, s.splits = (int)splits;
     s.groups = (int)((splits + kJoin - 1) / kJoin);
-    s.part_bytes = pairs * tiles * (splits + s.groups) * 16 * (d.head_dim + 4) * 4;
+    s.part_bytes = pairs * tiles * (splits + s.groups) * s.cols * (d.head_dim + 4) * 4;
     return PK_OK;
 }
 
@@ -134,7 +138,7 @@ int attend_call(const char *what, const pk_kv4_attend_desc *d, Launch launch) {
     p.vec = aligned(d->q, 16) && d->q_row % 8 == 0 && d->q_head % 8 == 0;
     p.vec_out = aligned(d->out, 8) && d->out_row % 4 == 0 && d->out_head % 4 == 0;
     const unsigned grid = (unsigned)((int64_t)d->requests * d->kv_heads * sh.tiles * sh.splits);
-    launch(p, sh.prompt, grid);
+    launch(p, sh, grid);
     return launched(what);
 }
 

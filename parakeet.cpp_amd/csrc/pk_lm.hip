@@ -11,7 +11,7 @@
 #include <cstring>
 
 #include "last_error.h"
-#include "lm_attend4.h"
+#include "lm_attend.h"
 #include "lm_attend_host.h"
 #include "lm_cache.h"
 #include "lm_host.h"
@@ -164,6 +164,9 @@ struct HostKv4 {
         return check_cache(what, cache, page_stride, page, n_pages, heads, dim);
     }
     static bool has_prompt(int dtype, int dim) { return !(dtype == PK_DTYPE_F16 && dim == 256); }
+    static int prompt_cols(int) { return kPromptCols; }
+    static int prompt_groups(int) { return kPromptGroups; }
+    static int tile_cols(int64_t, int) { return 16; }
 };
 
 template <class T, int D>
@@ -171,13 +174,13 @@ void launch_attend(const AttendParams &p, bool prompt, unsigned grid, hipStream_
     // pages of whole key tiles: addresses are worked out a wave at a time.  A prompt of 512 tokens x 4 on up to 8,191 keys
     // takes 431 us with f16 rows of 128 then, 443 otherwise; of D = 256, whose registers are full, 664 and 526.
     if constexpr (D == 256 && __is_same(T, BF16)) {
-        if (prompt) return attend_prompt_kernel<Kv4, T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt) return attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
     } else if constexpr (D < 256) {
-        if (prompt && p.page < kPromptKeys) return attend_prompt_kernel<Kv4, T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
-        if (prompt) return attend_prompt_kernel<Kv4, T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt && p.page < kPromptKeys) return attend_prompt_kernel<T, D, true><<<grid, kPromptThreads, 0, s>>>(p);
+        if (prompt) return attend_prompt_kernel<T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
     }
-    if (p.page < 32) attend_kernel<Kv4, T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
-    else attend_kernel<Kv4, T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
+    if (p.page < 32) attend_kernel<T, D, true><<<grid, kAttendThreads, 0, s>>>(p);
+    else attend_kernel<T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
 }
 
 template <class T>
@@ -225,9 +228,9 @@ PK_API int pk_kv4_attend_workspace(const pk_kv4_attend_desc *d, int64_t *bytes) 
 }
 
 PK_API int pk_kv4_attend(const pk_kv4_attend_desc *d, void *stream) {
-    return attend_call<HostKv4>("pk_kv4_attend", d, [&](const AttendParams &p, bool prompt, unsigned grid) {
-        if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
-        else launch_attend<BF16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
+    return attend_call<HostKv4>("pk_kv4_attend", d, [&](const AttendParams &p, const AttendShape &s, unsigned grid) {
+        if (d->dtype == PK_DTYPE_F16) launch_attend<F16>(p, s.prompt, d->head_dim, grid, (hipStream_t)stream);
+        else launch_attend<BF16>(p, s.prompt, d->head_dim, grid, (hipStream_t)stream);
     });
 }
 

@@ -83,17 +83,19 @@ struct HostKv8 {
     static int check(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
         return check_cache8(what, cache, page_stride, page, n_pages, heads, dim);
     }
-    static bool has_prompt(int dtype, int dim) { return !(dtype == PK_DTYPE_F16 && dim == 256); }
+    static bool has_prompt(int, int) { return true; }
+    static int prompt_cols(int) { return kPromptCols; }
+    static int prompt_groups(int) { return kPromptGroups; }
+    static int tile_cols(int64_t rows, int dim) { return rows <= 16 || dim == 256 ? 16 : 32; }
 };
 
 template <class T>
-void launch_attend8(const AttendParams &p, bool prompt, int dim, unsigned grid, hipStream_t s) {
+void launch_attend8(const AttendParams &p, const AttendShape &sh, int dim, unsigned grid, hipStream_t s) {
     by_dim(dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if constexpr (D < 256 || __is_same(T, BF16)) {
-            if (prompt) return attend_prompt_kernel<Kv8, T, D, false><<<grid, kPromptThreads, 0, s>>>(p);
-        }
-        attend_kernel<Kv8, T, D, false><<<grid, kAttendThreads, 0, s>>>(p);
+        if (sh.prompt) attend8_prompt_kernel<T, D><<<grid, kPromptThreads, 0, s>>>(p);
+        else if (sh.cols == 16) attend8_kernel<T, D, 1><<<grid, kAttendThreads, 0, s>>>(p);
+        else if constexpr (D < 256) attend8_kernel<T, D, 2><<<grid, kAttendThreads, 0, s>>>(p);
     });
 }
 
@@ -267,9 +269,9 @@ PK_API int pk_kv8_attend_workspace(const pk_kv4_attend_desc *d, int64_t *bytes) 
 }
 
 PK_API int pk_kv8_attend(const pk_kv4_attend_desc *d, void *stream) {
-    return attend_call<HostKv8>("pk_kv8_attend", d, [&](const AttendParams &p, bool prompt, unsigned grid) {
-        if (d->dtype == PK_DTYPE_F16) launch_attend8<F16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
-        else launch_attend8<BF16>(p, prompt, d->head_dim, grid, (hipStream_t)stream);
+    return attend_call<HostKv8>("pk_kv8_attend", d, [&](const AttendParams &p, const AttendShape &s, unsigned grid) {
+        if (d->dtype == PK_DTYPE_F16) launch_attend8<F16>(p, s, d->head_dim, grid, (hipStream_t)stream);
+        else launch_attend8<BF16>(p, s, d->head_dim, grid, (hipStream_t)stream);
     });
 }
 

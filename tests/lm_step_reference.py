@@ -133,6 +133,57 @@ def same_codes(a, b):
     return np.array_equal(va, vb, equal_nan=True)
 
 
+# ---- attention ----
+
+def attend(q, cache, table, lens, first, page, scale, window, dtype):
+    """(out, lse, tolerance of out, tolerance of lse) in f64, as lm_reference.attend's, of attention over the 8-bit cache.
+
+    Tolerances, of a query row with probabilities p over keys k, values v:
+      a score is off by at most ds = |scale| (2^-20 max|q| sum|k| + 2^-21 sum|q k|): products are exact, sums are f32;
+      out is rounded to its type (unit); p, f32 sums apart, to f16's 11 bits, 2^-11, down to 2^-28 of the largest p,
+      and below that to 2^-39 of it: unit |out| + (2^-11 + 2 ds + 2^-17) sum p |v| + 2^-38 sum |v| max p;
+      v, in f16 with the largest block's values at 2^8 .. 2^16, to 2^-25: 2^-32 of a value over half the block's largest code,
+      2^-39 of the largest |v| that the request's tiles meet.
+    """
+    N, Hq, D = q.shape
+    H = cache.shape[1]
+    out, lse = np.zeros(q.shape), np.full((N, Hq), -np.inf)
+    tol, ltol = np.zeros(q.shape), np.zeros((N, Hq))
+    for b in range(len(lens)):
+        n, new = int(lens[b]), int(first[b + 1] - first[b])
+        if n <= 0:
+            continue
+        for h in range(H):
+            rows = [get_row(cache[table[b, t // page], h], t % page, page, D) if 0 <= table[b, t // page] < cache.shape[0] else None
+                    for t in range(n)]
+            fine = np.array([r is not None for r in rows])
+            k = np.array([r[0] if r else np.zeros(D) for r in rows])
+            v = np.array([r[1] if r else np.zeros(D) for r in rows])
+            most = np.nanmax(np.abs(v), initial=0.0)
+            for i in range(new):
+                p = n - new + i
+                lo = max(0, p + 1 - window) if window else 0
+                at = np.arange(lo, p + 1)
+                at = at[fine[at]] if len(at) else at
+                if not len(at):
+                    continue
+                for hq in range(h * (Hq // H), (h + 1) * (Hq // H)):
+                    x = q[first[b] + i, hq]
+                    z = k[at] @ x * scale
+                    m = z.max()
+                    e = np.exp(z - m)
+                    w = e / e.sum()
+                    ds = abs(scale) * (2.0 ** -20 * np.abs(x).max() * np.abs(k[at]).sum(1)
+                                       + 2.0 ** -21 * (np.abs(k[at]) @ np.abs(x))).max()
+                    out[first[b] + i, hq] = w @ v[at]
+                    lse[first[b] + i, hq] = m + np.log(e.sum())
+                    tol[first[b] + i, hq] = (UNIT[dtype] * np.abs(w @ v[at]) + (2.0 ** -11 + 2 * ds + 2.0 ** -17) * (w @ np.abs(v[at]))
+                                             + 2.0 ** -38 * np.abs(v[at]).sum(0) * w.max() + 2.0 ** -39 * most
+                                             + (2.0 ** -24 if dtype == "f16" else 0))
+                    ltol[first[b] + i, hq] = ds + 2.0 ** -19 + 2.0 ** -22 * abs(m)
+    return out, lse, tol, ltol
+
+
 # ---- verification ----
 
 def weights(x, t):

@@ -1,5 +1,5 @@
 """pk_kv8_attend on the cases of pk_kv4_attend, over caches of 8 bits, by both kernels, within the tolerances that
-lm_reference.attend derives; NaNs, which lie at single values here, and offsets by cases of their own."""
+lm_step_reference.attend derives; NaNs, which lie at single values here, and offsets by cases of their own."""
 import numpy as np
 import pytest
 
@@ -15,7 +15,7 @@ def over_8_bits(request, monkeypatch):
     """The other cache's functions are this one's; `many`: a bound of many new tokens, which brings every call to the kernel
     for prompts."""
     from parakeet_amd import lm
-    for name in ("record_bytes", "store", "get_row"):
+    for name in ("record_bytes", "store", "get_row", "attend"):
         monkeypatch.setattr(R, name, getattr(S, name))
     monkeypatch.setattr(lm, "kv4_attend", lm.kv8_attend)
     own = A.problem
