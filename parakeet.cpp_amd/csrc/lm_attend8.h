@@ -665,7 +665,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 256 ? 1 : 2) void attend8_prom
 #pragma unroll
                         for (int i = 0; i < 2 * kAhead; ++i) {
                             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                            __builtin_amdgcn_sched_group_barrier(0x202, 8, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x202, 4, 0);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
