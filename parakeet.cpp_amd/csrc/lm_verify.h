@@ -26,14 +26,15 @@ struct RowWeights {
         greedy = !(t > 0);
         to_log2 = fminf(fmaxf(1.4426950408889634f / (greedy ? 1.0f : t), 1e-38f), 3e38f);
     }
-    __device__ void largest(float x) { top = x == -INFINITY ? 0.0f : x; }      // a row of -inf has no weight
+    // a row of -inf has no weight, in one with +inf those are alike
+    __device__ void largest(float x) { top = x == -INFINITY ? 0.0f : fminf(x, 0x1.fffffep127f); }
     // exp2 of one rounded product: off by 2^-23 and 2^-24 of the exponent, 2^-19 of itself where weights end.  (The library's expf takes
-    // half as long again: weights are what bounds long rows.)
-    __device__ unsigned weight(float x, int i) const {
-        if (greedy) return i == top_at ? 1u << 30 : 0u;
-        const float d = x == top ? 0.0f : x - top;
-        return (unsigned)rintf(__builtin_amdgcn_exp2f(d * to_log2) * 1073741824.0f);
+    // half as long again: weights are what bounds long rows.)  The median of -200, 0 and the exponent is -200 for -inf and NaN.
+    __device__ float weight_f(float x, int i) const {
+        if (greedy) return i == top_at ? 1073741824.0f : 0.0f;
+        return rintf(__builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f((x - top) * to_log2, -200.0f, 0.0f)) * 1073741824.0f);
     }
+    __device__ unsigned weight(float x, int i) const { return (unsigned)weight_f(x, i); }
     __device__ void total(u64 sum) { inv_sum = sum ? 1.0 / (double)sum : 0.0; }
     __device__ double share_of(unsigned w) const { return __dmul_rn((double)w, inv_sum); }
 };
@@ -51,10 +52,18 @@ struct Tokens8 {
             for (int e = 0; e < 8; ++e) raw[e] = i < end ? row[min(i + e, end - 1)] : (typename T::Raw)0;
         }
     }
-    // -inf behind the row's end and for NaN
-    __device__ float get(int e, int i, int end) const {
-        const float x = T::get(raw[e]);
-        return x != x || i + e >= end ? -INFINITY : x;
+    // -inf behind the row's end
+    __device__ float get(int e, int i, int end) const { return i + e >= end ? -INFINITY : T::get(raw[e]); }
+    // f(e, value) of each, of a wave's pass that may reach past the row's end
+    template <class F>
+    __device__ void each(int i, int end, F f) const {
+        if (__all(i + 8 <= end)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f(e, T::get(raw[e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f(e, get(e, i, end));
+        }
     }
 };
 __device__ inline int wave_min(int v) { return lane_value(wave_scan(v, kNever, [](int a, int b) { return min(a, b); }), 63); }
@@ -154,7 +163,7 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         for (int q = 0; q < kSources; ++q) {
             int at = kNever;
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e) at = x[q][e] == rw[q].top ? index(e / 8) + e % 8 : at;
+            for (int e = E - 1; e >= 0; --e) at = fminf(x[q][e], 0x1.fffffep127f) == rw[q].top ? index(e / 8) + e % 8 : at;
             at = wave_min(at);
             if (lane == 0) s_at[q][wave] = at;
         }
@@ -311,8 +320,9 @@ __device__ inline u64 row_rule(const pk_verify_desc &a, const SplitVerify &w, in
     const float m = in ? w.chunk_max[at] : -INFINITY;
     const u64 sum = summed && in ? w.chunk_sum[at] : 0;
     const int p = rw.greedy && in ? w.chunk_at[at] : kNever;
-    rw.largest(wave_max(m));
-    rw.top_at = rw.greedy ? wave_min(m == rw.top ? p : kNever) : kNever;
+    const float top = wave_max(m);
+    rw.largest(top);
+    rw.top_at = rw.greedy && top != -INFINITY ? wave_min(m == top ? p : kNever) : kNever;
     const u64 total = summed ? wave_sum(sum) : 0;
     rw.total(total);
     return total;
@@ -338,12 +348,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_max_kernel(pk_verify_de
         for (int p = 0; p < 2; ++p) i[p] = p0 + p < w.passes ? verify_token(w.passes, c.chunk, p0 + p) : V, x[p].load(row, i[p], V);
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = x[p].get(e, i[p], V);
+            x[p].each(i[p], V, [&](int e, float v) {
                 if (rw.greedy && v > top) at = i[p] + e;
                 top = fmaxf(top, v);
-            }
+            });
     }
     const float wave_top = wave_max(top);
     at = rw.greedy ? wave_min(top == wave_top ? at : kNever) : kNever;
@@ -377,8 +385,11 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(pk_verify_de
         const int i = verify_token(w.passes, c.chunk, p);
         Tokens8<T> y;
         y.load(row, p + 1 < w.passes ? verify_token(w.passes, c.chunk, p + 1) : V, V);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) sum += rw.weight(x.get(e, i, V), i + e) + rw.weight(x.get(e + 1, i, V), i + e + 1);
+        unsigned two = 0;                              // of at most 2^30 each
+        x.each(i, V, [&](int e, float v) {
+            two += rw.weight(v, i + e);
+            if (e & 1) sum += two, two = 0;
+        });
         x = y;
     }
     sum = wave_sum(sum);
@@ -446,28 +457,42 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
     const auto *x_row = verify_row<T>(a, 0, r), *y_row = two ? verify_row<T>(a, 1, r) : x_row;
     const u64 total = row_rule(a, w, b, place, 0, target, true);
     if (two) row_rule(a, w, b, place, 1, draft, true);
-    // what is left of a lane's 8 tokens of a pass
-    auto left_of_pass = [&](int ch, int pass, bool any, u64 (&left)[8]) {
-        const int i = verify_token(w.draw_passes, ch, pass);
+    // What is left of a lane's 8 tokens of a pass, whole numbers in f64, whose sums are exact: of p - q in steps of 2^-52 at most 2^52
+    // and a step a token, of weights at most 2^50.
+    const double scale_p = target.inv_sum * 0x1p52, scale_q = two ? draft.inv_sum * 0x1p52 : 0.0;
+    struct Pass {
         Tokens8<T> x, y;
-        x.load(x_row, i, V);
-        if (two && !any) y.load(y_row, i, V);
+    };
+    auto load_pass = [&](int ch, int pass, bool any, Pass &of) {
+        const int i = pass < w.draw_passes ? verify_token(w.draw_passes, ch, pass) : V;
+        of.x.load(x_row, i, V);
+        if (two && !any) of.y.load(y_row, i, V);
+    };
+    auto left_of_pass = [&](int ch, int pass, bool any, const Pass &of, double (&left)[8]) {
+        const int i = verify_token(w.draw_passes, ch, pass);
+        of.x.each(i, V, [&](int e, float v) { left[e] = (double)target.weight_f(v, i + e); });
+        if (any || !drafted) return;
+        if (two)
+            of.y.each(i, V, [&](int e, float v) {
+                left[e] = trunc(fmax(__dadd_rn(__dmul_rn(left[e], scale_p), -__dmul_rn((double)draft.weight_f(v, i + e), scale_q)), 0.0));
+            });
+        else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const unsigned wt = target.weight(x.get(e, i, V), i + e);
-            left[e] = wt;
-            if (!any && drafted) left[e] = two ? left_of(target.share_of(wt), draft.share_of(draft.weight(y.get(e, i, V), i + e))) : i + e == d ? 0 : left[e];
-        }
+            for (int e = 0; e < 8; ++e) left[e] = i + e == d ? 0.0 : left[e];
     };
     auto run_sum = [&](int ch, bool any) {
-        u64 mass = 0;
+        double mass = 0;
+        Pass now, next;
+        load_pass(ch, 0, any, now);
         for (int p = 0; p < w.draw_passes; ++p) {
-            u64 left[8];
-            left_of_pass(ch, p, any, left);
+            load_pass(ch, p + 1, any, next);
+            double left[8];
+            left_of_pass(ch, p, any, now, left);
 #pragma unroll
             for (int e = 0; e < 8; ++e) mass += left[e];
+            now = next;
         }
-        return wave_sum(mass);
+        return wave_sum((u64)mass);
     };
     {
         const u64 mass = run_sum(chunk, false);
@@ -513,21 +538,24 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
     for (int v = 0; v < wave; ++v) lead += s_sum[v];
     if (lead > t || lead + mass <= t) return;
     for (int p = 0; p < w.draw_passes; ++p) {
-        u64 left[8], own = 0;
-        left_of_pass(ch, p, any, left);
+        Pass now;
+        double left[8];
+        u64 own = 0;
+        load_pass(ch, p, any, now);
+        left_of_pass(ch, p, any, now, left);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) own += left[e];
+        for (int e = 0; e < 8; ++e) own += (u64)left[e];
         const u64 run = wave_scan(own), sum = lane_value(run, 63);
         u64 at = lead + run - own;
         if (at <= t && t < at + own) {
             const int i0 = verify_token(w.draw_passes, ch, p);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (at <= t && t < at + left[e]) {
+                if (at <= t && t < at + (u64)left[e]) {
                     a.out[r] = i0 + e;
                     if (a.prob) a.prob[r] = (float)target.share_of(target.weight(logit<T>(x_row, i0 + e), i0 + e));
                 }
-                at += left[e];
+                at += (u64)left[e];
             }
         }
         lead += sum;

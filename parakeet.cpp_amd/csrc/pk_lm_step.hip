@@ -116,14 +116,15 @@ VerifyShape verify_shape(const pk_verify_desc &d) {
         s.bytes = VerifyShape::kCounterBytes + rows * (int64_t)sizeof(RowVerdict);
         return s;
     }
-    // As many chunks as make 4,096 workgroups, 64 of a row at most (a lane has one each), of two passes at least.
-    auto cut = [&](int64_t each, int &chunks, int &passes) {
-        const int64_t aim = std::min<int64_t>(std::max<int64_t>(4096 / std::max<int64_t>(each, 1), 1), 64);
+    // As many chunks as make `want` workgroups, 64 of a row at most (a lane has one each), of two passes at least.  64 requests of 5 rows
+    // of 128,001: the rows' weights in 2,048 and 4,096 25.4 and 22.0 us, the draws, of which two fit a unit, in 512 and 1,024 32 and 36.
+    auto cut = [&](int64_t each, int &chunks, int &passes, int64_t want) {
+        const int64_t aim = std::min<int64_t>(std::max<int64_t>(want / std::max<int64_t>(each, 1), 1), 64);
         passes = (int)std::max<int64_t>(2, (d.vocab + aim * kVerifyPass - 1) / (aim * kVerifyPass));
         chunks = (d.vocab + passes * kVerifyPass - 1) / (passes * kVerifyPass);
     };
-    cut(rows * (d.draft ? 2 : 1), s.chunks, s.passes);
-    cut(d.requests, s.draw_chunks, s.draw_passes);
+    cut(rows * (d.draft ? 2 : 1), s.chunks, s.passes, 4096);
+    cut(d.requests, s.draw_chunks, s.draw_passes, 512);
     int64_t at = VerifyShape::kCounterBytes;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
