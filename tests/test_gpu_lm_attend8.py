@@ -65,6 +65,19 @@ def test_scales_and_large_values():
     A.test_scales_and_large_values()
 
 
+@pytest.mark.parametrize("scale", [0.0, 1e-20, -1e-30])
+def test_keys_of_zeros_at_scales_near_zero(scale):
+    """A block of zeros has the least scale, 2^-100: its product with the call's is none that f32 has."""
+    p = A.problem(17, 64, 32, 4, 2, [150, 70], [60, 70], "bf16")
+    for b, t in ((0, 96), (1, 32), (1, 64)):
+        for h in range(2):
+            k, _, scales = S.parts(p["cache"][p["table"][b, t // 32], h], 32, 64)
+            k[:] = 0
+            scales[0, 0] = 2.0 ** -100
+    A.check(p, scale=scale)
+    A.check(p, scale=scale, window=33)
+
+
 def test_page_ids_out_of_range_are_skipped():
     p = A.problem(13, 128, 32, 4, 2, [100, 50], [1, 3], "bf16")
     p["table"][0, 2], p["table"][1, 0] = -1, len(p["cache"])
