@@ -13,6 +13,7 @@
 namespace pklm {
 
 constexpr int kNever = 0x7FFFFFFF;
+constexpr float kMostLogit = 0x1.fffffep127f;         // +inf counts as this
 
 // One row's weights: the logits' largest, log2(e) / T, and where the largest alone counts its place.
 struct RowWeights {
@@ -27,7 +28,7 @@ struct RowWeights {
         to_log2 = fminf(fmaxf(1.4426950408889634f / (greedy ? 1.0f : t), 1e-38f), 3e38f);
     }
     // a row of -inf has no weight, in one with +inf those are alike
-    __device__ void largest(float x) { top = x == -INFINITY ? 0.0f : fminf(x, 0x1.fffffep127f); }
+    __device__ void largest(float x) { top = x == -INFINITY ? 0.0f : fminf(x, kMostLogit); }
     // exp2 of one rounded product: off by 2^-23 and 2^-24 of the exponent, 2^-19 of itself where weights end.  (The library's expf takes
     // half as long again: weights are what bounds long rows.)  The median of -200, 0 and the exponent is -200 for -inf and NaN.
     __device__ float weight_f(float x, int i) const {
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         for (int q = 0; q < kSources; ++q) {
             int at = kNever;
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e) at = fminf(x[q][e], 0x1.fffffep127f) == rw[q].top ? index(e / 8) + e % 8 : at;
+            for (int e = E - 1; e >= 0; --e) at = fminf(x[q][e], kMostLogit) == rw[q].top ? index(e / 8) + e % 8 : at;
             at = wave_min(at);
             if (lane == 0) s_at[q][wave] = at;
         }
@@ -349,10 +350,11 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_max_kernel(pk_verify_de
 #pragma unroll
         for (int p = 0; p < 2; ++p)
             x[p].each(i[p], V, [&](int e, float v) {
-                if (rw.greedy && v > top) at = i[p] + e;
+                if (rw.greedy && v > top && top < kMostLogit) at = i[p] + e;
                 top = fmaxf(top, v);
             });
     }
+    top = fminf(top, kMostLogit);
     const float wave_top = wave_max(top);
     at = rw.greedy ? wave_min(top == wave_top ? at : kNever) : kNever;
     if ((tid & 63) == 0) s_max[tid >> 6] = wave_top, s_at[tid >> 6] = at;

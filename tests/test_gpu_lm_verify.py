@@ -173,6 +173,16 @@ def test_greedy_rows_take_the_first_largest():
                 assert list(out) == want and acc[0] == (2 if d == 5 else 0) and prob[0] == 1
 
 
+@pytest.mark.parametrize("V", [70, 20000, 70000])
+def test_infinite_logits_count_as_the_largest_number(V):
+    x = np.zeros((2, V), np.float32)
+    x[:, 9], x[:, 12], x[:, V - 1] = np.inf, np.finfo(np.float32).max, np.inf
+    assert list(call(x, None, [0, 9], [0, 2], [0.5] * 2, [0.99], t=[0.0])[0]) == [9, 9]
+    x[:, 9], x[:, 12] = np.finfo(np.float32).max, np.inf
+    assert list(call(x, None, [0, 9], [0, 2], [0.5] * 2, [0.99], t=[0.0])[0]) == [9, 9]
+    assert list(call(x, None, [0, 12], [0, 2], [0.3] * 2, [0.4])[0]) == [12, 12]
+
+
 def test_counts_cut_first_and_out_of_range_offsets():
     V = 30
     x = np.zeros((6, V), np.float32)
