@@ -6,6 +6,8 @@
 // numbers again, whose sum is at most 2^52 and a half step for each token.
 #pragma once
 
+#include <type_traits>
+
 #include "lm_common.h"
 #include "lm_sample.h"
 #include "parakeet_lm.h"
@@ -207,11 +209,13 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         if (tid == 0) s_verdict = RowVerdict{ok, ok ? d : -1, ok ? (float)p_draft : 0.0f, 0};
     } else {
         // what is left to draw from
-        u64 left[E], mass = 0;
+        std::conditional_t<Draft, u64, unsigned> left[E];
+        u64 mass = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             left[e] = w[0][e];
-            if (drafted) left[e] = Draft ? left_of(rw[0].share_of(w[0][e]), rw[1].share_of(w[kSources - 1][e])) : index(e / 8) + e % 8 == d ? 0 : left[e];
+            if (drafted && Draft) left[e] = left_of(rw[0].share_of(w[0][e]), rw[1].share_of(w[kSources - 1][e]));
+            if (drafted && !Draft) left[e] = index(e / 8) + e % 8 == d ? 0 : left[e];
             mass += left[e];
         }
         mass = wave_sum(mass);

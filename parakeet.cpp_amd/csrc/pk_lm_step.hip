@@ -1,5 +1,5 @@
 // pk_lm_step.hip -- host side + C ABI of parakeet_lm.h's operators of a step with drafted tokens: norms and rotation, the
-// 8-bit cache, attention over it, verification.  The kernels are in lm_rope.h, lm_cache8.h, lm_attend.h and lm_verify.h.
+// 8-bit cache, attention over it, verification.  The kernels are in lm_rope.h, lm_cache8.h, lm_attend8.h and lm_verify.h.
 
 #include <hip/hip_runtime.h>
 
@@ -55,11 +55,13 @@ struct TurnGrid {
     int rows, parts;
     int64_t groups;
 };
-// As many rows as leave 1,024 workgroups, whole blocks where there are many, then parts of the heads as long as that gives more than
-// 2,048 workgroups or a part for each.
+// As many rows as leave 128 groups of them, whole blocks where that is more than half a block; beside each, as many parts of the heads as
+// make 2,048 workgroups.  32 heads on 8 x 128 in bf16, microseconds where 1,024, 128 and 32 groups are left: 1,000 rows normed
+// and turned 12.2, 9.8, 11.1; 4 x 200 appended 21.8, 14.7, 13.4, 4 x 1,000 56, 24, 24; a token of 64 sessions 7.4, 7.5, 10.9.  With parts
+// up to 1,024, 2,048 and 4,096 workgroups: 16,385 rows 90, 73, 77, 4 x 200 appended 17.4, 14.7, 14.8.
 TurnGrid turn_grid(int n_rows, int parts, int least) {
     TurnGrid g;
-    g.rows = (int)std::min<int64_t>(std::max<int64_t>(n_rows / 1024, least), kTurnRows);
+    g.rows = (int)std::min<int64_t>(std::max<int64_t>(n_rows / 128, least), kTurnRows);
     if (g.rows > kTurnRows / 2) g.rows = kTurnRows;
     g.groups = ((int64_t)n_rows + g.rows - 1) / g.rows;
     g.parts = (int)std::min<int64_t>(std::max<int64_t>((2048 + g.groups - 1) / g.groups, 1), std::max(parts, 1));
@@ -86,6 +88,9 @@ struct HostKv8 {
     static bool has_prompt(int, int) { return true; }
     static int prompt_cols(int) { return kPromptCols; }
     static int prompt_groups(int) { return kPromptGroups; }
+    // Two tiles that share each key's operands, where registers hold them.  32 heads on 8 x 128 in bf16, in one tile and in two: 64
+    // sessions' 5 tokens (20 rows) on up to 4,097 keys 94 and 65 us, 4 x 20 tokens on 8,191 keys 39 and 24, 64 x 20 on 1,000 keys 47 and
+    // 47; but one session's 6 tokens on 8,191 keys, whose splits do not fill the card, 13 and 17.
     static int tile_cols(int64_t rows, int dim) { return rows <= 16 || dim == 256 ? 16 : 32; }
 };
 
@@ -99,7 +104,10 @@ void launch_attend8(const AttendParams &p, const AttendShape &sh, int dim, unsig
     });
 }
 
-// Verification.  Rows of up to kVerifyVocab logits are a workgroup's each, in one launch; longer ones are cut in chunks.
+// Verification.  Rows of up to kVerifyVocab logits are a workgroup's each, in one launch, 16 tokens a lane at most; longer ones, which
+// no workgroup's registers hold, are cut in chunks.  f32 rows of 16,384 logits with draft logits, 5 and 1,280 of them, take 11 and 34 us in
+// one launch, 23 and 44 in three.  Fewer threads make room for more rows: 1,280 rows of 4,001 take 12 us on 512 threads each, 26 on
+// 1,024, of 8,001 19 and 28; 5 rows of 4,001 7.4 and 9.1.
 constexpr int kVerifyVocab = 16384;
 
 struct VerifyShape {
@@ -161,7 +169,8 @@ void launch_verify_rows(const pk_verify_desc &d, hipStream_t s) {
 template <class T>
 void launch_verify(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s) {
     if (d.vocab <= 2048) return launch_verify_rows<T, 256, 1>(d, s);
-    if (d.vocab <= 8192) return launch_verify_rows<T, 1024, 1>(d, s);
+    if (d.vocab <= 4096) return launch_verify_rows<T, 512, 1>(d, s);
+    if (d.vocab <= 8192) return launch_verify_rows<T, 512, 2>(d, s);
     if (d.vocab <= kVerifyVocab) return launch_verify_rows<T, 1024, 2>(d, s);
     char *w = (char *)d.workspace;
     SplitVerify p;
