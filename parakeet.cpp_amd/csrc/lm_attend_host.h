@@ -1,8 +1,7 @@
 // lm_attend_host.h -- host side of attention over a paged cache (pk_kv4_attend, pk_kv8_attend): checks, the choice of kernel and
 // how a call's work is dealt out.  C is the cache's kind, as in lm_attend.h, with what the host asks of it:
 //   check(...)            of a call's cache
-//   has_prompt(dtype, D)  whether its kernel for prompts takes it
-//   prompt_cols(D), prompt_groups(D)   query rows of that kernel's workgroup; as many of them are worth it
+//   prompt(call, rows, groups)   whether its kernel for prompts takes a call of `rows` to a request and kv head, in so many workgroups
 //   tile_cols(rows, D)    query rows of the other kernel's workgroup, of `rows` of a request and kv head
 #pragma once
 
@@ -19,22 +18,6 @@ namespace pklm {
 // no call's partial sums lie where another's counters are.  A split call has at most kSplitWork tiles times splits, and
 // a tile 1 + (splits + 15) / 16 counters.
 constexpr int kSplitWork = 512, kCounters = 4 * kSplitWork;
-// attend_prompt_kernel takes calls of more than kPromptRows query rows to a request and kv head that give it kPromptGroups
-// workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  The host has
-// bounds alone: where requests stay below them, workgroups stay empty and the others' keys make a tail.  32 heads on 8 of 128
-// channels in bf16, requests x new tokens on up to 8,191 keys, microseconds of the prompt kernel and of the other:
-//   workgroups             256                           512                                      1,024
-//   requests all alike     2 x 512: 226, 231             4 x 512: 278, 462; 16 x 128: 307, 512
-//   lengths spread evenly  4 x 256: 225, 132             4 x 512: 244, 224; 16 x 128: 233, 186    4 x 1,024: 314, 400
-//   one request            1 x 1,024: 224, 223           1 x 2,048: 269, 412                      1 x 4,096: 435, 709
-//   without keys held      4 x 256: 18, 21               4 x 512: 25, 42; 16 x 128: 17, 31
-// f16 at 512, 16 x 128: alike 486, 660; spread, on 6,000 keys 264, 175.  bf16 rows of 256 channels at 512, 4 x 512: alike 803,
-// 952; spread, on 6,000 keys 399, 365.  So 512 costs up to half where lengths are spread on long axes, and a higher
-// bound would cost as much or more where they are not.  64 requests of spread lengths on up to 2,047 keys: 64 rows each 69
-// and 43, 96 rows 69 and 55, 128 rows 70 and 70.  Not f16 rows of 256, which its registers do not hold: two requests of up
-// to 1,024 new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
-constexpr int kPromptRows = 128, kPromptGroups = 512;
-
 // How a call's work is dealt out, from its host-known sizes alone.
 struct AttendShape {
     bool prompt;             // the kernel for prompts; else the one that splits a long axis
@@ -47,14 +30,14 @@ struct AttendShape {
 template <class C>
 int attend_shape(const char *what, const pk_kv4_attend_desc &d, AttendShape &s) {
     const int64_t rows = (int64_t)d.max_new * (d.heads / d.kv_heads), pairs = (int64_t)d.requests * d.kv_heads;
-    const int64_t prompt_tiles = (rows + C::prompt_cols(d.head_dim) - 1) / C::prompt_cols(d.head_dim);
+    const int64_t prompt_tiles = (rows + kPromptCols - 1) / kPromptCols;
     auto too_many = [&] {
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %lld requests x kv heads of %lld query rows in one call", what, (long long)pairs,
                        (long long)rows);
     };
     if (pairs > most_groups(kPromptThreads)) return too_many();
-    s.prompt = rows > kPromptRows && pairs * prompt_tiles >= C::prompt_groups(d.head_dim) && C::has_prompt(d.dtype, d.head_dim);
-    s.cols = s.prompt ? C::prompt_cols(d.head_dim) : C::tile_cols(rows, d.head_dim);
+    s.prompt = C::prompt(d, rows, pairs * prompt_tiles);
+    s.cols = s.prompt ? kPromptCols : C::tile_cols(rows, d.head_dim);
     const int64_t tiles = (rows + s.cols - 1) / s.cols, step = 32 * kAttendWaves;
     // keys of one tile: its rows span at most as many tokens
     const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + s.cols + 64) : d.max_len;

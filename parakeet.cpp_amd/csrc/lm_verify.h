@@ -283,7 +283,10 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
 // that refuses its draft alone, what each chunk has left to draw from, of which the request's last chunk to arrive draws.
 // A launch's workgroups work out for themselves what follows from the launch before.
 
-constexpr int kVerifyThreads = 512, kVerifyWaves = kVerifyThreads / 64, kVerifyPass = 8 * kVerifyThreads;
+// Of the first two launches, and of the draws, whose workgroups each find the row that they draw from: 256 and 512 threads.  (64 requests of up
+// to 5 rows of 128,001 in bf16 with draft logits on 256, 512 and 1,024: 24, 28, 35 us the two, 29, 21, 27 the draws.)
+constexpr int kVerifyThreads = 256, kVerifyWaves = kVerifyThreads / 64, kVerifyPass = 8 * kVerifyThreads;
+constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64, kDrawPass = 8 * kDrawThreads;
 
 struct SplitVerify {
     float *chunk_max;       // [rows][2][chunks], of the target and of the draft
@@ -292,7 +295,7 @@ struct SplitVerify {
     u64 *left;              // [requests][chunks]
     int *arrived;           // [requests], zero between calls
     int chunks, passes, sources;        // a chunk is passes * kVerifyPass tokens, a wave's part of it in one run
-    int draw_chunks, draw_passes;       // likewise, of the one row of a request that is drawn from
+    int draw_chunks, draw_passes;       // likewise, with kDrawPass, of the one row of a request that is drawn from
 };
 
 // A workgroup's chunk of a row: (request, row of it, source).
@@ -311,9 +314,10 @@ __device__ inline const typename T::Raw *verify_row(const pk_verify_desc &a, int
     using Raw = typename T::Raw;
     return q ? (const Raw *)a.draft + (int64_t)r * a.draft_row : (const Raw *)a.logits + (int64_t)r * a.logits_row;
 }
-// The first token of this lane in a pass of a chunk.
+// The first token of this lane in a pass of a chunk of so many waves.
+template <int Waves>
 __device__ inline int verify_token(int passes, int chunk, int pass) {
-    return ((chunk * kVerifyWaves + (int)(threadIdx.x >> 6)) * passes + pass) * 512 + (int)(threadIdx.x & 63) * 8;
+    return ((chunk * Waves + (int)(threadIdx.x >> 6)) * passes + pass) * 512 + (int)(threadIdx.x & 63) * 8;
 }
 
 // A row's rule, from its chunks' maxima, and its weight where the chunks have theirs: by a whole wave.
@@ -350,7 +354,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_max_kernel(pk_verify_de
         Tokens8<T> x[2];
         int i[2];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) i[p] = p0 + p < w.passes ? verify_token(w.passes, c.chunk, p0 + p) : V, x[p].load(row, i[p], V);
+        for (int p = 0; p < 2; ++p) i[p] = p0 + p < w.passes ? verify_token<kVerifyWaves>(w.passes, c.chunk, p0 + p) : V, x[p].load(row, i[p], V);
 #pragma unroll
         for (int p = 0; p < 2; ++p)
             x[p].each(i[p], V, [&](int e, float v) {
@@ -383,14 +387,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(pk_verify_de
     const int tid = threadIdx.x, V = a.vocab;
     const int64_t place = (int64_t)c.b * a.max_new + c.j;
     Tokens8<T> x;
-    x.load(row, verify_token(w.passes, c.chunk, 0), V);       // on its way while the rule is worked out
+    x.load(row, verify_token<kVerifyWaves>(w.passes, c.chunk, 0), V);       // on its way while the rule is worked out
     RowWeights rw;
     row_rule(a, w, c.b, place, c.q, rw, false);
     u64 sum = 0;
     for (int p = 0; p < w.passes; ++p) {
-        const int i = verify_token(w.passes, c.chunk, p);
+        const int i = verify_token<kVerifyWaves>(w.passes, c.chunk, p);
         Tokens8<T> y;
-        y.load(row, p + 1 < w.passes ? verify_token(w.passes, c.chunk, p + 1) : V, V);
+        y.load(row, p + 1 < w.passes ? verify_token<kVerifyWaves>(w.passes, c.chunk, p + 1) : V, V);
         unsigned two = 0;                              // of at most 2^30 each
         x.each(i, V, [&](int e, float v) {
             two += rw.weight(v, i + e);
@@ -408,8 +412,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(pk_verify_de
 }
 
 template <class T>
-__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_desc a, SplitVerify w) {
-    __shared__ u64 s_sum[kVerifyWaves], s_base;
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(pk_verify_desc a, SplitVerify w) {
+    __shared__ u64 s_sum[kDrawWaves], s_base;
     __shared__ int s_stop[2], s_flag, s_chunk;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab;
     const int b = blockIdx.x / w.draw_chunks, chunk = blockIdx.x % w.draw_chunks;
@@ -437,7 +441,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
     if (tid < 2) s_stop[tid] = kNever;
     __syncthreads();
     int stop = kNever;
-    for (int j0 = 0, round = 0; stop == kNever; j0 += kVerifyWaves, round ^= 1) {      // ends: the last row has no draft
+    for (int j0 = 0, round = 0; stop == kNever; j0 += kDrawWaves, round ^= 1) {      // ends: the last row has no draft
         const int j = j0 + wave, d = j < rows.n ? rows.draft(a, j) : -1;
         double p = 0, q = 1;
         if (d >= 0) p = shares(j, d, q);
@@ -451,7 +455,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
         }
     }
     if (chunk == 0) {
-        for (int j = stop + 1 + tid; j < rows.n; j += kVerifyThreads) {
+        for (int j = stop + 1 + tid; j < rows.n; j += kDrawThreads) {
             a.out[rows.begin + j] = -1;
             if (a.prob) a.prob[rows.begin + j] = 0.0f;
         }
@@ -470,12 +474,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
         Tokens8<T> x, y;
     };
     auto load_pass = [&](int ch, int pass, bool any, Pass &of) {
-        const int i = pass < w.draw_passes ? verify_token(w.draw_passes, ch, pass) : V;
+        const int i = pass < w.draw_passes ? verify_token<kDrawWaves>(w.draw_passes, ch, pass) : V;
         of.x.load(x_row, i, V);
         if (two && !any) of.y.load(y_row, i, V);
     };
     auto left_of_pass = [&](int ch, int pass, bool any, const Pass &of, double (&left)[8]) {
-        const int i = verify_token(w.draw_passes, ch, pass);
+        const int i = verify_token<kDrawWaves>(w.draw_passes, ch, pass);
         of.x.each(i, V, [&](int e, float v) { left[e] = (double)target.weight_f(v, i + e); });
         if (any || !drafted) return;
         if (two)
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
         __syncthreads();
         if (tid == 0) {
             u64 s = 0;
-            for (int v = 0; v < kVerifyWaves; ++v) s += s_sum[v];
+            for (int v = 0; v < kDrawWaves; ++v) s += s_sum[v];
             put_shared(&w.left[(int64_t)b * w.draw_chunks + chunk], s);
         }
     }
@@ -536,7 +540,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
         if (lane == 0) s_sum[wave] = mass;
         __syncthreads();
         u64 of_chunk = 0;
-        for (int v = 0; v < kVerifyWaves; ++v) of_chunk += s_sum[v];
+        for (int v = 0; v < kDrawWaves; ++v) of_chunk += s_sum[v];
         if (t < lead + of_chunk || ch + 1 >= w.draw_chunks) break;
         lead += of_chunk;
         __syncthreads();
@@ -554,7 +558,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(pk_verify_d
         const u64 run = wave_scan(own), sum = lane_value(run, 63);
         u64 at = lead + run - own;
         if (at <= t && t < at + own) {
-            const int i0 = verify_token(w.draw_passes, ch, p);
+            const int i0 = verify_token<kDrawWaves>(w.draw_passes, ch, p);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (at <= t && t < at + (u64)left[e]) {

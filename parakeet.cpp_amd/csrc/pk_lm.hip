@@ -159,13 +159,29 @@ void launch_sample(const pk_sample_desc &d, const SampleShape &sh, hipStream_t s
     }
 }
 
+// attend_prompt_kernel takes calls of more than kPromptRows query rows to a request and kv head that give it kPromptGroups
+// workgroups or more, which the card holds at a time; attend_kernel splits long axes and takes the others.  The host has
+// bounds alone: where requests stay below them, workgroups stay empty and the others' keys make a tail.  32 heads on 8 of 128
+// channels in bf16, requests x new tokens on up to 8,191 keys, microseconds of the prompt kernel and of the other:
+//   workgroups             256                           512                                      1,024
+//   requests all alike     2 x 512: 226, 231             4 x 512: 278, 462; 16 x 128: 307, 512
+//   lengths spread evenly  4 x 256: 225, 132             4 x 512: 244, 224; 16 x 128: 233, 186    4 x 1,024: 314, 400
+//   one request            1 x 1,024: 224, 223           1 x 2,048: 269, 412                      1 x 4,096: 435, 709
+//   without keys held      4 x 256: 18, 21               4 x 512: 25, 42; 16 x 128: 17, 31
+// f16 at 512, 16 x 128: alike 486, 660; spread, on 6,000 keys 264, 175.  bf16 rows of 256 channels at 512, 4 x 512: alike 803,
+// 952; spread, on 6,000 keys 399, 365.  So 512 costs up to half where lengths are spread on long axes, and a higher
+// bound would cost as much or more where they are not.  64 requests of spread lengths on up to 2,047 keys: 64 rows each 69
+// and 43, 96 rows 69 and 55, 128 rows 70 and 70.  Not f16 rows of 256, which its registers do not hold: two requests of up
+// to 1,024 new tokens, 24 heads on 8 (384), 314 and 240 on up to 2,047 keys, 1,067 and 602 on 6,000.
+constexpr int kPromptRows = 128, kPromptGroups = 512;
+
 struct HostKv4 {
     static int check(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
         return check_cache(what, cache, page_stride, page, n_pages, heads, dim);
     }
-    static bool has_prompt(int dtype, int dim) { return !(dtype == PK_DTYPE_F16 && dim == 256); }
-    static int prompt_cols(int) { return kPromptCols; }
-    static int prompt_groups(int) { return kPromptGroups; }
+    static bool prompt(const pk_kv4_attend_desc &d, int64_t rows, int64_t groups) {
+        return rows > kPromptRows && groups >= kPromptGroups && !(d.dtype == PK_DTYPE_F16 && d.head_dim == 256);
+    }
     static int tile_cols(int64_t, int) { return 16; }
 };
 

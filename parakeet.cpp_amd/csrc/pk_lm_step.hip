@@ -85,9 +85,23 @@ struct HostKv8 {
     static int check(const char *what, const void *cache, int64_t page_stride, int page, int n_pages, int heads, int dim) {
         return check_cache8(what, cache, page_stride, page, n_pages, heads, dim);
     }
-    static bool has_prompt(int, int) { return true; }
-    static int prompt_cols(int) { return kPromptCols; }
-    static int prompt_groups(int) { return kPromptGroups; }
+    // The prompt kernel does not split keys: it takes calls that fill the card with workgroups, or half of it where no request has many
+    // more keys than new tokens; rows of 256 channels, which the other kernel takes 16 columns at a time, from a quarter on.  32 heads
+    // on 8 in bf16, lengths spread evenly, new tokens on up to so many keys, microseconds of the other kernel and of it:
+    //   workgroups         128 channels                            64 channels                           256 channels
+    //   128                512 on 8,191: 123, 199; on 512: 21, 20                                        512 on 8,191: 482, 391
+    //   256                4 x 256 on 8,191: 149, 207;             94, 157;                              514, 394
+    //                      on 2,047: 58, 56; on 512: 31, 20        37, 44; 18, 16
+    //   512                4 x 512 on 8,191: 258, 259;             159, 199;                             970, 567
+    //                      64 x 24 on 2,047: 75, 72                42, 56                                232, 214
+    //   1,024              4 x 1,024 on 8,191: 471, 336            275, 258                              1,832, 894
+    // 64 x 16 on 2,047, half a tile's rows, at 128 channels: 61, 73.
+    static bool prompt(const pk_kv4_attend_desc &d, int64_t rows, int64_t groups) {
+        const int64_t keys = d.window ? std::min<int64_t>(d.max_len, (int64_t)d.window + d.max_new) : d.max_len;
+        if (rows < 96) return false;
+        if (d.head_dim == 256) return groups >= 128;
+        return groups >= (d.head_dim == 64 ? 1024 : 512) || (groups >= 256 && keys <= (d.head_dim == 64 ? 2 : 8) * (int64_t)d.max_new);
+    }
     // Two tiles that share each key's operands, where registers hold them.  32 heads on 8 x 128 in bf16, in one tile and in two: 64
     // sessions' 5 tokens (20 rows) on up to 4,097 keys 94 and 65 us, 4 x 20 tokens on 8,191 keys 39 and 24, 64 x 20 on 1,000 keys 47 and
     // 47; but one session's 6 tokens on 8,191 keys, whose splits do not fill the card, 13 and 17.
@@ -124,15 +138,16 @@ VerifyShape verify_shape(const pk_verify_desc &d) {
         s.bytes = VerifyShape::kCounterBytes + rows * (int64_t)sizeof(RowVerdict);
         return s;
     }
-    // As many chunks as make `want` workgroups, 64 of a row at most (a lane has one each), of two passes at least.  64 requests of 5 rows
-    // of 128,001: the rows' weights in 2,048 and 4,096 25.4 and 22.0 us, the draws, of which two fit a unit, in 512 and 1,024 32 and 36.
-    auto cut = [&](int64_t each, int &chunks, int &passes, int64_t want) {
+    // As many chunks as make `want` workgroups, 64 of a row at most (a lane has one each), of two passes at least.  Requests of up to 5 rows
+    // of 128,001 in bf16 with draft logits: the first two launches in 2,048, 4,096, 8,192 and 16,384 take 31, 23, 25, 27 us for 64, 12.3, 13.5,
+    // 11.3, 11.5 for 16; the draws of 64, of which two fit a unit, in 256, 512 and 1,024 28, 21, 27.
+    auto cut = [&](int64_t each, int &chunks, int &passes, int64_t want, int pass) {
         const int64_t aim = std::min<int64_t>(std::max<int64_t>(want / std::max<int64_t>(each, 1), 1), 64);
-        passes = (int)std::max<int64_t>(2, (d.vocab + aim * kVerifyPass - 1) / (aim * kVerifyPass));
-        chunks = (d.vocab + passes * kVerifyPass - 1) / (passes * kVerifyPass);
+        passes = (int)std::max<int64_t>(2, (d.vocab + aim * pass - 1) / (aim * pass));
+        chunks = (d.vocab + passes * pass - 1) / (passes * pass);
     };
-    cut(rows * (d.draft ? 2 : 1), s.chunks, s.passes, 4096);
-    cut(d.requests, s.draw_chunks, s.draw_passes, 512);
+    cut(rows * (d.draft ? 2 : 1), s.chunks, s.passes, 8192, kVerifyPass);
+    cut(d.requests, s.draw_chunks, s.draw_passes, 512, kDrawPass);
     int64_t at = VerifyShape::kCounterBytes;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -181,7 +196,7 @@ void launch_verify(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s
     const unsigned grid = (unsigned)(d.requests * d.max_new * p.sources * p.chunks);
     verify_max_kernel<T><<<grid, kVerifyThreads, 0, s>>>(d, p);
     verify_sum_kernel<T><<<grid, kVerifyThreads, 0, s>>>(d, p);
-    verify_draw_kernel<T><<<(unsigned)(d.requests * p.draw_chunks), kVerifyThreads, 0, s>>>(d, p);
+    verify_draw_kernel<T><<<(unsigned)(d.requests * p.draw_chunks), kDrawThreads, 0, s>>>(d, p);
 }
 
 }  // namespace
