@@ -211,20 +211,22 @@ typedef struct pk_kv8_append_desc {
 PK_API int pk_kv8_append(const pk_kv8_append_desc *desc, void *stream);
 
 /* As pk_kv4_load and pk_kv4_attend, over the 8-bit cache.  Values at NaN codes are NaN; f16 results give held values of
- * 65,536, to which rows over 63,488 may be rounded, as 65,504. */
+ * 65,536, to which rows over 63,488 may be rounded, as 65,504.  Scores are f32 sums of exact products.  Probabilities go
+ * to the values in f16, 11 bits down to 2^-28 of a query's largest, values exactly down to 2^-22 of the largest block. */
 PK_API int pk_kv8_load(const pk_kv4_rows_desc *desc, void *stream);
 PK_API int pk_kv8_attend(const pk_kv4_attend_desc *desc, void *stream);
 PK_API int pk_kv8_attend_workspace(const pk_kv4_attend_desc *desc, int64_t *bytes);
 
 /* Drafted tokens.  Request b brought the tokens tokens[first[b] .. first[b + 1]) to the target: the last one that it had and
  * the drafts behind it.  Row r of logits is what the target says behind tokens[r]; its draft is tokens[r + 1], the last row
- * has none.  With the weights w of pk_sample (whole numbers, at the request's temperature) p = w / sum w; of draft logits,
- * at draft_temperature, likewise q; without draft logits q is 1 at the draft.  Drafts are accepted, first to last, while
- * u[r] q < p at the draft.  The token behind the accepted ones is drawn with u_draw[b] by rising index as pk_sample does:
+ * has none.  With weights w = round(2^30 exp((x - max) / T)) at the request's temperature (pk_sample's, but for the
+ * last bits of the exponential) p = w / sum w; of draft logits, at draft_temperature, likewise q; without draft logits q is
+ * 1 at the draft.  Drafts are accepted, first to last, while u[r] q < p at the draft.  The token behind the accepted ones is drawn with u_draw[b] by rising index as pk_sample does:
  * behind the last draft from p; where a draft was refused from max(p - q, 0) in steps of 2^-52 (without draft logits from p
  * less the draft), or from p where that leaves nothing.  So the tokens are distributed as if drawn from p one by one.  Tokens
  * that a filter bars are given as -inf.  All in whole numbers and single f64 steps: no result depends on the order of a sum.
- * A draft outside the vocabulary is refused, and the token then drawn from p; a row of -inf accepts nothing and gives -1. */
+ * A draft outside the vocabulary is refused, and the token then drawn from p; a row of -inf accepts nothing and gives -1.
+ * NaN counts as -inf, +inf as the largest number. */
 typedef struct pk_verify_desc {
     const void *logits;                 /* [n_rows][vocab], rows logits_row apart */
     const void *draft;                  /* [n_rows][vocab], rows draft_row apart, of the same type: what draft tokens[r + 1] was drawn

@@ -157,9 +157,9 @@ __device__ inline void load_weights(const float *weight, const LaneChannels<D> &
 // a time leaves too little on its way: 16,385 rows of 32 + 8 heads x 128, 8-byte partners through shuffles, took 104 us, 4 at a time 88.)
 template <class T, int D, int Batch, class Turn>
 __device__ inline void turn_some(const typename T::Raw *x, int64_t x_row, bool wide, typename T::Raw *y, int64_t y_row, bool y_wide,
-                                 const float (&w)[8], const Turn &turn, const TurnTable<D> &table, int64_t row0, int n) {
+                                 const float (&w)[8], const Turn &turn, const TurnTable<D> &table, int64_t row0, int n, int lane) {
     constexpr int kLanes = D / 8, kRows = 64 / kLanes;
-    const int lane = threadIdx.x & 63, c = lane % kLanes;
+    const int c = lane % kLanes;
     const LaneChannels<D> at(c, Turn::halves);
     for (int r0 = 0; r0 < n; r0 += kRows * Batch) {
         float v[Batch][8];
@@ -182,34 +182,42 @@ __device__ inline void turn_some(const typename T::Raw *x, int64_t x_row, bool w
 }
 template <class T, int D, int Batch, class Turn>
 __device__ inline void turn_rows(const typename T::Raw *x, int64_t x_row, bool wide, typename T::Raw *y, int64_t y_row, bool y_wide,
-                                 const float *weight, const Turn &turn, const TurnTable<D> &table, int64_t row0, int n) {
+                                 const float *weight, const Turn &turn, const TurnTable<D> &table, int64_t row0, int n, int lane) {
     float w[8];
-    load_weights(weight, LaneChannels<D>((threadIdx.x & 63) % (D / 8), Turn::halves), w);
-    if (n <= 512 / D) turn_some<T, D, 1>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n);
-    else turn_some<T, D, Batch>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n);
+    load_weights(weight, LaneChannels<D>(lane % (D / 8), Turn::halves), w);
+    if (n <= 512 / D) turn_some<T, D, 1>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n, lane);
+    else turn_some<T, D, Batch>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n, lane);
 }
 
-// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms take 74.6 us, 3.9 TB/s, where a
-// large copy reaches 5.2: 2 passes' loads a wave, 8 waves a vector unit (4 passes, of which 5 fit, 82.5).  One row of 16 heads takes 3.0 us,
-// a launch and the sines.
+// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms take 60 us, 4.9 TB/s, where a
+// large copy reaches 5.2: 4 passes' loads a wave of 16-bit types (2: 65; at 64 channels, where 4 are all rows, 28.5 and 29.6; f32 has no
+// registers for them), 8 waves a vector unit.  One row of 16 heads takes 3 us, a launch and the sines.
 template <class T, int D, bool Halves>
-__global__ __launch_bounds__(kTurnThreads, !Halves ? 4 : D == 256 ? 5 : 8) void rope_kernel(pk_qk_rope_desc a, int rows, int wide_q, int wide_k) {
+__global__ __launch_bounds__(kTurnThreads, !Halves || D == 256 ? 4 : 8) void rope_kernel(pk_qk_rope_desc a, int rows, int wide_q, int wide_k) {
     using Raw = typename T::Raw;
     __shared__ TurnTable<D> s_table;
     const Turn<Halves> turn{a.inv_freq, a.pos, a.rot_dim, a.norm, a.interleaved, a.eps};
     const int64_t row0 = (int64_t)blockIdx.x * rows;
     const int n = (int)min((int64_t)rows, a.n_rows - row0), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (a.rot_dim) {
+        // a padded call's last workgroups, all of whose rows are left out, read none
+        const bool live = turn.live(row0 + min((int)(threadIdx.x & 63), n - 1));
         s_table.fill(turn, row0, n);
+        if (!__any(live)) return;
         __syncthreads();
     }
+    constexpr int kBatch = sizeof(Raw) == 2 && D > 64 ? 4 : 2;
     for (int u = blockIdx.y * kTurnWaves + wave; u < a.heads + a.kv_heads; u += gridDim.y * kTurnWaves) {
+        // what follows from the lane is worked out behind this, not in front of the angles and the loop, over which it would be spilled:
+        // with 2 passes 48 registers instead of 62 and 10 spilled, 215 rows 4.2 us, not 5.7
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
         if (u < a.heads)
-            turn_rows<T, D, 2>((const Raw *)a.q + u * a.q_head, a.q_row, wide_q & 1, (Raw *)a.q_out + u * a.q_out_head, a.q_out_row, wide_q & 2,
-                            a.q_weight, turn, s_table, row0, n);
+            turn_rows<T, D, kBatch>((const Raw *)a.q + u * a.q_head, a.q_row, wide_q & 1, (Raw *)a.q_out + u * a.q_out_head, a.q_out_row, wide_q & 2,
+                            a.q_weight, turn, s_table, row0, n, lane);
         else
-            turn_rows<T, D, 2>((const Raw *)a.k + (u - a.heads) * a.k_head, a.k_row, wide_k & 1, (Raw *)a.k_out + (u - a.heads) * a.k_out_head,
-                            a.k_out_row, wide_k & 2, a.k_weight, turn, s_table, row0, n);
+            turn_rows<T, D, kBatch>((const Raw *)a.k + (u - a.heads) * a.k_head, a.k_row, wide_k & 1, (Raw *)a.k_out + (u - a.heads) * a.k_out_head,
+                            a.k_out_row, wide_k & 2, a.k_weight, turn, s_table, row0, n, lane);
     }
 }
 

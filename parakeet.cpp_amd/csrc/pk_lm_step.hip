@@ -57,8 +57,8 @@ struct TurnGrid {
 };
 // As many rows as leave 128 groups of them, whole blocks where that is more than half a block; beside each, as many parts of the heads as
 // make 2,048 workgroups.  32 heads on 8 x 128 in bf16, microseconds where 1,024, 128 and 32 groups are left: 1,000 rows normed
-// and turned 12.2, 9.8, 11.1; 4 x 200 appended 21.8, 14.7, 13.4, 4 x 1,000 56, 24, 24; a token of 64 sessions 7.4, 7.5, 10.9.  With parts
-// up to 1,024, 2,048 and 4,096 workgroups: 16,385 rows 90, 73, 77, 4 x 200 appended 17.4, 14.7, 14.8.
+// and turned 12.2, 9.8, 11.1; up to 4 x 200 appended 21.8, 14.7, 13.4, 4 x 1,000 56, 24, 24; a token of 64 sessions 7.4, 7.5, 10.9.  With parts
+// up to 1,024, 2,048 and 4,096 workgroups: 16,385 rows 90, 73, 77, up to 4 x 200 appended 17.4, 14.7, 14.8.
 TurnGrid turn_grid(int n_rows, int parts, int least) {
     TurnGrid g;
     g.rows = (int)std::min<int64_t>(std::max<int64_t>(n_rows / 128, least), kTurnRows);
@@ -87,7 +87,7 @@ struct HostKv8 {
     }
     // The prompt kernel does not split keys: it takes calls that fill the card with workgroups, or half of it where no request has many
     // more keys than new tokens; rows of 256 channels, which the other kernel takes 16 columns at a time, from a quarter on.  32 heads
-    // on 8 in bf16, lengths spread evenly, new tokens on up to so many keys, microseconds of the other kernel and of it:
+    // on 8 in bf16, new tokens and keys up to the numbers given, spread evenly over the requests, microseconds of the other kernel and of it:
     //   workgroups         128 channels                            64 channels                           256 channels
     //   128                512 on 8,191: 123, 199; on 512: 21, 20                                        512 on 8,191: 482, 391
     //   256                4 x 256 on 8,191: 149, 207;             94, 157;                              514, 394
@@ -103,8 +103,8 @@ struct HostKv8 {
         return groups >= (d.head_dim == 64 ? 1024 : 512) || (groups >= 256 && keys <= (d.head_dim == 64 ? 2 : 8) * (int64_t)d.max_new);
     }
     // Two tiles that share each key's operands, where registers hold them.  32 heads on 8 x 128 in bf16, in one tile and in two: 64
-    // sessions' 5 tokens (20 rows) on up to 4,097 keys 94 and 65 us, 4 x 20 tokens on 8,191 keys 39 and 24, 64 x 20 on 1,000 keys 47 and
-    // 47; but one session's 6 tokens on 8,191 keys, whose splits do not fill the card, 13 and 17.
+    // sessions' up to 5 tokens (20 rows) on up to 4,097 keys 94 and 65 us, 4 x 20 tokens on 8,191 keys 39 and 24, 64 x 20 on 1,000 keys 47
+    // and 47; but one session's 6 tokens on 8,191 keys, whose splits do not fill the card, 13 and 17.
     static int tile_cols(int64_t rows, int dim) { return rows <= 16 || dim == 256 ? 16 : 32; }
 };
 
@@ -119,9 +119,9 @@ void launch_attend8(const AttendParams &p, const AttendShape &sh, int dim, unsig
 }
 
 // Verification.  Rows of up to kVerifyVocab logits are a workgroup's each, in one launch, 16 tokens a lane at most; longer ones, which
-// no workgroup's registers hold, are cut in chunks.  f32 rows of 16,384 logits with draft logits, 5 and 1,280 of them, take 11 and 34 us in
-// one launch, 23 and 44 in three.  Fewer threads make room for more rows: 1,280 rows of 4,001 take 12 us on 512 threads each, 26 on
-// 1,024, of 8,001 19 and 28; 5 rows of 4,001 7.4 and 9.1.
+// no workgroup's registers hold, are cut in chunks.  Up to 5 f32 rows of 16,384 logits with draft logits, of 1 request and of 256, take 11 and 34
+// us in one launch, 23 and 44 in three.  Fewer threads make room for more rows: 256 requests' rows of 4,001 take 12 us on 512 threads each,
+// 26 on 1,024, of 8,001 19 and 28; one's of 4,001 7.4 and 9.1.
 constexpr int kVerifyVocab = 16384;
 
 struct VerifyShape {
