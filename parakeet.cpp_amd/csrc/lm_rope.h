@@ -189,7 +189,7 @@ __device__ inline void turn_rows(const typename T::Raw *x, int64_t x_row, bool w
     else turn_some<T, D, Batch>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n, lane);
 }
 
-// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms take 60 us, 4.9 TB/s, where a
+// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms take 61 us, 4.8 TB/s, where a
 // large copy reaches 5.2: 4 passes' loads a wave of 16-bit types (2: 65; at 64 channels, where 4 are all rows, 28.5 and 29.6; f32 has no
 // registers for them), 8 waves a vector unit.  One row of 16 heads takes 3 us, a launch and the sines.
 template <class T, int D, bool Halves>

@@ -57,8 +57,8 @@ struct TurnGrid {
 };
 // As many rows as leave 128 groups of them, whole blocks where that is more than half a block; beside each, as many parts of the heads as
 // make 2,048 workgroups.  32 heads on 8 x 128 in bf16, microseconds where 1,024, 128 and 32 groups are left: 1,000 rows normed
-// and turned 12.2, 9.8, 11.1; up to 4 x 200 appended 21.8, 14.7, 13.4, 4 x 1,000 56, 24, 24; a token of 64 sessions 7.4, 7.5, 10.9.  With parts
-// up to 1,024, 2,048 and 4,096 workgroups: 16,385 rows 90, 73, 77, up to 4 x 200 appended 17.4, 14.7, 14.8.
+// and turned 9.4, 8.6, 10.6; up to 4 x 200 appended 22, 15, 12, 4 x 1,000 56, 24, 24; a token of 64 sessions 7.5, 7.6, 11.1.  With parts
+// up to 1,024, 2,048 and 4,096 workgroups: 16,385 rows 79, 61, 67, up to 4 x 200 appended 17.5, 14.8, 14.1.
 TurnGrid turn_grid(int n_rows, int parts, int least) {
     TurnGrid g;
     g.rows = (int)std::min<int64_t>(std::max<int64_t>(n_rows / 128, least), kTurnRows);
