@@ -73,6 +73,16 @@ def test_many_rows():
     check(5000, 3, 1, 64, "bf16", 32)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, "f16"), (128, "bf16"), (128, "f32"), (256, "bf16")])
+def test_padding_behind_many_rows(D, dtype):
+    """Blocks of rows that begin in the padding, one that it begins in, a call of nothing else."""
+    pos = np.random.default_rng(7).integers(0, 9000, 4103)
+    pos[3300:] = -1
+    check(4103, 2, 1, D, dtype, D // 2, pos=pos)
+    check(4103, 2, 1, D, dtype, D // 2, pos=pos, inplace=True)
+    check(45, 5, 2, D, dtype, D // 2, pos=np.full(45, -1))
+
+
 def test_norms_of_small_and_large_rows():
     for size in (2.0 ** -40, 2.0 ** -12, 2.0 ** 40):
         check(5, 2, 1, 128, "f32", 64, size=size)
