@@ -163,12 +163,12 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
         for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_max[q][w]);
         rw[q].largest(top), rw[q].top_at = kNever;
     }
-    if (rw[0].greedy || (Draft && rw[1].greedy)) {       // the first place of the largest
+    if (rw[0].greedy || (Draft && rw[1].greedy)) {       // the first place of the largest; no NaN is as large as it
 #pragma unroll
         for (int q = 0; q < kSources; ++q) {
             int at = kNever;
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e) at = fminf(x[q][e], kMostLogit) == rw[q].top ? index(e / 8) + e % 8 : at;
+            for (int e = E - 1; e >= 0; --e) at = x[q][e] >= rw[q].top ? index(e / 8) + e % 8 : at;
             at = wave_min(at);
             if (lane == 0) s_at[q][wave] = at;
         }
