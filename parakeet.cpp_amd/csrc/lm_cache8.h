@@ -146,7 +146,13 @@ __device__ inline void append_rows(const pk_kv8_append_desc &a, const Turn &turn
         load_weights(a.k_weight, ch, w);
 #pragma unroll
         for (int p = 0; p < kPasses; ++p)
-            if (p * kRows < o0 + n && (p + 1) * kRows > o0) norm_and_turn<D>(x[p], c, turn, table, min(max(p * kRows + first - o0, 0), n - 1), w);
+            if (p * kRows < o0 + n && (p + 1) * kRows > o0) {
+                const int r = p * kRows + first - o0;
+                norm_and_turn<D>(x[p], c, turn, table, min(max(r, 0), n - 1), w);
+                // rows beside the run are zeros, whose norm with an eps of 0 is NaN: they count for nothing
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[p][i] = r >= 0 && r < n ? x[p][i] : 0.0f;
+            }
     }
     auto largest = [&](unsigned below) {
         unsigned top = 0;
