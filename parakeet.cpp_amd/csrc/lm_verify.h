@@ -14,6 +14,17 @@
 
 namespace pklm {
 
+// Single steps: neither is fused with the other, as the compiler would where it may (the header's __dmul_rn and __dadd_rn are plain
+// operators, which it fuses).
+__device__ inline double product(double a, double b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+__device__ inline double difference(double a, double b) {
+#pragma clang fp contract(off)
+    return a - b;
+}
+
 constexpr int kNever = 0x7FFFFFFF;
 constexpr float kMostLogit = 0x1.fffffep127f;         // +inf counts as this
 
@@ -39,7 +50,7 @@ struct RowWeights {
     }
     __device__ unsigned weight(float x, int i) const { return (unsigned)weight_f(x, i); }
     __device__ void total(u64 sum) { inv_sum = sum ? 1.0 / (double)sum : 0.0; }
-    __device__ double share_of(unsigned w) const { return __dmul_rn((double)w, inv_sum); }
+    __device__ double share_of(unsigned w) const { return product((double)w, inv_sum); }
 };
 
 // 8 adjacent logits of a row, from i on, as they come from memory; rows need not be aligned.
@@ -77,8 +88,8 @@ __device__ inline double uniform(float u) {
 }
 // In steps of 2^-52, cut to whole ones: at most 2^52, so that added to 2^52 they are the low bits.
 __device__ inline u64 left_of(double p, double q) {
-    const double d = __dadd_rn(p, -q);
-    return d > 0 ? __double_as_longlong(__dadd_rn(trunc(d * 0x1p52), 0x1p52)) - __double_as_longlong(0x1p52) : 0;
+    const double d = difference(p, q);
+    return d > 0 ? __double_as_longlong(trunc(d * 0x1p52) + 0x1p52) - __double_as_longlong(0x1p52) : 0;
 }
 
 // Rows of a request: [begin, begin + n) of the call's.
@@ -206,7 +217,7 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
     }
     const double p_draft = drafted ? rw[0].share_of(rw[0].weight(at_draft[0], d)) : 0.0;
     const double q_draft = Draft ? rw[1].share_of(rw[1].weight(at_draft[1], d)) : 1.0;
-    const bool ok = drafted && __dmul_rn(uniform(a.u[r]), q_draft) < p_draft;
+    const bool ok = drafted && product(uniform(a.u[r]), q_draft) < p_draft;
     if (ok || total[0] == 0) {
         if (tid == 0) s_verdict = RowVerdict{ok, ok ? d : -1, ok ? (float)p_draft : 0.0f, 0};
     } else {
@@ -449,7 +460,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(pk_verify_des
         const int j = j0 + wave, d = j < rows.n ? rows.draft(a, j) : -1;
         double p = 0, q = 1;
         if (d >= 0) p = shares(j, d, q);
-        const bool ok = d >= 0 && __dmul_rn(uniform(a.u[rows.begin + j]), q) < p;
+        const bool ok = d >= 0 && product(uniform(a.u[rows.begin + j]), q) < p;
         if (!ok && lane == 0 && j < rows.n) atomicMin(&s_stop[round], j);
         __syncthreads();
         stop = s_stop[round];
@@ -488,7 +499,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(pk_verify_des
         if (any || !drafted) return;
         if (two)
             of.y.each(i, V, [&](int e, float v) {
-                left[e] = trunc(fmax(__dadd_rn(__dmul_rn(left[e], scale_p), -__dmul_rn((double)draft.weight_f(v, i + e), scale_q)), 0.0));
+                left[e] = trunc(fmax(difference(product(left[e], scale_p), product((double)draft.weight_f(v, i + e), scale_q)), 0.0));
             });
         else
 #pragma unroll
