@@ -120,11 +120,12 @@ struct alignas(16) RowVerdict {
 
 // One launch, bound by its latency: 5 rows of 8,193 logits in f32 take 8.3 us, 256 requests of up to 6 rows of 1,027 with draft logits 9.8.
 //
-// A request's rows on a workgroup each, tokens in registers: wave w has tokens ((w n + g) 64 + lane) 8 + e of a row, g < n <= G.  Every
-// row that refuses its draft draws its own token, whether or not an earlier row has refused; the request's last workgroup to
-// arrive has the rows' verdicts and writes them up to the first refusal.
-template <class T, int BS, int G, bool Draft>
-__global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *arrived, RowVerdict *verdicts) {
+// A request has `each` workgroups, a row on each, or several in turn (Turns, which takes up to a tenth longer by its registers) where there
+// may be more rows.  Tokens are in registers: wave w has tokens ((w n + g) 64 + lane) 8 + e of a row, g < n <= G.  Every row that
+// refuses its draft draws its own token, whether or not an earlier row has refused; the request's last row to arrive has the rows'
+// verdicts and writes them up to the first refusal.
+template <class T, int BS, int G, bool Draft, bool Turns>
+__global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int each, int *arrived, RowVerdict *verdicts) {
     constexpr int kWaves = BS / 64, E = 8 * G, kSources = Draft ? 2 : 1;
     __shared__ float s_max[2][kWaves];
     __shared__ int s_at[2][kWaves];
@@ -132,162 +133,174 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int *a
     __shared__ RowVerdict s_verdict;
     __shared__ int s_flag;
     using Raw = typename T::Raw;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), V = a.vocab;
-    const int b = blockIdx.x / a.max_new, j = blockIdx.x % a.max_new;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Of Turns most may have no row: those go last.  Turned on by a request, so that one's rows are not all on one XCD.
+    const int first = Turns ? blockIdx.x / a.requests : blockIdx.x % each;
+    const int b = Turns ? (blockIdx.x + first) % a.requests : blockIdx.x / each;
     const RequestRows rows(a, b);
-    if (rows.n == 0 && j == 0 && tid == 0) verify_counts(a, b, 0, 0);
-    if (j >= rows.n) return;
-    const int r = rows.begin + j, d = rows.draft(a, j);
-    const bool drafted = d >= 0;
-    const int n = (V + 8 * BS - 1) / (8 * BS);
-    auto index = [&](int g) { return ((wave * n + g) * 64 + lane) * 8; };
-    const Raw *row[2] = {(const Raw *)a.logits + (int64_t)r * a.logits_row, Draft ? (const Raw *)a.draft + (int64_t)r * a.draft_row : nullptr};
-    Tokens8<T> raw[kSources][G];
-    float at_draft[2];
-    RowWeights rw[2];
-#pragma unroll
-    for (int q = 0; q < kSources; ++q) {
-        const int end = q == 0 || drafted ? V : 0;      // without a draft its row is not read
-#pragma unroll
-        for (int g = 0; g < G; ++g) raw[q][g].load(row[q], g < n ? index(g) : end, end);
-        at_draft[q] = drafted ? logit<T>(row[q], d) : -INFINITY;
-        rw[q].settings(q ? a.draft_temperature : a.temperature, b);
-    }
-    float x[kSources][E];
-#pragma unroll
-    for (int q = 0; q < kSources; ++q) {
-        const int end = q == 0 || drafted ? V : 0;
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[q][e] = raw[q][e / 8].get(e % 8, e / 8 < n ? index(e / 8) : end, end);
-            top = fmaxf(top, x[q][e]);
-        }
-        top = wave_max(top);
-        if (lane == 0) s_max[q][wave] = top;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kSources; ++q) {
-        float top = s_max[q][0];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_max[q][w]);
-        rw[q].largest(top), rw[q].top_at = kNever;
-    }
-    if (rw[0].greedy || (Draft && rw[1].greedy)) {       // the first place of the largest; no NaN is as large as it
+    if (rows.n == 0 && first == 0 && tid == 0) verify_counts(a, b, 0, 0);
+#pragma nounroll
+    for (int j = first; j < rows.n; j += each) {
+        // what follows from these is worked out for each row, not once in front of them all, over which it would be spilled
+        int lane = tid & 63, V = a.vocab;
+        if (Turns) asm volatile("" : "+v"(lane), "+s"(V));
+        const int r = rows.begin + j, d = rows.draft(a, j);
+        const bool drafted = d >= 0;
+        const int n = (V + 8 * BS - 1) / (8 * BS);
+        auto index = [&](int g) { return ((wave * n + g) * 64 + lane) * 8; };
+        const Raw *row[2] = {(const Raw *)a.logits + (int64_t)r * a.logits_row, Draft ? (const Raw *)a.draft + (int64_t)r * a.draft_row : nullptr};
+        Tokens8<T> raw[kSources][G];
+        float at_draft[2];
+        RowWeights rw[2];
 #pragma unroll
         for (int q = 0; q < kSources; ++q) {
-            int at = kNever;
+            const int end = q == 0 || drafted ? V : 0;      // without a draft its row is not read
 #pragma unroll
-            for (int e = E - 1; e >= 0; --e) at = x[q][e] >= rw[q].top ? index(e / 8) + e % 8 : at;
-            at = wave_min(at);
-            if (lane == 0) s_at[q][wave] = at;
+            for (int g = 0; g < G; ++g) raw[q][g].load(row[q], g < n ? index(g) : end, end);
+            at_draft[q] = drafted ? logit<T>(row[q], d) : -INFINITY;
+            rw[q].settings(q ? a.draft_temperature : a.temperature, b);
         }
-        __syncthreads();
+        float x[kSources][E];
 #pragma unroll
-        for (int q = 0; q < kSources; ++q)
+        for (int q = 0; q < kSources; ++q) {
+            const int end = q == 0 || drafted ? V : 0;
+            float top = -INFINITY;
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) rw[q].top_at = min(rw[q].top_at, s_at[q][v]);
-    }
-    unsigned w[kSources][E];
-#pragma unroll
-    for (int q = 0; q < kSources; ++q) {
-        u64 sum = 0;
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-            if (g < n)
-#pragma unroll
-                for (int e = 8 * g; e < 8 * g + 8; ++e) {
-                    w[q][e] = rw[q].weight(x[q][e], index(g) + e % 8);
-                    sum += w[q][e];
-                }
-            else
-#pragma unroll
-                for (int e = 8 * g; e < 8 * g + 8; ++e) w[q][e] = 0;
-        sum = wave_sum(sum);
-        if (lane == 0) s_sum[q][wave] = sum;
-    }
-    __syncthreads();
-    u64 total[2] = {0, 0};
-#pragma unroll
-    for (int q = 0; q < kSources; ++q) {
-#pragma unroll
-        for (int v = 0; v < kWaves; ++v) total[q] += s_sum[q][v];
-        rw[q].total(total[q]);
-    }
-    const double p_draft = drafted ? rw[0].share_of(rw[0].weight(at_draft[0], d)) : 0.0;
-    const double q_draft = Draft ? rw[1].share_of(rw[1].weight(at_draft[1], d)) : 1.0;
-    const bool ok = drafted && product(uniform(a.u[r]), q_draft) < p_draft;
-    if (ok || total[0] == 0) {
-        if (tid == 0) s_verdict = RowVerdict{ok, ok ? d : -1, ok ? (float)p_draft : 0.0f, 0};
-    } else {
-        // what is left to draw from
-        std::conditional_t<Draft, u64, unsigned> left[E];
-        u64 mass = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            left[e] = w[0][e];
-            if (drafted && Draft) left[e] = left_of(rw[0].share_of(w[0][e]), rw[1].share_of(w[kSources - 1][e]));
-            if (drafted && !Draft) left[e] = index(e / 8) + e % 8 == d ? 0 : left[e];
-            mass += left[e];
-        }
-        mass = wave_sum(mass);
-        if (lane == 0) s_left[wave] = mass;
-        __syncthreads();
-        u64 all = 0, lead = 0;
-#pragma unroll
-        for (int v = 0; v < kWaves; ++v) {
-            if (v < wave) lead += s_left[v];
-            all += s_left[v];
-        }
-        if (all == 0) {                          // nothing: from the target itself
-#pragma unroll
-            for (int e = 0; e < E; ++e) left[e] = w[0][e];
-            mass = s_sum[0][wave], all = total[0], lead = 0;
-#pragma unroll
-            for (int v = 0; v < kWaves; ++v)
-                if (v < wave) lead += s_sum[0][v];
-        }
-        const u64 u = part31(a.u_draw[b]), t = share(all, u > 0x7FFFFFFFull ? 0x7FFFFFFFull : u);
-        if (lead <= t && t < lead + mass)
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                u64 own = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) own += left[8 * g + e];
-                const u64 run = wave_scan(own);
-                u64 at = lead + run - own;
-                if (at <= t && t < at + own)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (at <= t && t < at + left[8 * g + e])
-                            s_verdict = RowVerdict{0, index(g) + e, (float)rw[0].share_of(w[0][8 * g + e]), 0};
-                        at += left[8 * g + e];
-                    }
-                lead += lane_value(run, 63);
+            for (int e = 0; e < E; ++e) {
+                x[q][e] = raw[q][e / 8].get(e % 8, e / 8 < n ? index(e / 8) : end, end);
+                top = fmaxf(top, x[q][e]);
             }
-    }
-    __syncthreads();
-    auto write = [&](int at, const RowVerdict &v, bool kept) {
-        a.out[rows.begin + at] = kept ? v.token : -1;
-        if (a.prob) a.prob[rows.begin + at] = kept ? v.prob : 0.0f;
-    };
-    if (rows.n == 1) {
-        if (tid == 0) write(0, s_verdict, true), verify_counts(a, b, 1, 0);
+            top = wave_max(top);
+            if (lane == 0) s_max[q][wave] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < kSources; ++q) {
+            float top = s_max[q][0];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_max[q][w]);
+            rw[q].largest(top), rw[q].top_at = kNever;
+        }
+        if (rw[0].greedy || (Draft && rw[1].greedy)) {       // the first place of the largest; no NaN is as large as it
+#pragma unroll
+            for (int q = 0; q < kSources; ++q) {
+                int at = kNever;
+#pragma unroll
+                for (int e = E - 1; e >= 0; --e) at = x[q][e] >= rw[q].top ? index(e / 8) + e % 8 : at;
+                at = wave_min(at);
+                if (lane == 0) s_at[q][wave] = at;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < kSources; ++q)
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) rw[q].top_at = min(rw[q].top_at, s_at[q][v]);
+        }
+        unsigned w[kSources][E];
+#pragma unroll
+        for (int q = 0; q < kSources; ++q) {
+            u64 sum = 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (g < n)
+#pragma unroll
+                    for (int e = 8 * g; e < 8 * g + 8; ++e) {
+                        w[q][e] = rw[q].weight(x[q][e], index(g) + e % 8);
+                        sum += w[q][e];
+                    }
+                else
+#pragma unroll
+                    for (int e = 8 * g; e < 8 * g + 8; ++e) w[q][e] = 0;
+            sum = wave_sum(sum);
+            if (lane == 0) s_sum[q][wave] = sum;
+        }
+        __syncthreads();
+        u64 total[2] = {0, 0};
+#pragma unroll
+        for (int q = 0; q < kSources; ++q) {
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) total[q] += s_sum[q][v];
+            rw[q].total(total[q]);
+        }
+        const double p_draft = drafted ? rw[0].share_of(rw[0].weight(at_draft[0], d)) : 0.0;
+        const double q_draft = Draft ? rw[1].share_of(rw[1].weight(at_draft[1], d)) : 1.0;
+        const bool ok = drafted && product(uniform(a.u[r]), q_draft) < p_draft;
+        if (ok || total[0] == 0) {
+            if (tid == 0) s_verdict = RowVerdict{ok, ok ? d : -1, ok ? (float)p_draft : 0.0f, 0};
+        } else {
+            // what is left to draw from
+            std::conditional_t<Draft, u64, unsigned> left[E];
+            u64 mass = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                left[e] = w[0][e];
+                if (drafted && Draft) left[e] = left_of(rw[0].share_of(w[0][e]), rw[1].share_of(w[kSources - 1][e]));
+                if (drafted && !Draft) left[e] = index(e / 8) + e % 8 == d ? 0 : left[e];
+                mass += left[e];
+            }
+            mass = wave_sum(mass);
+            if (lane == 0) s_left[wave] = mass;
+            __syncthreads();
+            u64 all = 0, lead = 0;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                if (v < wave) lead += s_left[v];
+                all += s_left[v];
+            }
+            if (all == 0) {                          // nothing: from the target itself
+#pragma unroll
+                for (int e = 0; e < E; ++e) left[e] = w[0][e];
+                mass = s_sum[0][wave], all = total[0], lead = 0;
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v)
+                    if (v < wave) lead += s_sum[0][v];
+            }
+            const u64 u = part31(a.u_draw[b]), t = share(all, u > 0x7FFFFFFFull ? 0x7FFFFFFFull : u);
+            if (lead <= t && t < lead + mass)
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    u64 own = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) own += left[8 * g + e];
+                    const u64 run = wave_scan(own);
+                    u64 at = lead + run - own;
+                    if (at <= t && t < at + own)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (at <= t && t < at + left[8 * g + e])
+                                s_verdict = RowVerdict{0, index(g) + e, (float)rw[0].share_of(w[0][8 * g + e]), 0};
+                            at += left[8 * g + e];
+                        }
+                    lead += lane_value(run, 63);
+                }
+        }
+        __syncthreads();
+        auto write = [&](int at, const RowVerdict &v, bool kept) {
+            a.out[rows.begin + at] = kept ? v.token : -1;
+            if (a.prob) a.prob[rows.begin + at] = kept ? v.prob : 0.0f;
+        };
+        if (rows.n == 1) {
+            if (tid == 0) write(0, s_verdict, true), verify_counts(a, b, 1, 0);
+            return;
+        }
+        RowVerdict *mine = verdicts + rows.begin;
+        if (tid == 0) store_shared4((unsigned *)(mine + j), 0, __builtin_bit_cast(u4, s_verdict));
+        if (!last_to_arrive(&arrived[b], rows.n, &s_flag)) {
+            if (Turns) continue;
+            return;
+        }
+        if (wave != 0) return;
+        int stop = kNever;
+        for (int j0 = 0; j0 < rows.n; j0 += 64) {
+            RowVerdict v{1, 0, 0, 0};
+            if (j0 + lane < rows.n) v = __builtin_bit_cast(RowVerdict, load_shared4((const unsigned *)(mine + j0), 4 * lane));
+            const u64 refused = __ballot(!v.ok || j0 + lane == rows.n - 1);
+            if (stop == kNever && refused) stop = j0 + __ffsll(refused) - 1;
+            if (j0 + lane < rows.n) write(j0 + lane, v, j0 + lane <= stop);
+        }
+        if (lane == 0) verify_counts(a, b, rows.n, stop);
         return;
     }
-    RowVerdict *mine = verdicts + (int64_t)b * a.max_new;
-    if (tid == 0) store_shared4((unsigned *)(mine + j), 0, __builtin_bit_cast(u4, s_verdict));
-    if (!last_to_arrive(&arrived[b], rows.n, &s_flag) || wave != 0) return;
-    int stop = kNever;
-    for (int j0 = 0; j0 < rows.n; j0 += 64) {
-        RowVerdict v{1, 0, 0, 0};
-        if (j0 + lane < rows.n) v = __builtin_bit_cast(RowVerdict, load_shared4((const unsigned *)(mine + j0), 4 * lane));
-        const u64 refused = __ballot(!v.ok);
-        if (stop == kNever && refused) stop = j0 + __ffsll(refused) - 1;
-        if (j0 + lane < rows.n) write(j0 + lane, v, j0 + lane <= stop);
-    }
-    if (lane == 0) verify_counts(a, b, rows.n, stop);
 }
 
 // ---- rows too long for one workgroup's registers ----
@@ -304,7 +317,7 @@ constexpr int kVerifyThreads = 256, kVerifyWaves = kVerifyThreads / 64, kVerifyP
 constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64, kDrawPass = 8 * kDrawThreads;
 
 struct SplitVerify {
-    float *chunk_max;       // [rows][2][chunks], of the target and of the draft
+    float *chunk_max;       // [rows of the call][2][chunks], of the target and of the draft
     int *chunk_at;          // likewise; where the largest alone counts
     u64 *chunk_sum;         // likewise
     u64 *left;              // [requests][chunks]
@@ -313,15 +326,30 @@ struct SplitVerify {
     int draw_chunks, draw_passes;       // likewise, with kDrawPass, of the one row of a request that is drawn from
 };
 
-// A workgroup's chunk of a row: (request, row of it, source).
-struct VerifyChunk {
-    int b, j, q, chunk;
-    __device__ VerifyChunk(const pk_verify_desc &a, const SplitVerify &w) {
-        unsigned id = blockIdx.x;
-        chunk = id % w.chunks, id /= w.chunks;
-        q = id % w.sources, id /= w.sources;
-        j = id % a.max_new, b = id / a.max_new;
+// The request of the call's row r, the first one that ends behind it: by a whole wave, among 64 runs of requests, then in the run.
+static_assert(PK_LM_MAX_REQUESTS <= 64 * 64, "a lane looks at one run, then at one request");
+__device__ inline int request_of(const pk_verify_desc &a, int r) {
+    const int lane = threadIdx.x & 63, run = (a.requests + 63) / 64;
+    auto behind = [&](int request) { return __ballot(a.first[min(request + 1, a.requests)] > r); };
+    const u64 runs = behind((lane + 1) * run - 1);
+    int b = runs ? __builtin_ctzll(runs) * run : a.requests - 1;
+    if (run > 1) {
+        const u64 in = behind(b + lane);
+        b += in ? __builtin_ctzll(in) : 0;
     }
+    return min(b, a.requests - 1);
+}
+
+// A workgroup's chunk of a row of the call: its request and place in it, none where j is not below rows.n.
+struct VerifyChunk {
+    int q, chunk, r, b, j;
+    RequestRows rows;
+    __device__ VerifyChunk(const pk_verify_desc &a, const SplitVerify &w)
+        : q(blockIdx.x / w.chunks % w.sources), chunk(blockIdx.x % w.chunks), r(blockIdx.x / w.chunks / w.sources), b(request_of(a, r)), rows(a, b) {
+        j = r >= rows.begin ? r - rows.begin : rows.n;
+    }
+    __device__ bool none(const pk_verify_desc &a) const { return j >= rows.n || (q && rows.draft(a, j) < 0); }
+    __device__ int64_t place(const SplitVerify &w) const { return ((int64_t)r * 2 + q) * w.chunks + chunk; }
 };
 
 template <class T>
@@ -335,10 +363,10 @@ __device__ inline int verify_token(int passes, int chunk, int pass) {
     return ((chunk * Waves + (int)(threadIdx.x >> 6)) * passes + pass) * 512 + (int)(threadIdx.x & 63) * 8;
 }
 
-// A row's rule, from its chunks' maxima, and its weight where the chunks have theirs: by a whole wave.
-__device__ inline u64 row_rule(const pk_verify_desc &a, const SplitVerify &w, int b, int64_t place, int q, RowWeights &rw, bool summed) {
+// The rule of row r of the call, from its chunks' maxima, and its weight where the chunks have theirs: by a whole wave.
+__device__ inline u64 row_rule(const pk_verify_desc &a, const SplitVerify &w, int b, int r, int q, RowWeights &rw, bool summed) {
     const int lane = threadIdx.x & 63;
-    const int64_t at = (place * 2 + q) * w.chunks + lane;
+    const int64_t at = ((int64_t)r * 2 + q) * w.chunks + lane;
     rw.settings(q ? a.draft_temperature : a.temperature, b);
     const bool in = lane < w.chunks;
     const float m = in ? w.chunk_max[at] : -INFINITY;
@@ -357,9 +385,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_max_kernel(pk_verify_de
     __shared__ float s_max[kVerifyWaves];
     __shared__ int s_at[kVerifyWaves];
     const VerifyChunk c(a, w);
-    const RequestRows rows(a, c.b);
-    if (c.j >= rows.n || (c.q && rows.draft(a, c.j) < 0)) return;
-    const auto *row = verify_row<T>(a, c.q, rows.begin + c.j);
+    if (c.none(a)) return;
+    const auto *row = verify_row<T>(a, c.q, c.r);
     const int tid = threadIdx.x, V = a.vocab;
     RowWeights rw;
     rw.settings(c.q ? a.draft_temperature : a.temperature, c.b);
@@ -387,8 +414,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_max_kernel(pk_verify_de
         int p = s_at[0];
         for (int v = 1; v < kVerifyWaves; ++v)
             if (s_max[v] > m || (s_max[v] == m && s_at[v] < p)) m = s_max[v], p = s_at[v];
-        const int64_t place = (((int64_t)c.b * a.max_new + c.j) * 2 + c.q) * w.chunks + c.chunk;
-        w.chunk_max[place] = m, w.chunk_at[place] = p;
+        w.chunk_max[c.place(w)] = m, w.chunk_at[c.place(w)] = p;
     }
 }
 
@@ -396,15 +422,13 @@ template <class T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(pk_verify_desc a, SplitVerify w) {
     __shared__ u64 s_sum[kVerifyWaves];
     const VerifyChunk c(a, w);
-    const RequestRows rows(a, c.b);
-    if (c.j >= rows.n || (c.q && rows.draft(a, c.j) < 0)) return;
-    const auto *row = verify_row<T>(a, c.q, rows.begin + c.j);
+    if (c.none(a)) return;
+    const auto *row = verify_row<T>(a, c.q, c.r);
     const int tid = threadIdx.x, V = a.vocab;
-    const int64_t place = (int64_t)c.b * a.max_new + c.j;
     Tokens8<T> x;
     x.load(row, verify_token<kVerifyWaves>(w.passes, c.chunk, 0), V);       // on its way while the rule is worked out
     RowWeights rw;
-    row_rule(a, w, c.b, place, c.q, rw, false);
+    row_rule(a, w, c.b, c.r, c.q, rw, false);
     u64 sum = 0;
     for (int p = 0; p < w.passes; ++p) {
         const int i = verify_token<kVerifyWaves>(w.passes, c.chunk, p);
@@ -422,7 +446,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(pk_verify_de
     __syncthreads();
     if (tid < 64) {
         sum = wave_sum(tid < kVerifyWaves ? s_sum[tid] : 0);
-        if (tid == 0) w.chunk_sum[(place * 2 + c.q) * w.chunks + c.chunk] = sum;
+        if (tid == 0) w.chunk_sum[c.place(w)] = sum;
     }
 }
 
@@ -442,11 +466,10 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(pk_verify_des
     // p and q of a row's draft; by a whole wave
     auto shares = [&](int j, int d, double &q) {
         const float x = logit<T>(verify_row<T>(a, 0, rows.begin + j), d), y = two_sources ? logit<T>(verify_row<T>(a, 1, rows.begin + j), d) : 0.0f;
-        const int64_t place = (int64_t)b * a.max_new + j;
-        row_rule(a, w, b, place, 0, target, true);
+        row_rule(a, w, b, rows.begin + j, 0, target, true);
         q = 1.0;
         if (two_sources) {
-            row_rule(a, w, b, place, 1, draft, true);
+            row_rule(a, w, b, rows.begin + j, 1, draft, true);
             q = draft.share_of(draft.weight(y, d));
         }
         return target.share_of(target.weight(x, d));
@@ -477,11 +500,10 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(pk_verify_des
         if (tid == 0) verify_counts(a, b, rows.n, stop);
     }
     const int d = rows.draft(a, stop), r = rows.begin + stop;
-    const int64_t place = (int64_t)b * a.max_new + stop;
     const bool drafted = d >= 0, two = drafted && two_sources;
     const auto *x_row = verify_row<T>(a, 0, r), *y_row = two ? verify_row<T>(a, 1, r) : x_row;
-    const u64 total = row_rule(a, w, b, place, 0, target, true);
-    if (two) row_rule(a, w, b, place, 1, draft, true);
+    const u64 total = row_rule(a, w, b, r, 0, target, true);
+    if (two) row_rule(a, w, b, r, 1, draft, true);
     // What is left of a lane's 8 tokens of a pass, whole numbers in f64, whose sums are exact: of p - q in steps of 2^-52 at most 2^52
     // and a step a token, of weights at most 2^50.
     const double scale_p = target.inv_sum * 0x1p52, scale_q = two ? draft.inv_sum * 0x1p52 : 0.0;

@@ -122,9 +122,18 @@ void launch_attend8(const AttendParams &p, const AttendShape &sh, int dim, unsig
 // no workgroup's registers hold, are cut in chunks.  Up to 5 f32 rows of 16,384 logits with draft logits, of 1 request and of 256, take 11 and 34
 // us in one launch, 23 and 44 in three.  Fewer threads make room for more rows: 256 requests' rows of 4,001 take 12 us on 512 threads each,
 // 26 on 1,024, of 8,001 19 and 28; one's of 4,001 7.4 and 9.1.
-constexpr int kVerifyVocab = 16384;
+//
+// In one launch a request has as many workgroups as it may bring rows.  Where that bound says nothing (it is all rows of the call) or
+// is far, it has twice the mean's, or what makes kVerifyGroups in all, and they take its rows in turn: with the bound and without,
+// 256 requests' 5 rows of 1,027 with draft logits take 10.4 and 10.5 us, 64 requests' 5 of 4,001 7.5 and 9.0, one request's 300 rows of
+// 1,027 among 63 of one row 11.2 and 17.5.  Half of kVerifyGroups: 10.5, 7.7 and 25.9.  Several launches have workgroups for the call's
+// rows alone.
+constexpr int kVerifyVocab = 16384, kVerifyGroups = 8192, kVerifyMost = 1 << 17;
 
 struct VerifyShape {
+    bool turns;          // see verify_row_kernel
+    int each;
+    int64_t groups;      // workgroups of it, or of the first launch of several
     int passes, chunks, draw_passes, draw_chunks;        // see SplitVerify
     // counters first, the same place for every shape: they are zero between calls
     static constexpr int64_t kCounterBytes = PK_LM_MAX_REQUESTS * 4;
@@ -133,9 +142,13 @@ struct VerifyShape {
 
 VerifyShape verify_shape(const pk_verify_desc &d) {
     VerifyShape s{};
-    const int64_t rows = (int64_t)d.requests * d.max_new;
+    const int64_t requests = std::max(d.requests, 1), most = std::max(std::min(d.max_new, d.n_rows), 1);
+    const int64_t mean = (d.n_rows + requests - 1) / requests;
     if (d.vocab <= kVerifyVocab) {
-        s.bytes = VerifyShape::kCounterBytes + rows * (int64_t)sizeof(RowVerdict);
+        const bool known = (d.max_new < d.n_rows || requests == 1) && requests * most <= kVerifyMost;
+        s.each = (int)(known ? most : std::min(most, std::max(2 * mean, kVerifyGroups / requests)));
+        s.turns = s.each < most, s.groups = requests * s.each;
+        s.bytes = VerifyShape::kCounterBytes + d.n_rows * (int64_t)sizeof(RowVerdict);
         return s;
     }
     // As many chunks as make `want` workgroups, 64 of a row at most (a lane has one each), of two passes at least.  Requests of up to 5 rows
@@ -146,8 +159,10 @@ VerifyShape verify_shape(const pk_verify_desc &d) {
         passes = (int)std::max<int64_t>(2, (d.vocab + aim * pass - 1) / (aim * pass));
         chunks = (d.vocab + passes * pass - 1) / (passes * pass);
     };
-    cut(rows * (d.draft ? 2 : 1), s.chunks, s.passes, 8192, kVerifyPass);
+    const int64_t rows = d.n_rows, sources = d.draft ? 2 : 1;
+    cut(std::min(requests * most, 2 * rows) * sources, s.chunks, s.passes, 8192, kVerifyPass);
     cut(d.requests, s.draw_chunks, s.draw_passes, 512, kDrawPass);
+    s.groups = rows * sources * s.chunks;
     int64_t at = VerifyShape::kCounterBytes;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -166,36 +181,36 @@ int verify_check(const char *what, const pk_verify_desc *d) {
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests (at most %d)", what, d->requests, PK_LM_MAX_REQUESTS);
     if (d->n_rows < 0 || d->max_new < 0 || d->vocab <= 0 || d->vocab > PK_LM_MAX_VOCAB)
         return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d rows, max_new %d, %d logits (1 .. %d)", what, d->n_rows, d->max_new, d->vocab, PK_LM_MAX_VOCAB);
-    // with 64 chunks a row at most of two sources
-    if ((int64_t)d->requests * d->max_new > most_groups(kVerifyThreads) / 128)
-        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests of up to %d rows in one call", what, d->requests, d->max_new);
+    if ((int64_t)d->requests * d->max_new > INT32_MAX || verify_shape(*d).groups > most_groups(1024))       // threads of the largest workgroup
+        return pk_fail(PK_ERR_UNSUPPORTED, "%s: %d requests of up to %d rows, %d in all, in one call", what, d->requests, d->max_new, d->n_rows);
     return PK_OK;
 }
 
 template <class T, int BS, int G>
-void launch_verify_rows(const pk_verify_desc &d, hipStream_t s) {
+void launch_verify_rows(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s) {
     int *arrived = (int *)d.workspace;
     auto *verdicts = (RowVerdict *)((char *)d.workspace + VerifyShape::kCounterBytes);
-    const unsigned grid = (unsigned)(d.requests * d.max_new);
-    if (d.draft) verify_row_kernel<T, BS, G, true><<<grid, BS, 0, s>>>(d, arrived, verdicts);
-    else verify_row_kernel<T, BS, G, false><<<grid, BS, 0, s>>>(d, arrived, verdicts);
+    auto launch = [&](auto draft, auto turns) {
+        verify_row_kernel<T, BS, G, draft.value, turns.value><<<(unsigned)sh.groups, BS, 0, s>>>(d, sh.each, arrived, verdicts);
+    };
+    if (sh.turns) d.draft ? launch(std::true_type{}, std::true_type{}) : launch(std::false_type{}, std::true_type{});
+    else d.draft ? launch(std::true_type{}, std::false_type{}) : launch(std::false_type{}, std::false_type{});
 }
 
 template <class T>
 void launch_verify(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s) {
-    if (d.vocab <= 2048) return launch_verify_rows<T, 256, 1>(d, s);
-    if (d.vocab <= 4096) return launch_verify_rows<T, 512, 1>(d, s);
-    if (d.vocab <= 8192) return launch_verify_rows<T, 512, 2>(d, s);
-    if (d.vocab <= kVerifyVocab) return launch_verify_rows<T, 1024, 2>(d, s);
+    if (d.vocab <= 2048) return launch_verify_rows<T, 256, 1>(d, sh, s);
+    if (d.vocab <= 4096) return launch_verify_rows<T, 512, 1>(d, sh, s);
+    if (d.vocab <= 8192) return launch_verify_rows<T, 512, 2>(d, sh, s);
+    if (d.vocab <= kVerifyVocab) return launch_verify_rows<T, 1024, 2>(d, sh, s);
     char *w = (char *)d.workspace;
     SplitVerify p;
     p.arrived = (int *)w, p.chunk_max = (float *)(w + sh.max_at), p.chunk_at = (int *)(w + sh.at_at), p.chunk_sum = (u64 *)(w + sh.sum_at);
     p.left = (u64 *)(w + sh.left_at);
     p.chunks = sh.chunks, p.passes = sh.passes, p.sources = d.draft ? 2 : 1;
     p.draw_chunks = sh.draw_chunks, p.draw_passes = sh.draw_passes;
-    const unsigned grid = (unsigned)(d.requests * d.max_new * p.sources * p.chunks);
-    verify_max_kernel<T><<<grid, kVerifyThreads, 0, s>>>(d, p);
-    verify_sum_kernel<T><<<grid, kVerifyThreads, 0, s>>>(d, p);
+    if (sh.groups) verify_max_kernel<T><<<(unsigned)sh.groups, kVerifyThreads, 0, s>>>(d, p);
+    if (sh.groups) verify_sum_kernel<T><<<(unsigned)sh.groups, kVerifyThreads, 0, s>>>(d, p);
     verify_draw_kernel<T><<<(unsigned)(d.requests * p.draw_chunks), kDrawThreads, 0, s>>>(d, p);
 }
 

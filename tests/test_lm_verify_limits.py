@@ -1,0 +1,23 @@
+"""What pk_verify takes and refuses by its sizes (no GPU needed)."""
+import ctypes as C
+
+import pytest
+
+
+def workspace(n, B, V, max_new, draft=True):
+    """Bytes, None where the call is refused."""
+    from parakeet_amd import lm, pk
+    wanted = C.c_int64()
+    try:
+        lm._call("pk_verify_workspace", lm._VERIFY.pack(1 << 20, draft << 20, *[0] * 13, V, V, n, B, V, 0, max_new, 0), C.addressof(wanted))
+    except pk.PkError as e:
+        assert "in one call" in str(e)
+        return None
+    return wanted.value
+
+
+@pytest.mark.parametrize("n,B,V", [(1280, 256, 1027), (810, 162, 128001), (320, 64, 128001), (20480, 4096, 8193), (20480, 4096, 128001)])
+def test_the_bound_defaults_to_all_rows(pkg, n, B, V):
+    """The sizes of a call go by the rows that there are, not by how many each request might have had."""
+    assert 0 < workspace(n, B, V, n) <= 2 * workspace(n, B, V, 5)
+    assert workspace(n, B, V, (2 ** 31 - 1) // B) and workspace(n, B, V, 2 ** 31 // B + 1) is None
