@@ -238,9 +238,9 @@ typedef struct pk_verify_desc {
     const float *u_draw;                /* [requests] */
     const int32_t *lens;                /* [requests] tokens held, those of this call included; nullable */
     int32_t *out;                       /* out [n_rows]: the accepted drafts, the token drawn behind them, then -1; rows of no
-                                           request stay as they are */
+                                           request stay as they are; not over tokens */
     int32_t *accepted;                  /* out [requests]: how many drafts were accepted */
-    int32_t *lens_out;                  /* out [requests]: lens less the refused drafts, not lens itself; nullable */
+    int32_t *lens_out;                  /* out [requests]: lens less the refused drafts, not over lens; nullable */
     float *prob;                        /* out [n_rows]: p of the token in out, 0 at -1; nullable */
     void *workspace;                    /* pk_verify_workspace() bytes, zeroed once before its first use.  One call at a time may
                                            use it. */

@@ -186,6 +186,12 @@ int verify_check(const char *what, const pk_verify_desc *d) {
     return PK_OK;
 }
 
+// Whether two arrays of n whole numbers have a place in common.
+bool overlap(const int32_t *a, const int32_t *b, int64_t n) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return (x < y ? y - x : x - y) < (uintptr_t)n * sizeof(int32_t);
+}
+
 template <class T, int BS, int G>
 void launch_verify_rows(const pk_verify_desc &d, const VerifyShape &sh, hipStream_t s) {
     int *arrived = (int *)d.workspace;
@@ -331,8 +337,9 @@ PK_API int pk_verify(const pk_verify_desc *d, void *stream) {
     if (d->requests == 0) return PK_OK;
     if (d->max_new == 0) return pk_fail(PK_ERR_ARG, "%s: max_new 0", what);
     if (!d->logits || !d->tokens || !d->first || !d->u || !d->u_draw || !d->out || !d->accepted) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
-    if (d->lens_out && (!d->lens || d->lens_out == d->lens)) return pk_fail(PK_ERR_ARG, "%s: lens_out without lens, or lens itself", what);
-    if (d->out == d->tokens) return pk_fail(PK_ERR_ARG, "%s: out is written while tokens are read", what);
+    if (d->lens_out && (!d->lens || overlap(d->lens_out, d->lens, d->requests)))
+        return pk_fail(PK_ERR_ARG, "%s: lens_out without lens, or over lens", what);
+    if (overlap(d->out, d->tokens, d->n_rows)) return pk_fail(PK_ERR_ARG, "%s: out is written while tokens are read", what);
     const int size = type_size(d->dtype);
     if (!aligned(d->logits, size) || !aligned(d->draft, size)) return pk_fail(PK_ERR_ARG, "%s: logits not aligned to their type", what);
     const VerifyShape sh = verify_shape(*d);
