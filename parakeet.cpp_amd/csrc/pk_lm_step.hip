@@ -335,8 +335,10 @@ PK_API int pk_verify(const pk_verify_desc *d, void *stream) {
     if (int rc = verify_check(what, d)) return rc;
     if (!float_type(d->dtype)) return pk_fail(PK_ERR_UNSUPPORTED, "%s: dtype %d", what, d->dtype);
     if (d->requests == 0) return PK_OK;
-    if (d->max_new == 0) return pk_fail(PK_ERR_ARG, "%s: max_new 0", what);
-    if (!d->logits || !d->tokens || !d->first || !d->u || !d->u_draw || !d->out || !d->accepted) return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
+    // without rows the requests' counts are written all the same
+    if (d->n_rows > 0 && d->max_new == 0) return pk_fail(PK_ERR_ARG, "%s: max_new 0", what);
+    if (!d->first || !d->u_draw || !d->accepted || (d->n_rows > 0 && (!d->logits || !d->tokens || !d->u || !d->out)))
+        return pk_fail(PK_ERR_ARG, "%s: NULL array", what);
     if (d->lens_out && (!d->lens || overlap(d->lens_out, d->lens, d->requests)))
         return pk_fail(PK_ERR_ARG, "%s: lens_out without lens, or over lens", what);
     if (overlap(d->out, d->tokens, d->n_rows)) return pk_fail(PK_ERR_ARG, "%s: out is written while tokens are read", what);

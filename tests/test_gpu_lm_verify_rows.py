@@ -1,4 +1,8 @@
 """pk_verify without max_new, and calls whose requests bring rows of very different numbers: the same answers, whatever bound is given."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -77,3 +81,37 @@ def test_offsets_outside_the_rows_and_over_each_other(V):
         for first in ([0, 5, 2, 6], [4, 1, 6, 0], [-9, 99, -9, 99]):
             _, acc, _, _ = call(x, None, [0, 3, 3, 3, 3, 3], first, [0.5] * 6, [0.5] * 3, max_new=9)
             assert (0 <= acc).all() and (acc < 6).all()
+
+
+TORCH_EMPTY = """
+import sys
+import torch
+sys.path.insert(0, sys.argv[1])
+import __graft_entry__ as graft
+graft.load_package()
+from parakeet_amd import lm
+i32 = dict(dtype=torch.int32, device="cuda")
+for V in (50, 17000):
+    for more in (dict(), dict(max_new=5), dict(draft=torch.zeros(0, V, device="cuda"))):
+        accepted, cut = torch.full((3,), -9, **i32), torch.full((3,), -9, **i32)
+        lens = torch.tensor([5, 0, 77], **i32)
+        lm.verify(torch.zeros(0, V, device="cuda"), torch.zeros(0, **i32), torch.zeros(4, **i32), torch.zeros(0, device="cuda"),
+                  torch.zeros(3, device="cuda"), torch.zeros(0, **i32), accepted, lens=lens, lens_out=cut, **more)
+        assert accepted.tolist() == [0, 0, 0] and cut.tolist() == [5, 0, 77], (V, accepted, cut)
+print("ok empty")
+"""
+
+
+@pytest.mark.parametrize("V", [50, 17000])
+def test_a_call_without_rows(V):
+    """A step to which no request brings a token: nothing is accepted, lengths stay."""
+    for m in (None, 0, 5):
+        for y in (None, np.zeros((0, V), np.float32)):
+            out, acc, lens, _ = call(np.zeros((0, V), np.float32), y, [], [0] * 4, [], [0.5] * 3, lens=[5, 0, 77], max_new=m)
+            assert list(acc) == [0, 0, 0] and list(lens) == [5, 0, 77]
+
+
+def test_a_call_without_rows_on_torch_tensors():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", TORCH_EMPTY, root], capture_output=True, text=True, timeout=110)
+    assert p.returncode == 0 and "ok empty" in p.stdout, p.stdout[-1000:] + p.stderr[-3000:]

@@ -36,3 +36,11 @@ def test_outputs_that_lie_over_what_is_read_are_refused(pkg, kw, err):
              out=Arr((7,), "i32", ptr=1 << 16), accepted=Arr((3,), "i32"), workspace=Arr((1 << 20,), "u8"))
     a.update(kw)
     refused(lm.verify, a, err)
+
+
+def test_a_call_without_rows_is_asked_for_its_requests_arrays(pkg):
+    from parakeet_amd import lm
+    none = dict(logits=Arr((0, 50), "f32", ptr=0), tokens=Arr((0,), "i32", ptr=0), u=Arr((0,), "f32", ptr=0), out=Arr((0,), "i32", ptr=0))
+    a = dict(none, first=Arr((4,), "i32"), u_draw=Arr((3,), "f32"), accepted=Arr((3,), "i32"), workspace=Arr((1 << 20,), "u8"))
+    for name in ("first", "u_draw", "accepted"):
+        refused(lm.verify, dict(a, **{name: Arr(a[name].shape, a[name].dtype, ptr=0)}), "NULL")
