@@ -133,7 +133,7 @@ __device__ inline void append_rows(const pk_kv8_append_desc &a, const Turn &turn
     const Record8 rec{a.page, D};
     uint8_t *at = (uint8_t *)a.cache + (int64_t)(slot0 >> page_shift) * a.page_stride + h * rec.bytes();
     unsigned *scale_at = (unsigned *)(at + rec.scales() + (page_off / kBlock) * 16 + (V ? 4 : 0));
-    const unsigned before = rows.before;
+    unsigned before = rows.before;
     const LaneChannels<D> ch(c, !V && Turn::halves);
     float x[kPasses][8];
 #pragma unroll
@@ -169,6 +169,8 @@ __device__ inline void append_rows(const pk_kv8_append_desc &a, const Turn &turn
     const bool mine_bad = __any(top_any >= 0x7F800000u);
     unsigned top = mine_bad ? largest(0x7F800000u) : top_any;
     if ((t & 63) == 63) s_top[t >> 6] = top | (mine_bad ? 0x80000000u : 0u);
+    // every wave has the scale before it lets the others go on, who write the new one
+    asm volatile("" : "+v"(before));
     lds_barrier();
     top = s_top[0];
 #pragma unroll
