@@ -25,6 +25,9 @@ and with --draft N each step brings up to N tokens more, guessed from what follo
     lm.verify                which of them stand, by the target's own logits, and the token behind them
     lm.kv_plan               cuts the cache back to those that stand
 
+lm.verify has a temperature and no filters: what lm.sample's top-k, top-p and min-p would leave out is barred in the logits
+(torch's part), so that replies are drawn from the same distribution with drafts and without.
+
 --check reads the cache back (lm.kv4_load, lm.kv8_load) and compares the last step's logits with dense attention over it in
 f32.
 """
@@ -158,6 +161,17 @@ def turns(n: int):
     return [torch.tensor([int(t) for t in r["tokens"]] or [0]) for r in res], vocab
 
 
+def barred(logits, temperature, top_k, top_p, min_p):
+    """logits [n, vocab] with the tokens that lm.sample's filters leave out at -inf; the settings are the rows'."""
+    x = logits.double()
+    weight, order = torch.exp((x - x.amax(-1, keepdim=True)) / temperature[:, None]).sort(dim=-1, descending=True, stable=True)
+    rank = torch.arange(x.shape[1], device=x.device)
+    weight = weight * (rank < top_k[:, None])
+    keep = (weight.cumsum(-1) - weight < top_p[:, None] * weight.sum(-1, keepdim=True)) & (weight >= min_p[:, None] * weight[:, :1]) & (weight > 0)
+    keep[:, 0] = True
+    return logits.masked_fill(~torch.zeros_like(keep).scatter(1, order, keep), float("-inf"))
+
+
 def guesses(history, most: int):
     """Up to `most` tokens that followed the last token of a session's history when it was there before."""
     for i in range(len(history) - 2, -1, -1):
@@ -198,7 +212,7 @@ def main():
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     if a.draft:
-        replies, steps, fed, logits, took = drafted(a, sessions, forward, token, prompts, uniform, settings["temperature"])
+        replies, steps, fed, logits, took = drafted(a, sessions, forward, token, prompts, uniform, settings)
     else:
         got, fed = [token.clone()], token
         for steps in range(1, a.reply):
@@ -226,7 +240,7 @@ def main():
     print(f"{made / took:.0f} tokens/s, {took / steps * 1e6:.0f} us a step ({LAYERS} layers)")
 
 
-def drafted(a, sessions, forward, token, prompts, uniform, temperature):
+def drafted(a, sessions, forward, token, prompts, uniform, settings):
     """Steps that bring each session's last token with what was guessed behind it, until all have their reply.  Returns the
     replies, how many steps, and of the last one the tokens that stood last, their logits and the time of all."""
     t0 = time.perf_counter()
@@ -245,7 +259,9 @@ def drafted(a, sessions, forward, token, prompts, uniform, temperature):
         first = sessions.first.clone()
         logits = forward(tokens.long(), slots, pos, max(counts), sessions.longest)
         out = torch.zeros(n, **I32)
-        lm.verify(logits, tokens, first, uniform(n), uniform(a.sessions), out, accepted, max_new=max(counts), temperature=temperature,
+        own = torch.repeat_interleave(torch.arange(a.sessions, device="cuda"), torch.tensor(counts, device="cuda"), output_size=n)
+        allowed = barred(logits, **{k: v[own] for k, v in settings.items()})
+        lm.verify(allowed, tokens, first, uniform(n), uniform(a.sessions), out, accepted, max_new=max(counts), temperature=settings["temperature"],
                   lens=sessions.lens[0], lens_out=cut)
         sessions.plan(cut, 0)
         stood = accepted.tolist()
