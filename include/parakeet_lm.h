@@ -193,8 +193,10 @@ PK_API int pk_qk_rope(const pk_qk_rope_desc *desc, void *stream);
  * whose slot is outside the cache, or at positions below 0, are skipped (a query's row goes by its position alone).  Tokens are
  * appended: of a block, a call's rows lie one after the other in the call, their slots rising by one; the block's rows
  * before them are held already (none where they begin it, and then its scale begins anew), those behind them are not held
- * any more.  Held rows are rounded again where the block's scale grows with a new one, which loses at most the last bits
- * of values below 2^-6 of the scale.  Rows in another order leave the block's rows undefined (not other blocks). */
+ * any more.  Held rows are rounded again where the block's scale grows with a new one: values below 2^-6 of the new scale
+ * go to multiples of 2^-9 of it, the smallest to zero.  A scale does not shrink, nor a mark go, before the block begins
+ * anew: rows that are cut off again, as refused drafts are, leave the up to 31 before them as they made them.  Rows in
+ * another order leave the block's rows undefined (not other blocks). */
 typedef struct pk_kv8_append_desc {
     const void *k, *v, *q;              /* q nullable where heads is 0 */
     void *q_out;                        /* may be q itself */
@@ -212,7 +214,8 @@ PK_API int pk_kv8_append(const pk_kv8_append_desc *desc, void *stream);
 
 /* As pk_kv4_load and pk_kv4_attend, over the 8-bit cache.  Values at NaN codes are NaN; f16 results give held values of
  * 65,536, to which rows over 63,488 may be rounded, as 65,504.  Scores are f32 sums of exact products.  Probabilities go
- * to the values in f16, 11 bits down to 2^-28 of a query's largest, values exactly down to 2^-22 of the largest block. */
+ * to the values in f16, 11 bits down to 2^-28 of a query's largest, values exactly down to 2^-22 of the largest block: up to
+ * 2^-11 of sum p |v| beside a result's own rounding.  (pk_kv4_attend has 2^-16 of it for f16 results, 2^-8 for bf16.) */
 PK_API int pk_kv8_load(const pk_kv4_rows_desc *desc, void *stream);
 PK_API int pk_kv8_attend(const pk_kv4_attend_desc *desc, void *stream);
 PK_API int pk_kv8_attend_workspace(const pk_kv4_attend_desc *desc, int64_t *bytes);
@@ -221,10 +224,11 @@ PK_API int pk_kv8_attend_workspace(const pk_kv4_attend_desc *desc, int64_t *byte
  * the drafts behind it.  Row r of logits is what the target says behind tokens[r]; its draft is tokens[r + 1], the last row
  * has none.  With weights w = round(2^30 exp((x - max) / T)) at the request's temperature (pk_sample's, but for the
  * last bits of the exponential) p = w / sum w; of draft logits, at draft_temperature, likewise q; without draft logits q is
- * 1 at the draft.  Drafts are accepted, first to last, while u[r] q < p at the draft.  The token behind the accepted ones is drawn with u_draw[b] by rising index as pk_sample does:
- * behind the last draft from p; where a draft was refused from max(p - q, 0) in steps of 2^-52 (without draft logits from p
- * less the draft), or from p where that leaves nothing.  So the tokens are distributed as if drawn from p one by one.  Tokens
- * that a filter bars are given as -inf.  All in whole numbers and single f64 steps: no result depends on the order of a sum.
+ * 1 at the draft.  Drafts are accepted, first to last, while u[r] q < p at the draft.  The token behind the accepted ones is
+ * drawn with u_draw[b] by rising index as pk_sample does: behind the last draft from p; where a draft was refused from
+ * max(p - q, 0) in steps of 2^-52 (without draft logits from p less the draft), or from p where that leaves nothing.  So the
+ * tokens are distributed as if drawn from p one by one.  There are no filters as pk_sample's: tokens that one bars are given
+ * as -inf.  All in whole numbers and single f64 steps: no result depends on the order of a sum.
  * A draft outside the vocabulary is refused, and the token then drawn from p; a row of -inf accepts nothing and gives -1.
  * NaN counts as -inf, +inf as the largest number. */
 typedef struct pk_verify_desc {
@@ -247,7 +251,8 @@ typedef struct pk_verify_desc {
     int64_t workspace_bytes;
     int64_t logits_row, draft_row;
     int32_t n_rows, requests, vocab, dtype;
-    int32_t max_new;                    /* no request brings more rows (those behind are left out) */
+    int32_t max_new;                    /* no request brings more rows; those behind are left out, and lens_out counts them as
+                                           held.  n_rows where no bound is known */
     int32_t reserved;
 } pk_verify_desc;
 PK_API int pk_verify(const pk_verify_desc *desc, void *stream);

@@ -161,9 +161,11 @@ struct KeyTile8 {
 // Tiles of 16 columns that share each key's operands, their keys dealt to the eight waves 32 at a time; `splits` workgroups
 // share a tile's keys.  Each wave keeps its own maximum, sum and O of all columns, in registers, and they meet once at the end.
 // Two tiles where a request and kv head have more rows than one holds, as steps with drafted tokens do: unpacking a key's codes costs
-// the vector unit more than its products cost the matrix core, and is done once for both.  64 sessions' up to 5 tokens on up to 4,097
-// keys, 32 heads on 8 x 128 in bf16, 272 MB: 65 us (4.2 TB/s, a large copy 5.2), 100 with a tile a workgroup; 2 tokens on 200,003 and
-// 100,001 keys of 2 x 128, 154 MB: 37 us (4.2 TB/s).  One token on 733 keys of 8 x 64: 7 us, two splits of at most two steps and their join.
+// the vector unit more than its products cost the matrix core, and is done once for both.  On inputs that rotate 64 sessions' up to 5
+// tokens on up to 4,097 keys, 32 heads on 8 x 128 in bf16, 272 MB, take 72 us (3.8 TB/s, a large copy 5.2), 2 tokens on 200,003 and 100,001
+// keys of 2 x 128, 154 MB, 48 us (3.2 TB/s: 336 of 512 resident workgroups have keys).  On one input again and again, which the memory-side
+// cache holds in part: 64 and 37; the former 100 with a tile a workgroup.  One token on 733 keys of 8 x 64: 7 us, two splits of at most
+// two steps and their join.
 constexpr int kLogShift = 14;      // of P in attend8_kernel
 
 template <class T, int D, int Tiles>
@@ -401,10 +403,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 || Tiles == 2 ? 2 : 4) voi
 //
 // A workgroup takes 128 columns, a wave 32 of them, and goes over the keys 64 at a time, K and V as 16-bit values in LDS, two buffers
 // deep: see lm_attend.h.  4 prompts of up to 2,047 tokens on up to 4,095 keys, 32 heads on 8 x 128 in bf16, 162 GFLOP: 219 to 234 us a
-// call (0.72 PFLOP/s; a large product 1.22); through a window of 1,000, up to 4,001 on 8,191, 16 heads on 4 in f16, 77 GFLOP: 135 to 143.
-// Nothing bounds it alone: of 253 us under the profiler 204 are left without loads and unpacking, 224 with a quarter of the
-// products with V, 215 with an eighth of those with K, 239 without exponentials; the matrix cores are busy for a third of the cycles,
-// the vector units for 44%.  (Tried: 64 columns a wave, 358, by its registers; 256 columns a workgroup, four waves unpacking K and four V,
+// call (0.72 PFLOP/s; a large product 1.22); through a window of 1,000, up to 4,001 on 8,191, 16 heads on 4 in f16, 77 GFLOP: 135 to 152.
+// Under the profiler, which both take longer with (256 to 274 and 150 to 160): at 64 channels 189 and 117, at 256 657 and 420.
+// No unit is full: of 253 us 204 are left without loads and unpacking, 224 with a quarter of the products with V, 215 with
+// an eighth of those with K, 239 without exponentials; the matrix cores are busy for a third of the cycles, the vector units for
+// 44%.  The rest is waiting: whether one workgroup's products meet the other's exponentials is left to chance.  (Tried: 64 columns a wave, 358, by its registers; 256 columns a workgroup, four waves unpacking K and four V,
 // 274 and 204 through the window, whose one workgroup a unit waits as one.)
 
 constexpr float kPromptLogShift = 9.0f;      // of P: maxima lag by up to 2^6

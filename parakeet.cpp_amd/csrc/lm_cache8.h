@@ -223,9 +223,12 @@ __device__ inline void append_rows(const pk_kv8_append_desc &a, const Turn &turn
 // A workgroup has `rows` rows of the call (at most kTurnRows) and takes the runs that begin in them: rows one after the other
 // whose slots are one after the other in one block, 32 at most, the last of them perhaps behind its own rows.  It goes over
 // the run's heads of K and of V, its waves over those of the queries where they are given.  Rows without a slot are runs of one,
-// for their query.  A prompt's rows are bound by memory: 26,617 rows of 32 query heads on 8 x 128 in bf16 with norms, 600 MB, take
-// 188 us (3.2 TB/s; a large copy 5.2), 421 with a head of K or V a wave, whose registers leave two waves a vector unit, 204 without the next
-// head's rows on their way.  A step of 64 sessions, 215 rows: 9.4 us, the chain from slots to angles, norm, scale and codes.
+// for their query.  26,617 rows of 32 query heads on 8 x 128 in bf16 with norms, 600 MB, take 186 us (3.2 TB/s; a large copy
+// 5.2), 421 with a head of K or V a wave, whose registers leave two waves a vector unit, 204 without the next head's rows on their way:
+// memory, the wait for each block's largest magnitude, and queries that a workgroup begins behind all its K and V.  In f32, 1.15 GB,
+// 298 us; with half of the channels turned, or partners beside each other, 216 in bf16 and 339 in f32.  (f32 spills 2 to 18 registers at 64 and
+// 128 channels, the latter forms in 16 bits up to 6 at 128.)  A step of 64 sessions, 215 rows: 10 us, the chain from slots to angles,
+// norm, scale and codes.
 template <class T, int D, bool Halves>
 __global__ __launch_bounds__(kTurnThreads, D == 256 ? 2 : 4) void append_kernel(pk_kv8_append_desc a, int rows, int page_shift, int wide_q, int wide_kv) {
     using Raw = typename T::Raw;
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(kTurnThreads, D == 256 ? 2 : 4) void append_kernel(
 }
 
 // Rows out of the cache: 8 channels a thread, of V eight adjacent threads the same channels of 8 rows, whose entries lie side by side.
-// 26,617 rows of 8 x 128, 163 MB read and written: 39 us, 4.2 TB/s.
+// 26,617 rows of 8 x 128, 163 MB read and written: 39 us, 4.2 TB/s, on inputs that rotate or not.
 template <class T, int D, bool V>
 __device__ inline void load_rows8(const pk_kv4_rows_desc &a, int page_shift, bool wide, int h) {
     constexpr int kLanes = D / 8, kEach = kRowThreads / kLanes;

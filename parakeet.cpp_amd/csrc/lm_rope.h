@@ -189,9 +189,11 @@ __device__ inline void turn_rows(const typename T::Raw *x, int64_t x_row, bool w
     else turn_some<T, D, Batch>(x, x_row, wide, y, y_row, y_wide, w, turn, table, row0, n, lane);
 }
 
-// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms take 61 us, 4.8 TB/s, where a
-// large copy reaches 5.2: 4 passes' loads a wave of 16-bit types (2: 65; at 64 channels, where 4 are all rows, 28.5 and 29.6; f32 has no
-// registers for them), 8 waves a vector unit.  One row of 16 heads takes 3 us, a launch and the sines.
+// Memory bounds it: 16,385 rows (2,048 of them left out) of 32 + 8 heads x 128 in bf16 with norms, 294 MB, take 74 us on inputs that
+// rotate, 4.0 TB/s, where a large copy reaches 5.2; 62 on one input again and again, which the memory-side cache holds in part, as
+// in the next figures.  4 passes' loads a wave of 16-bit types (2: 65; at 64 channels, where 4 are all rows, 28.5 and 29.6; f32
+// has no registers for them), 8 waves a vector unit.  In f32 134 us (588 MB, 4.4 TB/s).  With half of the channels turned, or partners beside
+// each other, 103 in bf16 and 168 in f32: four waves a vector unit.  One row of 16 heads takes 3 us, a launch and the sines.
 template <class T, int D, bool Halves>
 __global__ __launch_bounds__(kTurnThreads, !Halves || D == 256 ? 4 : 8) void rope_kernel(pk_qk_rope_desc a, int rows, int wide_q, int wide_k) {
     using Raw = typename T::Raw;

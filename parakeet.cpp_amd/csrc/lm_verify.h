@@ -118,7 +118,8 @@ struct alignas(16) RowVerdict {
     int unused;
 };
 
-// One launch, bound by its latency: 5 rows of 8,193 logits in f32 take 8.3 us, 256 requests of up to 6 rows of 1,027 with draft logits 9.8.
+// One launch, bound by its latency: 5 rows of 8,193 logits in f32 take 8.0 us a call, 256 requests of up to 6 rows of 1,027 with draft logits
+// 9.6.
 //
 // A request has `each` workgroups, a row on each, or several in turn (Turns, which takes up to a tenth longer by its registers) where there
 // may be more rows.  Tokens are in registers: wave w has tokens ((w n + g) 64 + lane) 8 + e of a row, g < n <= G.  Every row that
@@ -308,8 +309,9 @@ __global__ __launch_bounds__(BS) void verify_row_kernel(pk_verify_desc a, int ea
 // Three launches over chunks of rows: each chunk's largest logit and its place; its weight; then, of each request's first row
 // that refuses its draft alone, what each chunk has left to draw from, of which the request's last chunk to arrive draws.
 // A launch's workgroups work out for themselves what follows from the launch before.  64 requests of up to 5 rows of 128,001 in bf16 with draft
-// logits, 57 MB: 14 us (memory), 19 (the vector unit: 28 million exponentials, the rows again from the cache behind the L2) and
-// 32 (the chain to each request's row, its own exponentials and f64 sums, the last chunk's search).
+// logits, 57 MB: 18 us (memory; 15 on one input again and again), 17 (the vector unit: 28 million exponentials, the rows again from the
+// cache behind the L2) and 31 (the chain to each request's row, its own exponentials and f64 sums, the drawn chunk summed again and
+// searched).
 
 // Of the first two launches, and of the draws, whose workgroups each find the row that they draw from: 256 and 512 threads.  (64 requests of up
 // to 5 rows of 128,001 in bf16 with draft logits on 256, 512 and 1,024: 24, 28, 35 us the two, 29, 21, 27 the draws.)

@@ -56,7 +56,7 @@ struct TurnGrid {
     int64_t groups;
 };
 // As many rows as leave 128 groups of them, whole blocks where that is more than half a block; beside each, as many parts of the heads as
-// make 2,048 workgroups.  32 heads on 8 x 128 in bf16, microseconds where 1,024, 128 and 32 groups are left: 1,000 rows normed
+// make 2,048 workgroups.  32 heads on 8 x 128 in bf16, one input again and again, microseconds where 1,024, 128 and 32 groups are left: 1,000 rows normed
 // and turned 9.4, 8.6, 10.6; up to 4 x 200 appended 22, 15, 12, 4 x 1,000 56, 24, 24; a token of 64 sessions 7.5, 7.6, 11.1.  With parts
 // up to 1,024, 2,048 and 4,096 workgroups: 16,385 rows 79, 61, 67, up to 4 x 200 appended 17.5, 14.8, 14.1.
 TurnGrid turn_grid(int n_rows, int parts, int least) {
@@ -104,7 +104,7 @@ struct HostKv8 {
     }
     // Two tiles that share each key's operands, where registers hold them.  32 heads on 8 x 128 in bf16, in one tile and in two: 64
     // sessions' up to 5 tokens (20 rows) on up to 4,097 keys 94 and 65 us, 4 x 20 tokens on 8,191 keys 39 and 24, 64 x 20 on 1,000 keys 47
-    // and 47; but one session's 6 tokens on 8,191 keys, whose splits do not fill the card, 13 and 17.
+    // and 47; but one session's 6 tokens on 8,191 keys, whose splits do not fill the card, 13 and 17, which this rule does not see.
     static int tile_cols(int64_t rows, int dim) { return rows <= 16 || dim == 256 ? 16 : 32; }
 };
 

@@ -479,8 +479,9 @@ def verify(logits, tokens, first, u, u_draw, out, accepted, *, max_new: int | No
 
     Uniform numbers u [n] decide on the drafts, u_draw [requests] on the token behind those accepted.  Written: out [n] int32
     (the accepted drafts, that token, then -1), accepted [requests], lens_out [requests] (lens less the refused drafts, what
-    kv_plan is to cut the cache back to) and prob [n] f32.  max_new bounds the rows of any request (None: n).
-    temperature and draft_temperature [requests] f32 (None = 1).
+    kv_plan is to cut the cache back to) and prob [n] f32.  max_new bounds the rows of any request (None: n); rows behind it
+    are left out, and lens_out counts them as held.  temperature and draft_temperature [requests] f32 (None = 1).  Tokens that
+    a filter as sample's bars are given as -inf.
     """
     if isinstance(logits, _Tensor) or _new_torch(logits):
         rc = _torch_calls.verify(logits, tokens, first, u, u_draw, out, accepted, max_new, draft, temperature, draft_temperature, lens, lens_out,
