@@ -14,7 +14,7 @@
 
 namespace pklm {
 
-// Single steps: neither is fused with the other, as the compiler would where it may (the header's __dmul_rn and __dadd_rn are plain
+// Single steps: neither is fused with the other, as the compiler would where it may (HIP's __dmul_rn and __dadd_rn are plain
 // operators, which it fuses).
 __device__ inline double product(double a, double b) {
 #pragma clang fp contract(off)
